@@ -707,6 +707,99 @@ mg_status mg_mcmc_add_noise(float* means, const float* quats, const float* log_s
                             mg_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
+/* Operators on rows of per-pixel features (no reference counterpart)       */
+/* ------------------------------------------------------------------------ */
+
+/* Element types of the entry points below. */
+#define MG_F32 0
+#define MG_BF16 1
+#define MG_F16 2
+
+/* Layer normalisation of each row of x (rows, channels), contiguous:
+ *   y = (x - mean) * rstd * weight + bias, rstd = 1 / sqrt(var + eps),
+ * var the mean of (x - mean)^2. Sums, mean and rstd are fp32; y has x's
+ * type and is rounded once. weight and bias (channels,) of param_dtype may
+ * each be NULL (1 and 0). mean and rstd (rows,) are written when not NULL
+ * (the adjoint needs them). With codes and scales given, x is also written
+ * in the 8-bit form of mg_pack8 in the same pass. channels <=
+ * MG_LAYER_NORM_MAX_CHANNELS: a row stays in registers. y may not overlap x. */
+#define MG_LAYER_NORM_MAX_CHANNELS 8192
+mg_status mg_layer_norm_forward(const void* x, int32_t dtype, const void* weight,
+                                const void* bias, int32_t param_dtype, int64_t rows,
+                                int64_t channels, float eps, void* y, float* mean, float* rstd,
+                                int8_t* codes, float* scales, mg_stream_t stream);
+
+/* The adjoint: dx (rows, channels), dweight and dbias (channels,) of
+ * param_dtype, each OVERWRITTEN, each NULL to leave it out. x comes either
+ * as it was or in its 8-bit form (codes, scales; x NULL). The sums over
+ * rows are fp32 in a fixed order. scratch (NULL when neither dweight nor
+ * dbias is wanted): mg_layer_norm_backward_scratch_bytes. */
+size_t mg_layer_norm_backward_scratch_bytes(int64_t rows, int64_t channels);
+mg_status mg_layer_norm_backward(const void* dy, const void* x, const int8_t* codes,
+                                 const float* scales, int32_t dtype, const void* weight,
+                                 int32_t param_dtype, const float* mean, const float* rstd,
+                                 int64_t rows, int64_t channels, void* dx, void* dweight,
+                                 void* dbias, void* scratch, size_t scratch_bytes,
+                                 mg_stream_t stream);
+
+/* The 8-bit form of x (rows, channels): codes (rows, channels) and scales
+ * (rows, ceil(channels / 128)). For each 128 channels of a row (fewer at its
+ * end) with largest magnitude a: scale = a / 127, code = round half even(x *
+ * (127 / a)), each operation a correctly rounded fp32 one. a below 1e-30:
+ * scale and codes 0. An infinity or a NaN among them: scale NaN. codes must
+ * be 8-byte aligned. */
+mg_status mg_pack8(const void* x, int32_t dtype, int64_t rows, int64_t channels, int8_t* codes,
+                   float* scales, mg_stream_t stream);
+
+/* x = code * scale, rounded once to dtype. */
+mg_status mg_unpack8(const int8_t* codes, const float* scales, int64_t rows, int64_t channels,
+                     int32_t dtype, void* x, mg_stream_t stream);
+
+/* Softmax cross entropy of features (rows, channels) against class
+ * embeddings (n_classes, channels), both of `dtype` and contiguous:
+ *   z[p, v] = scale * features[p] . classes[v] + class_bias[v]
+ *   loss[p] = log(sum_v exp(z[p, v])) - z[p, label[p]]
+ * class_bias (n_classes,) fp32 may be NULL; -infinity there takes a class
+ * out. No logit is stored in the forward pass; logits, sums and losses are
+ * fp32. labels are uint8, int32 or int64 (label_bytes 1, 4, 8). A row whose
+ * label equals ignore_index has loss 0, takes no part in a mean and gets and
+ * gives no gradient, whatever its features hold. A label outside [0,
+ * n_classes) makes the loss NaN, records code 3 in the device error word, and
+ * gives no gradient. reduction: MG_REDUCE_NONE writes `rows` losses,
+ * MG_REDUCE_SUM and MG_REDUCE_MEAN one; the mean of no live rows is 0.
+ * For the backward pass stats (2, rows) and live (1,) are written when not
+ * NULL (live: sum and mean only): the log of the sum, 1 - softmax(label), and
+ * the count of rows that take part. */
+#define MG_REDUCE_NONE 0
+#define MG_REDUCE_MEAN 1
+#define MG_REDUCE_SUM 2
+#define MG_LABEL_MAX_CHANNELS 512
+#define MG_LABEL_MAX_CLASSES (1 << 20)
+#define MG_LABEL_MAX_ROWS ((int64_t)1 << 30)
+size_t mg_label_loss_scratch_bytes(int64_t rows, int64_t channels, int64_t n_classes,
+                                   int32_t dtype, int32_t backward);
+mg_status mg_label_loss_forward(const void* features, const void* classes, int32_t dtype,
+                                const float* class_bias, const void* labels,
+                                int32_t label_bytes, int64_t ignore_index, int64_t rows,
+                                int64_t channels, int64_t n_classes, float scale,
+                                int32_t reduction, float* loss, float* stats, float* live,
+                                void* scratch, size_t scratch_bytes, mg_stream_t stream);
+
+/* Its adjoint: d_features, d_classes (of `dtype`) and d_bias (fp32), each
+ * OVERWRITTEN, each NULL to leave it out. grad_loss: one float, or one per
+ * row with MG_REDUCE_NONE. The scratch (backward = 1) holds pieces of the
+ * logits' gradient, never all of it when it is large. Sums run in a fixed
+ * order: equal calls give equal bits. */
+mg_status mg_label_loss_backward(const void* features, const void* classes, int32_t dtype,
+                                 const float* class_bias, const void* labels,
+                                 int32_t label_bytes, int64_t ignore_index, int64_t rows,
+                                 int64_t channels, int64_t n_classes, float scale,
+                                 int32_t reduction, const float* grad_loss, const float* stats,
+                                 const float* live, void* d_features, void* d_classes,
+                                 float* d_bias, void* scratch, size_t scratch_bytes,
+                                 mg_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
 /* Device error word                                                        */
 /* ------------------------------------------------------------------------ */
 
@@ -714,7 +807,7 @@ mg_status mg_mcmc_add_noise(float* means, const float* quats, const float* log_s
  * spins that gave up, checked-mode index faults). Synchronises `stream`.
  * *code_out receives 0 when nothing was recorded, else the first code:
  * 1 a sort look-back wait gave up, 2 a tile list reached past the sized pair
- * count. The reference refuses instead of continuing silently
+ * count, 3 a label outside the classes. The reference refuses instead of continuing silently
  * (metal_gauss/api.py:18-26); callers raise on a non-zero code. */
 mg_status mg_read_device_error(int32_t* code_out, mg_stream_t stream);
 

@@ -137,6 +137,17 @@ SIGNATURES = {
     "mg_l1_ssim_scratch_bytes": (sz, [i32, i32]),
     "mg_l1_ssim_loss": (i32, [vp, vp, vp, i32, i32, f32, f32, f32, vp, vp, vp, sz, vp]),
     "mg_l1_ssim_loss_u8": (i32, [vp, vp, vp, i32, i32, f32, f32, f32, vp, vp, vp, sz, vp]),
+    "mg_layer_norm_forward": (i32, [vp, i32, vp, vp, i32, i64, i64, f32, vp, vp, vp, vp, vp, vp]),
+    "mg_layer_norm_backward_scratch_bytes": (sz, [i64, i64]),
+    "mg_layer_norm_backward": (i32, [vp, vp, vp, vp, i32, vp, i32, vp, vp, i64, i64, vp, vp, vp,
+                                     vp, sz, vp]),
+    "mg_pack8": (i32, [vp, i32, i64, i64, vp, vp, vp]),
+    "mg_unpack8": (i32, [vp, vp, i64, i64, i32, vp, vp]),
+    "mg_label_loss_scratch_bytes": (sz, [i64, i64, i64, i32, i32]),
+    "mg_label_loss_forward": (i32, [vp, vp, i32, vp, vp, i32, i64, i64, i64, i64, f32, i32, vp, vp,
+                                    vp, vp, sz, vp]),
+    "mg_label_loss_backward": (i32, [vp, vp, i32, vp, vp, i32, i64, i64, i64, i64, f32, i32, vp,
+                                     vp, vp, vp, vp, vp, vp, sz, vp]),
     "mg_read_device_error": (i32, [C.POINTER(i32), vp]),
     "mg_peek_device_error": (i32, [vp, vp]),
     "mg_sort_lookback_selftest_scratch_bytes": (sz, []),
@@ -214,7 +225,8 @@ def make_camera(viewmat: torch.Tensor, fx: float, fy: float, cx: float, cy: floa
 
 
 DEVICE_ERRORS = {1: "a radix-sort look-back wait gave up (a predecessor tile never published)",
-                 2: "a tile list reached past the sized pair count"}
+                 2: "a tile list reached past the sized pair count",
+                 3: "a label outside the classes"}
 
 
 class DeviceError(RuntimeError):

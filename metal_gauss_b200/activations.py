@@ -1,0 +1,129 @@
+"""Activation checkpoints in 8 bits.
+
+The feature maps of a step's views are the largest tensors its backward pass
+holds. `pack8` puts a map into one byte per element and one fp32 scale per 128
+channels (`mg_pack8`), `unpack8` reads it back, and `checkpoint8(fn, x, ...)`
+runs a segment of the graph whose input is held in that form and computed
+again in the backward pass. `layernorm.layer_norm(saved="int8")` uses the same
+form without the second forward pass.
+
+    a = largest magnitude of 128 channels of a row (fewer at its end)
+    scale = a / 127,  code = round half even(x * (127 / a)),  value = code * scale
+
+so a value comes back within a / 254 of itself.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from ._lib import ptr
+
+BLOCK = 128
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # MG_F32, MG_BF16, MG_F16
+
+
+def dtype_code(t: torch.Tensor, what: str) -> int:
+    if t.dtype not in DTYPES:
+        raise TypeError(f"{what} must be float32, bfloat16 or float16, got {t.dtype}")
+    return DTYPES[t.dtype]
+
+
+def check_cuda(t: torch.Tensor, what: str) -> None:
+    if t.device.type != "cuda":
+        raise RuntimeError(f"{what} is on '{t.device}': the CUDA backend needs CUDA tensors and "
+                           "does not move data or fall back")
+
+
+def _rows(t: torch.Tensor, what: str) -> tuple[int, int]:
+    if t.dim() < 1 or t.shape[-1] < 1:
+        raise ValueError(f"{what} must be (..., channels) with at least one channel, "
+                         f"got {tuple(t.shape)}")
+    return t.numel() // t.shape[-1], t.shape[-1]
+
+
+@torch.no_grad()
+def pack8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """x (..., channels) in 8 bits: codes int8 (..., channels) and scales
+    float32 (..., ceil(channels / 128)). 128 channels with an infinity or a
+    NaN among them read back as NaN; below 1e-30 they read back as 0."""
+    code, (n, d) = dtype_code(x, "pack8: x"), _rows(x, "pack8: x")
+    check_cuda(x, "pack8: x")
+    with torch.cuda.device(x.device):
+        x = x.detach().contiguous()
+        codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+        scales = torch.empty(*x.shape[:-1], -(-d // BLOCK), dtype=torch.float32, device=x.device)
+        _lib.call("mg_pack8", ptr(x), code, n, d, ptr(codes), ptr(scales), _lib.stream())
+    return codes, scales
+
+
+@torch.no_grad()
+def unpack8(codes: torch.Tensor, scales: torch.Tensor,
+            dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The tensor that `pack8` gave codes and scales for, as `dtype`."""
+    if codes.dtype != torch.int8 or scales.dtype != torch.float32:
+        raise TypeError(f"unpack8 takes int8 codes and float32 scales, got {codes.dtype} and "
+                        f"{scales.dtype}")
+    if dtype not in DTYPES:
+        raise TypeError(f"unpack8: dtype must be float32, bfloat16 or float16, got {dtype}")
+    n, d = _rows(codes, "unpack8: codes")
+    want = (*codes.shape[:-1], -(-d // BLOCK))
+    if tuple(scales.shape) != want:
+        raise ValueError(f"unpack8: scales must be {want} for codes {tuple(codes.shape)}, "
+                         f"got {tuple(scales.shape)}")
+    if scales.device != codes.device:
+        raise RuntimeError(f"unpack8: codes on {codes.device}, scales on {scales.device}")
+    check_cuda(codes, "unpack8: codes")
+    with torch.cuda.device(codes.device):
+        codes, scales = codes.contiguous(), scales.contiguous()
+        if codes.data_ptr() % 8:
+            codes = codes.clone()
+        x = torch.empty(codes.shape, dtype=dtype, device=codes.device)
+        _lib.call("mg_unpack8", ptr(codes), ptr(scales), n, d, DTYPES[dtype], ptr(x),
+                  _lib.stream())
+    return x
+
+
+class _Checkpoint8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, fn, x, *args):
+        ctx.fn, ctx.dtype = fn, x.dtype
+        ctx.where = [i for i, a in enumerate(args) if torch.is_tensor(a)]
+        ctx.others = [None if torch.is_tensor(a) else a for a in args]
+        codes, scales = pack8(x)
+        ctx.save_for_backward(codes, scales, *(args[i] for i in ctx.where))
+        with torch.no_grad():
+            out = fn(x, *args)
+        if not torch.is_tensor(out):
+            raise TypeError(f"checkpoint8: fn must return one tensor, got {type(out).__name__}")
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        codes, scales, *tensors = ctx.saved_tensors
+        need = ctx.needs_input_grad[1:]
+        x = unpack8(codes, scales, ctx.dtype)
+        args = list(ctx.others)
+        with torch.enable_grad():
+            x.requires_grad_(need[0])
+            for i, t in zip(ctx.where, tensors):
+                args[i] = t.detach().requires_grad_(need[1 + i])
+            out = ctx.fn(x, *args)
+        leaves = [t for t, k in zip([x] + args, need) if k]
+        found = iter(torch.autograd.grad(out, leaves, grad, allow_unused=True))
+        return (None,) + tuple(next(found) if k else None for k in need)
+
+
+def checkpoint8(fn, x: torch.Tensor, *args) -> torch.Tensor:
+    """fn(x, *args), differentiable in x and the tensors among args, holding
+    x in 8 bits and nothing that fn computes: the backward pass reads x back
+    and runs fn again. The result is fn's own; the gradients are those of fn
+    at the x that was read back. fn must return one tensor, do the same work
+    both times, and take every tensor that needs a gradient as an argument
+    (one that it closes over gets none)."""
+    dtype_code(x, "checkpoint8: x")
+    _rows(x, "checkpoint8: x")
+    check_cuda(x, "checkpoint8: x")
+    return _Checkpoint8.apply(fn, x, *args)

@@ -1,0 +1,512 @@
+// Layer normalisation of rows of channels, forward and adjoint.
+//
+//   mean, var over the row; rstd = 1 / sqrt(var + eps); h = (x - mean) rstd
+//   y  = h w + b
+//   dx = rstd (g - mean(g) - h mean(g h)),  g = dy w
+//   dw = sum over rows of dy h,  db = sum over rows of dy
+//
+// Memory bounds it: forward reads x and writes y, the adjoint reads dy and x
+// (or x's 8-bit form) and writes dx. A row is held in the registers of a team
+// of lanes between its reductions, so each tensor crosses HBM once: LPR lanes
+// of a warp for rows up to 1024 channels (several rows to a warp when they are
+// short), the 8 warps of a block above that. The variance is the mean of
+// (x - mean)^2 from those registers, never E[x^2] - mean^2.
+// dw and db: a lane owns the same channels of every row its team takes, so
+// the sums over rows stay in its registers; teams of a block join in shared
+// memory, blocks through one fp32 row each in scratch, summed in a fixed order
+// by a second kernel (no atomics: equal calls give equal bits).
+#include "rows.cuh"
+
+namespace mg {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+// The channel of register group k (VEC channels) of this lane. A warp's 32
+// lanes cover 128 consecutive channels (4 groups at VEC 1, one at VEC 4, half
+// of one at VEC 8), so the channels that share an 8-bit scale are in one warp.
+template <int VEC, int LPR, int WARPS>
+__device__ __forceinline__ int channel_of(int k, int warp, int lane) {
+    if constexpr (WARPS == 1) return (k * LPR + lane) * VEC;
+    if constexpr (VEC == 1) return ((k / 4) * WARPS + warp) * 128 + (k % 4) * 32 + lane;
+    return ((k * WARPS + warp) * 32 + lane) * VEC;
+}
+
+// Sum over the team that holds a row.
+template <int LPR, int WARPS>
+__device__ __forceinline__ float2 team_sum(float a, float b, float2* sh, int warp, int lane) {
+    a = lanes_sum<LPR>(a);
+    b = lanes_sum<LPR>(b);
+    if constexpr (WARPS > 1) {
+        __syncthreads();  // the previous sum's readers are done
+        if (lane == 0) sh[warp] = make_float2(a, b);
+        __syncthreads();
+        a = b = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            a += sh[w].x;
+            b += sh[w].y;
+        }
+    }
+    return make_float2(a, b);
+}
+
+__device__ __forceinline__ float param_at(const void* p, int dtype, int c) {
+    if (dtype == MG_F32) return static_cast<const float*>(p)[c];
+    if (dtype == MG_BF16) return to_f32(static_cast<const __nv_bfloat16*>(p)[c]);
+    return to_f32(static_cast<const __half*>(p)[c]);
+}
+
+template <typename T, int VEC, int LPR, int NV, int WARPS>
+__global__ void __launch_bounds__(kThreads)
+norm_forward_kernel(const T* __restrict__ x, const void* __restrict__ weight,
+                    const void* __restrict__ bias, int param_dtype, int64_t rows, int channels,
+                    float eps, T* __restrict__ y, float* __restrict__ mean_out,
+                    float* __restrict__ rstd_out, int8_t* __restrict__ codes,
+                    float* __restrict__ scales) {
+    __shared__ float2 sh[WARPS > 1 ? WARPS : 1];
+    constexpr int kTeams = WARPS > 1 ? 1 : kThreads / LPR;
+    const int lane = WARPS > 1 ? threadIdx.x % 32 : threadIdx.x % LPR;
+    const int warp = WARPS > 1 ? threadIdx.x / 32 : 0;
+    const int team = WARPS > 1 ? 0 : threadIdx.x / LPR;
+    const float inv_n = 1.0f / (float)channels;
+    const int nb = (channels + kBlock8 - 1) / kBlock8;
+
+    float w[NV * VEC], b[NV * VEC];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int c = channel_of<VEC, LPR, WARPS>(k, warp, lane);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            w[k * VEC + i] = (weight != nullptr && c < channels) ? param_at(weight, param_dtype, c + i) : 1.0f;
+            b[k * VEC + i] = (bias != nullptr && c < channels) ? param_at(bias, param_dtype, c + i) : 0.0f;
+        }
+    }
+
+    // every lane of a warp takes every round: the reductions are warp-wide
+    const int64_t rounds = (rows + (int64_t)gridDim.x * kTeams - 1) / ((int64_t)gridDim.x * kTeams);
+    for (int64_t r = 0; r < rounds; ++r) {
+        const int64_t row = (r * gridDim.x + blockIdx.x) * kTeams + team;
+        const bool live = row < rows;
+        const T* xr = x + row * channels;
+        float v[NV * VEC];
+        float s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int c = channel_of<VEC, LPR, WARPS>(k, warp, lane);
+            if (live && c < channels) {
+                load_row<T, VEC>(xr + c, v + k * VEC);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) v[k * VEC + i] = 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) s += v[k * VEC + i];
+        }
+        const float mean = team_sum<LPR, WARPS>(s, 0.0f, sh, warp, lane).x * inv_n;
+        float q = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            if (channel_of<VEC, LPR, WARPS>(k, warp, lane) < channels) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    const float d = v[k * VEC + i] - mean;
+                    q = fmaf(d, d, q);
+                }
+            }
+        }
+        const float var = team_sum<LPR, WARPS>(q, 0.0f, sh, warp, lane).x * inv_n;
+        const float rstd = 1.0f / sqrtf(var + eps);
+        if (codes != nullptr) {
+            // one scale per 128 channels, the maximum over the lanes that hold them
+            constexpr int kGroup = VEC == 8 ? (LPR < 16 ? LPR : 16) : LPR;
+            constexpr int kStep = VEC == 1 ? (NV < 4 ? NV : 4) : 1;
+#pragma unroll
+            for (int k0 = 0; k0 < NV; k0 += kStep) {
+                float a = 0.0f;
+#pragma unroll
+                for (int i = 0; i < kStep * VEC; ++i) a = fmaxf(a, mag8(v[k0 * VEC + i]));
+                a = lanes_max<kGroup>(a);
+                const Scale8 s8 = scale8(a);
+#pragma unroll
+                for (int k = k0; k < k0 + kStep; ++k) {
+                    const int c = channel_of<VEC, LPR, WARPS>(k, warp, lane);
+                    if (live && c < channels) {
+                        int qv[VEC];
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) qv[i] = code8(v[k * VEC + i], s8.inv);
+                        store_codes<VEC>(codes + row * channels + c, qv);
+                        if (c % kBlock8 == 0) scales[row * nb + c / kBlock8] = s8.scale;
+                    }
+                }
+            }
+        }
+        if (live) {
+            T* yr = y + row * channels;
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const int c = channel_of<VEC, LPR, WARPS>(k, warp, lane);
+                if (c < channels) {
+                    float o[VEC];
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i)
+                        o[i] = fmaf((v[k * VEC + i] - mean) * rstd, w[k * VEC + i], b[k * VEC + i]);
+                    store_row<T, VEC>(yr + c, o);
+                }
+            }
+            if (mean_out != nullptr && lane == 0 && warp == 0) {
+                mean_out[row] = mean;
+                rstd_out[row] = rstd;
+            }
+        }
+    }
+}
+
+template <typename T, int VEC, int LPR, int NV, int WARPS, bool HELD8>
+__global__ void __launch_bounds__(kThreads)
+norm_backward_kernel(const T* __restrict__ dy, const T* __restrict__ x,
+                     const int8_t* __restrict__ codes, const float* __restrict__ scales,
+                     const void* __restrict__ weight, int param_dtype,
+                     const float* __restrict__ mean_in, const float* __restrict__ rstd_in,
+                     int64_t rows, int channels, T* __restrict__ dx,
+                     float* __restrict__ partial) {
+    __shared__ float2 sh[WARPS > 1 ? WARPS : 1];
+    constexpr int kTeams = WARPS > 1 ? 1 : kThreads / LPR;
+    const int lane = WARPS > 1 ? threadIdx.x % 32 : threadIdx.x % LPR;
+    const int warp = WARPS > 1 ? threadIdx.x / 32 : 0;
+    const int team = WARPS > 1 ? 0 : threadIdx.x / LPR;
+    const float inv_n = 1.0f / (float)channels;
+    const int nb = (channels + kBlock8 - 1) / kBlock8;
+
+    float w[NV * VEC], dw[NV * VEC], db[NV * VEC];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int c = channel_of<VEC, LPR, WARPS>(k, warp, lane);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            w[k * VEC + i] = (weight != nullptr && c < channels) ? param_at(weight, param_dtype, c + i) : 1.0f;
+            dw[k * VEC + i] = db[k * VEC + i] = 0.0f;
+        }
+    }
+
+    const int64_t rounds = (rows + (int64_t)gridDim.x * kTeams - 1) / ((int64_t)gridDim.x * kTeams);
+    for (int64_t r = 0; r < rounds; ++r) {
+        const int64_t row = (r * gridDim.x + blockIdx.x) * kTeams + team;
+        const bool live = row < rows;
+        const float mean = live ? __ldg(mean_in + row) : 0.0f;
+        const float rstd = live ? __ldg(rstd_in + row) : 0.0f;
+        float h[NV * VEC], g[NV * VEC];
+        float sg = 0.0f, sgh = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int c = channel_of<VEC, LPR, WARPS>(k, warp, lane);
+            if (live && c < channels) {
+                load_row<T, VEC>(dy + row * channels + c, g + k * VEC);
+                if constexpr (HELD8) {
+                    load_codes<VEC>(codes + row * channels + c, h + k * VEC);
+                    const float sc = __ldg(scales + row * nb + c / kBlock8);
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) h[k * VEC + i] = __fmul_rn(h[k * VEC + i], sc);
+                } else {
+                    load_row<T, VEC>(x + row * channels + c, h + k * VEC);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    g[k * VEC + i] = 0.0f;
+                    h[k * VEC + i] = mean;
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NV * VEC; ++i) {
+            h[i] = (h[i] - mean) * rstd;
+            dw[i] = fmaf(g[i], h[i], dw[i]);
+            db[i] += g[i];
+            g[i] *= w[i];
+            sg += g[i];
+            sgh = fmaf(g[i], h[i], sgh);
+        }
+        if (dx != nullptr) {
+            const float2 m = team_sum<LPR, WARPS>(sg, sgh, sh, warp, lane);
+            const float c1 = m.x * inv_n, c2 = m.y * inv_n;
+            if (live) {
+#pragma unroll
+                for (int k = 0; k < NV; ++k) {
+                    const int c = channel_of<VEC, LPR, WARPS>(k, warp, lane);
+                    if (c < channels) {
+                        float o[VEC];
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i)
+                            o[i] = rstd * (g[k * VEC + i] - c1 - h[k * VEC + i] * c2);
+                        store_row<T, VEC>(dx + row * channels + c, o);
+                    }
+                }
+            }
+        }
+    }
+
+    if (partial == nullptr) return;
+    // lanes of a warp that hold the same channels, then the block's warps
+    float* out = partial + (int64_t)blockIdx.x * 2 * channels;
+    if constexpr (WARPS == 1) {
+        extern __shared__ float join[];  // 8 warps x channels
+        const int wid = threadIdx.x / 32;
+#pragma unroll
+        for (int i = 0; i < NV * VEC; ++i) {
+#pragma unroll
+            for (int o = LPR; o < 32; o <<= 1) {
+                dw[i] += __shfl_xor_sync(0xffffffffu, dw[i], o);
+                db[i] += __shfl_xor_sync(0xffffffffu, db[i], o);
+            }
+        }
+#pragma unroll
+        for (int pass = 0; pass < 2; ++pass) {
+            __syncthreads();
+            if (threadIdx.x % 32 < LPR) {
+#pragma unroll
+                for (int k = 0; k < NV; ++k) {
+                    const int c = channel_of<VEC, LPR, WARPS>(k, warp, lane);
+                    if (c < channels) {
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i)
+                            join[wid * channels + c + i] = pass == 0 ? dw[k * VEC + i] : db[k * VEC + i];
+                    }
+                }
+            }
+            __syncthreads();
+            for (int c = threadIdx.x; c < channels; c += kThreads) {
+                float s = 0.0f;
+#pragma unroll
+                for (int q = 0; q < kThreads / 32; ++q) s += join[q * channels + c];
+                out[pass * channels + c] = s;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int c = channel_of<VEC, LPR, WARPS>(k, warp, lane);
+            if (c < channels) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    out[c + i] = dw[k * VEC + i];
+                    out[channels + c + i] = db[k * VEC + i];
+                }
+            }
+        }
+    }
+}
+
+// Column sums of the blocks' partial rows: 32 columns and 32 row groups to a
+// block; columns [0, channels) are dw, the rest db.
+__global__ void __launch_bounds__(1024)
+norm_join_kernel(const float* __restrict__ partial, int blocks, int channels, int param_dtype,
+                 void* __restrict__ dweight, void* __restrict__ dbias) {
+    __shared__ float sh[32][33];
+    const int col = blockIdx.x * 32 + threadIdx.x;
+    float s = 0.0f;
+    if (col < 2 * channels) {
+#pragma unroll 4
+        for (int r = threadIdx.y; r < blocks; r += 32) s += partial[(int64_t)r * 2 * channels + col];
+    }
+    sh[threadIdx.y][threadIdx.x] = s;
+    __syncthreads();
+    s = lanes_sum<32>(sh[threadIdx.x][threadIdx.y]);
+    const int c = blockIdx.x * 32 + threadIdx.y;
+    if (threadIdx.x != 0 || c >= 2 * channels) return;
+    void* dst = c < channels ? dweight : dbias;
+    if (dst == nullptr) return;
+    const int i = c < channels ? c : c - channels;
+    if (param_dtype == MG_F32) static_cast<float*>(dst)[i] = s;
+    else if (param_dtype == MG_BF16) static_cast<__nv_bfloat16*>(dst)[i] = from_f32<__nv_bfloat16>(s);
+    else static_cast<__half*>(dst)[i] = from_f32<__half>(s);
+}
+
+// Blocks of the adjoint: enough to fill the device, few enough that the join
+// stays short. Depends on the sizes only, so scratch and launch agree.
+int64_t backward_blocks(int64_t rows, int64_t channels) {
+    const int64_t teams = channels > 1024 ? 1 : std::max<int64_t>(8, 256 / std::max<int64_t>(1, channels));
+    const int64_t want = (rows + teams - 1) / teams;
+    return std::max<int64_t>(1, std::min<int64_t>(want, 4 * (int64_t)sm_count()));
+}
+
+struct Forward {
+    const void *x, *weight, *bias;
+    int param_dtype;
+    int64_t rows;
+    int channels;
+    float eps;
+    void* y;
+    float *mean, *rstd;
+    int8_t* codes;
+    float* scales;
+    cudaStream_t st;
+
+    template <typename T, int VEC, int LPR, int NV, int WARPS>
+    mg_status run() const {
+        constexpr int kTeams = WARPS > 1 ? 1 : kThreads / LPR;
+        const int64_t want = (rows + kTeams - 1) / kTeams;
+        const int grid = (int)std::min<int64_t>(want, 8 * (int64_t)sm_count());
+        norm_forward_kernel<T, VEC, LPR, NV, WARPS><<<grid, kThreads, 0, st>>>(
+            static_cast<const T*>(x), weight, bias, param_dtype, rows, channels, eps,
+            static_cast<T*>(y), mean, rstd, codes, scales);
+        return check_launch("layer_norm_forward");
+    }
+};
+
+struct Backward {
+    const void *dy, *x;
+    const int8_t* codes;
+    const float* scales;
+    const void* weight;
+    int param_dtype;
+    const float *mean, *rstd;
+    int64_t rows;
+    int channels;
+    void* dx;
+    float* partial;
+    int grid;
+    cudaStream_t st;
+
+    template <typename T, int VEC, int LPR, int NV, int WARPS>
+    mg_status run() const {
+        const size_t smem = WARPS == 1 ? sizeof(float) * 8 * (size_t)channels : 0;
+        if (codes != nullptr)
+            norm_backward_kernel<T, VEC, LPR, NV, WARPS, true><<<grid, kThreads, smem, st>>>(
+                static_cast<const T*>(dy), nullptr, codes, scales, weight, param_dtype, mean, rstd,
+                rows, channels, static_cast<T*>(dx), partial);
+        else
+            norm_backward_kernel<T, VEC, LPR, NV, WARPS, false><<<grid, kThreads, smem, st>>>(
+                static_cast<const T*>(dy), static_cast<const T*>(x), nullptr, nullptr, weight,
+                param_dtype, mean, rstd, rows, channels, static_cast<T*>(dx), partial);
+        return check_launch("layer_norm_backward");
+    }
+};
+
+// The team for a row length: the fewest lanes that hold the row with one
+// vector each, then more vectors per lane, then a block.
+template <typename T, int VEC, typename Op>
+mg_status pick_team(const Op& op, int channels) {
+    const int vecs = (channels + VEC - 1) / VEC;
+    if (vecs <= 4) return op.template run<T, VEC, 4, 1, 1>();
+    if (vecs <= 8) return op.template run<T, VEC, 8, 1, 1>();
+    if (vecs <= 16) return op.template run<T, VEC, 16, 1, 1>();
+    if (vecs <= 32) return op.template run<T, VEC, 32, 1, 1>();
+    if (vecs <= 64) return op.template run<T, VEC, 32, 2, 1>();
+    if (vecs <= 128) return op.template run<T, VEC, 32, 4, 1>();
+    if constexpr (VEC <= 4) {
+        if (vecs <= 256) return op.template run<T, VEC, 32, 8, 1>();
+    }
+    if constexpr (VEC == 1) {
+        if (vecs <= 512) return op.template run<T, VEC, 32, 16, 1>();
+        if (vecs <= 1024) return op.template run<T, VEC, 32, 32, 1>();
+        if (vecs <= 4096) return op.template run<T, VEC, 32, 16, 8>();
+        return op.template run<T, VEC, 32, 32, 8>();
+    } else {
+        if (vecs <= 512) return op.template run<T, VEC, 32, 2, 8>();
+        if (VEC == 8 || vecs <= 1024) return op.template run<T, VEC, 32, 4, 8>();
+        return op.template run<T, VEC, 32, VEC == 8 ? 4 : 8, 8>();
+    }
+}
+
+template <typename Op>
+mg_status pick_type(const Op& op, int dtype, int channels, bool aligned) {
+    if (dtype == MG_F32)
+        return aligned && channels % 4 == 0 ? pick_team<float, 4>(op, channels)
+                                            : pick_team<float, 1>(op, channels);
+    if (dtype == MG_BF16)
+        return aligned && channels % 8 == 0 ? pick_team<__nv_bfloat16, 8>(op, channels)
+                                            : pick_team<__nv_bfloat16, 1>(op, channels);
+    return aligned && channels % 8 == 0 ? pick_team<__half, 8>(op, channels)
+                                        : pick_team<__half, 1>(op, channels);
+}
+
+bool known_dtype(int d) { return d == MG_F32 || d == MG_BF16 || d == MG_F16; }
+
+}  // namespace
+
+int sm_count() {
+    static int cached[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    if (cached[dev] == 0) {
+        int n = 0;
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1)
+            n = 148;
+        cached[dev] = n;
+    }
+    return cached[dev];
+}
+
+}  // namespace mg
+
+using namespace mg;
+
+extern "C" mg_status mg_layer_norm_forward(const void* x, int32_t dtype, const void* weight,
+                                           const void* bias, int32_t param_dtype, int64_t rows,
+                                           int64_t channels, float eps, void* y, float* mean,
+                                           float* rstd, int8_t* codes, float* scales,
+                                           mg_stream_t stream) {
+    MG_REQUIRE(known_dtype(dtype) && known_dtype(param_dtype), "layer_norm_forward: unknown dtype");
+    MG_REQUIRE(rows >= 0, "layer_norm_forward: negative row count");
+    MG_REQUIRE(channels >= 1 && channels <= MG_LAYER_NORM_MAX_CHANNELS,
+               "layer_norm_forward: channels must be 1..8192");
+    MG_REQUIRE(eps >= 0.0f, "layer_norm_forward: eps must not be negative");
+    MG_REQUIRE((mean == nullptr) == (rstd == nullptr) && (codes == nullptr) == (scales == nullptr),
+               "layer_norm_forward: mean comes with rstd, codes with scales");
+    if (rows == 0) return MG_OK;
+    MG_REQUIRE(x && y, "layer_norm_forward: null pointer");
+    MG_REQUIRE(codes == nullptr || (reinterpret_cast<uintptr_t>(codes) & 7u) == 0u,
+               "layer_norm_forward: codes must be 8-byte aligned");
+    const Forward op{x, weight, bias, param_dtype, rows, (int)channels, eps, y, mean, rstd,
+                     codes, scales, reinterpret_cast<cudaStream_t>(stream)};
+    return pick_type(op, dtype, (int)channels, aligned16(x) && aligned16(y));
+}
+
+extern "C" size_t mg_layer_norm_backward_scratch_bytes(int64_t rows, int64_t channels) {
+    if (rows <= 0 || channels <= 0 || channels > MG_LAYER_NORM_MAX_CHANNELS) return 0;
+    return sizeof(float) * 2 * (size_t)channels * (size_t)backward_blocks(rows, channels);
+}
+
+extern "C" mg_status mg_layer_norm_backward(const void* dy, const void* x, const int8_t* codes,
+                                            const float* scales, int32_t dtype, const void* weight,
+                                            int32_t param_dtype, const float* mean,
+                                            const float* rstd, int64_t rows, int64_t channels,
+                                            void* dx, void* dweight, void* dbias, void* scratch,
+                                            size_t scratch_bytes, mg_stream_t stream) {
+    MG_REQUIRE(known_dtype(dtype) && known_dtype(param_dtype), "layer_norm_backward: unknown dtype");
+    MG_REQUIRE(rows >= 0, "layer_norm_backward: negative row count");
+    MG_REQUIRE(channels >= 1 && channels <= MG_LAYER_NORM_MAX_CHANNELS,
+               "layer_norm_backward: channels must be 1..8192");
+    MG_REQUIRE((x == nullptr) != (codes == nullptr) || rows == 0,
+               "layer_norm_backward: give x or its 8-bit form");
+    MG_REQUIRE((codes == nullptr) == (scales == nullptr),
+               "layer_norm_backward: codes come with scales");
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    const bool params = dweight != nullptr || dbias != nullptr;
+    if (rows == 0) {
+        const size_t bytes = (size_t)channels * (param_dtype == MG_F32 ? 4 : 2);
+        if (dweight && cudaMemsetAsync(dweight, 0, bytes, st) != cudaSuccess)
+            return check_launch("layer_norm_backward memset");
+        if (dbias && cudaMemsetAsync(dbias, 0, bytes, st) != cudaSuccess)
+            return check_launch("layer_norm_backward memset");
+        return MG_OK;
+    }
+    if (!params && dx == nullptr) return MG_OK;
+    MG_REQUIRE(dy && mean && rstd, "layer_norm_backward: null pointer");
+    MG_REQUIRE(codes == nullptr || (reinterpret_cast<uintptr_t>(codes) & 7u) == 0u,
+               "layer_norm_backward: codes must be 8-byte aligned");
+    MG_REQUIRE(!params || (scratch != nullptr &&
+                           scratch_bytes >= mg_layer_norm_backward_scratch_bytes(rows, channels)),
+               "layer_norm_backward: scratch too small");
+    const int grid = (int)backward_blocks(rows, channels);
+    const Backward op{dy, x, codes, scales, weight, param_dtype, mean, rstd, rows, (int)channels,
+                      dx, params ? static_cast<float*>(scratch) : nullptr, grid, st};
+    MG_TRY(pick_type(op, dtype, (int)channels,
+                     aligned16(dy) && (x == nullptr || aligned16(x)) && (dx == nullptr || aligned16(dx))));
+    if (!params) return MG_OK;
+    norm_join_kernel<<<ceil_div(2 * channels, 32), dim3(32, 32), 0, st>>>(
+        static_cast<const float*>(scratch), grid, (int)channels, param_dtype, dweight, dbias);
+    return check_launch("layer_norm_backward join");
+}
