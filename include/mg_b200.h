@@ -807,7 +807,8 @@ mg_status mg_label_loss_backward(const void* features, const void* classes, int3
  * spins that gave up, checked-mode index faults). Synchronises `stream`.
  * *code_out receives 0 when nothing was recorded, else the first code:
  * 1 a sort look-back wait gave up, 2 a tile list reached past the sized pair
- * count, 3 a label outside the classes. The reference refuses instead of continuing silently
+ * count, 3 a label outside the classes, 4 a wait of a tensor-core tile gave
+ * up. The reference refuses instead of continuing silently
  * (metal_gauss/api.py:18-26); callers raise on a non-zero code. */
 mg_status mg_read_device_error(int32_t* code_out, mg_stream_t stream);
 

@@ -226,7 +226,8 @@ def make_camera(viewmat: torch.Tensor, fx: float, fy: float, cx: float, cy: floa
 
 DEVICE_ERRORS = {1: "a radix-sort look-back wait gave up (a predecessor tile never published)",
                  2: "a tile list reached past the sized pair count",
-                 3: "a label outside the classes"}
+                 3: "a label outside the classes",
+                 4: "a wait of a tensor-core tile gave up"}
 
 
 class DeviceError(RuntimeError):

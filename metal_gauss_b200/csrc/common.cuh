@@ -58,6 +58,7 @@ enum DeviceErrorCode : int32_t {
     DEV_ERR_SORT_LOOKBACK_TIMEOUT = 1,
     DEV_ERR_INDEX = 2,
     DEV_ERR_LABEL = 3,
+    DEV_ERR_TILE_WAIT = 4,
 };
 
 __device__ __forceinline__ void record_device_error(int32_t* word, int32_t code) {

@@ -6,126 +6,582 @@
 //   G[p, v] = r[p] (softmax(z[p])[v] - [v == label])
 //   dx = scale G w,  dw = scale G^T x,  db = column sums of G
 //
-// Forward: a block owns 64 rows and walks its share of the classes in tiles,
-// keeping per row the running maximum, the sum of exponentials of every class
-// but the label's, and the label's logit. The label's own share is kept apart
-// so that 1 - softmax(label) of a confident row is not a difference of two
-// numbers near 1. The backward kernels compute each tile of z again.
-// The classes (forward, dx) or the rows (dw) are split over blocks when there
-// are few of the others, and the shares joined in a fixed order.
+// All four products run on the tensor cores as bf16 tiles of 128 x up to 256
+// with fp32 sums. A feature or embedding becomes PARTS bf16 numbers that add up
+// to it: one for bf16 (exact), two for fp16 (exact: 11 bits), three for fp32
+// (24 bits); a product is the sum of the products of its parts, smallest first,
+// down to those of 2^-24 of it (fp32) or all (fp16). So fp32 features keep
+// fp32 logits, which a single tf32 or bf16 product would not.
+//
+//   split_kernel   x and w as parts; rows that are ignored become zeros, so
+//                  whatever they hold meets nothing
+//   kStats         a block takes 128 rows and walks its share of the classes,
+//                  keeping per row the running maximum and the sum of
+//                  exponentials of every class but the label's, and the
+//                  label's logit. The label's own share is kept apart so that
+//                  1 - softmax(label) of a confident row is not a difference
+//                  of two numbers near 1.
+//   kLogitGrad     the backward pass's logits again, turned into G, which goes
+//                  to scratch as PARTS bf16 numbers, a piece of rows at a time
+//   kProductRow    dx = G w of the piece
+//   kProductClass  dw += G^T x of the piece
+//
+// Products that sum over more than a few hundred entries leave the tensor
+// cores' accumulator for registers after every kSegment entries (fp32), since
+// its additions truncate. Classes or rows are split over blocks when there are
+// few of the others; shares are joined in a fixed order.
 #include "labels.cuh"
+#include "tensor.cuh"
 
 namespace mg {
 
 namespace {
 
-constexpr int kTile = 64;    // rows x classes of a score tile
-constexpr int kDepth = 16;   // channels per step
-constexpr int kThreads = 256;  // 16 x 16 threads, 4 x 4 scores each
 constexpr float kInf = __builtin_huge_valf();
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kM = 128;        // rows of a tile
+constexpr int kN = 256;        // columns of a tile, at most
+constexpr int kThreads = 320;  // a copying warp, an issuing warp, 8 warps that take tiles out
 
-// acc[i][j] += a[ty * 4 + i] . b[tx * 4 + j] over the channels; a and b are
-// 64 rows of row-major (n, channels) tensors, rows at or past n read as 0.
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// --------------------------------------------------------------------- parts
+
+// The number of bf16 parts of a type.
 template <typename T>
-__device__ __forceinline__ void score_tile(const T* __restrict__ a, int64_t a0, int64_t an,
-                                           const T* __restrict__ b, int64_t b0, int64_t bn,
-                                           int channels, float (*sa)[kTile + 4],
-                                           float (*sb)[kTile + 4], float acc[4][4]) {
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    for (int k0 = 0; k0 < channels; k0 += kDepth) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < kTile * kDepth; i += kThreads) {
-            const int r = i / kDepth, k = i % kDepth;
-            const bool in = k0 + k < channels;
-            sa[k][r] = in && a0 + r < an ? to_f32<T>(a[(a0 + r) * channels + k0 + k]) : 0.0f;
-            sb[k][r] = in && b0 + r < bn ? to_f32<T>(b[(b0 + r) * channels + k0 + k]) : 0.0f;
+constexpr int kPartsOf = sizeof(T) == 4 ? 3 : 2;
+template <>
+constexpr int kPartsOf<__nv_bfloat16> = 1;
+
+template <int PARTS>
+__device__ __forceinline__ void split_parts(float v, __nv_bfloat16 (&p)[PARTS]) {
+    p[0] = __float2bfloat16_rn(v);
+#pragma unroll
+    for (int i = 1; i < PARTS; ++i) {
+        v -= __bfloat162float(p[i - 1]);
+        p[i] = __float2bfloat16_rn(v);
+    }
+}
+
+// Features (live rows) and embeddings as (row, part, depth) bf16, depth the
+// channels rounded up to 8 with zeros. One thread: 8 channels of one row.
+template <typename T>
+__global__ void __launch_bounds__(256)
+split_kernel(const T* __restrict__ x, const T* __restrict__ w, LabelSource labels, int64_t rows,
+             int classes, int channels, int depth, __nv_bfloat16* __restrict__ xs,
+             __nv_bfloat16* __restrict__ ws) {
+    constexpr int PARTS = kPartsOf<T>;
+    const int groups = depth / 8;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t all = i / groups;
+    const int c = (int)(i - all * groups) * 8;
+    if (all >= rows + classes) return;
+    const bool feature = all < rows;
+    const int64_t row = feature ? all : all - rows;
+    const T* src = (feature ? x : w) + row * channels + c;
+    const bool live = !feature || labels.at(row) >= 0;
+    __nv_bfloat16 out[PARTS][8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const float v = live && c + k < channels ? to_f32<T>(src[k]) : 0.0f;
+        __nv_bfloat16 p[PARTS];
+        split_parts<PARTS>(v, p);
+        // an infinity is its first part alone: the rest would be inf - inf
+#pragma unroll
+        for (int j = 0; j < PARTS; ++j)
+            out[j][k] = j > 0 && fabsf(v) == kInf ? __float2bfloat16_rn(0.0f) : p[j];
+    }
+    __nv_bfloat16* dst = (feature ? xs : ws) + row * PARTS * depth + c;
+#pragma unroll
+    for (int j = 0; j < PARTS; ++j) {
+        uint4 r;
+        memcpy(&r, out[j], 16);
+        *reinterpret_cast<uint4*>(dst + j * depth) = r;
+    }
+}
+
+// ------------------------------------------------------------- the tile kernel
+
+enum Mode { kStats, kLogitGrad, kProductRow, kProductClass };
+
+template <int MODE, int PARTS>
+struct Shape {
+    static constexpr bool kProduct = MODE >= kProductRow;
+    static constexpr bool kAmn = MODE == kProductClass;  // A's row index runs fastest
+    static constexpr bool kBmn = kProduct;
+    static constexpr int kChunk = PARTS == 1 ? 64 : 32;  // contraction entries per stage
+    static constexpr int kA = kM * kChunk * 2;           // bytes of one part
+    static constexpr int kB = kN * kChunk * 2;
+    static constexpr int kStage = PARTS * (kA + kB);
+    static constexpr int kStages = PARTS == 3 ? (MODE == kLogitGrad ? 2 : 3) : (MODE == kLogitGrad ? 3 : 4);
+    // G on its way out: 128 x 32 bf16 for each half of the taking warps, part and buffer
+    static constexpr int kOutBuffers = PARTS == 3 ? 1 : 2;
+    static constexpr int kOut = MODE == kLogitGrad ? 2 * PARTS * kOutBuffers * kM * 64 : 0;
+    static constexpr int kDynamic = 1024 + kStages * kStage + kOut;
+    // Products of parts (a, b), smallest first.
+    static constexpr int kPairs = PARTS == 1 ? 1 : PARTS == 3 ? 6 : kProduct ? 3 : 4;
+};
+
+template <int PARTS>
+__device__ constexpr int pair_a(int pairs, int i) {
+    if (PARTS == 1) return 0;
+    if (PARTS == 2) return (i + 4 - pairs) == 0 || (i + 4 - pairs) == 1 ? 1 : 0;
+    return i == 0 ? 2 : i == 1 || i == 3 ? 1 : 0;
+}
+template <int PARTS>
+__device__ constexpr int pair_b(int pairs, int i) {
+    if (PARTS == 1) return 0;
+    if (PARTS == 2) return (i + 4 - pairs) == 0 || (i + 4 - pairs) == 2 ? 1 : 0;
+    return i == 2 ? 2 : i == 1 || i == 4 ? 1 : 0;
+}
+
+struct TileArgs {
+    int64_t units;
+    int64_t a_rows;         // rows of the A side (of the piece, or classes)
+    int64_t depth;          // contraction entries
+    int columns;            // columns of the B side in all (classes, or channels)
+    int splits;             // shares of the classes (kStats) or of the contraction
+    int64_t per_split;      // column tiles, or chunks, per share
+    int per_segment;        // chunks between visits to the registers
+    int64_t row0;           // the piece's first row
+    int64_t rows;           // rows in all
+    float scale;
+    const float* bias;
+    LabelSource labels;
+    RowGrad rg;
+    const float* stats;     // kLogitGrad: log2 of the sum, 1 - softmax(label)
+    float *part_m, *part_s, *label_z;  // kStats
+    float* part_bias;       // kLogitGrad: sums of 32 rows of G, or NULL
+    float* part;            // products: fp32 shares (splits, a_rows, part_ld), or NULL
+    int part_ld;
+    int add;                // to what the share holds
+    void* out;              // products: the result itself
+    int out_type;
+    int32_t* error_word;
+};
+
+// The tiles of a unit. Scores: a unit is a row tile and a share of the column
+// tiles (kStats) or one column tile (kLogitGrad). Products: a unit is a row
+// tile, a column tile and a share of the contraction, in segments.
+struct Walk {
+    int64_t a_row, c0, c1;
+    int b_row, split, tiles, first;
+};
+
+template <int MODE, int PARTS>
+__device__ __forceinline__ Walk walk_unit(const TileArgs& p, int64_t u) {
+    Walk w;
+    const int col_tiles = (p.columns + kN - 1) / kN;
+    if (MODE == kStats) {
+        w.a_row = u / p.splits * kM;
+        w.split = (int)(u % p.splits);
+        w.first = (int)(w.split * p.per_split);
+        w.tiles = (int)min((int64_t)col_tiles, w.first + p.per_split) - w.first;
+        w.c0 = 0;
+        w.c1 = (p.depth + Shape<MODE, PARTS>::kChunk - 1) / Shape<MODE, PARTS>::kChunk;
+    } else if (MODE == kLogitGrad) {
+        w.a_row = u / col_tiles * kM;
+        w.first = (int)(u % col_tiles);
+        w.tiles = 1;
+        w.split = 0;
+        w.c0 = 0;
+        w.c1 = (p.depth + Shape<MODE, PARTS>::kChunk - 1) / Shape<MODE, PARTS>::kChunk;
+    } else {
+        const int64_t chunks = (p.depth + Shape<MODE, PARTS>::kChunk - 1) / Shape<MODE, PARTS>::kChunk;
+        w.split = (int)(u % p.splits);
+        const int64_t t = u / p.splits;
+        w.first = (int)(t % col_tiles);
+        w.a_row = t / col_tiles * kM;
+        w.c0 = w.split * p.per_split;
+        w.c1 = min(chunks, w.c0 + p.per_split);
+        w.tiles = (int)((w.c1 - w.c0 + p.per_segment - 1) / p.per_segment);
+    }
+    return w;
+}
+
+template <int MODE, int PARTS>
+__global__ void __launch_bounds__(kThreads, 1)
+tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensorMap map_a,
+            const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_out) {
+    using S = Shape<MODE, PARTS>;
+    extern __shared__ uint8_t dynamic[];
+    __shared__ alignas(16) float bias_s[2][kN];
+    __shared__ uint64_t bars[2 * S::kStages + 5];
+    __shared__ uint32_t tmem_s;
+    __shared__ volatile int stop;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t base = (smem_u32(dynamic) + 1023u) & ~1023u;
+    const uint32_t full = smem_u32(bars), empty = full + 8 * S::kStages;
+    const uint32_t taken_full = empty + 8 * S::kStages, taken_empty = taken_full + 16;
+    const uint32_t drain = taken_empty + 16;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S::kStages; ++i) {
+            mbar_init(full + 8 * i, 1);
+            mbar_init(empty + 8 * i, 1);
         }
-        __syncthreads();
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(taken_full + 8 * i, 1);
+            mbar_init(taken_empty + 8 * i, 8);
+        }
+        mbar_init(drain, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async_shared();
+        stop = 0;
+    }
+    if (warp == 1) tmem_alloc(smem_u32(&tmem_s), 512);
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    const uint32_t tmem = tmem_s;
+
+    if (warp == 0) {
+        if (lane == 0) {  // copies tiles in
+            int stage = 0;
+            uint32_t phase = 0;
+            int64_t issued = 0;
+            bool ok = true;
+            for (int64_t u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
+                const Walk w = walk_unit<MODE, PARTS>(p, u);
+                for (int t = 0; ok && t < w.tiles; ++t) {
+                    const int b0 = (S::kProduct ? w.first : w.first + t) * kN;
+                    const int64_t c0 = S::kProduct ? w.c0 + (int64_t)t * p.per_segment : w.c0;
+                    const int64_t c1 = S::kProduct ? min(w.c1, c0 + p.per_segment) : w.c1;
+                    const int blocks = S::kProduct ? (min(kN, p.columns - b0) + 63) / 64 : 0;
+                    const uint32_t bytes =
+                        PARTS * (S::kA + (S::kProduct ? blocks * S::kChunk * 128 : S::kB));
+                    for (int64_t c = c0; c < c1; ++c) {
+                        ok = mbar_wait(empty + 8 * stage, phase ^ 1, &stop, p.error_word, DEV_ERR_TILE_WAIT);
+                        if (!ok) break;
+                        const uint32_t bar = full + 8 * stage;
+                        mbar_expect(bar, bytes);
+                        const int k = (int)(c * S::kChunk);
 #pragma unroll
-        for (int k = 0; k < kDepth; ++k) {
-            float x[4], y[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[i] = sa[k][ty * 4 + i];
-                y[i] = sb[k][tx * 4 + i];
+                        for (int i = 0; i < PARTS; ++i) {
+                            const uint32_t a = base + stage * S::kStage + i * S::kA;
+                            const uint32_t b = base + stage * S::kStage + PARTS * S::kA + i * S::kB;
+                            if (S::kAmn) {
+                                for (int q = 0; q < 2; ++q)
+                                    tma_load(a + q * S::kChunk * 128, &map_a, (int)w.a_row + 64 * q, k, i, bar);
+                            } else {
+                                tma_load(a, &map_a, k, (int)w.a_row, i, bar);
+                            }
+                            if (S::kBmn) {
+                                for (int q = 0; q < blocks; ++q)
+                                    tma_load(b + q * S::kChunk * 128, &map_b, b0 + 64 * q, k, i, bar);
+                            } else {
+                                tma_load(b, &map_b, k, b0, i, bar);
+                            }
+                        }
+                        ++issued;
+                        if (++stage == S::kStages) {
+                            stage = 0;
+                            phase ^= 1;
+                        }
+                    }
+                }
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(x[i], y[j], acc[i][j]);
-        }
-    }
-}
-
-// (m, s) of two shares of one row: maximum and sum of exp(z - m).
-__device__ __forceinline__ void join_stats(float& m, float& s, float m2, float s2) {
-    const float t = fmaxf(m, m2);
-    if (t == -kInf) return;  // neither share has a finite logit
-    s = s * expf(m - t) + s2 * expf(m2 - t);
-    m = t;
-}
-
-// NaN logits: m stays a number, s becomes NaN and the row's loss with it.
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
-label_stats_kernel(const T* __restrict__ x, const T* __restrict__ w,
-                   const float* __restrict__ bias, LabelSource labels, int64_t rows, int channels,
-                   int classes, float scale, int tiles_per_split, float* __restrict__ part_m,
-                   float* __restrict__ part_s, float* __restrict__ label_z) {
-    __shared__ float sa[kDepth][kTile + 4], sb[kDepth][kTile + 4];
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    const int64_t row0 = (int64_t)blockIdx.x * kTile;
-    int lab[4];
-    float m[4], s[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int64_t row = row0 + ty * 4 + i;
-        lab[i] = row < rows ? labels.at(row) : kIgnored;
-        m[i] = -kInf;
-        s[i] = 0.0f;
-    }
-    const int first = blockIdx.y * tiles_per_split;
-    const int last = min((classes + kTile - 1) / kTile, first + tiles_per_split);
-    for (int t = first; t < last; ++t) {
-        float acc[4][4] = {};
-        score_tile<T>(x, row0, rows, w, (int64_t)t * kTile, classes, channels, sa, sb, acc);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int v = t * kTile + tx * 4 + j;
-                if (v >= classes) continue;
-                const float z = fmaf(acc[i][j], scale, bias != nullptr ? bias[v] : 0.0f);
-                if (v == lab[i]) {
-                    label_z[row0 + ty * 4 + i] = z;
-                } else if (z > m[i]) {
-                    s[i] = fmaf(s[i], expf(m[i] - z), 1.0f);
-                    m[i] = z;
-                } else if (z > -kInf || z != z) {
-                    s[i] += expf(z - m[i]);
+            if (stop) {  // this block gave up: its copies in flight land before it ends
+                const int n = (int)min(issued, (int64_t)S::kStages);
+                for (int j = 0; j < n; ++j) {
+                    if (--stage < 0) {
+                        stage = S::kStages - 1;
+                        phase ^= 1;
+                    }
+                    for (int i = 0; i < kMbarRounds; ++i)
+                        if (mbar_try(full + 8 * stage, phase)) break;
                 }
             }
         }
+    } else if (warp == 1) {
+        if (lane == 0) {  // issues products
+            int stage = 0, buf = 0;
+            uint32_t phase = 0, buf_phase = 0;
+            bool ok = true;
+            for (int64_t u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
+                const Walk w = walk_unit<MODE, PARTS>(p, u);
+                for (int t = 0; ok && t < w.tiles; ++t) {
+                    const int b0 = (S::kProduct ? w.first : w.first + t) * kN;
+                    const int64_t c0 = S::kProduct ? w.c0 + (int64_t)t * p.per_segment : w.c0;
+                    const int64_t c1 = S::kProduct ? min(w.c1, c0 + p.per_segment) : w.c1;
+                    const int n = min(kN, (p.columns - b0 + 15) / 16 * 16);
+                    const uint32_t idesc = mma_idesc(n, S::kAmn, S::kBmn);
+                    ok = mbar_wait(taken_empty + 8 * buf, buf_phase ^ 1, &stop, p.error_word, DEV_ERR_TILE_WAIT);
+                    if (!ok) break;
+                    tmem_fence_after();
+                    const uint32_t d = tmem + buf * kN;
+                    bool add = false;
+                    for (int64_t c = c0; c < c1; ++c) {
+                        ok = mbar_wait(full + 8 * stage, phase, &stop, p.error_word, DEV_ERR_TILE_WAIT);
+                        if (!ok) break;
+                        tmem_fence_after();
+                        const int steps = (int)min((int64_t)(S::kChunk / 16), (p.depth - c * S::kChunk + 15) / 16);
+                        const uint32_t a0 = base + stage * S::kStage, b1 = a0 + PARTS * S::kA;
+#pragma unroll
+                        for (int i = 0; i < S::kPairs; ++i) {
+                            const uint32_t a = a0 + pair_a<PARTS>(S::kPairs, i) * S::kA;
+                            const uint32_t b = b1 + pair_b<PARTS>(S::kPairs, i) * S::kB;
+                            const uint64_t ad = S::kAmn ? desc_mn_major(a, S::kChunk * 128)
+                                                        : desc_k_major(a, S::kChunk * 2);
+                            const uint64_t bd = S::kBmn ? desc_mn_major(b, S::kChunk * 128)
+                                                        : desc_k_major(b, S::kChunk * 2);
+                            for (int s = 0; s < steps; ++s) {
+                                // 16 entries on: 32 bytes along a row, or 16 rows of 128 bytes
+                                mma_bf16(d, ad + s * (S::kAmn ? 128 : 2), bd + s * (S::kBmn ? 128 : 2), idesc, add);
+                                add = true;
+                            }
+                        }
+                        mma_commit(empty + 8 * stage);
+                        if (++stage == S::kStages) {
+                            stage = 0;
+                            phase ^= 1;
+                        }
+                    }
+                    if (!ok) break;
+                    mma_commit(taken_full + 8 * buf);
+                    buf ^= 1;
+                    if (buf == 0) buf_phase ^= 1;
+                }
+            }
+            if (stop) {
+                mma_commit(drain);
+                for (int i = 0; i < kMbarRounds; ++i)
+                    if (mbar_try(drain, 0)) break;
+            }
+        }
+    } else {
+        // Takes tiles out: warp % 4 is the quarter of the rows it can reach,
+        // `half` the 32-column chunks it takes (even or odd ones). After a wait
+        // that gave up the remaining waits fail at once and the block runs to
+        // its end on whatever is there; the error word says so.
+        const int quarter = warp & 3, half = (warp - 2) / 4, et = threadIdx.x - 64;
+        const int in_tile = quarter * 32 + lane;
+        const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+        const bool speaks = quarter == 0 && lane == 0;  // for its half's stores
+        const float c2 = p.scale * kLog2e;
+        int buf = 0, out_buf = 0;
+        uint32_t buf_phase = 0;
+        for (int64_t u = blockIdx.x; u < p.units; u += gridDim.x) {
+            const Walk w = walk_unit<MODE, PARTS>(p, u);
+            const int64_t a_row = w.a_row + in_tile;
+            const bool mine = a_row < p.a_rows;
+            if constexpr (!S::kProduct) {
+                const int64_t row = p.row0 + a_row;
+                const int lab = mine ? p.labels.at(row) : kIgnored;
+                float m = -kInf, s = 0.0f;
+                float lse = kInf, at_label = 0.0f, r = 0.0f;
+                if (MODE == kLogitGrad && lab >= 0) {
+                    r = p.rg.at(row, lab);
+                    lse = p.stats[row];
+                    at_label = -p.stats[p.rows + row] * r;
+                }
+                for (int t = 0; t < w.tiles; ++t) {
+                    const int v0 = (w.first + t) * kN;
+                    const int n = min(kN, p.columns - v0);
+                    // bias times log2 e; classes past the end are taken out
+                    bias_s[buf][et] = et < n ? (p.bias != nullptr ? p.bias[v0 + et] * kLog2e : 0.0f) : -kInf;
+                    named_sync(1, 256);
+                    mbar_wait(taken_full + 8 * buf, buf_phase, &stop, p.error_word, DEV_ERR_TILE_WAIT);
+                    tmem_fence_after();
+                    for (int k = half; k * 32 < n; k += 2) {
+                        float z[32];
+                        tmem_load32(lanes + buf * kN + k * 32, z);
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) {
+                            const float4 b = *reinterpret_cast<const float4*>(&bias_s[buf][k * 32 + j]);
+                            z[j] = fmaf(z[j], c2, b.x);
+                            z[j + 1] = fmaf(z[j + 1], c2, b.y);
+                            z[j + 2] = fmaf(z[j + 2], c2, b.z);
+                            z[j + 3] = fmaf(z[j + 3], c2, b.w);
+                        }
+                        const int rel = lab - v0 - k * 32;
+                        const bool here = (unsigned)rel < 32u;
+                        const bool any = __any_sync(0xffffffffu, here);
+                        if constexpr (MODE == kStats) {
+                            if (any) {
+                                float zl = 0.0f;
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) {
+                                    if (j == rel) {
+                                        zl = z[j];
+                                        z[j] = -kInf;
+                                    }
+                                }
+                                if (here) p.label_z[row] = zl;
+                            }
+                            float top = m;
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) top = fmaxf(top, z[j]);
+                            const float ref = top == -kInf ? 0.0f : top;
+                            float q[4] = {s * exp2_fast(m - ref), 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) q[j % 4] += exp2_fast(z[j] - ref);
+                            s = (q[0] + q[1]) + (q[2] + q[3]);
+                            m = top;
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) z[j] = exp2_fast(z[j] - lse) * r;
+                            if (any) {
+#pragma unroll
+                                for (int j = 0; j < 32; ++j)
+                                    if (j == rel) z[j] = at_label;
+                            }
+                            // staging is free again once the store before last has read it
+                            const uint32_t stage0 = base + S::kStages * S::kStage +
+                                                    (half * S::kOutBuffers + out_buf) * (PARTS * kM * 64);
+                            if (speaks) tma_store_wait_read<S::kOutBuffers - 1>();
+                            named_sync(2 + half, 128);
+                            const uint32_t line = stage0 + in_tile * 64;
+#pragma unroll
+                            for (int g = 0; g < 4; ++g) {
+                                const uint32_t at = line + ((g ^ ((in_tile >> 1) & 3)) * 16);
+                                __nv_bfloat16 o[PARTS][8];
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) {
+                                    __nv_bfloat16 q[PARTS];
+                                    split_parts<PARTS>(z[8 * g + j], q);
+#pragma unroll
+                                    for (int i = 0; i < PARTS; ++i) o[i][j] = q[i];
+                                }
+#pragma unroll
+                                for (int i = 0; i < PARTS; ++i) {
+                                    uint4 v;
+                                    memcpy(&v, o[i], 16);
+                                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + i * kM * 64),
+                                                 "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                                                 : "memory");
+                                }
+                            }
+                            fence_async_shared();
+                            named_sync(2 + half, 128);
+                            if (speaks) {
+#pragma unroll
+                                for (int i = 0; i < PARTS; ++i)
+                                    tma_store(&map_out, v0 + k * 32, (int)w.a_row, i, stage0 + i * kM * 64);
+                                tma_store_commit();
+                            }
+                            if (++out_buf == S::kOutBuffers) out_buf = 0;
+                            if (p.part_bias != nullptr) {
+                                // lane c ends with the sum of column c over the warp's 32 rows
+#pragma unroll
+                                for (int o = 16; o > 0; o >>= 1) {
+#pragma unroll
+                                    for (int j = 0; j < o; ++j) {
+                                        const bool up = (lane & o) != 0;
+                                        const float send = up ? z[j] : z[j + o];
+                                        const float keep = up ? z[j + o] : z[j];
+                                        z[j] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+                                    }
+                                }
+                                const int v = v0 + k * 32 + lane;
+                                const int64_t line32 = w.a_row / 32 + quarter;
+                                if (v < p.columns) p.part_bias[line32 * p.columns + v] = z[0];
+                            }
+                        }
+                    }
+                    tmem_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(taken_empty + 8 * buf);
+                    buf ^= 1;
+                    if (buf == 0) buf_phase ^= 1;
+                }
+                if (MODE == kStats && mine) {
+                    const int64_t at = (int64_t)(w.split * 2 + half) * p.rows + row;
+                    p.part_m[at] = m;
+                    p.part_s[at] = s;
+                }
+            } else {
+                const int d0 = w.first * kN;
+                const int n = min(kN, p.columns - d0);
+                float acc[4][32];
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) acc[q][j] = 0.0f;
+                for (int t = 0; t < w.tiles; ++t) {
+                    mbar_wait(taken_full + 8 * buf, buf_phase, &stop, p.error_word, DEV_ERR_TILE_WAIT);
+                    tmem_fence_after();
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        if ((2 * q + half) * 32 < n) {
+                            float v[32];
+                            tmem_load32(lanes + buf * kN + (2 * q + half) * 32, v);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) acc[q][j] += v[j];
+                        }
+                    }
+                    tmem_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(taken_empty + 8 * buf);
+                    buf ^= 1;
+                    if (buf == 0) buf_phase ^= 1;
+                }
+                if (mine) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int c = d0 + (2 * q + half) * 32;
+                        if (c >= p.columns) continue;
+                        if (p.part != nullptr) {
+                            float* dst = p.part + ((int64_t)w.split * p.a_rows + a_row) * p.part_ld + c;
+#pragma unroll
+                            for (int j = 0; j < 32; j += 4) {
+                                if (c + j >= p.part_ld) continue;
+                                float4* d4 = reinterpret_cast<float4*>(dst + j);
+                                float4 o = make_float4(acc[q][j], acc[q][j + 1], acc[q][j + 2], acc[q][j + 3]);
+                                if (p.add) {
+                                    const float4 e = *d4;
+                                    o.x += e.x;
+                                    o.y += e.y;
+                                    o.z += e.z;
+                                    o.w += e.w;
+                                }
+                                *d4 = o;
+                            }
+                        } else {
+                            const int64_t at = (p.row0 + a_row) * p.columns + c;
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) {
+                                if (c + j >= p.columns) continue;
+                                const float v = acc[q][j] * p.scale;
+                                if (p.out_type == MG_F32) static_cast<float*>(p.out)[at + j] = v;
+                                else if (p.out_type == MG_BF16) static_cast<__nv_bfloat16*>(p.out)[at + j] = from_f32<__nv_bfloat16>(v);
+                                else static_cast<__half*>(p.out)[at + j] = from_f32<__half>(v);
+                            }
+                        }
+                    }
+                }
+            }
+        }
+        if (MODE == kLogitGrad && speaks) tma_store_wait_all();
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) {
-            const float m2 = __shfl_xor_sync(0xffffffffu, m[i], o);
-            const float s2 = __shfl_xor_sync(0xffffffffu, s[i], o);
-            join_stats(m[i], s[i], m2, s2);
-            if (m[i] == -kInf) s[i] += s2;  // carries a NaN
-        }
-        const int64_t row = row0 + ty * 4 + i;
-        if (tx == 0 && row < rows) {
-            part_m[(int64_t)blockIdx.y * rows + row] = m[i];
-            part_s[(int64_t)blockIdx.y * rows + row] = s[i];
-        }
+    tmem_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tmem_fence_after();
+        tmem_free(tmem, 512);
     }
 }
 
+// ------------------------------------------------------------- rows and joins
+
+// (m, s) of two shares of one row: maximum and sum of exp2(z - m).
+__device__ __forceinline__ void join_stats(float& m, float& s, float m2, float s2) {
+    const float t = fmaxf(m, m2);
+    if (t == -kInf) {  // neither share has a finite logit; a NaN stays
+        s += s2;
+        return;
+    }
+    s = s * exp2f(m - t) + s2 * exp2f(m2 - t);
+    m = t;
+}
+
 // Per row: the shares' join, the loss, and what the backward pass needs
-// (stats: lse, then 1 - softmax(label)); per block the sum of the losses and
+// (stats: log2 of the sum, then 1 - softmax(label)); per block the sum of the losses and
 // the count of live rows.
 __global__ void __launch_bounds__(256)
 label_rows_kernel(const float* __restrict__ part_m, const float* __restrict__ part_s,
@@ -145,20 +601,19 @@ label_rows_kernel(const float* __restrict__ part_m, const float* __restrict__ pa
                 const float m2 = part_m[(int64_t)k * rows + row];
                 const float s2 = part_s[(int64_t)k * rows + row];
                 join_stats(m, s, m2, s2);
-                if (m == -kInf) s += s2;
             }
             const float z = label_z[row];
-            // others = sum over the other classes of exp(z_v - top)
+            // all in base 2; others = sum over the other classes of exp2(z_v - top)
             const float top = fmaxf(m, z);
             if (top == -kInf || z != z || s != s) {
                 lse = loss = miss = __int_as_float(0x7fc00000);
             } else {
-                const float others = m == -kInf ? 0.0f : s * expf(m - top);
-                const float own = expf(z - top);
+                const float others = m == -kInf ? 0.0f : s * exp2f(m - top);
+                const float own = exp2f(z - top);
                 const float total = others + own;
-                lse = top + logf(total);
+                lse = top + log2f(total);
                 miss = others / total;
-                loss = z == top ? log1pf(others) : (top - z) + logf(total);
+                loss = z == top ? log1pf(others) : (top - z) * kLn2 + logf(total);
             }
         } else if (lab == kBadLabel) {
             live = 1;
@@ -210,131 +665,137 @@ label_total_kernel(const double* __restrict__ block_sum, int blocks, int mean,
     }
 }
 
-// One side's gradient for 64 of its items (BY_CLASS: classes, else rows) and
-// 64 of its channels, over a share of the other side's items:
-//   out[i, c] = scale sum_j G[i, j] other[j, c].
-// A row that is ignored counts as zeros on both sides, whatever its features.
-template <typename T, bool BY_CLASS>
-__global__ void __launch_bounds__(kThreads)
-label_grad_kernel(const T* __restrict__ x, const T* __restrict__ w,
-                  const float* __restrict__ bias, LabelSource labels, RowGrad rg,
-                  const float* __restrict__ stats, int64_t rows, int channels, int classes,
-                  float scale, int64_t tiles_per_split, float* __restrict__ part,
-                  float* __restrict__ part_bias) {
-    __shared__ float sa[kDepth][kTile + 4], sb[kDepth][kTile + 4];
-    __shared__ float g[kTile][kTile + 1], other[kTile][kTile + 1];
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    const int64_t mine_n = BY_CLASS ? classes : rows, other_n = BY_CLASS ? rows : classes;
-    const int64_t i0 = (int64_t)blockIdx.x * kTile;
-    const int c0 = blockIdx.y * kTile;
-    const int64_t first = blockIdx.z * tiles_per_split;
-    const int64_t last = min((other_n + kTile - 1) / kTile, first + tiles_per_split);
-    float out[4][4] = {};
-    float bsum = 0.0f;
-    for (int64_t t = first; t < last; ++t) {
-        const int64_t j0 = t * kTile;
-        float acc[4][4] = {};
-        if constexpr (BY_CLASS) score_tile<T>(w, i0, classes, x, j0, rows, channels, sa, sb, acc);
-        else score_tile<T>(x, i0, rows, w, j0, classes, channels, sa, sb, acc);
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int64_t mi = i0 + ty * 4 + i, oj = j0 + tx * 4 + j;
-                const int64_t p = BY_CLASS ? oj : mi, v = BY_CLASS ? mi : oj;
-                float e = 0.0f;
-                if (p < rows && v < classes) {
-                    const int lab = labels.at(p);
-                    if (lab >= 0) {
-                        const float z = fmaf(acc[i][j], scale, bias != nullptr ? bias[v] : 0.0f);
-                        e = (v == lab ? -stats[rows + p] : expf(z - stats[p])) * rg.at(p, lab);
-                    }
-                }
-                g[ty * 4 + i][tx * 4 + j] = e;
-            }
-        }
-        for (int i = threadIdx.x; i < kTile * kTile; i += kThreads) {
-            const int r = i / kTile, c = i % kTile;
-            const int64_t j = j0 + r;
-            float v = 0.0f;
-            if (j < other_n && c0 + c < channels && (!BY_CLASS || labels.at(j) >= 0))
-                v = to_f32<T>((BY_CLASS ? x : w)[j * channels + c0 + c]);
-            other[r][c] = v;
-        }
-        __syncthreads();
-        for (int r = 0; r < kTile; ++r) {
-            float a[4], b[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                a[i] = g[ty * 4 + i][r];
-                b[i] = other[r][tx * 4 + i];
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) out[i][j] = fmaf(a[i], b[j], out[i][j]);
-        }
-        if (part_bias != nullptr && blockIdx.y == 0 && threadIdx.x < kTile) {
-            for (int r = 0; r < kTile; ++r) bsum += g[threadIdx.x][r];
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t mi = i0 + ty * 4 + i;
-            const int c = c0 + tx * 4 + j;
-            if (mi < mine_n && c < channels)
-                part[((int64_t)blockIdx.z * mine_n + mi) * channels + c] = out[i][j] * scale;
-        }
-    }
-    if (part_bias != nullptr && blockIdx.y == 0 && threadIdx.x < kTile && i0 + threadIdx.x < mine_n)
-        part_bias[(int64_t)blockIdx.z * mine_n + i0 + threadIdx.x] = bsum;
-}
-
+// out = scale times the sum of the shares (splits, n, ld), columns of each row.
 template <typename T>
 __global__ void __launch_bounds__(256)
-label_join_kernel(const float* __restrict__ part, int splits, int64_t n, T* __restrict__ out) {
+join_kernel(const float* __restrict__ part, int splits, int64_t n, int ld, int columns, float scale,
+            T* __restrict__ out) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
+    if (i >= n * columns) return;
+    const int64_t row = i / columns;
+    const int c = (int)(i - row * columns);
     float s = 0.0f;
-    for (int k = 0; k < splits; ++k) s += part[(int64_t)k * n + i];
-    out[i] = from_f32<T>(s);
+    for (int k = 0; k < splits; ++k) s += part[((int64_t)k * n + row) * ld + c];
+    out[i] = from_f32<T>(s * scale);
 }
+
+// Column sums of (lines, columns): block (x, y) takes 32 columns and the y-th
+// share of the lines.
+__global__ void __launch_bounds__(1024)
+column_sum_kernel(const float* __restrict__ in, int64_t lines, int64_t per_block, int columns,
+                  float* __restrict__ out) {
+    __shared__ float sh[32][33];
+    const int col = blockIdx.x * 32 + threadIdx.x;
+    const int64_t end = min(lines, (int64_t)(blockIdx.y + 1) * per_block);
+    float s = 0.0f;
+    if (col < columns) {
+#pragma unroll 4
+        for (int64_t r = (int64_t)blockIdx.y * per_block + threadIdx.y; r < end; r += 32) s += in[r * columns + col];
+    }
+    sh[threadIdx.y][threadIdx.x] = s;
+    __syncthreads();
+    s = lanes_sum<32>(sh[threadIdx.x][threadIdx.y]);
+    const int c = blockIdx.x * 32 + threadIdx.y;
+    if (threadIdx.x == 0 && c < columns) out[(int64_t)blockIdx.y * columns + c] = s;
+}
+
+// ------------------------------------------------------------------- the host
 
 struct Shares {
     int splits;
     int64_t per_split;
 };
 
-// Splits `tiles` over blocks when `blocks` others alone would not fill the device.
-Shares split(int64_t tiles, int64_t blocks) {
-    const int64_t want = std::max<int64_t>(1, 2 * (int64_t)sm_count() / std::max<int64_t>(1, blocks));
+// Splits `tiles` over blocks when `others` blocks alone would not fill the
+// device (one block to an SM).
+Shares split(int64_t tiles, int64_t others) {
+    const int64_t want = std::max<int64_t>(1, sm_count() / std::max<int64_t>(1, others));
     const int64_t per = (tiles + std::min(tiles, want) - 1) / std::min(tiles, want);
     return {(int)((tiles + per - 1) / per), per};
 }
 
+inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// G of a piece of rows is kept to about this much scratch.
+constexpr int64_t kPieceBytes = (int64_t)256 << 20;
+constexpr int64_t kPieceRows = 1024;  // and to at least this many rows
+constexpr int64_t kBiasLines = 1024;
+
 struct Sizes {
     int64_t rows;
-    int channels, classes;
+    int channels, classes, parts;
 
-    int64_t row_tiles() const { return (rows + kTile - 1) / kTile; }
-    int64_t class_tiles() const { return (classes + kTile - 1) / kTile; }
-    int64_t depth_tiles() const { return (channels + kTile - 1) / kTile; }
-    Shares stats() const { return split(class_tiles(), row_tiles()); }
-    Shares by_row() const { return split(class_tiles(), row_tiles() * depth_tiles()); }
-    Shares by_class() const { return split(row_tiles(), class_tiles() * depth_tiles()); }
-    int64_t row_blocks() const { return (rows + 255) / 256; }
-
-    size_t forward_bytes() const {
-        return 16 * (size_t)row_blocks() +
-               sizeof(float) * (size_t)rows * (2 * (size_t)stats().splits + 1);
+    int chunk() const { return parts == 1 ? 64 : 32; }
+    // fp32: 256 entries between visits to the registers; the others round their
+    // result to 11 bits or fewer and go 4096
+    int segment() const { return (parts == 3 ? 256 : 4096) / chunk(); }
+    int depth() const { return (int)up(channels, 8) * 8; }
+    int part_ld() const { return (int)up(channels, 4) * 4; }
+    int64_t row_tiles() const { return up(rows, kM); }
+    int64_t class_columns() const { return up(classes, kN); }
+    int64_t channel_columns() const { return up(channels, kN); }
+    int64_t g_ld() const { return up(classes, 64) * 64; }
+    int64_t piece() const {
+        const int64_t fit = kPieceBytes / (2 * parts * g_ld()) / kM * kM;
+        return std::min(up(rows, kM) * kM, std::max(kPieceRows, fit));
     }
-    size_t backward_bytes() const {
-        const size_t a = (size_t)by_row().splits * rows * channels;
-        const size_t b = (size_t)by_class().splits * classes * (channels + 1);
-        return sizeof(float) * std::max(a, b);
+    Shares stats() const { return split(class_columns(), row_tiles()); }
+    Shares by_row() const {
+        return split(up(classes, chunk()), up(piece(), kM) * channel_columns());
+    }
+    Shares by_class() const {
+        return split(up(piece(), chunk()), up(classes, kM) * channel_columns());
+    }
+    int64_t row_blocks() const { return up(rows, 256); }
+    // the bias's gradient: sums of 32 rows, then of up to kBiasLines of those
+    int64_t pieces() const { return up(rows, piece()); }
+    int64_t bias_lines() const { return piece() / 32; }
+    int64_t bias_shares() const { return up(bias_lines(), kBiasLines); }
+};
+
+struct Scratch {
+    char* p;
+    template <typename T>
+    T* take(size_t n) {
+        T* r = reinterpret_cast<T*>(p);
+        p += align256(n * sizeof(T));
+        return r;
+    }
+};
+
+struct ForwardScratch {
+    __nv_bfloat16 *xs, *ws;
+    float *m, *s, *z;
+    double* sums;
+    size_t bytes;
+    ForwardScratch(void* base, const Sizes& n) {
+        Scratch a{static_cast<char*>(base)};
+        xs = a.take<__nv_bfloat16>((size_t)n.rows * n.parts * n.depth());
+        ws = a.take<__nv_bfloat16>((size_t)n.classes * n.parts * n.depth());
+        m = a.take<float>((size_t)n.stats().splits * 2 * n.rows);
+        s = a.take<float>((size_t)n.stats().splits * 2 * n.rows);
+        z = a.take<float>((size_t)n.rows);
+        sums = a.take<double>(2 * (size_t)n.row_blocks());
+        bytes = (size_t)(a.p - static_cast<char*>(base));
+    }
+};
+
+struct BackwardScratch {
+    __nv_bfloat16 *xs, *ws, *g;
+    float *row_part, *class_part, *bias_part, *bias_part2;
+    size_t bytes;
+    BackwardScratch(void* base, const Sizes& n) {
+        Scratch a{static_cast<char*>(base)};
+        xs = a.take<__nv_bfloat16>((size_t)n.rows * n.parts * n.depth());
+        ws = a.take<__nv_bfloat16>((size_t)n.classes * n.parts * n.depth());
+        g = a.take<__nv_bfloat16>((size_t)n.piece() * n.parts * n.g_ld());
+        const int rs = n.by_row().splits;
+        row_part = a.take<float>(rs > 1 ? (size_t)rs * n.piece() * n.part_ld() : 0);
+        class_part = a.take<float>((size_t)n.by_class().splits * n.classes * n.part_ld());
+        bias_part = a.take<float>((size_t)n.bias_lines() * n.classes);
+        bias_part2 = a.take<float>((size_t)(n.pieces() * n.bias_shares()) * n.classes);
+        bytes = (size_t)(a.p - static_cast<char*>(base));
     }
 };
 
@@ -348,49 +809,183 @@ struct Args {
     cudaStream_t st;
 };
 
+template <int MODE, int PARTS>
+mg_status launch_tiles(const TileArgs& p, const CUtensorMap& a, const CUtensorMap& b,
+                       const CUtensorMap& out, cudaStream_t st, const char* what) {
+    constexpr int bytes = Shape<MODE, PARTS>::kDynamic;
+    static bool ready[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+    if (!ready[dev]) {
+        if (cudaFuncSetAttribute(tile_kernel<MODE, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 bytes) != cudaSuccess)
+            return check_launch(what);
+        ready[dev] = true;
+    }
+    const int grid = (int)std::min<int64_t>(p.units, sm_count());
+    tile_kernel<MODE, PARTS><<<grid, kThreads, bytes, st>>>(p, a, b, out);
+    return check_launch(what);
+}
+
+template <typename T>
+mg_status split_inputs(const Args& a, __nv_bfloat16* xs, __nv_bfloat16* ws) {
+    const int64_t threads = (a.n.rows + a.n.classes) * (a.n.depth() / 8);
+    split_kernel<T><<<(unsigned)up(threads, 256), 256, 0, a.st>>>(
+        static_cast<const T*>(a.x), static_cast<const T*>(a.w), a.labels, a.n.rows, a.n.classes,
+        a.n.channels, a.n.depth(), xs, ws);
+    return check_launch("label_loss split");
+}
+
+// Maps of the parts of features or embeddings: contraction along the channels
+// (box_rows rows of a tile) or along the rows (box_rows 0).
+mg_status parts_map(CUtensorMap* m, const __nv_bfloat16* base, const Sizes& n, int64_t rows,
+                    int box_rows) {
+    const int64_t part = 2 * (int64_t)n.depth(), row = n.parts * part;
+    if (box_rows > 0)
+        return make_tensor_map(m, base, n.depth(), rows, n.parts, row, part, n.chunk(), box_rows,
+                               n.chunk() == 64, "label_loss parts");
+    return make_tensor_map(m, base, n.depth(), rows, n.parts, row, part, 64, n.chunk(), true,
+                           "label_loss parts");
+}
+
 template <typename T>
 mg_status forward(const Args& a, int reduction, float* loss, float* stats, float* live,
                   void* scratch) {
+    constexpr int PARTS = kPartsOf<T>;
+    const ForwardScratch f(scratch, a.n);
+    MG_TRY((split_inputs<T>(a, f.xs, f.ws)));
+    CUtensorMap mx, mw;
+    MG_TRY(parts_map(&mx, f.xs, a.n, a.n.rows, kM));
+    MG_TRY(parts_map(&mw, f.ws, a.n, a.n.classes, kN));
     const Shares sh = a.n.stats();
-    double* sums = static_cast<double*>(scratch);
-    float* m = reinterpret_cast<float*>(sums + 2 * a.n.row_blocks());
-    float* s = m + sh.splits * a.n.rows;
-    float* z = s + sh.splits * a.n.rows;
-    label_stats_kernel<T><<<dim3((unsigned)a.n.row_tiles(), sh.splits), kThreads, 0, a.st>>>(
-        static_cast<const T*>(a.x), static_cast<const T*>(a.w), a.bias, a.labels, a.n.rows,
-        a.n.channels, a.n.classes, a.scale, (int)sh.per_split, m, s, z);
-    MG_TRY(check_launch("label_loss_forward"));
+    TileArgs p{};
+    p.units = a.n.row_tiles() * sh.splits;
+    p.a_rows = p.rows = a.n.rows;
+    p.depth = a.n.depth();
+    p.columns = a.n.classes;
+    p.splits = sh.splits;
+    p.per_split = sh.per_split;
+    p.scale = a.scale;
+    p.bias = a.bias;
+    p.labels = a.labels;
+    p.part_m = f.m;
+    p.part_s = f.s;
+    p.label_z = f.z;
+    p.error_word = device_error_word();
+    MG_TRY((launch_tiles<kStats, PARTS>(p, mx, mw, mw, a.st, "label_loss_forward")));
     label_rows_kernel<<<(unsigned)a.n.row_blocks(), 256, 0, a.st>>>(
-        m, s, z, a.labels, sh.splits, a.n.rows, stats, reduction == MG_REDUCE_NONE ? loss : nullptr,
-        reduction == MG_REDUCE_NONE ? nullptr : sums, device_error_word());
+        f.m, f.s, f.z, a.labels, sh.splits * 2, a.n.rows, stats,
+        reduction == MG_REDUCE_NONE ? loss : nullptr, reduction == MG_REDUCE_NONE ? nullptr : f.sums,
+        p.error_word);
     MG_TRY(check_launch("label_loss_forward rows"));
     if (reduction == MG_REDUCE_NONE) return MG_OK;
-    label_total_kernel<<<1, 1024, 0, a.st>>>(sums, (int)a.n.row_blocks(),
+    label_total_kernel<<<1, 1024, 0, a.st>>>(f.sums, (int)a.n.row_blocks(),
                                              reduction == MG_REDUCE_MEAN, loss, live);
     return check_launch("label_loss_forward total");
 }
 
-template <typename T, bool BY_CLASS>
-mg_status grad(const Args& a, const RowGrad& rg, const float* stats, void* out, float* out_bias,
-               float* scratch) {
-    const Shares sh = BY_CLASS ? a.n.by_class() : a.n.by_row();
-    const int64_t n = BY_CLASS ? a.n.classes : a.n.rows;
-    float* part_bias = out_bias != nullptr ? scratch + (int64_t)sh.splits * n * a.n.channels : nullptr;
-    const dim3 grid((unsigned)((n + kTile - 1) / kTile), (unsigned)a.n.depth_tiles(), sh.splits);
-    label_grad_kernel<T, BY_CLASS><<<grid, kThreads, 0, a.st>>>(
-        static_cast<const T*>(a.x), static_cast<const T*>(a.w), a.bias, a.labels, rg, stats,
-        a.n.rows, a.n.channels, a.n.classes, a.scale, sh.per_split, scratch, part_bias);
-    MG_TRY(check_launch("label_loss_backward"));
-    if (out != nullptr) {
-        const int64_t e = n * a.n.channels;
-        label_join_kernel<T><<<ceil_div(e, 256), 256, 0, a.st>>>(scratch, sh.splits, e,
-                                                                 static_cast<T*>(out));
-        MG_TRY(check_launch("label_loss_backward join"));
-    }
-    if (out_bias == nullptr) return MG_OK;
-    label_join_kernel<float><<<ceil_div(n, 256), 256, 0, a.st>>>(part_bias, sh.splits, n, out_bias);
+template <typename T>
+mg_status join(const float* part, int splits, int64_t n, int ld, int columns, float scale, T* out,
+               cudaStream_t st) {
+    join_kernel<T><<<(unsigned)up(n * columns, 256), 256, 0, st>>>(part, splits, n, ld, columns, scale, out);
+    return check_launch("label_loss_backward join");
+}
+
+// Sums of shares of per_block lines each.
+mg_status column_sum(const float* in, int64_t lines, int64_t per_block, int columns, float* out,
+                     cudaStream_t st) {
+    const dim3 grid((unsigned)up(columns, 32), (unsigned)up(lines, per_block));
+    column_sum_kernel<<<grid, dim3(32, 32), 0, st>>>(in, lines, per_block, columns, out);
     return check_launch("label_loss_backward bias");
 }
+
+template <typename T>
+mg_status backward(const Args& a, const RowGrad& rg, const float* stats, T* dx, T* dw, float* db,
+                   void* scratch) {
+    constexpr int PARTS = kPartsOf<T>;
+    const Sizes& n = a.n;
+    const BackwardScratch f(scratch, n);
+    MG_TRY((split_inputs<T>(a, f.xs, f.ws)));
+    CUtensorMap mw_score, mw_prod;
+    MG_TRY(parts_map(&mw_score, f.ws, n, n.classes, kN));
+    MG_TRY(parts_map(&mw_prod, f.ws, n, n.classes, 0));
+    const int64_t g_part = n.piece() * n.g_ld() * 2;
+    for (int64_t row0 = 0; row0 < n.rows; row0 += n.piece()) {
+        const int64_t rows = std::min(n.piece(), n.rows - row0);
+        const __nv_bfloat16* xs = f.xs + row0 * PARTS * n.depth();
+        CUtensorMap mx, mg_out;
+        MG_TRY(parts_map(&mx, xs, n, rows, kM));
+        MG_TRY(make_tensor_map(&mg_out, f.g, n.classes, rows, PARTS, n.g_ld() * 2, g_part, 32, kM,
+                               false, "label_loss G"));
+        TileArgs p{};
+        p.units = up(rows, kM) * n.class_columns();
+        p.a_rows = rows;
+        p.rows = n.rows;
+        p.row0 = row0;
+        p.depth = n.depth();
+        p.columns = n.classes;
+        p.splits = 1;
+        p.scale = a.scale;
+        p.bias = a.bias;
+        p.labels = a.labels;
+        p.rg = rg;
+        p.stats = stats;
+        p.part_bias = db != nullptr ? f.bias_part : nullptr;
+        p.error_word = device_error_word();
+        MG_TRY((launch_tiles<kLogitGrad, PARTS>(p, mx, mw_score, mg_out, a.st, "label_loss_backward logits")));
+        if (db != nullptr) {
+            float* sums = f.bias_part2 + row0 / n.piece() * n.bias_shares() * n.classes;
+            MG_TRY(column_sum(f.bias_part, up(rows, kM) * 4, kBiasLines, n.classes,
+                              n.pieces() * n.bias_shares() > 1 ? sums : db, a.st));
+        }
+        p.part_bias = nullptr;
+        p.per_segment = n.segment();
+        p.columns = n.channels;
+        if (dx != nullptr) {
+            CUtensorMap mg_in;
+            MG_TRY(make_tensor_map(&mg_in, f.g, n.classes, rows, PARTS, n.g_ld() * 2, g_part, n.chunk(),
+                                   kM, n.chunk() == 64, "label_loss G"));
+            const Shares sh = n.by_row();
+            p.units = up(rows, kM) * n.channel_columns() * sh.splits;
+            p.depth = n.classes;
+            p.splits = sh.splits;
+            p.per_split = sh.per_split;
+            p.part = sh.splits > 1 ? f.row_part : nullptr;
+            p.part_ld = n.part_ld();
+            p.out = dx;
+            p.out_type = a.dtype;
+            MG_TRY((launch_tiles<kProductRow, PARTS>(p, mg_in, mw_prod, mw_prod, a.st, "label_loss_backward rows")));
+            if (sh.splits > 1)
+                MG_TRY(join(f.row_part, sh.splits, rows, n.part_ld(), n.channels, a.scale,
+                            dx + row0 * n.channels, a.st));
+        }
+        if (dw != nullptr) {
+            CUtensorMap mg_in, mx_prod;
+            MG_TRY(make_tensor_map(&mg_in, f.g, n.classes, rows, PARTS, n.g_ld() * 2, g_part, 64,
+                                   n.chunk(), true, "label_loss G"));
+            MG_TRY(parts_map(&mx_prod, xs, n, rows, 0));
+            const Shares sh = n.by_class();
+            p.units = up(n.classes, kM) * n.channel_columns() * sh.splits;
+            p.a_rows = n.classes;
+            p.depth = rows;
+            p.splits = sh.splits;
+            p.per_split = sh.per_split;
+            p.part = f.class_part;
+            p.part_ld = n.part_ld();
+            p.add = row0 > 0;
+            MG_TRY((launch_tiles<kProductClass, PARTS>(p, mg_in, mx_prod, mx_prod, a.st, "label_loss_backward classes")));
+        }
+    }
+    if (dw != nullptr)
+        MG_TRY(join(f.class_part, n.by_class().splits, n.classes, n.part_ld(), n.channels, a.scale, dw, a.st));
+    if (db != nullptr && n.pieces() * n.bias_shares() > 1) {
+        const int64_t shares = n.pieces() * n.bias_shares();
+        MG_TRY(column_sum(f.bias_part2, shares, shares, n.classes, db, a.st));
+    }
+    return MG_OK;
+}
+
+int parts_of_dtype(int32_t dtype) { return dtype == MG_F32 ? 3 : dtype == MG_F16 ? 2 : 1; }
 
 mg_status check_args(const char* who, const void* x, const void* w, int32_t dtype,
                      const void* labels, int32_t label_bytes, int64_t rows, int64_t channels,
@@ -411,18 +1006,44 @@ mg_status check_args(const char* who, const void* x, const void* w, int32_t dtyp
 
 }  // namespace
 
+mg_status make_tensor_map(CUtensorMap* map, const void* base, int64_t columns, int64_t rows,
+                          int64_t parts, int64_t row_bytes, int64_t part_bytes, int box_columns,
+                          int box_rows, bool swizzle128, const char* what) {
+    using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static Encode encode = [] {
+        void* f = nullptr;
+        return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault) == cudaSuccess
+                   ? reinterpret_cast<Encode>(f)
+                   : nullptr;
+    }();
+    if (encode == nullptr) return fail(MG_ERR_CUDA, std::string(what) + ": the driver has no tensor maps");
+    const cuuint64_t dims[3] = {(cuuint64_t)columns, (cuuint64_t)rows, (cuuint64_t)parts};
+    const cuuint64_t strides[2] = {(cuuint64_t)row_bytes, (cuuint64_t)part_bytes};
+    const cuuint32_t box[3] = {(cuuint32_t)box_columns, (cuuint32_t)box_rows, 1};
+    const cuuint32_t step[3] = {1, 1, 1};
+    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims,
+                              strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail(MG_ERR_CUDA, std::string(what) + ": cuTensorMapEncodeTiled returned " + std::to_string((int)r));
+    return MG_OK;
+}
+
 }  // namespace mg
 
 using namespace mg;
 
 extern "C" size_t mg_label_loss_scratch_bytes(int64_t rows, int64_t channels, int64_t classes,
                                               int32_t dtype, int32_t backward) {
-    (void)dtype;
     if (rows <= 0 || rows > MG_LABEL_MAX_ROWS || channels < 1 || channels > MG_LABEL_MAX_CHANNELS ||
         classes < 1 || classes > MG_LABEL_MAX_CLASSES)
         return 0;
-    const Sizes n{rows, (int)channels, (int)classes};
-    return backward ? n.backward_bytes() : n.forward_bytes();
+    const Sizes n{rows, (int)channels, (int)classes, parts_of_dtype(dtype)};
+    return backward ? BackwardScratch(nullptr, n).bytes : ForwardScratch(nullptr, n).bytes;
 }
 
 extern "C" mg_status mg_label_loss_forward(const void* features, const void* classes, int32_t dtype,
@@ -450,7 +1071,7 @@ extern "C" mg_status mg_label_loss_forward(const void* features, const void* cla
                "label_loss_forward: scratch too small or not 256-byte aligned");
     const Args a{features, classes, dtype, class_bias,
                  LabelSource{labels, label_bytes, ignore_index, (int)n_classes},
-                 Sizes{rows, (int)channels, (int)n_classes}, scale, st};
+                 Sizes{rows, (int)channels, (int)n_classes, parts_of_dtype(dtype)}, scale, st};
     if (dtype == MG_F32) return forward<float>(a, reduction, loss, stats, live, scratch);
     if (dtype == MG_BF16) return forward<__nv_bfloat16>(a, reduction, loss, stats, live, scratch);
     return forward<__half>(a, reduction, loss, stats, live, scratch);
@@ -472,6 +1093,7 @@ extern "C" mg_status mg_label_loss_backward(
             return check_launch("label_loss_backward memset");
         return MG_OK;
     }
+    if (d_features == nullptr && d_classes == nullptr && d_bias == nullptr) return MG_OK;
     MG_REQUIRE(grad_loss && stats && (reduction != MG_REDUCE_MEAN || live),
                "label_loss_backward: null pointer");
     MG_REQUIRE(scratch != nullptr && (reinterpret_cast<uintptr_t>(scratch) & 255u) == 0u &&
@@ -480,19 +1102,13 @@ extern "C" mg_status mg_label_loss_backward(
                "label_loss_backward: scratch too small or not 256-byte aligned");
     const Args a{features, classes, dtype, class_bias,
                  LabelSource{labels, label_bytes, ignore_index, (int)n_classes},
-                 Sizes{rows, (int)channels, (int)n_classes}, scale, st};
+                 Sizes{rows, (int)channels, (int)n_classes, parts_of_dtype(dtype)}, scale, st};
     const RowGrad rg{grad_loss, reduction == MG_REDUCE_MEAN ? live : nullptr,
                      reduction == MG_REDUCE_NONE};
-    float* f = static_cast<float*>(scratch);
-    if (d_features != nullptr) {
-        if (dtype == MG_F32) MG_TRY((grad<float, false>(a, rg, stats, d_features, nullptr, f)));
-        else if (dtype == MG_BF16) MG_TRY((grad<__nv_bfloat16, false>(a, rg, stats, d_features, nullptr, f)));
-        else MG_TRY((grad<__half, false>(a, rg, stats, d_features, nullptr, f)));
-    }
-    if (d_classes != nullptr || d_bias != nullptr) {
-        if (dtype == MG_F32) MG_TRY((grad<float, true>(a, rg, stats, d_classes, d_bias, f)));
-        else if (dtype == MG_BF16) MG_TRY((grad<__nv_bfloat16, true>(a, rg, stats, d_classes, d_bias, f)));
-        else MG_TRY((grad<__half, true>(a, rg, stats, d_classes, d_bias, f)));
-    }
-    return MG_OK;
+    if (dtype == MG_F32)
+        return backward(a, rg, stats, static_cast<float*>(d_features), static_cast<float*>(d_classes), d_bias, scratch);
+    if (dtype == MG_BF16)
+        return backward(a, rg, stats, static_cast<__nv_bfloat16*>(d_features),
+                        static_cast<__nv_bfloat16*>(d_classes), d_bias, scratch);
+    return backward(a, rg, stats, static_cast<__half*>(d_features), static_cast<__half*>(d_classes), d_bias, scratch);
 }
