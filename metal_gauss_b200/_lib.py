@@ -199,6 +199,30 @@ def call(name: str, *args) -> None:
     check(getattr(load(), name)(*args), name)
 
 
+class Launcher:
+    """One mg_* entry point whose last argument is the stream, called with the
+    index of the device its tensors are on: it runs on that device's current
+    stream whichever device is current, and raises on a non-zero status. The
+    binding and the switch are looked up once: a call costs the ctypes call."""
+
+    __slots__ = ("name", "fn")
+
+    def __init__(self, name: str):
+        self.name, self.fn = name, None
+
+    def __call__(self, device: int, *args) -> None:
+        fn = self.fn
+        if fn is None:
+            fn = self.fn = getattr(load(), self.name)
+        if torch._C._cuda_getDevice() == device:
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+        else:
+            with torch.cuda.device(device):
+                status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+        if status:
+            check(status, self.name)
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 

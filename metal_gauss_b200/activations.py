@@ -20,8 +20,13 @@ import torch
 from . import _lib
 from ._lib import ptr
 
+_PACK, _UNPACK = _lib.Launcher("mg_pack8"), _lib.Launcher("mg_unpack8")
 BLOCK = 128
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # MG_F32, MG_BF16, MG_F16
+
+
+def wants_grad(*tensors: torch.Tensor | None) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def dtype_code(t: torch.Tensor, what: str) -> int:
@@ -31,7 +36,7 @@ def dtype_code(t: torch.Tensor, what: str) -> int:
 
 
 def check_cuda(t: torch.Tensor, what: str) -> None:
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise RuntimeError(f"{what} is on '{t.device}': the CUDA backend needs CUDA tensors and "
                            "does not move data or fall back")
 
@@ -43,22 +48,19 @@ def _rows(t: torch.Tensor, what: str) -> tuple[int, int]:
     return t.numel() // t.shape[-1], t.shape[-1]
 
 
-@torch.no_grad()
 def pack8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """x (..., channels) in 8 bits: codes int8 (..., channels) and scales
     float32 (..., ceil(channels / 128)). 128 channels with an infinity or a
     NaN among them read back as NaN; below 1e-30 they read back as 0."""
     code, (n, d) = dtype_code(x, "pack8: x"), _rows(x, "pack8: x")
     check_cuda(x, "pack8: x")
-    with torch.cuda.device(x.device):
-        x = x.detach().contiguous()
-        codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-        scales = torch.empty(*x.shape[:-1], -(-d // BLOCK), dtype=torch.float32, device=x.device)
-        _lib.call("mg_pack8", ptr(x), code, n, d, ptr(codes), ptr(scales), _lib.stream())
+    x = x.detach().contiguous()
+    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scales = torch.empty((*x.shape[:-1], -(-d // BLOCK)), dtype=torch.float32, device=x.device)
+    _PACK(x.get_device(), ptr(x), code, n, d, ptr(codes), ptr(scales))
     return codes, scales
 
 
-@torch.no_grad()
 def unpack8(codes: torch.Tensor, scales: torch.Tensor,
             dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The tensor that `pack8` gave codes and scales for, as `dtype`."""
@@ -75,13 +77,11 @@ def unpack8(codes: torch.Tensor, scales: torch.Tensor,
     if scales.device != codes.device:
         raise RuntimeError(f"unpack8: codes on {codes.device}, scales on {scales.device}")
     check_cuda(codes, "unpack8: codes")
-    with torch.cuda.device(codes.device):
-        codes, scales = codes.contiguous(), scales.contiguous()
-        if codes.data_ptr() % 8:
-            codes = codes.clone()
-        x = torch.empty(codes.shape, dtype=dtype, device=codes.device)
-        _lib.call("mg_unpack8", ptr(codes), ptr(scales), n, d, DTYPES[dtype], ptr(x),
-                  _lib.stream())
+    codes, scales = codes.contiguous(), scales.contiguous()
+    if codes.data_ptr() % 8:
+        codes = codes.clone()
+    x = torch.empty(codes.shape, dtype=dtype, device=codes.device)
+    _UNPACK(codes.get_device(), ptr(codes), ptr(scales), n, d, DTYPES[dtype], ptr(x))
     return x
 
 

@@ -11,67 +11,80 @@ again (`mg_label_loss_forward`, `mg_label_loss_backward`).
 
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
 
 from . import _lib
 from ._lib import ptr
-from .activations import DTYPES, check_cuda, dtype_code
+from .activations import DTYPES, check_cuda, dtype_code, wants_grad
 
 MAX_CHANNELS, MAX_CLASSES = 512, 1 << 20      # MG_LABEL_MAX_CHANNELS, MG_LABEL_MAX_CLASSES
 REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 LABEL_BYTES = {torch.uint8: 1, torch.int32: 4, torch.int64: 8}
 
 
-def _scratch(n, d, v, code, backward, device):
-    nbytes = _lib.load().mg_label_loss_scratch_bytes(n, d, v, code, backward)
-    return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes
+_FORWARD = _lib.Launcher("mg_label_loss_forward")
+_BACKWARD = _lib.Launcher("mg_label_loss_backward")
+
+
+@lru_cache(maxsize=256)
+def _scratch_bytes(n: int, d: int, v: int, code: int, backward: int) -> int:
+    return _lib.load().mg_label_loss_scratch_bytes(n, d, v, code, backward)
+
+
+def _forward(features, classes, labels, bias, scale, ignore_index, reduction, train):
+    """The loss and what the backward pass needs; stats is (2 n + 1,): the two
+    values of each row and the count of live ones."""
+    d, v = features.shape[-1], classes.shape[0]
+    n = labels.numel()
+    code = DTYPES[features.dtype]
+    x = features.detach().contiguous()
+    w = classes.detach().contiguous()
+    lab = labels.contiguous()
+    b = None if bias is None else bias.detach().to(torch.float32).contiguous()
+    loss = torch.empty(labels.shape if reduction == 0 else (), dtype=torch.float32,
+                       device=x.device)
+    stats = torch.empty(2 * n + 1, dtype=torch.float32, device=x.device) if train else None
+    at = ptr(stats)
+    nbytes = _scratch_bytes(n, d, v, code, 0)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    _FORWARD(x.get_device(), ptr(x), ptr(w), code, ptr(b), ptr(lab), LABEL_BYTES[lab.dtype],
+             ignore_index, n, d, v, scale, reduction, ptr(loss), at,
+             at + 8 * n if train and reduction else None, ptr(scratch), nbytes)
+    return loss, (x, w, lab, b, stats)
 
 
 class _LabelLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, features, classes, labels, bias, scale, ignore_index, reduction):
-        d, v = features.shape[-1], classes.shape[0]
-        n = labels.numel()
-        code = DTYPES[features.dtype]
-        train = any(ctx.needs_input_grad[:4])
-        with torch.cuda.device(features.device):
-            x = features.detach().contiguous()
-            w = classes.detach().contiguous()
-            lab = labels.contiguous()
-            b = None if bias is None else bias.detach().to(torch.float32).contiguous()
-            opts = {"dtype": torch.float32, "device": x.device}
-            loss = torch.empty(labels.shape if reduction == 0 else (), **opts)
-            stats = torch.empty(2, n, **opts) if train else None
-            live = torch.empty(1, **opts) if train and reduction else None
-            scratch, nbytes = _scratch(n, d, v, code, 0, x.device)
-            _lib.call("mg_label_loss_forward", ptr(x), ptr(w), code, ptr(b), ptr(lab),
-                      LABEL_BYTES[lab.dtype], ignore_index, n, d, v, scale, reduction, ptr(loss),
-                      ptr(stats), ptr(live), ptr(scratch), nbytes, _lib.stream())
-        if train:
-            ctx.save_for_backward(x, w, lab, b, stats, live)
-            ctx.meta = (scale, ignore_index, reduction)
-            ctx.bias_dtype = None if bias is None else bias.dtype
+        loss, kept = _forward(features, classes, labels, bias, scale, ignore_index, reduction,
+                              True)
+        ctx.save_for_backward(*kept)
+        ctx.meta = (scale, ignore_index, reduction)
+        ctx.bias_dtype = None if bias is None else bias.dtype
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        x, w, lab, b, stats, live = ctx.saved_tensors
+        x, w, lab, b, stats = ctx.saved_tensors
         scale, ignore_index, reduction = ctx.meta
         need_x, need_w, _, need_b = ctx.needs_input_grad[:4]
         d, v, n = x.shape[-1], w.shape[0], lab.numel()
         code = DTYPES[x.dtype]
-        with torch.cuda.device(x.device):
-            g = grad.to(torch.float32).contiguous()
-            dx = torch.empty_like(x) if need_x else None
-            dw = torch.empty_like(w) if need_w else None
-            db = torch.empty(v, dtype=torch.float32, device=x.device) if need_b else None
-            scratch, nbytes = _scratch(n, d, v, code, 1, x.device)
-            _lib.call("mg_label_loss_backward", ptr(x), ptr(w), code, ptr(b), ptr(lab),
-                      LABEL_BYTES[lab.dtype], ignore_index, n, d, v, scale, reduction, ptr(g),
-                      ptr(stats), ptr(live), ptr(dx), ptr(dw), ptr(db), ptr(scratch), nbytes,
-                      _lib.stream())
-        if db is not None:
+        g = grad.to(torch.float32).contiguous()
+        dx = torch.empty_like(x) if need_x else None
+        dw = torch.empty_like(w) if need_w else None
+        db = torch.empty(v, dtype=torch.float32, device=x.device) if need_b else None
+        nbytes = _scratch_bytes(n, d, v, code, 1)
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        at = stats.data_ptr()
+        _BACKWARD(x.get_device(), ptr(x), ptr(w), code, ptr(b), ptr(lab), LABEL_BYTES[lab.dtype],
+                  ignore_index, n, d, v, scale, reduction, ptr(g), at,
+                  at + 8 * n if reduction else None, ptr(dx), ptr(dw), ptr(db), ptr(scratch),
+                  nbytes)
+        if db is not None and ctx.bias_dtype != torch.float32:
             db = db.to(ctx.bias_dtype)
         return dx, dw, None, db, None, None, None
 
@@ -120,5 +133,8 @@ def label_loss(features: torch.Tensor, classes: torch.Tensor, labels: torch.Tens
         raise ValueError(f"label_loss: reduction must be one of {tuple(REDUCTIONS)}, got "
                          f"{reduction!r}")
     check_cuda(features, "label_loss: features")
-    return _LabelLoss.apply(features, classes, labels, bias, float(scale), int(ignore_index),
-                            REDUCTIONS[reduction])
+    args = (features, classes, labels, bias, float(scale), int(ignore_index),
+            REDUCTIONS[reduction])
+    if not wants_grad(features, classes, bias):
+        return _forward(*args, False)[0]
+    return _LabelLoss.apply(*args)

@@ -9,61 +9,76 @@ fp32 in a fixed order, so equal calls give equal bits.
 
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
 
 from . import _lib
 from ._lib import ptr
-from .activations import BLOCK, DTYPES, check_cuda, dtype_code
+from .activations import BLOCK, DTYPES, check_cuda, dtype_code, wants_grad
 
 MAX_CHANNELS = 8192      # MG_LAYER_NORM_MAX_CHANNELS
+_FORWARD = _lib.Launcher("mg_layer_norm_forward")
+_BACKWARD = _lib.Launcher("mg_layer_norm_backward")
+
+
+@lru_cache(maxsize=256)
+def _scratch_bytes(n: int, d: int) -> int:
+    return _lib.load().mg_layer_norm_backward_scratch_bytes(n, d)
+
+
+def _forward(x, weight, bias, eps, train, saved):
+    """y and what the backward pass needs: x, or codes and scales; mean and
+    rstd as one (2 n,) tensor."""
+    d = x.shape[-1]
+    n = x.numel() // d
+    params = weight if weight is not None else bias
+    pcode = 0 if params is None else DTYPES[params.dtype]
+    x = x.detach().contiguous()
+    w = None if weight is None else weight.detach().contiguous()
+    b = None if bias is None else bias.detach().contiguous()
+    y = torch.empty_like(x)
+    stats = codes = scales = None
+    mean = rstd = None
+    if train:
+        stats = torch.empty(2 * n, dtype=torch.float32, device=x.device)
+        mean = stats.data_ptr()
+        rstd = mean + 4 * n
+        if saved == "int8":
+            codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+            scales = torch.empty((n, -(-d // BLOCK)), dtype=torch.float32, device=x.device)
+    _FORWARD(x.get_device(), ptr(x), DTYPES[x.dtype], ptr(w), ptr(b), pcode, n, d, eps, ptr(y),
+             mean, rstd, ptr(codes), ptr(scales))
+    return y, (x if codes is None else None, codes, scales, w, stats), pcode
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, saved):
-        d = x.shape[-1]
-        n = x.numel() // d
-        params = weight if weight is not None else bias
-        pcode = DTYPES[torch.float32 if params is None else params.dtype]
-        train = any(ctx.needs_input_grad[:3])
-        with torch.cuda.device(x.device):
-            x = x.detach().contiguous()
-            w = None if weight is None else weight.detach().contiguous()
-            b = None if bias is None else bias.detach().contiguous()
-            y = torch.empty_like(x)
-            mean = rstd = codes = scales = None
-            if train:
-                mean, rstd = torch.empty(2, n, dtype=torch.float32, device=x.device).unbind(0)
-                if saved == "int8":
-                    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-                    scales = torch.empty(n, -(-d // BLOCK), dtype=torch.float32, device=x.device)
-            _lib.call("mg_layer_norm_forward", ptr(x), DTYPES[x.dtype], ptr(w), ptr(b), pcode, n,
-                      d, eps, ptr(y), ptr(mean), ptr(rstd), ptr(codes), ptr(scales),
-                      _lib.stream())
-        if train:
-            ctx.save_for_backward(x if codes is None else None, codes, scales, w, mean, rstd)
-            ctx.pcode, ctx.bias_like = pcode, bias is not None
+        y, kept, ctx.pcode = _forward(x, weight, bias, eps, True, saved)
+        ctx.save_for_backward(*kept)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, codes, scales, w, mean, rstd = ctx.saved_tensors
+        x, codes, scales, w, stats = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        n, d = mean.shape[0], dy.shape[-1]
-        pdtype = [t for t, c in DTYPES.items() if c == ctx.pcode][0]
-        with torch.cuda.device(dy.device):
-            dy = dy.contiguous()
-            dx = torch.empty_like(dy) if need_x else None
-            dw = torch.empty(d, dtype=pdtype, device=dy.device) if need_w else None
-            db = torch.empty(d, dtype=pdtype, device=dy.device) if need_b else None
-            scratch, nbytes = None, 0
-            if need_w or need_b:
-                nbytes = _lib.load().mg_layer_norm_backward_scratch_bytes(n, d)
-                scratch = torch.empty(nbytes, dtype=torch.uint8, device=dy.device)
-            _lib.call("mg_layer_norm_backward", ptr(dy), ptr(x), ptr(codes), ptr(scales),
-                      DTYPES[dy.dtype], ptr(w), ctx.pcode, ptr(mean), ptr(rstd), n, d, ptr(dx),
-                      ptr(dw), ptr(db), ptr(scratch), nbytes, _lib.stream())
+        d = dy.shape[-1]
+        n = dy.numel() // d
+        pdtype = (torch.float32, torch.bfloat16, torch.float16)[ctx.pcode]
+        dy = dy.contiguous()
+        dx = torch.empty_like(dy) if need_x else None
+        dw = torch.empty(d, dtype=pdtype, device=dy.device) if need_w else None
+        db = torch.empty(d, dtype=pdtype, device=dy.device) if need_b else None
+        scratch, nbytes = None, 0
+        if need_w or need_b:
+            nbytes = _scratch_bytes(n, d)
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=dy.device)
+        mean = stats.data_ptr()
+        _BACKWARD(dy.get_device(), ptr(dy), ptr(x), ptr(codes), ptr(scales), DTYPES[dy.dtype],
+                  ptr(w), ctx.pcode, mean, mean + 4 * n, n, d, ptr(dx), ptr(dw), ptr(db),
+                  ptr(scratch), nbytes)
         return dx, dw, db, None, None
 
 
@@ -97,4 +112,6 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise TypeError(f"layer_norm: weight is {weight.dtype}, bias {bias.dtype}")
     check_cuda(x, "layer_norm: x")
+    if not wants_grad(x, weight, bias):
+        return _forward(x, weight, bias, float(eps), False, saved)[0]
     return _LayerNorm.apply(x, weight, bias, float(eps), saved)
