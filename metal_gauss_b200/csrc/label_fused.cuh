@@ -1,0 +1,598 @@
+// The label loss's gradients with the logits' gradient never leaving the SM.
+//
+// A unit owns 128 items of one side (rows for dx, classes for dw) and a share
+// of the other side, which streams past in tiles of 64:
+//   S = own . stream^T       128 x 64, fp32 in tensor memory
+//   G = r (softmax - onehot) from S by one of two groups of four warps, back
+//       into tensor memory as bf16 parts
+//   acc += G stream          128 x channels, G the A operand from tensor memory
+// One streamed tile in shared memory serves both products: its channels are
+// the contraction of the first and the columns of the second.
+//
+// Bound by the exponentials of the groups (one per logit: 16 a clock and SM)
+// while there are few channels, by the tensor cores above. The logits are
+// computed twice in all (dx and dw), which costs less than 2 x PARTS bytes a
+// logit of G written and read twice.
+// acc leaves tensor memory for the registers of eight more warps every
+// `per_segment` tiles: the tensor cores' fp32 additions truncate, and fp32
+// results keep their precision only over short runs of them.
+#pragma once
+
+#include "labels.cuh"
+
+namespace mg {
+
+namespace {
+
+constexpr int kOwn = 128;
+constexpr int kStream = 64;
+constexpr int kFusedThreads = 576;  // copy, issue, 2 x 4 score warps, 8 warps for acc
+constexpr int kFusedStages = 8;     // at most
+constexpr int kFusedShared = 222 * 1024;  // of it 1 KB to align; 5 KB are static
+
+// Parts of G: two also for bf16 features, whose gradients then carry no other
+// rounding than their own (one part would add its 2^-9 to theirs).
+template <int PARTS>
+constexpr int kGParts = PARTS == 1 ? 2 : PARTS;
+
+// Products (G part, stream part), smallest first.
+template <int PARTS>
+__device__ constexpr int g_pairs() { return PARTS == 1 ? 2 : PARTS == 2 ? 3 : 6; }
+template <int PARTS>
+__device__ constexpr int g_pair_a(int i) {
+    return PARTS == 1 ? 1 - i : pair_a<PARTS>(g_pairs<PARTS>(), i);
+}
+template <int PARTS>
+__device__ constexpr int g_pair_b(int i) {
+    return PARTS == 1 ? 0 : pair_b<PARTS>(g_pairs<PARTS>(), i);
+}
+
+// The features' type, by its parts.
+template <int PARTS>
+struct PartsType;
+template <>
+struct PartsType<1> { using type = __nv_bfloat16; };
+template <>
+struct PartsType<2> { using type = __half; };
+template <>
+struct PartsType<3> { using type = float; };
+template <int PARTS>
+using TypeOf = typename PartsType<PARTS>::type;
+
+struct FusedArgs {
+    int64_t units;
+    int64_t own;           // items of the owning side
+    int64_t streamed;      // items of the streaming side
+    int64_t per_split;     // tiles of a share
+    int splits;
+    int per_segment;
+    int64_t rows;
+    int classes, channels;
+    int chunks;            // of 64 channels
+    int stages, own_buffers, acc_buffers;
+    float scale;
+    const float* bias;
+    LabelSource labels;
+    RowGrad rg;
+    const float* stats;
+    float* part_bias;      // by class: (splits, 2, classes), or NULL
+    float* part;           // fp32 shares (splits, own, part_ld), or NULL
+    int part_ld;
+    void* out;             // the result itself
+    int32_t* error_word;
+};
+
+struct FusedWalk {
+    int64_t own0, t0, t1;
+    int split;
+};
+
+__device__ __forceinline__ FusedWalk fused_unit(const FusedArgs& p, int64_t u) {
+    FusedWalk w;
+    w.own0 = u / p.splits * kOwn;
+    w.split = (int)(u % p.splits);
+    w.t0 = w.split * p.per_split;
+    w.t1 = min((p.streamed + kStream - 1) / kStream, w.t0 + p.per_split);
+    return w;
+}
+
+__device__ __forceinline__ void tmem_store8(uint32_t addr, const uint32_t (&r)[8]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_load16(uint32_t addr, float (&v)[16]) {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15])
+        : "r"(addr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_store_wait() {
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    uint32_t r;
+    memcpy(&r, &v, 4);
+    return r;
+}
+
+// 16 values as GP parts, two to a word.
+template <int GP>
+__device__ __forceinline__ void store_parts(uint32_t addr, float (&z)[16]) {
+#pragma unroll
+    for (int i = 0; i < GP; ++i) {
+        uint32_t r[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            r[j] = pack_bf16(z[2 * j], z[2 * j + 1]);
+            if (i + 1 < GP) {
+                z[2 * j] -= __uint_as_float(r[j] << 16);
+                z[2 * j + 1] -= __uint_as_float(r[j] & 0xffff0000u);
+            }
+        }
+        tmem_store8(addr + i * (kStream / 2), r);
+    }
+}
+
+template <bool BY_CLASS, int PARTS>
+__global__ void __launch_bounds__(kFusedThreads, 1)
+fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtensorMap map_own,
+             const __grid_constant__ CUtensorMap map_stream) {
+    constexpr int GP = kGParts<PARTS>;
+    constexpr int kScorePairs = PARTS == 1 ? 1 : PARTS == 2 ? 4 : 6;
+    constexpr int kOwnChunk = kOwn * 128, kStreamChunk = kStream * 128;  // 64 channels, bytes
+    constexpr uint32_t kGBase = 2 * kStream, kAccBase = kGBase + 2 * GP * (kStream / 2);
+    extern __shared__ uint8_t dynamic[];
+    // per group and of two tiles in turn: bias (by row), or the rows' values (by class)
+    __shared__ alignas(16) float col_a[2][2][kStream], col_b[2][2][kStream], col_c[2][2][kStream];
+    __shared__ alignas(16) int col_l[2][2][kStream];
+    __shared__ uint64_t bars[2 * kFusedStages + 17];
+    __shared__ uint32_t tmem_s;
+    __shared__ volatile int stop;
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x / 32, 0), lane = threadIdx.x % 32;
+    const uint32_t base = (smem_u32(dynamic) + 1023u) & ~1023u;
+    const uint32_t own_bytes = PARTS * p.chunks * kOwnChunk;
+    const uint32_t stage_bytes = PARTS * p.chunks * kStreamChunk;
+    const uint32_t stream0 = base + p.own_buffers * own_bytes;
+    const uint32_t full = smem_u32(bars), empty = full + 8 * kFusedStages;
+    const uint32_t own_full = empty + 8 * kFusedStages, own_empty = own_full + 16;
+    const uint32_t s_full = own_empty + 16, s_empty = s_full + 16;
+    const uint32_t g_full = s_empty + 16, g_empty = g_full + 16;
+    const uint32_t acc_full = g_empty + 16, acc_empty = acc_full + 16;
+    const uint32_t drain = acc_empty + 16;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kFusedStages; ++i) {
+            mbar_init(full + 8 * i, 1);
+            mbar_init(empty + 8 * i, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(own_full + 8 * i, 1);
+            mbar_init(own_empty + 8 * i, 1);
+            mbar_init(s_full + 8 * i, 1);
+            mbar_init(s_empty + 8 * i, 4);
+            mbar_init(g_full + 8 * i, 4);
+            mbar_init(g_empty + 8 * i, 1);
+            mbar_init(acc_full + 8 * i, 1);
+            mbar_init(acc_empty + 8 * i, 8);
+        }
+        mbar_init(drain, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async_shared();
+        stop = 0;
+    }
+    if (warp == 1) tmem_alloc(smem_u32(&tmem_s), kTmemColumns);
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    constexpr uint32_t tmem = kTmemBase;
+    const auto wait = [&](uint32_t bar, uint32_t parity) {
+        return mbar_wait(bar, parity, &stop, p.error_word, DEV_ERR_TILE_WAIT);
+    };
+
+    const auto wait_warp = [&](uint32_t bar, uint32_t parity) {
+        return mbar_wait_warp(bar, parity, &stop, p.error_word, DEV_ERR_TILE_WAIT);
+    };
+
+    if (warp == 0) {
+        {  // copies tiles in
+            const uint32_t on = elect_lane();
+            int stage = 0, ob = 0;
+            uint32_t phase = 0, ob_phase = 0;
+            int64_t issued = 0, owns = 0;
+            bool ok = true;
+            for (int64_t u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
+                const FusedWalk w = fused_unit(p, u);
+                ok = wait_warp(own_empty + 8 * ob, ob_phase ^ 1);
+                if (!ok) break;
+                mbar_expect(own_full + 8 * ob, own_bytes, on);
+                for (int i = 0; i < PARTS; ++i)
+                    for (int c = 0; c < p.chunks; ++c)
+                        tma_load(base + ob * own_bytes + (i * p.chunks + c) * kOwnChunk, &map_own,
+                                 c * 64, (int)w.own0, i, own_full + 8 * ob, on);
+                ++owns;
+                if (++ob == p.own_buffers) {
+                    ob = 0;
+                    ob_phase ^= 1;
+                }
+                for (int64_t t = w.t0; t < w.t1; ++t) {
+                    ok = wait_warp(empty + 8 * stage, phase ^ 1);
+                    if (!ok) break;
+                    mbar_expect(full + 8 * stage, stage_bytes, on);
+                    for (int i = 0; i < PARTS; ++i)
+                        for (int c = 0; c < p.chunks; ++c)
+                            tma_load(stream0 + stage * stage_bytes + (i * p.chunks + c) * kStreamChunk,
+                                     &map_stream, c * 64, (int)(t * kStream), i, full + 8 * stage, on);
+                    ++issued;
+                    if (++stage == p.stages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+            }
+            if (stop) {  // this block gave up: its copies in flight land before it ends
+                for (int j = (int)min(issued, (int64_t)p.stages); j > 0; --j) {
+                    if (--stage < 0) {
+                        stage = p.stages - 1;
+                        phase ^= 1;
+                    }
+                    for (int i = 0; i < kMbarRounds; ++i)
+                        if (mbar_try(full + 8 * stage, phase)) break;
+                }
+                for (int j = (int)min(owns, (int64_t)p.own_buffers); j > 0; --j) {
+                    if (--ob < 0) {
+                        ob = p.own_buffers - 1;
+                        ob_phase ^= 1;
+                    }
+                    for (int i = 0; i < kMbarRounds; ++i)
+                        if (mbar_try(own_full + 8 * ob, ob_phase)) break;
+                }
+            }
+        }
+    } else if (warp == 1) {
+        {  // issues products
+            const uint32_t on = elect_lane();
+            // the scores of a tile go before the G product of the tile `ahead`
+            // before it, so that a group finds its next scores ready when it
+            // hands over G (two ahead against one: 2438 -> @@ cycles a tile,
+            // bf16, 16 channels); two take three streamed tiles
+            const uint32_t idesc_s = mma_idesc(kStream, false, false);
+            const int n = (p.channels + 15) / 16 * 16;
+            const uint32_t idesc_g = uniform(mma_idesc(n, false, true));
+            int stage = 0, ob = 0, ab = 0;
+            uint32_t phase = 0, ob_phase = 0, ab_phase = 0;
+            int64_t i = 0;         // tiles whose scores are issued
+            int in_segment = 0;    // G products in acc
+            const int ahead = p.stages > 2 ? 2 : 1;
+            int stage1 = 0, stage2 = 0;          // of the last tile and the one before
+            bool ends1 = false, ends2 = false, ok = true;
+            // the G product of a tile; `ends`: acc is complete after it
+            const auto product = [&](int64_t tile, int st, bool ends) {
+                const int g = (int)(tile & 1);
+                if (!wait_warp(g_full + 8 * g, (uint32_t)(tile >> 1) & 1)) return false;
+                if (in_segment == 0 && !wait_warp(acc_empty + 8 * ab, ab_phase ^ 1)) return false;
+                tmem_fence_after();
+                const uint32_t d = uniform(tmem + kAccBase + ab * n);
+                const uint32_t a0 = uniform(tmem + kGBase + g * (GP * (kStream / 2)));
+                const uint32_t b0 = uniform(mn_major_lo(stream0 + st * stage_bytes, kStreamChunk));
+                const uint32_t part = uniform(p.chunks * kStreamChunk / 16);
+                const uint32_t more = uniform(in_segment > 0);
+#pragma unroll
+                for (int q = 0; q < g_pairs<PARTS>(); ++q) {
+#pragma unroll
+                    for (int s = 0; s < kStream / 16; ++s)
+                        mma_bf16_ta<kMnMajorHi>(d, a0 + g_pair_a<PARTS>(q) * (kStream / 2) + 8 * s,
+                                                b0 + g_pair_b<PARTS>(q) * part + 128 * s, idesc_g,
+                                                q > 0 || s > 0 ? true : more != 0, on);
+                }
+                mma_commit(empty + 8 * st, on);
+                mma_commit(g_empty + 8 * g, on);
+                if (++in_segment == p.per_segment || ends) {
+                    mma_commit(acc_full + 8 * ab, on);
+                    in_segment = 0;
+                    if (++ab == p.acc_buffers) {
+                        ab = 0;
+                        ab_phase ^= 1;
+                    }
+                }
+                return true;
+            };
+            for (int64_t u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
+                const FusedWalk w = fused_unit(p, u);
+                ok = wait_warp(own_full + 8 * ob, ob_phase);
+                for (int64_t t = w.t0; ok && t < w.t1; ++t) {
+                    const int g = (int)(i & 1);
+                    ok = wait_warp(full + 8 * stage, phase) && wait_warp(s_empty + 8 * g, ((uint32_t)(i >> 1) & 1) ^ 1);
+                    if (!ok) break;
+                    tmem_fence_after();
+                    const uint32_t d = uniform(tmem + g * kStream);
+                    const uint32_t a0 = uniform(k_major_lo(base + ob * own_bytes));
+                    const uint32_t b0 = uniform(k_major_lo(stream0 + stage * stage_bytes));
+                    const uint32_t a_part = uniform(p.chunks * kOwnChunk / 16);
+                    const uint32_t b_part = uniform(p.chunks * kStreamChunk / 16);
+                    for (int c = 0; c < p.chunks; ++c) {
+                        const uint32_t a1 = uniform(a0 + c * (kOwnChunk / 16)), b1 = uniform(b0 + c * (kStreamChunk / 16));
+#pragma unroll
+                        for (int q = 0; q < kScorePairs; ++q) {
+#pragma unroll
+                            for (int s = 0; s < 4; ++s)
+                                if (64 * c + 16 * s < p.channels)
+                                    mma_bf16<k_major_hi(128), k_major_hi(128)>(
+                                        d, a1 + pair_a<PARTS>(kScorePairs, q) * a_part + 2 * s,
+                                        b1 + pair_b<PARTS>(kScorePairs, q) * b_part + 2 * s, idesc_s,
+                                        q > 0 || s > 0 ? true : c > 0, on);
+                        }
+                    }
+                    mma_commit(s_full + 8 * g, on);
+                    if (t + 1 == w.t1) mma_commit(own_empty + 8 * ob, on);
+                    if (i >= ahead) ok = ahead == 2 ? product(i - 2, stage2, ends2) : product(i - 1, stage1, ends1);
+                    stage2 = stage1;
+                    ends2 = ends1;
+                    stage1 = stage;
+                    ends1 = t + 1 == w.t1;
+                    ++i;
+                    if (++stage == p.stages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+                if (++ob == p.own_buffers) {
+                    ob = 0;
+                    ob_phase ^= 1;
+                }
+            }
+            if (ok && ahead == 2 && i > 1) ok = product(i - 2, stage2, ends2);
+            if (ok && i > 0) product(i - 1, stage1, ends1);
+            if (stop) {
+                mma_commit(drain, on);
+                for (int k = 0; k < kMbarRounds; ++k)
+                    if (mbar_try(drain, 0)) break;
+            }
+        }
+    } else if (warp < 10) {
+        // Scores to G: group g takes every other tile. After a wait that gave
+        // up the rest fail at once and the block runs out on what is there.
+        const int g = (warp - 2) / 4, quarter = warp & 3, in_tile = quarter * 32 + lane;
+        const int gt = (threadIdx.x - 64) & 127;  // thread of the group
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+        const uint32_t s_addr = tmem + lanes + g * kStream;
+        const uint32_t g_addr = tmem + lanes + kGBase + g * (GP * (kStream / 2));
+        const float c2 = p.scale * kLog2e;
+        int64_t i = 0;
+        int buf = 0;
+        uint32_t phase = 0;
+        for (int64_t u = blockIdx.x; u < p.units; u += gridDim.x) {
+            const FusedWalk w = fused_unit(p, u);
+            const int64_t own = w.own0 + in_tile;
+            int lab = kIgnored;
+            float lse = kInf, r = 0.0f, at_label = 0.0f, own_bias = 0.0f, bias_sum = 0.0f;
+            if constexpr (BY_CLASS) {
+                if (p.bias != nullptr && own < p.own) own_bias = p.bias[own] * kLog2e;
+            } else if (own < p.own) {
+                lab = p.labels.at(own);
+                if (lab >= 0) {
+                    r = p.rg.at(own, lab);
+                    lse = p.stats[own];
+                    at_label = -p.stats[p.rows + own] * r;
+                }
+            }
+            for (int64_t t = w.t0; t < w.t1; ++t, ++i) {
+                if ((int)(i & 1) != g) continue;
+                if (gt < kStream) {
+                    const int64_t j = t * kStream + gt;
+                    if constexpr (BY_CLASS) {
+                        const int l = j < p.rows ? p.labels.at(j) : kIgnored;
+                        const float rj = p.rg.at(j < p.rows ? j : 0, l);
+                        col_l[g][buf][gt] = l;
+                        col_a[g][buf][gt] = l >= 0 ? p.stats[j] : kInf;
+                        col_b[g][buf][gt] = rj;
+                        col_c[g][buf][gt] = l >= 0 ? -p.stats[p.rows + j] * rj : 0.0f;
+                    } else {
+                        col_a[g][buf][gt] = j < p.classes ? (p.bias != nullptr ? p.bias[j] * kLog2e : 0.0f) : -kInf;
+                    }
+                }
+                named_sync(2 + g, 128);
+                wait(s_full + 8 * g, phase);
+                tmem_fence_after();
+                // 16 columns at a time in a loop that is not unrolled: its code has
+                // to stay in the instruction cache of eight warps out of step
+                // (both halves of 32 unrolled: 38 % of the stalls were fetches)
+#pragma unroll 1
+                for (int k = 0; k < kStream; k += 16) {
+                    float z[16];
+                    tmem_load16(s_addr + k, z);
+                    if (k + 16 == kStream) {
+                        tmem_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(s_empty + 8 * g);
+                    }
+                    if constexpr (BY_CLASS) {
+#pragma unroll
+                        for (int j = 0; j < 16; j += 4) {
+                            const float4 a = *reinterpret_cast<const float4*>(&col_a[g][buf][k + j]);
+                            const float4 b = *reinterpret_cast<const float4*>(&col_b[g][buf][k + j]);
+                            z[j] = exp2_fast(fmaf(z[j], c2, own_bias) - a.x) * b.x;
+                            z[j + 1] = exp2_fast(fmaf(z[j + 1], c2, own_bias) - a.y) * b.y;
+                            z[j + 2] = exp2_fast(fmaf(z[j + 2], c2, own_bias) - a.z) * b.z;
+                            z[j + 3] = exp2_fast(fmaf(z[j + 3], c2, own_bias) - a.w) * b.w;
+                        }
+                        // rows labelled with one of this warp's classes
+                        const int mine = col_l[g][buf][k + (lane & 15)] - (int)w.own0 - quarter * 32;
+                        if (__any_sync(0xffffffffu, (unsigned)mine < 32u)) {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j)
+                                if (col_l[g][buf][k + j] == (int)own) z[j] = col_c[g][buf][k + j];
+                        }
+                        if (p.part_bias != nullptr) {
+                            float q[4] = {bias_sum, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) q[j % 4] += z[j];
+                            bias_sum = (q[0] + q[1]) + (q[2] + q[3]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; j += 4) {
+                            const float4 b = *reinterpret_cast<const float4*>(&col_a[g][buf][k + j]);
+                            z[j] = exp2_fast(fmaf(z[j], c2, b.x) - lse) * r;
+                            z[j + 1] = exp2_fast(fmaf(z[j + 1], c2, b.y) - lse) * r;
+                            z[j + 2] = exp2_fast(fmaf(z[j + 2], c2, b.z) - lse) * r;
+                            z[j + 3] = exp2_fast(fmaf(z[j + 3], c2, b.w) - lse) * r;
+                        }
+                        const int rel = lab - (int)(t * kStream) - k;
+                        if (__any_sync(0xffffffffu, (unsigned)rel < 16u)) {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j)
+                                if (j == rel) z[j] = at_label;
+                        }
+                    }
+                    // the G product of the tile before last has read this buffer
+                    if (k == 0) {
+                        wait(g_empty + 8 * g, phase ^ 1);
+                        tmem_fence_after();
+                    }
+                    store_parts<GP>(g_addr + k / 2, z);
+                }
+                tmem_store_wait();
+                tmem_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(g_full + 8 * g);
+                buf ^= 1;
+                phase ^= 1;
+            }
+            if (BY_CLASS && p.part_bias != nullptr && own < p.own)
+                p.part_bias[(int64_t)(w.split * 2 + g) * p.own + own] = bias_sum;
+        }
+    } else {
+        // acc: quarter of the rows, and every other 32 channels
+        const int quarter = warp & 3, half = (warp - 10) / 4;
+        const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + kAccBase;
+        const int n = (p.channels + 15) / 16 * 16;
+        constexpr int kKept = PARTS == 3 ? 2 : 1;  // fp32: all (<= 128 channels) stay here
+        int ab = 0;
+        uint32_t ab_phase = 0;
+        for (int64_t u = blockIdx.x; u < p.units; u += gridDim.x) {
+            const FusedWalk w = fused_unit(p, u);
+            const int64_t own = w.own0 + quarter * 32 + lane;
+            float kept[kKept][32];
+            if constexpr (PARTS == 3) {
+#pragma unroll
+                for (int q = 0; q < kKept; ++q)
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) kept[q][j] = 0.0f;
+            }
+            const auto write = [&](const float (&v)[32], int c, bool add) {
+                if (own >= p.own) return;
+                if (p.part != nullptr) {
+                    float* dst = p.part + ((int64_t)w.split * p.own + own) * p.part_ld + c;
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        if (c + j >= p.part_ld) continue;
+                        float4* d4 = reinterpret_cast<float4*>(dst + j);
+                        float4 o = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                        if (add) {
+                            const float4 e = *d4;
+                            o.x += e.x;
+                            o.y += e.y;
+                            o.z += e.z;
+                            o.w += e.w;
+                        }
+                        *d4 = o;
+                    }
+                    return;
+                }
+                TypeOf<PARTS>* dst = static_cast<TypeOf<PARTS>*>(p.out) + own * p.channels + c;
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    if (c + j < p.channels) dst[j] = from_f32<TypeOf<PARTS>>(v[j] * p.scale);
+            };
+            bool first = true;
+            for (int64_t t = w.t0; t < w.t1; t += p.per_segment) {
+                wait(acc_full + 8 * ab, ab_phase);
+                tmem_fence_after();
+                if constexpr (PARTS == 3) {
+#pragma unroll
+                    for (int q = 0; q < kKept; ++q) {
+                        const int c = (2 * q + half) * 32;
+                        if (c < n) {
+#pragma unroll
+                            for (int h = 0; h < 32; h += 16) {  // 16 at a time: 96 registers a thread
+                                float v[16];
+                                tmem_load16(lanes + ab * n + c + h, v);
+#pragma unroll
+                                for (int j = 0; j < 16; ++j) kept[q][h + j] += v[j];
+                            }
+                        }
+                    }
+                } else {
+                    for (int c = half * 32; c < n; c += 64) {
+                        tmem_load32(lanes + ab * n + c, kept[0]);
+                        if (c + 64 >= n) break;
+                        write(kept[0], c, !first);
+                    }
+                }
+                tmem_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(acc_empty + 8 * ab);
+                if constexpr (PARTS < 3) {
+                    // the last chunk is written after the buffer is given back
+                    const int chunks = (n + 31) / 32;
+                    const int mine = (chunks - half + 1) / 2;
+                    if (mine > 0) write(kept[0], (2 * (mine - 1) + half) * 32, !first);
+                }
+                first = false;
+                if (++ab == p.acc_buffers) {
+                    ab = 0;
+                    ab_phase ^= 1;
+                }
+            }
+            if constexpr (PARTS == 3) {
+#pragma unroll
+                for (int q = 0; q < kKept; ++q) {
+                    const int c = (2 * q + half) * 32;
+                    if (c < n) write(kept[q], c, false);
+                }
+            }
+        }
+    }
+    tmem_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tmem_fence_after();
+        tmem_free(tmem_s, kTmemColumns);
+    }
+}
+
+// Whether the owning side, two streamed tiles and acc fit an SM: up to 128
+// channels of fp32, 192 of fp16, 256 of bf16.
+inline bool fused_fits(int parts, int channels) {
+    const int chunks = (channels + 63) / 64, n = (channels + 15) / 16 * 16;
+    const int g_parts = parts == 1 ? 2 : parts;
+    return parts * chunks * (kOwn * 128 + 2 * kStream * 128) <= kFusedShared - 1024 &&
+           2 * kStream + g_parts * kStream + n <= 512;
+}
+
+// Buffers for what is left: a second one for the owning side if four streamed
+// tiles fit beside it, then streamed tiles.
+inline void fused_buffers(FusedArgs& p, int parts) {
+    const int own = parts * p.chunks * kOwn * 128, stage = parts * p.chunks * kStream * 128;
+    const int room = kFusedShared - 1024, n = (p.channels + 15) / 16 * 16;
+    p.own_buffers = 2 * own + 4 * stage <= room ? 2 : 1;
+    p.stages = std::min(kFusedStages, (room - p.own_buffers * own) / stage);
+    const int g_parts = parts == 1 ? 2 : parts;
+    p.acc_buffers = 2 * kStream + g_parts * kStream + 2 * n <= 512 ? 2 : 1;
+}
+
+}  // namespace
+
+}  // namespace mg

@@ -1,0 +1,470 @@
+// The tile kernel of the label loss (labels.cu): one pipeline of TMA copies,
+// tcgen05 products and epilogue warps with four uses.
+#pragma once
+
+#include "labels.cuh"
+
+namespace mg {
+
+namespace {
+
+constexpr int kM = 128;        // rows of a tile
+constexpr int kN = 256;        // columns of a tile, at most
+constexpr int kThreads = 320;  // a copying warp, an issuing warp, 8 warps that take tiles out
+
+enum Mode { kStats, kLogitGrad, kProductRow, kProductClass };
+
+template <int MODE, int PARTS>
+struct Shape {
+    static constexpr bool kProduct = MODE >= kProductRow;
+    static constexpr bool kAmn = MODE == kProductClass;  // A's row index runs fastest
+    static constexpr bool kBmn = kProduct;
+    static constexpr int kChunk = PARTS == 1 ? 64 : 32;  // contraction entries per stage
+    static constexpr int kA = kM * kChunk * 2;           // bytes of one part
+    static constexpr int kB = kN * kChunk * 2;
+    static constexpr int kStage = PARTS * (kA + kB);
+    static constexpr int kStages = PARTS == 3 ? (MODE == kLogitGrad ? 2 : 3) : (MODE == kLogitGrad ? 3 : 4);
+    // G on its way out: 128 x 32 bf16 for each half of the taking warps, part and buffer
+    static constexpr int kOutBuffers = PARTS == 3 ? 1 : 2;
+    static constexpr int kOut = MODE == kLogitGrad ? 2 * PARTS * kOutBuffers * kM * 64 : 0;
+    static constexpr int kDynamic = 1024 + kStages * kStage + kOut;
+    // Products of parts (a, b), smallest first.
+    static constexpr int kPairs = PARTS == 1 ? 1 : PARTS == 3 ? 6 : kProduct ? 3 : 4;
+};
+
+struct TileArgs {
+    int64_t units;
+    int64_t a_rows;         // rows of the A side (of the piece, or classes)
+    int64_t depth;          // contraction entries
+    int columns;            // columns of the B side in all (classes, or channels)
+    int splits;             // shares of the classes (kStats) or of the contraction
+    int64_t per_split;      // column tiles, or chunks, per share
+    int per_segment;        // chunks between visits to the registers
+    int64_t row0;           // the piece's first row
+    int64_t rows;           // rows in all
+    float scale;
+    const float* bias;
+    LabelSource labels;
+    RowGrad rg;
+    const float* stats;     // kLogitGrad: log2 of the sum, 1 - softmax(label)
+    float *part_m, *part_s, *label_z;  // kStats
+    float* part_bias;       // kLogitGrad: sums of 32 rows of G, or NULL
+    float* part;            // products: fp32 shares (splits, a_rows, part_ld), or NULL
+    int part_ld;
+    int add;                // to what the share holds
+    void* out;              // products: the result itself
+    int out_type;
+    int32_t* error_word;
+};
+
+// The tiles of a unit. Scores: a unit is a row tile and a share of the column
+// tiles (kStats) or one column tile (kLogitGrad). Products: a unit is a row
+// tile, a column tile and a share of the contraction, in segments.
+struct Walk {
+    int64_t a_row, c0, c1;
+    int b_row, split, tiles, first;
+};
+
+template <int MODE, int PARTS>
+__device__ __forceinline__ Walk walk_unit(const TileArgs& p, int64_t u) {
+    Walk w;
+    const int col_tiles = (p.columns + kN - 1) / kN;
+    if (MODE == kStats) {
+        w.a_row = u / p.splits * kM;
+        w.split = (int)(u % p.splits);
+        w.first = (int)(w.split * p.per_split);
+        w.tiles = (int)min((int64_t)col_tiles, w.first + p.per_split) - w.first;
+        w.c0 = 0;
+        w.c1 = (p.depth + Shape<MODE, PARTS>::kChunk - 1) / Shape<MODE, PARTS>::kChunk;
+    } else if (MODE == kLogitGrad) {
+        w.a_row = u / col_tiles * kM;
+        w.first = (int)(u % col_tiles);
+        w.tiles = 1;
+        w.split = 0;
+        w.c0 = 0;
+        w.c1 = (p.depth + Shape<MODE, PARTS>::kChunk - 1) / Shape<MODE, PARTS>::kChunk;
+    } else {
+        const int64_t chunks = (p.depth + Shape<MODE, PARTS>::kChunk - 1) / Shape<MODE, PARTS>::kChunk;
+        w.split = (int)(u % p.splits);
+        const int64_t t = u / p.splits;
+        w.first = (int)(t % col_tiles);
+        w.a_row = t / col_tiles * kM;
+        w.c0 = w.split * p.per_split;
+        w.c1 = min(chunks, w.c0 + p.per_split);
+        w.tiles = (int)((w.c1 - w.c0 + p.per_segment - 1) / p.per_segment);
+    }
+    return w;
+}
+
+template <int MODE, int PARTS>
+__global__ void __launch_bounds__(kThreads, 1)
+tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensorMap map_a,
+            const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_out) {
+    using S = Shape<MODE, PARTS>;
+    extern __shared__ uint8_t dynamic[];
+    __shared__ alignas(16) float bias_s[2][kN];
+    __shared__ uint64_t bars[2 * S::kStages + 5];
+    __shared__ uint32_t tmem_s;
+    __shared__ volatile int stop;
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x / 32, 0), lane = threadIdx.x % 32;
+    const uint32_t base = (smem_u32(dynamic) + 1023u) & ~1023u;
+    const uint32_t full = smem_u32(bars), empty = full + 8 * S::kStages;
+    const uint32_t taken_full = empty + 8 * S::kStages, taken_empty = taken_full + 16;
+    const uint32_t drain = taken_empty + 16;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S::kStages; ++i) {
+            mbar_init(full + 8 * i, 1);
+            mbar_init(empty + 8 * i, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(taken_full + 8 * i, 1);
+            mbar_init(taken_empty + 8 * i, 8);
+        }
+        mbar_init(drain, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async_shared();
+        stop = 0;
+    }
+    if (warp == 1) tmem_alloc(smem_u32(&tmem_s), kTmemColumns);
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    constexpr uint32_t tmem = kTmemBase;
+
+    if (warp == 0) {
+        {  // copies tiles in
+            const uint32_t on = elect_lane();
+            int stage = 0;
+            uint32_t phase = 0;
+            int64_t issued = 0;
+            bool ok = true;
+            for (int64_t u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
+                const Walk w = walk_unit<MODE, PARTS>(p, u);
+                for (int t = 0; ok && t < w.tiles; ++t) {
+                    const int b0 = (S::kProduct ? w.first : w.first + t) * kN;
+                    const int64_t c0 = S::kProduct ? w.c0 + (int64_t)t * p.per_segment : w.c0;
+                    const int64_t c1 = S::kProduct ? min(w.c1, c0 + p.per_segment) : w.c1;
+                    const int blocks = S::kProduct ? (min(kN, p.columns - b0) + 63) / 64 : 0;
+                    const uint32_t bytes =
+                        PARTS * (S::kA + (S::kProduct ? blocks * S::kChunk * 128 : S::kB));
+                    for (int64_t c = c0; c < c1; ++c) {
+                        ok = mbar_wait_warp(empty + 8 * stage, phase ^ 1, &stop, p.error_word, DEV_ERR_TILE_WAIT);
+                        if (!ok) break;
+                        const uint32_t bar = full + 8 * stage;
+                        mbar_expect(bar, bytes, on);
+                        const int k = (int)(c * S::kChunk);
+#pragma unroll
+                        for (int i = 0; i < PARTS; ++i) {
+                            const uint32_t a = base + stage * S::kStage + i * S::kA;
+                            const uint32_t b = base + stage * S::kStage + PARTS * S::kA + i * S::kB;
+                            if (S::kAmn) {
+                                for (int q = 0; q < 2; ++q)
+                                    tma_load(a + q * S::kChunk * 128, &map_a, (int)w.a_row + 64 * q, k, i, bar, on);
+                            } else {
+                                tma_load(a, &map_a, k, (int)w.a_row, i, bar, on);
+                            }
+                            if (S::kBmn) {
+                                for (int q = 0; q < blocks; ++q)
+                                    tma_load(b + q * S::kChunk * 128, &map_b, b0 + 64 * q, k, i, bar, on);
+                            } else {
+                                tma_load(b, &map_b, k, b0, i, bar, on);
+                            }
+                        }
+                        ++issued;
+                        if (++stage == S::kStages) {
+                            stage = 0;
+                            phase ^= 1;
+                        }
+                    }
+                }
+            }
+            if (stop) {  // this block gave up: its copies in flight land before it ends
+                const int n = (int)min(issued, (int64_t)S::kStages);
+                for (int j = 0; j < n; ++j) {
+                    if (--stage < 0) {
+                        stage = S::kStages - 1;
+                        phase ^= 1;
+                    }
+                    for (int i = 0; i < kMbarRounds; ++i)
+                        if (mbar_try(full + 8 * stage, phase)) break;
+                }
+            }
+        }
+    } else if (warp == 1) {
+        {  // issues products
+            const uint32_t on = elect_lane();
+            int stage = 0, buf = 0;
+            uint32_t phase = 0, buf_phase = 0;
+            bool ok = true;
+            for (int64_t u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
+                const Walk w = walk_unit<MODE, PARTS>(p, u);
+                for (int t = 0; ok && t < w.tiles; ++t) {
+                    const int b0 = (S::kProduct ? w.first : w.first + t) * kN;
+                    const int64_t c0 = S::kProduct ? w.c0 + (int64_t)t * p.per_segment : w.c0;
+                    const int64_t c1 = S::kProduct ? min(w.c1, c0 + p.per_segment) : w.c1;
+                    const int n = min(kN, (p.columns - b0 + 15) / 16 * 16);
+                    const uint32_t idesc = uniform(mma_idesc(n, S::kAmn, S::kBmn));
+                    const int chunks = (int)uniform((uint32_t)(c1 - c0));
+                    // 16-entry steps of the last chunk
+                    const int tail = (int)uniform((uint32_t)min((int64_t)(S::kChunk / 16), (p.depth - (c1 - 1) * S::kChunk + 15) / 16));
+                    ok = mbar_wait_warp(taken_empty + 8 * buf, buf_phase ^ 1, &stop, p.error_word, DEV_ERR_TILE_WAIT);
+                    if (!ok) break;
+                    tmem_fence_after();
+                    const uint32_t d = uniform(tmem + buf * kN);
+                    for (int c = 0; c < chunks; ++c) {
+                        ok = mbar_wait_warp(full + 8 * stage, phase, &stop, p.error_word, DEV_ERR_TILE_WAIT);
+                        if (!ok) break;
+                        tmem_fence_after();
+                        const int steps = c + 1 < chunks ? S::kChunk / 16 : tail;
+                        const uint32_t a_at = base + stage * S::kStage, b_at = a_at + PARTS * S::kA;
+                        const uint32_t a = uniform(S::kAmn ? mn_major_lo(a_at, S::kChunk * 128) : k_major_lo(a_at));
+                        const uint32_t b = uniform(S::kBmn ? mn_major_lo(b_at, S::kChunk * 128) : k_major_lo(b_at));
+                        constexpr uint32_t a_hi = S::kAmn ? kMnMajorHi : k_major_hi(S::kChunk * 2);
+                        constexpr uint32_t b_hi = S::kBmn ? kMnMajorHi : k_major_hi(S::kChunk * 2);
+#pragma unroll
+                        for (int i = 0; i < S::kPairs; ++i) {
+#pragma unroll
+                            for (int s = 0; s < S::kChunk / 16; ++s) {
+                                // 16 entries on: 32 bytes along a row, or 16 rows of 128 bytes
+                                if (s < steps)
+                                    mma_bf16<a_hi, b_hi>(
+                                        d, a + pair_a<PARTS>(S::kPairs, i) * (S::kA / 16) + s * (S::kAmn ? 128 : 2),
+                                        b + pair_b<PARTS>(S::kPairs, i) * (S::kB / 16) + s * (S::kBmn ? 128 : 2), idesc,
+                                        i > 0 || s > 0 ? true : c > 0, on);
+                            }
+                        }
+                        mma_commit(empty + 8 * stage, on);
+                        if (++stage == S::kStages) {
+                            stage = 0;
+                            phase ^= 1;
+                        }
+                    }
+                    if (!ok) break;
+                    mma_commit(taken_full + 8 * buf, on);
+                    buf ^= 1;
+                    if (buf == 0) buf_phase ^= 1;
+                }
+            }
+            if (stop) {
+                mma_commit(drain, on);
+                for (int i = 0; i < kMbarRounds; ++i)
+                    if (mbar_try(drain, 0)) break;
+            }
+        }
+    } else {
+        // Takes tiles out: warp % 4 is the quarter of the rows it can reach,
+        // `half` the 32-column chunks it takes (even or odd ones). After a wait
+        // that gave up the remaining waits fail at once and the block runs to
+        // its end on whatever is there; the error word says so.
+        const int quarter = warp & 3, half = (warp - 2) / 4, et = threadIdx.x - 64;
+        const int in_tile = quarter * 32 + lane;
+        const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+        const bool speaks = quarter == 0 && lane == 0;  // for its half's stores
+        const float c2 = p.scale * kLog2e;
+        int buf = 0, out_buf = 0;
+        uint32_t buf_phase = 0;
+        for (int64_t u = blockIdx.x; u < p.units; u += gridDim.x) {
+            const Walk w = walk_unit<MODE, PARTS>(p, u);
+            const int64_t a_row = w.a_row + in_tile;
+            const bool mine = a_row < p.a_rows;
+            if constexpr (!S::kProduct) {
+                const int64_t row = p.row0 + a_row;
+                const int lab = mine ? p.labels.at(row) : kIgnored;
+                float m = -kInf, s = 0.0f;
+                float lse = kInf, at_label = 0.0f, r = 0.0f;
+                if (MODE == kLogitGrad && lab >= 0) {
+                    r = p.rg.at(row, lab);
+                    lse = p.stats[row];
+                    at_label = -p.stats[p.rows + row] * r;
+                }
+                for (int t = 0; t < w.tiles; ++t) {
+                    const int v0 = (w.first + t) * kN;
+                    const int n = min(kN, p.columns - v0);
+                    // bias times log2 e; classes past the end are taken out
+                    bias_s[buf][et] = et < n ? (p.bias != nullptr ? p.bias[v0 + et] * kLog2e : 0.0f) : -kInf;
+                    named_sync(1, 256);
+                    mbar_wait(taken_full + 8 * buf, buf_phase, &stop, p.error_word, DEV_ERR_TILE_WAIT);
+                    tmem_fence_after();
+                    for (int k = half; k * 32 < n; k += 2) {
+                        float z[32];
+                        tmem_load32(lanes + buf * kN + k * 32, z);
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) {
+                            const float4 b = *reinterpret_cast<const float4*>(&bias_s[buf][k * 32 + j]);
+                            z[j] = fmaf(z[j], c2, b.x);
+                            z[j + 1] = fmaf(z[j + 1], c2, b.y);
+                            z[j + 2] = fmaf(z[j + 2], c2, b.z);
+                            z[j + 3] = fmaf(z[j + 3], c2, b.w);
+                        }
+                        const int rel = lab - v0 - k * 32;
+                        const bool here = (unsigned)rel < 32u;
+                        const bool any = __any_sync(0xffffffffu, here);
+                        if constexpr (MODE == kStats) {
+                            if (any) {
+                                float zl = 0.0f;
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) {
+                                    if (j == rel) {
+                                        zl = z[j];
+                                        z[j] = -kInf;
+                                    }
+                                }
+                                if (here) p.label_z[row] = zl;
+                            }
+                            float top = m;
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) top = fmaxf(top, z[j]);
+                            const float ref = top == -kInf ? 0.0f : top;
+                            float q[4] = {s * exp2_fast(m - ref), 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) q[j % 4] += exp2_fast(z[j] - ref);
+                            s = (q[0] + q[1]) + (q[2] + q[3]);
+                            m = top;
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) z[j] = exp2_fast(z[j] - lse) * r;
+                            if (any) {
+#pragma unroll
+                                for (int j = 0; j < 32; ++j)
+                                    if (j == rel) z[j] = at_label;
+                            }
+                            // staging is free again once the store before last has read it
+                            const uint32_t stage0 = base + S::kStages * S::kStage +
+                                                    (half * S::kOutBuffers + out_buf) * (PARTS * kM * 64);
+                            if (speaks) tma_store_wait_read<S::kOutBuffers - 1>();
+                            named_sync(2 + half, 128);
+                            const uint32_t line = stage0 + in_tile * 64;
+#pragma unroll
+                            for (int g = 0; g < 4; ++g) {
+                                const uint32_t at = line + ((g ^ ((in_tile >> 1) & 3)) * 16);
+                                __nv_bfloat16 o[PARTS][8];
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) {
+                                    __nv_bfloat16 q[PARTS];
+                                    split_parts<PARTS>(z[8 * g + j], q);
+#pragma unroll
+                                    for (int i = 0; i < PARTS; ++i) o[i][j] = q[i];
+                                }
+#pragma unroll
+                                for (int i = 0; i < PARTS; ++i) {
+                                    uint4 v;
+                                    memcpy(&v, o[i], 16);
+                                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + i * kM * 64),
+                                                 "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                                                 : "memory");
+                                }
+                            }
+                            fence_async_shared();
+                            named_sync(2 + half, 128);
+                            if (speaks) {
+#pragma unroll
+                                for (int i = 0; i < PARTS; ++i)
+                                    tma_store(&map_out, v0 + k * 32, (int)w.a_row, i, stage0 + i * kM * 64);
+                                tma_store_commit();
+                            }
+                            if (++out_buf == S::kOutBuffers) out_buf = 0;
+                            if (p.part_bias != nullptr) {
+                                // lane c ends with the sum of column c over the warp's 32 rows
+#pragma unroll
+                                for (int o = 16; o > 0; o >>= 1) {
+#pragma unroll
+                                    for (int j = 0; j < o; ++j) {
+                                        const bool up = (lane & o) != 0;
+                                        const float send = up ? z[j] : z[j + o];
+                                        const float keep = up ? z[j + o] : z[j];
+                                        z[j] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+                                    }
+                                }
+                                const int v = v0 + k * 32 + lane;
+                                const int64_t line32 = w.a_row / 32 + quarter;
+                                if (v < p.columns) p.part_bias[line32 * p.columns + v] = z[0];
+                            }
+                        }
+                    }
+                    tmem_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(taken_empty + 8 * buf);
+                    buf ^= 1;
+                    if (buf == 0) buf_phase ^= 1;
+                }
+                if (MODE == kStats && mine) {
+                    const int64_t at = (int64_t)(w.split * 2 + half) * p.rows + row;
+                    p.part_m[at] = m;
+                    p.part_s[at] = s;
+                }
+            } else {
+                const int d0 = w.first * kN;
+                const int n = min(kN, p.columns - d0);
+                float acc[4][32];
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) acc[q][j] = 0.0f;
+                for (int t = 0; t < w.tiles; ++t) {
+                    mbar_wait(taken_full + 8 * buf, buf_phase, &stop, p.error_word, DEV_ERR_TILE_WAIT);
+                    tmem_fence_after();
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        if ((2 * q + half) * 32 < n) {
+                            float v[32];
+                            tmem_load32(lanes + buf * kN + (2 * q + half) * 32, v);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) acc[q][j] += v[j];
+                        }
+                    }
+                    tmem_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(taken_empty + 8 * buf);
+                    buf ^= 1;
+                    if (buf == 0) buf_phase ^= 1;
+                }
+                if (mine) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int c = d0 + (2 * q + half) * 32;
+                        if (c >= p.columns) continue;
+                        if (p.part != nullptr) {
+                            float* dst = p.part + ((int64_t)w.split * p.a_rows + a_row) * p.part_ld + c;
+#pragma unroll
+                            for (int j = 0; j < 32; j += 4) {
+                                if (c + j >= p.part_ld) continue;
+                                float4* d4 = reinterpret_cast<float4*>(dst + j);
+                                float4 o = make_float4(acc[q][j], acc[q][j + 1], acc[q][j + 2], acc[q][j + 3]);
+                                if (p.add) {
+                                    const float4 e = *d4;
+                                    o.x += e.x;
+                                    o.y += e.y;
+                                    o.z += e.z;
+                                    o.w += e.w;
+                                }
+                                *d4 = o;
+                            }
+                        } else {
+                            const int64_t at = (p.row0 + a_row) * p.columns + c;
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) {
+                                if (c + j >= p.columns) continue;
+                                const float v = acc[q][j] * p.scale;
+                                if (p.out_type == MG_F32) static_cast<float*>(p.out)[at + j] = v;
+                                else if (p.out_type == MG_BF16) static_cast<__nv_bfloat16*>(p.out)[at + j] = from_f32<__nv_bfloat16>(v);
+                                else static_cast<__half*>(p.out)[at + j] = from_f32<__half>(v);
+                            }
+                        }
+                    }
+                }
+            }
+        }
+        if (MODE == kLogitGrad && speaks) tma_store_wait_all();
+    }
+    tmem_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tmem_fence_after();
+        tmem_free(tmem_s, kTmemColumns);
+    }
+}
+
+}  // namespace
+
+}  // namespace mg

@@ -2,6 +2,7 @@
 #pragma once
 
 #include "rows.cuh"
+#include "tensor.cuh"
 
 namespace mg {
 
@@ -39,5 +40,47 @@ struct RowGrad {
         return live != nullptr ? g / fmaxf(live[0], 1.0f) : g;
     }
 };
+
+constexpr float kInf = __builtin_huge_valf();
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// --------------------------------------------------------------------- parts
+
+// The number of bf16 parts of a type.
+template <typename T>
+constexpr int kPartsOf = sizeof(T) == 4 ? 3 : 2;
+template <>
+constexpr int kPartsOf<__nv_bfloat16> = 1;
+
+template <int PARTS>
+__device__ __forceinline__ void split_parts(float v, __nv_bfloat16 (&p)[PARTS]) {
+    p[0] = __float2bfloat16_rn(v);
+#pragma unroll
+    for (int i = 1; i < PARTS; ++i) {
+        v -= __bfloat162float(p[i - 1]);
+        p[i] = __float2bfloat16_rn(v);
+    }
+}
+
+// Products of parts (a, b), smallest first: of the 1, 3, 4 or 6 pairs that
+// matter at PARTS parts, the i-th.
+template <int PARTS>
+__device__ constexpr int pair_a(int pairs, int i) {
+    if (PARTS == 1) return 0;
+    if (PARTS == 2) return (i + 4 - pairs) == 0 || (i + 4 - pairs) == 1 ? 1 : 0;
+    return i == 0 ? 2 : i == 1 || i == 3 ? 1 : 0;
+}
+template <int PARTS>
+__device__ constexpr int pair_b(int pairs, int i) {
+    if (PARTS == 1) return 0;
+    if (PARTS == 2) return (i + 4 - pairs) == 0 || (i + 4 - pairs) == 2 ? 1 : 0;
+    return i == 2 ? 2 : i == 1 || i == 4 ? 1 : 0;
+}
 
 }  // namespace mg

@@ -18,9 +18,26 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) {
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
-__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
-                 : "memory");
+// The copying and the issuing warp run their loops with all lanes, so that
+// addresses and descriptors stay in uniform registers, and one lane (`on`)
+// executes the instruction. A product's operands come from uniform registers:
+// moving them there from a lane's takes 50 to 210 cycles a product, where 64
+// columns keep the tensor core for 32 (measured, 128 x n x 16).
+__device__ __forceinline__ uint32_t elect_lane() {
+    uint32_t on;
+    asm volatile(
+        "{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}"
+        : "=r"(on));
+    return on;
+}
+// v, the same in all lanes, as a uniform register.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __reduce_or_sync(0xffffffffu, v); }
+__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes, uint32_t on) {
+    asm volatile(
+        "{\n.reg .pred q;\nsetp.ne.u32 q, %2, 0;\n"
+        "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n}" ::"r"(bar),
+        "r"(bytes), "r"(on)
+        : "memory");
 }
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -52,14 +69,21 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     return false;
 }
 
+// The same for a whole warp, which agrees on the answer (and stays in step).
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* stop,
+                                               int32_t* error_word, int32_t code) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, stop, error_word, code));
+}
+
 // ------------------------------------------------------------------------ TMA
 
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, int z,
-                                         uint32_t bar) {
+                                         uint32_t bar, uint32_t on) {
     asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-        "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        "{\n.reg .pred q;\nsetp.ne.u32 q, %6, 0;\n"
+        "@q cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4}], [%5];\n}" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar), "r"(on)
         : "memory");
 }
 __device__ __forceinline__ void tma_store(const CUtensorMap* map, int x, int y, int z, uint32_t src) {
@@ -92,6 +116,9 @@ __device__ __forceinline__ void tmem_alloc(uint32_t dst_smem, uint32_t columns) 
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
 }
+// A block that asks for all 512 columns has them from address 0 on.
+constexpr uint32_t kTmemColumns = 512;
+constexpr uint32_t kTmemBase = 0;
 __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t columns) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(columns)
                  : "memory");
@@ -123,19 +150,37 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
 }
 
 // D (fp32, tensor memory) = or += A B, one step of 16 along the contraction;
-// A and B are bf16 tiles in shared memory behind their descriptors.
-__device__ __forceinline__ void mma_bf16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                         bool add) {
+// A and B are bf16 tiles in shared memory behind their descriptors, given as
+// the low word (address and block stride) and the constant high word.
+template <uint32_t A_HI, uint32_t B_HI>
+__device__ __forceinline__ void mma_bf16(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc,
+                                         bool add, uint32_t on) {
     asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        "{\n.reg .pred p, q;\n.reg .b64 da, db;\nsetp.ne.u32 p, %4, 0;\nsetp.ne.u32 q, %5, 0;\n"
+        "mov.b64 da, {%1, %6};\nmov.b64 db, {%2, %7};\n"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)add), "r"(on), "n"(A_HI), "n"(B_HI)
+        : "memory");
+}
+// The same with A in tensor memory: row i in lane i, two contraction entries
+// to a 32-bit column.
+template <uint32_t B_HI>
+__device__ __forceinline__ void mma_bf16_ta(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc,
+                                            bool add, uint32_t on) {
+    asm volatile(
+        "{\n.reg .pred p, q;\n.reg .b64 db;\nsetp.ne.u32 p, %4, 0;\nsetp.ne.u32 q, %5, 0;\n"
+        "mov.b64 db, {%2, %6};\n"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)add), "r"(on), "n"(B_HI)
         : "memory");
 }
 // The barrier gets an arrival when every product issued so far is done.
-__device__ __forceinline__ void mma_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
-                 : "memory");
+__device__ __forceinline__ void mma_commit(uint32_t bar, uint32_t on) {
+    asm volatile(
+        "{\n.reg .pred q;\nsetp.ne.u32 q, %1, 0;\n"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(bar),
+        "r"(on)
+        : "memory");
 }
 
 // bf16 x bf16 -> fp32, 128 rows by n columns; *_mn: the operand is stored with
@@ -145,18 +190,19 @@ __device__ __forceinline__ uint32_t mma_idesc(int n, bool a_mn, bool b_mn) {
            ((uint32_t)(n >> 3) << 17) | (8u << 24);
 }
 
-// A tile whose contraction index runs fastest, `bytes` (128 or 64) to a row:
-// groups of 8 rows follow one another.
-__device__ __forceinline__ uint64_t desc_k_major(uint32_t addr, int bytes) {
-    return (uint64_t)((addr & 0x3ffffu) >> 4) | ((uint64_t)1 << 16) |
-           ((uint64_t)(8 * bytes / 16) << 32) | ((uint64_t)1 << 46) |
-           ((uint64_t)(bytes == 128 ? 2 : 4) << 61);
+// Descriptors. A tile whose contraction index runs fastest, `bytes` (128 or
+// 64) to a row: groups of 8 rows follow one another.
+__host__ __device__ constexpr uint32_t k_major_hi(int bytes) {
+    return (uint32_t)(8 * bytes / 16) | 1u << 14 | (bytes == 128 ? 2u : 4u) << 29;
 }
-// A tile whose row index runs fastest: blocks of 64 rows (128 bytes) by `depth`
-// contraction steps, block_bytes from one block of rows to the next.
-__device__ __forceinline__ uint64_t desc_mn_major(uint32_t addr, int block_bytes) {
-    return (uint64_t)((addr & 0x3ffffu) >> 4) | ((uint64_t)(block_bytes / 16) << 16) |
-           ((uint64_t)(1024 / 16) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+__device__ __forceinline__ uint32_t k_major_lo(uint32_t addr) {
+    return ((addr & 0x3ffffu) >> 4) | 1u << 16;
+}
+// A tile whose row index runs fastest: blocks of 64 rows (128 bytes) by the
+// contraction, block_bytes from one block of rows to the next.
+constexpr uint32_t kMnMajorHi = (1024u / 16) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t mn_major_lo(uint32_t addr, int block_bytes) {
+    return ((addr & 0x3ffffu) >> 4) | (uint32_t)(block_bytes / 16) << 16;
 }
 
 // ----------------------------------------------------------------------- host
