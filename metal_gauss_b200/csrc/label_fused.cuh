@@ -26,9 +26,9 @@ namespace {
 
 constexpr int kOwn = 128;
 constexpr int kStream = 64;
-constexpr int kFusedThreads = 576;  // copy, issue, 2 x 4 score warps, 8 warps for acc
+constexpr int kFusedThreads = 608;  // copy, issue, 2 x 4 score warps, 8 warps for acc, issue
 constexpr int kFusedStages = 8;     // at most
-constexpr int kFusedShared = 222 * 1024;  // of it 1 KB to align; 5 KB are static
+constexpr int kFusedShared = 226 * 1024;  // of it 1 KB to align
 
 // Parts of G: two also for bf16 features, whose gradients then carry no other
 // rounding than their own (one part would add its 2^-9 to theirs).
@@ -71,16 +71,19 @@ struct FusedArgs {
     int chunks;            // of 64 channels
     int stages, own_buffers, acc_buffers;
     float scale;
-    const float* bias;
-    LabelSource labels;
-    RowGrad rg;
-    const float* stats;
+    const float* row_values;   // kRowValues per row, in blocks of 64 rows
+    const float* class_bias;   // bias times log2 e, -infinity past the last class
     float* part_bias;      // by class: (splits, 2, classes), or NULL
     float* part;           // fp32 shares (splits, own, part_ld), or NULL
     int part_ld;
     void* out;             // the result itself
     int32_t* error_word;
 };
+
+// What the scores need of a row: log2 of its sum, r, G at its label, its label
+// (an int), each 64 in a row per block of 64 rows.
+constexpr int kRowValues = 4;
+constexpr int kColumnBytes = kRowValues * kStream * 4;  // of a streamed tile, beside its parts
 
 struct FusedWalk {
     int64_t own0, t0, t1;
@@ -120,6 +123,28 @@ __device__ __forceinline__ void tmem_store_wait() {
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
+// `bytes` (a multiple of 16) from global to shared memory.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes,
+                                          uint32_t bar, uint32_t on) {
+    asm volatile(
+        "{\n.reg .pred q;\nsetp.ne.u32 q, %4, 0;\n"
+        "@q cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n}" ::"r"(dst),
+        "l"(src), "r"(bytes), "r"(bar), "r"(on)
+        : "memory");
+}
+__device__ __forceinline__ float4 shared_float4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ int shared_int(uint32_t addr) {
+    int v;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr));
+    return v;
+}
+
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     uint32_t r;
@@ -154,16 +179,15 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
     constexpr int kOwnChunk = kOwn * 128, kStreamChunk = kStream * 128;  // 64 channels, bytes
     constexpr uint32_t kGBase = 2 * kStream, kAccBase = kGBase + 2 * GP * (kStream / 2);
     extern __shared__ uint8_t dynamic[];
-    // per group and of two tiles in turn: bias (by row), or the rows' values (by class)
-    __shared__ alignas(16) float col_a[2][2][kStream], col_b[2][2][kStream], col_c[2][2][kStream];
-    __shared__ alignas(16) int col_l[2][2][kStream];
-    __shared__ uint64_t bars[2 * kFusedStages + 17];
+    __shared__ uint64_t bars[2 * kFusedStages + 18];
     __shared__ uint32_t tmem_s;
     __shared__ volatile int stop;
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x / 32, 0), lane = threadIdx.x % 32;
     const uint32_t base = (smem_u32(dynamic) + 1023u) & ~1023u;
     const uint32_t own_bytes = PARTS * p.chunks * kOwnChunk;
-    const uint32_t stage_bytes = PARTS * p.chunks * kStreamChunk;
+    const uint32_t tile_bytes = PARTS * p.chunks * kStreamChunk;
+    const uint32_t stage_bytes = tile_bytes + kColumnBytes;  // parts, then the columns' values
+    constexpr uint32_t column_bytes = BY_CLASS ? kColumnBytes : kStream * 4;
     const uint32_t stream0 = base + p.own_buffers * own_bytes;
     const uint32_t full = smem_u32(bars), empty = full + 8 * kFusedStages;
     const uint32_t own_full = empty + 8 * kFusedStages, own_empty = own_full + 16;
@@ -188,6 +212,7 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
             mbar_init(acc_empty + 8 * i, 8);
         }
         mbar_init(drain, 1);
+        mbar_init(drain + 8, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_shared();
         stop = 0;
@@ -229,7 +254,10 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
                 for (int64_t t = w.t0; t < w.t1; ++t) {
                     ok = wait_warp(empty + 8 * stage, phase ^ 1);
                     if (!ok) break;
-                    mbar_expect(full + 8 * stage, stage_bytes, on);
+                    mbar_expect(full + 8 * stage, tile_bytes + column_bytes, on);
+                    bulk_load(stream0 + stage * stage_bytes + tile_bytes,
+                              (BY_CLASS ? p.row_values : p.class_bias) + t * (column_bytes / 4), column_bytes,
+                              full + 8 * stage, on);
                     for (int i = 0; i < PARTS; ++i)
                         for (int c = 0; c < p.chunks; ++c)
                             tma_load(stream0 + stage * stage_bytes + (i * p.chunks + c) * kStreamChunk,
@@ -261,44 +289,91 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
             }
         }
     } else if (warp == 1) {
-        {  // issues products
-            const uint32_t on = elect_lane();
-            // the scores of a tile go before the G product of the tile `ahead`
-            // before it, so that a group finds its next scores ready when it
-            // hands over G (two ahead against one: 2438 -> @@ cycles a tile,
-            // bf16, 16 channels); two take three streamed tiles
-            const uint32_t idesc_s = mma_idesc(kStream, false, false);
-            const int n = (p.channels + 15) / 16 * 16;
-            const uint32_t idesc_g = uniform(mma_idesc(n, false, true));
-            int stage = 0, ob = 0, ab = 0;
-            uint32_t phase = 0, ob_phase = 0, ab_phase = 0;
-            int64_t i = 0;         // tiles whose scores are issued
-            int in_segment = 0;    // G products in acc
-            const int ahead = p.stages > 2 ? 2 : 1;
-            int stage1 = 0, stage2 = 0;          // of the last tile and the one before
-            bool ends1 = false, ends2 = false, ok = true;
-            // the G product of a tile; `ends`: acc is complete after it
-            const auto product = [&](int64_t tile, int st, bool ends) {
-                const int g = (int)(tile & 1);
-                if (!wait_warp(g_full + 8 * g, (uint32_t)(tile >> 1) & 1)) return false;
-                if (in_segment == 0 && !wait_warp(acc_empty + 8 * ab, ab_phase ^ 1)) return false;
+        // Issues the scores. They run ahead of the G products, which have a warp
+        // of their own (the last): one issuing warp for both was what a tile of
+        // few channels took (1750 cycles a tile, bf16).
+        const uint32_t on = elect_lane();
+        const uint32_t idesc = mma_idesc(kStream, false, false);
+        const uint32_t a_part = uniform(p.chunks * kOwnChunk / 16);
+        const uint32_t b_part = uniform(p.chunks * kStreamChunk / 16);
+        int stage = 0, ob = 0, g = 0;
+        uint32_t phase = 0, ob_phase = 0, g_phase = 0;
+        bool ok = true;
+        for (int64_t u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
+            const FusedWalk w = fused_unit(p, u);
+            const int tiles = (int)uniform((uint32_t)(w.t1 - w.t0));
+            ok = wait_warp(own_full + 8 * ob, ob_phase);
+            const uint32_t a0 = uniform(k_major_lo(base + ob * own_bytes));
+            for (int t = 0; ok && t < tiles; ++t) {
+                ok = wait_warp(full + 8 * stage, phase) && wait_warp(s_empty + 8 * g, g_phase ^ 1);
+                if (!ok) break;
+                tmem_fence_after();
+                const uint32_t b0 = uniform(k_major_lo(stream0 + stage * stage_bytes));
+                const uint32_t d = uniform(tmem + g * kStream);
+                for (int c = 0; c < p.chunks; ++c) {
+                    const uint32_t a1 = a0 + c * (kOwnChunk / 16), b1 = b0 + c * (kStreamChunk / 16);
+#pragma unroll
+                    for (int q = 0; q < kScorePairs; ++q) {
+#pragma unroll
+                        for (int s = 0; s < 4; ++s)
+                            if (64 * c + 16 * s < p.channels)
+                                mma_bf16<k_major_hi(128), k_major_hi(128)>(
+                                    d, a1 + pair_a<PARTS>(kScorePairs, q) * a_part + 2 * s,
+                                    b1 + pair_b<PARTS>(kScorePairs, q) * b_part + 2 * s, idesc,
+                                    q > 0 || s > 0 ? true : c > 0, on);
+                    }
+                }
+                mma_commit(s_full + 8 * g, on);
+                if (++stage == p.stages) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+                g ^= 1;
+                if (g == 0) g_phase ^= 1;
+            }
+            mma_commit(own_empty + 8 * ob, on);
+            if (++ob == p.own_buffers) {
+                ob = 0;
+                ob_phase ^= 1;
+            }
+        }
+        if (stop) {
+            mma_commit(drain, on);
+            for (int k = 0; k < kMbarRounds; ++k)
+                if (mbar_try(drain, 0)) break;
+        }
+    } else if (warp == kFusedThreads / 32 - 1) {
+        // issues the G products
+        const uint32_t on = elect_lane();
+        const int n = (p.channels + 15) / 16 * 16;
+        const uint32_t idesc = uniform(mma_idesc(n, false, true));
+        const uint32_t part = uniform(p.chunks * kStreamChunk / 16);
+        int stage = 0, ab = 0, g = 0;
+        uint32_t g_phase = 0, ab_phase = 0;
+        bool ok = true;
+        for (int64_t u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
+            const FusedWalk w = fused_unit(p, u);
+            const int tiles = (int)uniform((uint32_t)(w.t1 - w.t0));
+            int in_segment = 0;  // G products in acc
+            for (int t = 0; ok && t < tiles; ++t) {
+                ok = wait_warp(g_full + 8 * g, g_phase);
+                if (ok && in_segment == 0) ok = wait_warp(acc_empty + 8 * ab, ab_phase ^ 1);
+                if (!ok) break;
                 tmem_fence_after();
                 const uint32_t d = uniform(tmem + kAccBase + ab * n);
                 const uint32_t a0 = uniform(tmem + kGBase + g * (GP * (kStream / 2)));
-                const uint32_t b0 = uniform(mn_major_lo(stream0 + st * stage_bytes, kStreamChunk));
-                const uint32_t part = uniform(p.chunks * kStreamChunk / 16);
-                const uint32_t more = uniform(in_segment > 0);
+                const uint32_t b0 = uniform(mn_major_lo(stream0 + stage * stage_bytes, kStreamChunk));
 #pragma unroll
                 for (int q = 0; q < g_pairs<PARTS>(); ++q) {
 #pragma unroll
                     for (int s = 0; s < kStream / 16; ++s)
                         mma_bf16_ta<kMnMajorHi>(d, a0 + g_pair_a<PARTS>(q) * (kStream / 2) + 8 * s,
-                                                b0 + g_pair_b<PARTS>(q) * part + 128 * s, idesc_g,
-                                                q > 0 || s > 0 ? true : more != 0, on);
+                                                b0 + g_pair_b<PARTS>(q) * part + 128 * s, idesc,
+                                                q > 0 || s > 0 ? true : in_segment > 0, on);
                 }
-                mma_commit(empty + 8 * st, on);
                 mma_commit(g_empty + 8 * g, on);
-                if (++in_segment == p.per_segment || ends) {
+                mma_commit(empty + 8 * stage, on);
+                if (++in_segment == p.per_segment || t + 1 == tiles) {
                     mma_commit(acc_full + 8 * ab, on);
                     in_segment = 0;
                     if (++ab == p.acc_buffers) {
@@ -306,103 +381,53 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
                         ab_phase ^= 1;
                     }
                 }
-                return true;
-            };
-            for (int64_t u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
-                const FusedWalk w = fused_unit(p, u);
-                ok = wait_warp(own_full + 8 * ob, ob_phase);
-                for (int64_t t = w.t0; ok && t < w.t1; ++t) {
-                    const int g = (int)(i & 1);
-                    ok = wait_warp(full + 8 * stage, phase) && wait_warp(s_empty + 8 * g, ((uint32_t)(i >> 1) & 1) ^ 1);
-                    if (!ok) break;
-                    tmem_fence_after();
-                    const uint32_t d = uniform(tmem + g * kStream);
-                    const uint32_t a0 = uniform(k_major_lo(base + ob * own_bytes));
-                    const uint32_t b0 = uniform(k_major_lo(stream0 + stage * stage_bytes));
-                    const uint32_t a_part = uniform(p.chunks * kOwnChunk / 16);
-                    const uint32_t b_part = uniform(p.chunks * kStreamChunk / 16);
-                    for (int c = 0; c < p.chunks; ++c) {
-                        const uint32_t a1 = uniform(a0 + c * (kOwnChunk / 16)), b1 = uniform(b0 + c * (kStreamChunk / 16));
-#pragma unroll
-                        for (int q = 0; q < kScorePairs; ++q) {
-#pragma unroll
-                            for (int s = 0; s < 4; ++s)
-                                if (64 * c + 16 * s < p.channels)
-                                    mma_bf16<k_major_hi(128), k_major_hi(128)>(
-                                        d, a1 + pair_a<PARTS>(kScorePairs, q) * a_part + 2 * s,
-                                        b1 + pair_b<PARTS>(kScorePairs, q) * b_part + 2 * s, idesc_s,
-                                        q > 0 || s > 0 ? true : c > 0, on);
-                        }
-                    }
-                    mma_commit(s_full + 8 * g, on);
-                    if (t + 1 == w.t1) mma_commit(own_empty + 8 * ob, on);
-                    if (i >= ahead) ok = ahead == 2 ? product(i - 2, stage2, ends2) : product(i - 1, stage1, ends1);
-                    stage2 = stage1;
-                    ends2 = ends1;
-                    stage1 = stage;
-                    ends1 = t + 1 == w.t1;
-                    ++i;
-                    if (++stage == p.stages) {
-                        stage = 0;
-                        phase ^= 1;
-                    }
-                }
-                if (++ob == p.own_buffers) {
-                    ob = 0;
-                    ob_phase ^= 1;
-                }
+                if (++stage == p.stages) stage = 0;
+                g ^= 1;
+                if (g == 0) g_phase ^= 1;
             }
-            if (ok && ahead == 2 && i > 1) ok = product(i - 2, stage2, ends2);
-            if (ok && i > 0) product(i - 1, stage1, ends1);
-            if (stop) {
-                mma_commit(drain, on);
-                for (int k = 0; k < kMbarRounds; ++k)
-                    if (mbar_try(drain, 0)) break;
-            }
+        }
+        if (stop) {
+            mma_commit(drain + 8, on);
+            for (int k = 0; k < kMbarRounds; ++k)
+                if (mbar_try(drain + 8, 0)) break;
         }
     } else if (warp < 10) {
         // Scores to G: group g takes every other tile. After a wait that gave
         // up the rest fail at once and the block runs out on what is there.
         const int g = (warp - 2) / 4, quarter = warp & 3, in_tile = quarter * 32 + lane;
-        const int gt = (threadIdx.x - 64) & 127;  // thread of the group
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         const uint32_t s_addr = tmem + lanes + g * kStream;
         const uint32_t g_addr = tmem + lanes + kGBase + g * (GP * (kStream / 2));
         const float c2 = p.scale * kLog2e;
         int64_t i = 0;
-        int buf = 0;
-        uint32_t phase = 0;
+        int stage = 0;
+        uint32_t phase = 0, stage_phase = 0;
         for (int64_t u = blockIdx.x; u < p.units; u += gridDim.x) {
             const FusedWalk w = fused_unit(p, u);
             const int64_t own = w.own0 + in_tile;
             int lab = kIgnored;
             float lse = kInf, r = 0.0f, at_label = 0.0f, own_bias = 0.0f, bias_sum = 0.0f;
-            if constexpr (BY_CLASS) {
-                if (p.bias != nullptr && own < p.own) own_bias = p.bias[own] * kLog2e;
-            } else if (own < p.own) {
-                lab = p.labels.at(own);
-                if (lab >= 0) {
-                    r = p.rg.at(own, lab);
-                    lse = p.stats[own];
-                    at_label = -p.stats[p.rows + own] * r;
+            if (own < p.own) {
+                if constexpr (BY_CLASS) {
+                    own_bias = p.class_bias[own];
+                } else {
+                    const float* v = p.row_values + own / kStream * (kRowValues * kStream) + own % kStream;
+                    lse = v[0];
+                    r = v[kStream];
+                    at_label = v[2 * kStream];
+                    lab = __float_as_int(v[3 * kStream]);
                 }
             }
             for (int64_t t = w.t0; t < w.t1; ++t, ++i) {
-                if ((int)(i & 1) != g) continue;
-                if (gt < kStream) {
-                    const int64_t j = t * kStream + gt;
-                    if constexpr (BY_CLASS) {
-                        const int l = j < p.rows ? p.labels.at(j) : kIgnored;
-                        const float rj = p.rg.at(j < p.rows ? j : 0, l);
-                        col_l[g][buf][gt] = l;
-                        col_a[g][buf][gt] = l >= 0 ? p.stats[j] : kInf;
-                        col_b[g][buf][gt] = rj;
-                        col_c[g][buf][gt] = l >= 0 ? -p.stats[p.rows + j] * rj : 0.0f;
-                    } else {
-                        col_a[g][buf][gt] = j < p.classes ? (p.bias != nullptr ? p.bias[j] * kLog2e : 0.0f) : -kInf;
-                    }
+                const int at = stage;
+                const uint32_t at_phase = stage_phase;
+                if (++stage == p.stages) {
+                    stage = 0;
+                    stage_phase ^= 1;
                 }
-                named_sync(2 + g, 128);
+                if ((int)(i & 1) != g) continue;
+                const uint32_t col = stream0 + at * stage_bytes + tile_bytes;
+                wait(full + 8 * at, at_phase);  // the columns' values
                 wait(s_full + 8 * g, phase);
                 tmem_fence_after();
                 // 16 columns at a time in a loop that is not unrolled: its code has
@@ -420,19 +445,20 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
                     if constexpr (BY_CLASS) {
 #pragma unroll
                         for (int j = 0; j < 16; j += 4) {
-                            const float4 a = *reinterpret_cast<const float4*>(&col_a[g][buf][k + j]);
-                            const float4 b = *reinterpret_cast<const float4*>(&col_b[g][buf][k + j]);
+                            const float4 a = shared_float4(col + 4 * (k + j));
+                            const float4 b = shared_float4(col + 4 * (kStream + k + j));
                             z[j] = exp2_fast(fmaf(z[j], c2, own_bias) - a.x) * b.x;
                             z[j + 1] = exp2_fast(fmaf(z[j + 1], c2, own_bias) - a.y) * b.y;
                             z[j + 2] = exp2_fast(fmaf(z[j + 2], c2, own_bias) - a.z) * b.z;
                             z[j + 3] = exp2_fast(fmaf(z[j + 3], c2, own_bias) - a.w) * b.w;
                         }
                         // rows labelled with one of this warp's classes
-                        const int mine = col_l[g][buf][k + (lane & 15)] - (int)w.own0 - quarter * 32;
+                        const int mine = shared_int(col + 4 * (3 * kStream + k + (lane & 15))) - (int)w.own0 - quarter * 32;
                         if (__any_sync(0xffffffffu, (unsigned)mine < 32u)) {
 #pragma unroll
                             for (int j = 0; j < 16; ++j)
-                                if (col_l[g][buf][k + j] == (int)own) z[j] = col_c[g][buf][k + j];
+                                if (shared_int(col + 4 * (3 * kStream + k + j)) == (int)own)
+                                    z[j] = __int_as_float(shared_int(col + 4 * (2 * kStream + k + j)));
                         }
                         if (p.part_bias != nullptr) {
                             float q[4] = {bias_sum, 0.0f, 0.0f, 0.0f};
@@ -443,7 +469,7 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
                     } else {
 #pragma unroll
                         for (int j = 0; j < 16; j += 4) {
-                            const float4 b = *reinterpret_cast<const float4*>(&col_a[g][buf][k + j]);
+                            const float4 b = shared_float4(col + 4 * (k + j));
                             z[j] = exp2_fast(fmaf(z[j], c2, b.x) - lse) * r;
                             z[j + 1] = exp2_fast(fmaf(z[j + 1], c2, b.y) - lse) * r;
                             z[j + 2] = exp2_fast(fmaf(z[j + 2], c2, b.z) - lse) * r;
@@ -467,7 +493,6 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
                 tmem_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(g_full + 8 * g);
-                buf ^= 1;
                 phase ^= 1;
             }
             if (BY_CLASS && p.part_bias != nullptr && own < p.own)
@@ -578,14 +603,15 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
 inline bool fused_fits(int parts, int channels) {
     const int chunks = (channels + 63) / 64, n = (channels + 15) / 16 * 16;
     const int g_parts = parts == 1 ? 2 : parts;
-    return parts * chunks * (kOwn * 128 + 2 * kStream * 128) <= kFusedShared - 1024 &&
+    return parts * chunks * (kOwn * 128 + 2 * kStream * 128) + 2 * kColumnBytes <= kFusedShared - 1024 &&
            2 * kStream + g_parts * kStream + n <= 512;
 }
 
 // Buffers for what is left: a second one for the owning side if four streamed
 // tiles fit beside it, then streamed tiles.
 inline void fused_buffers(FusedArgs& p, int parts) {
-    const int own = parts * p.chunks * kOwn * 128, stage = parts * p.chunks * kStream * 128;
+    const int own = parts * p.chunks * kOwn * 128;
+    const int stage = parts * p.chunks * kStream * 128 + kColumnBytes;
     const int room = kFusedShared - 1024, n = (p.channels + 15) / 16 * 16;
     p.own_buffers = 2 * own + 4 * stage <= room ? 2 : 1;
     p.stages = std::min(kFusedStages, (room - p.own_buffers * own) / stage);

@@ -37,18 +37,44 @@ namespace mg {
 
 namespace {
 
+// What the backward pass's scores need beside the parts (label_fused.cuh).
+struct ColumnValues {
+    RowGrad rg;
+    const float* stats;
+    const float* bias;
+    float* row_values;  // NULL in the forward pass
+    float* class_bias;
+};
+
 // Features (live rows) and embeddings as (row, part, depth) bf16, depth the
 // channels rounded up to 8 with zeros. One thread: 8 channels of one row.
 template <typename T>
 __global__ void __launch_bounds__(256)
 split_kernel(const T* __restrict__ x, const T* __restrict__ w, LabelSource labels, int64_t rows,
-             int classes, int channels, int depth, __nv_bfloat16* __restrict__ xs,
+             int classes, int channels, int depth, ColumnValues cv, __nv_bfloat16* __restrict__ xs,
              __nv_bfloat16* __restrict__ ws) {
     constexpr int PARTS = kPartsOf<T>;
     const int groups = depth / 8;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int64_t all = i / groups;
     const int c = (int)(i - all * groups) * 8;
+    if (cv.row_values != nullptr && i < (rows + kStream - 1) / kStream * kStream) {
+        float v[kRowValues] = {kInf, 0.0f, 0.0f, __int_as_float(kIgnored)};
+        if (i < rows) {
+            const int lab = labels.at(i);
+            if (lab >= 0) {
+                v[0] = cv.stats[i];
+                v[1] = cv.rg.at(i, lab);
+                v[2] = -cv.stats[rows + i] * v[1];
+                v[3] = __int_as_float(lab);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kRowValues; ++k)
+            cv.row_values[i / kStream * (kRowValues * kStream) + k * kStream + i % kStream] = v[k];
+    }
+    if (cv.class_bias != nullptr && i < (classes + kOwn - 1) / kOwn * kOwn)
+        cv.class_bias[i] = i < classes ? (cv.bias != nullptr ? cv.bias[i] * kLog2e : 0.0f) : -kInf;
     if (all >= rows + classes) return;
     const bool feature = all < rows;
     const int64_t row = feature ? all : all - rows;
@@ -299,7 +325,7 @@ struct ForwardScratch {
 
 struct BackwardScratch {
     __nv_bfloat16 *xs, *ws, *g;
-    float *row_part, *class_part, *bias_part, *bias_part2;
+    float *row_values, *class_bias, *row_part, *class_part, *bias_part, *bias_part2;
     size_t bytes;
     BackwardScratch(void* base, const Sizes& n) {
         Scratch a{static_cast<char*>(base)};
@@ -308,11 +334,14 @@ struct BackwardScratch {
         if (n.fused()) {
             const Shares rs = n.fused_by_row(), cs = n.fused_by_class();
             g = nullptr;
+            row_values = a.take<float>((size_t)up(n.rows, kStream) * kStream * kRowValues);
+            class_bias = a.take<float>((size_t)up(n.classes, kOwn) * kOwn);
             row_part = a.take<float>(n.fused_direct() ? 0 : (size_t)rs.splits * n.rows * n.part_ld());
             class_part = a.take<float>((size_t)cs.splits * n.classes * n.part_ld());
             bias_part = a.take<float>((size_t)cs.splits * 2 * n.classes);
             bias_part2 = nullptr;
         } else {
+            row_values = class_bias = nullptr;
             g = a.take<__nv_bfloat16>((size_t)n.piece() * n.parts * n.g_ld());
             const int rs = n.by_row().splits;
             row_part = a.take<float>(rs > 1 ? (size_t)rs * n.piece() * n.part_ld() : 0);
@@ -353,11 +382,14 @@ mg_status launch_tiles(const TileArgs& p, const CUtensorMap& a, const CUtensorMa
 }
 
 template <typename T>
-mg_status split_inputs(const Args& a, __nv_bfloat16* xs, __nv_bfloat16* ws) {
-    const int64_t threads = (a.n.rows + a.n.classes) * (a.n.depth() / 8);
+mg_status split_inputs(const Args& a, __nv_bfloat16* xs, __nv_bfloat16* ws,
+                       const ColumnValues& cv = {}) {
+    // a thread for each 8 channels, and for each of the padded rows and classes
+    const int64_t threads = std::max({(a.n.rows + a.n.classes) * (a.n.depth() / 8),
+                                      up(a.n.rows, kStream) * kStream, up(a.n.classes, kOwn) * kOwn});
     split_kernel<T><<<(unsigned)up(threads, 256), 256, 0, a.st>>>(
         static_cast<const T*>(a.x), static_cast<const T*>(a.w), a.labels, a.n.rows, a.n.classes,
-        a.n.channels, a.n.depth(), xs, ws);
+        a.n.channels, a.n.depth(), cv, xs, ws);
     return check_launch("label_loss split");
 }
 
@@ -448,7 +480,7 @@ mg_status backward_fused(const Args& a, const RowGrad& rg, const float* stats, T
     constexpr int PARTS = kPartsOf<T>;
     const Sizes& n = a.n;
     const BackwardScratch f(scratch, n);
-    MG_TRY((split_inputs<T>(a, f.xs, f.ws)));
+    MG_TRY((split_inputs<T>(a, f.xs, f.ws, ColumnValues{rg, stats, a.bias, f.row_values, f.class_bias})));
     const int64_t part = 2 * (int64_t)n.depth(), row = n.parts * part;
     const auto map = [&](CUtensorMap* m, const __nv_bfloat16* b, int64_t rows, int box) {
         return make_tensor_map(m, b, n.depth(), rows, PARTS, row, part, 64, box, true, "label_loss parts");
@@ -460,10 +492,8 @@ mg_status backward_fused(const Args& a, const RowGrad& rg, const float* stats, T
     p.chunks = (int)up(n.channels, 64);
     p.per_segment = n.fused_segment();
     p.scale = a.scale;
-    p.bias = a.bias;
-    p.labels = a.labels;
-    p.rg = rg;
-    p.stats = stats;
+    p.row_values = f.row_values;
+    p.class_bias = f.class_bias;
     p.part_ld = n.part_ld();
     p.error_word = device_error_word();
     CUtensorMap own, stream;
