@@ -3,7 +3,7 @@
 // A unit owns 128 items of one side (rows for dx, classes for dw) and a share
 // of the other side, which streams past in tiles of 64:
 //   S = own . stream^T       128 x 64, fp32 in tensor memory
-//   G = r (softmax - onehot) from S by one of two groups of four warps, back
+//   G = r (softmax - onehot) from S by one of four groups of four warps, back
 //       into tensor memory as bf16 parts
 //   acc += G stream          128 x channels, G the A operand from tensor memory
 // One streamed tile in shared memory serves both products: its channels are
@@ -26,7 +26,12 @@ namespace {
 
 constexpr int kOwn = 128;
 constexpr int kStream = 64;
-constexpr int kFusedThreads = 608;  // copy, issue, 2 x 4 score warps, 8 warps for acc, issue
+constexpr int kGroups = 4;          // of four warps that turn scores into G
+// copy, issue scores, issue G products, (none); the groups; 8 warps for acc
+constexpr int kFusedThreads = 128 * (1 + kGroups + 2);
+// Registers a thread: 72 at launch; the first four warps give up 32 and the
+// groups 8 each for the acc warps' 32 more: 40 + 4 * 64 + 2 * 104 = 7 * 72.
+constexpr int kIssueRegs = 72, kScoreRegs = 64, kAccRegs = 88;
 constexpr int kFusedStages = 8;     // at most
 constexpr int kFusedShared = 226 * 1024;  // of it 1 KB to align
 
@@ -59,21 +64,20 @@ struct PartsType<3> { using type = float; };
 template <int PARTS>
 using TypeOf = typename PartsType<PARTS>::type;
 
-struct FusedArgs {
-    int64_t units;
-    int64_t own;           // items of the owning side
-    int64_t streamed;      // items of the streaming side
-    int64_t per_split;     // tiles of a share
+struct FusedArgs {         // counts below 2^31: at most 2^30 rows
+    int units;
+    int own;               // items of the owning side
+    int streamed;          // items of the streaming side
+    int per_split;         // tiles of a share
     int splits;
     int per_segment;
-    int64_t rows;
-    int classes, channels;
+    int channels;
     int chunks;            // of 64 channels
     int stages, own_buffers, acc_buffers;
     float scale;
     const float* row_values;   // kRowValues per row, in blocks of 64 rows
     const float* class_bias;   // bias times log2 e, -infinity past the last class
-    float* part_bias;      // by class: (splits, 2, classes), or NULL
+    float* part_bias;      // by class: (splits, kGroups, classes), or NULL
     float* part;           // fp32 shares (splits, own, part_ld), or NULL
     int part_ld;
     void* out;             // the result itself
@@ -86,26 +90,53 @@ constexpr int kRowValues = 4;
 constexpr int kColumnBytes = kRowValues * kStream * 4;  // of a streamed tile, beside its parts
 
 struct FusedWalk {
-    int64_t own0, t0, t1;
-    int split;
+    int own0, t0, t1, split;
 };
 
-__device__ __forceinline__ FusedWalk fused_unit(const FusedArgs& p, int64_t u) {
+template <int N>
+__device__ __forceinline__ void registers_down() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void registers_up() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// Tensor memory of a group: 64 columns of scores, in which G's first two parts
+// take the place of the scores they came from (16 entries of a part are 8
+// columns: part i of entries [16 s, 16 s + 16) at 16 s + 8 i), and 32 columns
+// for a third part.
+template <int PARTS>
+constexpr int kGroupColumns = kStream + (PARTS == 3 ? kStream / 2 : 0);
+__device__ __forceinline__ constexpr int g_column(int part, int entry) {
+    return part < 2 ? entry + 8 * part : kStream + entry / 2;
+}
+
+__device__ __forceinline__ FusedWalk fused_unit(const FusedArgs& p, int u) {
     FusedWalk w;
     w.own0 = u / p.splits * kOwn;
-    w.split = (int)(u % p.splits);
+    w.split = u % p.splits;
     w.t0 = w.split * p.per_split;
     w.t1 = min((p.streamed + kStream - 1) / kStream, w.t0 + p.per_split);
     return w;
 }
 
-__device__ __forceinline__ void tmem_store8(uint32_t addr, const uint32_t (&r)[8]) {
+__device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t (&r)[8]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr),
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
         : "memory");
 }
-__device__ __forceinline__ void tmem_load16(uint32_t addr, float (&v)[16]) {
+__device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+        "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[16]) {
     uint32_t r[16];
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
@@ -119,6 +150,7 @@ __device__ __forceinline__ void tmem_load16(uint32_t addr, float (&v)[16]) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
+__device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32]) { tmem_load32(addr, v); }
 __device__ __forceinline__ void tmem_store_wait() {
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
@@ -152,21 +184,22 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return r;
 }
 
-// 16 values as GP parts, two to a word.
+// kStep values as GP parts, two to a word.
+constexpr int kStep = 16;
 template <int GP>
-__device__ __forceinline__ void store_parts(uint32_t addr, float (&z)[16]) {
+__device__ __forceinline__ void store_parts(uint32_t group, int k, float (&z)[kStep]) {
 #pragma unroll
     for (int i = 0; i < GP; ++i) {
-        uint32_t r[8];
+        uint32_t r[kStep / 2];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < kStep / 2; ++j) {
             r[j] = pack_bf16(z[2 * j], z[2 * j + 1]);
             if (i + 1 < GP) {
                 z[2 * j] -= __uint_as_float(r[j] << 16);
                 z[2 * j + 1] -= __uint_as_float(r[j] & 0xffff0000u);
             }
         }
-        tmem_store8(addr + i * (kStream / 2), r);
+        tmem_store(group + g_column(i, k), r);
     }
 }
 
@@ -177,9 +210,9 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
     constexpr int GP = kGParts<PARTS>;
     constexpr int kScorePairs = PARTS == 1 ? 1 : PARTS == 2 ? 4 : 6;
     constexpr int kOwnChunk = kOwn * 128, kStreamChunk = kStream * 128;  // 64 channels, bytes
-    constexpr uint32_t kGBase = 2 * kStream, kAccBase = kGBase + 2 * GP * (kStream / 2);
+    constexpr uint32_t kAccBase = kGroups * kGroupColumns<PARTS>;
     extern __shared__ uint8_t dynamic[];
-    __shared__ uint64_t bars[2 * kFusedStages + 18];
+    __shared__ uint64_t bars[2 * kFusedStages + 3 * kGroups + 10];
     __shared__ uint32_t tmem_s;
     __shared__ volatile int stop;
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x / 32, 0), lane = threadIdx.x % 32;
@@ -191,9 +224,9 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
     const uint32_t stream0 = base + p.own_buffers * own_bytes;
     const uint32_t full = smem_u32(bars), empty = full + 8 * kFusedStages;
     const uint32_t own_full = empty + 8 * kFusedStages, own_empty = own_full + 16;
-    const uint32_t s_full = own_empty + 16, s_empty = s_full + 16;
-    const uint32_t g_full = s_empty + 16, g_empty = g_full + 16;
-    const uint32_t acc_full = g_empty + 16, acc_empty = acc_full + 16;
+    const uint32_t s_full = own_empty + 16, g_full = s_full + 8 * kGroups;
+    const uint32_t g_empty = g_full + 8 * kGroups;
+    const uint32_t acc_full = g_empty + 8 * kGroups, acc_empty = acc_full + 16;
     const uint32_t drain = acc_empty + 16;
 
     if (threadIdx.x == 0) {
@@ -204,12 +237,13 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
         for (int i = 0; i < 2; ++i) {
             mbar_init(own_full + 8 * i, 1);
             mbar_init(own_empty + 8 * i, 1);
-            mbar_init(s_full + 8 * i, 1);
-            mbar_init(s_empty + 8 * i, 4);
-            mbar_init(g_full + 8 * i, 4);
-            mbar_init(g_empty + 8 * i, 1);
             mbar_init(acc_full + 8 * i, 1);
             mbar_init(acc_empty + 8 * i, 8);
+        }
+        for (int i = 0; i < kGroups; ++i) {
+            mbar_init(s_full + 8 * i, 1);
+            mbar_init(g_full + 8 * i, 4);
+            mbar_init(g_empty + 8 * i, 1);
         }
         mbar_init(drain, 1);
         mbar_init(drain + 8, 1);
@@ -230,14 +264,18 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
         return mbar_wait_warp(bar, parity, &stop, p.error_word, DEV_ERR_TILE_WAIT);
     };
 
+    if (warp < 4) registers_down<kIssueRegs>();
+    else if (warp < 4 + 4 * kGroups) registers_down<kScoreRegs>();
+    else registers_up<kAccRegs>();
+
     if (warp == 0) {
         {  // copies tiles in
             const uint32_t on = elect_lane();
             int stage = 0, ob = 0;
             uint32_t phase = 0, ob_phase = 0;
-            int64_t issued = 0, owns = 0;
+            int issued = 0, owns = 0;  // of the last ring, for a stop
             bool ok = true;
-            for (int64_t u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
+            for (int u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
                 const FusedWalk w = fused_unit(p, u);
                 ok = wait_warp(own_empty + 8 * ob, ob_phase ^ 1);
                 if (!ok) break;
@@ -245,24 +283,24 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
                 for (int i = 0; i < PARTS; ++i)
                     for (int c = 0; c < p.chunks; ++c)
                         tma_load(base + ob * own_bytes + (i * p.chunks + c) * kOwnChunk, &map_own,
-                                 c * 64, (int)w.own0, i, own_full + 8 * ob, on);
-                ++owns;
+                                 c * 64, w.own0, i, own_full + 8 * ob, on);
+                owns = min(owns + 1, p.own_buffers);
                 if (++ob == p.own_buffers) {
                     ob = 0;
                     ob_phase ^= 1;
                 }
-                for (int64_t t = w.t0; t < w.t1; ++t) {
+                for (int t = w.t0; t < w.t1; ++t) {
                     ok = wait_warp(empty + 8 * stage, phase ^ 1);
                     if (!ok) break;
                     mbar_expect(full + 8 * stage, tile_bytes + column_bytes, on);
                     bulk_load(stream0 + stage * stage_bytes + tile_bytes,
-                              (BY_CLASS ? p.row_values : p.class_bias) + t * (column_bytes / 4), column_bytes,
+                              (BY_CLASS ? p.row_values : p.class_bias) + (int64_t)t * (column_bytes / 4), column_bytes,
                               full + 8 * stage, on);
                     for (int i = 0; i < PARTS; ++i)
                         for (int c = 0; c < p.chunks; ++c)
                             tma_load(stream0 + stage * stage_bytes + (i * p.chunks + c) * kStreamChunk,
-                                     &map_stream, c * 64, (int)(t * kStream), i, full + 8 * stage, on);
-                    ++issued;
+                                     &map_stream, c * 64, t * kStream, i, full + 8 * stage, on);
+                    issued = min(issued + 1, p.stages);
                     if (++stage == p.stages) {
                         stage = 0;
                         phase ^= 1;
@@ -270,7 +308,7 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
                 }
             }
             if (stop) {  // this block gave up: its copies in flight land before it ends
-                for (int j = (int)min(issued, (int64_t)p.stages); j > 0; --j) {
+                for (int j = issued; j > 0; --j) {
                     if (--stage < 0) {
                         stage = p.stages - 1;
                         phase ^= 1;
@@ -278,7 +316,7 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
                     for (int i = 0; i < kMbarRounds; ++i)
                         if (mbar_try(full + 8 * stage, phase)) break;
                 }
-                for (int j = (int)min(owns, (int64_t)p.own_buffers); j > 0; --j) {
+                for (int j = owns; j > 0; --j) {
                     if (--ob < 0) {
                         ob = p.own_buffers - 1;
                         ob_phase ^= 1;
@@ -290,8 +328,8 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
         }
     } else if (warp == 1) {
         // Issues the scores. They run ahead of the G products, which have a warp
-        // of their own (the last): one issuing warp for both was what a tile of
-        // few channels took (1750 cycles a tile, bf16).
+        // of their own: one issuing warp for both was what a tile of few channels
+        // took (1750 cycles a tile, bf16).
         const uint32_t on = elect_lane();
         const uint32_t idesc = mma_idesc(kStream, false, false);
         const uint32_t a_part = uniform(p.chunks * kOwnChunk / 16);
@@ -299,17 +337,17 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
         int stage = 0, ob = 0, g = 0;
         uint32_t phase = 0, ob_phase = 0, g_phase = 0;
         bool ok = true;
-        for (int64_t u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
+        for (int u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
             const FusedWalk w = fused_unit(p, u);
             const int tiles = (int)uniform((uint32_t)(w.t1 - w.t0));
             ok = wait_warp(own_full + 8 * ob, ob_phase);
             const uint32_t a0 = uniform(k_major_lo(base + ob * own_bytes));
             for (int t = 0; ok && t < tiles; ++t) {
-                ok = wait_warp(full + 8 * stage, phase) && wait_warp(s_empty + 8 * g, g_phase ^ 1);
+                ok = wait_warp(full + 8 * stage, phase) && wait_warp(g_empty + 8 * g, g_phase ^ 1);
                 if (!ok) break;
                 tmem_fence_after();
                 const uint32_t b0 = uniform(k_major_lo(stream0 + stage * stage_bytes));
-                const uint32_t d = uniform(tmem + g * kStream);
+                const uint32_t d = uniform(tmem + g * kGroupColumns<PARTS>);
                 for (int c = 0; c < p.chunks; ++c) {
                     const uint32_t a1 = a0 + c * (kOwnChunk / 16), b1 = b0 + c * (kStreamChunk / 16);
 #pragma unroll
@@ -328,8 +366,10 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
                     stage = 0;
                     phase ^= 1;
                 }
-                g ^= 1;
-                if (g == 0) g_phase ^= 1;
+                if (++g == kGroups) {
+                    g = 0;
+                    g_phase ^= 1;
+                }
             }
             mma_commit(own_empty + 8 * ob, on);
             if (++ob == p.own_buffers) {
@@ -342,7 +382,7 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
             for (int k = 0; k < kMbarRounds; ++k)
                 if (mbar_try(drain, 0)) break;
         }
-    } else if (warp == kFusedThreads / 32 - 1) {
+    } else if (warp == 2) {
         // issues the G products
         const uint32_t on = elect_lane();
         const int n = (p.channels + 15) / 16 * 16;
@@ -351,7 +391,7 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
         int stage = 0, ab = 0, g = 0;
         uint32_t g_phase = 0, ab_phase = 0;
         bool ok = true;
-        for (int64_t u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
+        for (int u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
             const FusedWalk w = fused_unit(p, u);
             const int tiles = (int)uniform((uint32_t)(w.t1 - w.t0));
             int in_segment = 0;  // G products in acc
@@ -361,13 +401,13 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
                 if (!ok) break;
                 tmem_fence_after();
                 const uint32_t d = uniform(tmem + kAccBase + ab * n);
-                const uint32_t a0 = uniform(tmem + kGBase + g * (GP * (kStream / 2)));
+                const uint32_t a0 = uniform(tmem + g * kGroupColumns<PARTS>);
                 const uint32_t b0 = uniform(mn_major_lo(stream0 + stage * stage_bytes, kStreamChunk));
 #pragma unroll
                 for (int q = 0; q < g_pairs<PARTS>(); ++q) {
 #pragma unroll
                     for (int s = 0; s < kStream / 16; ++s)
-                        mma_bf16_ta<kMnMajorHi>(d, a0 + g_pair_a<PARTS>(q) * (kStream / 2) + 8 * s,
+                        mma_bf16_ta<kMnMajorHi>(d, a0 + g_column(g_pair_a<PARTS>(q), 16 * s),
                                                 b0 + g_pair_b<PARTS>(q) * part + 128 * s, idesc,
                                                 q > 0 || s > 0 ? true : in_segment > 0, on);
                 }
@@ -382,8 +422,10 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
                     }
                 }
                 if (++stage == p.stages) stage = 0;
-                g ^= 1;
-                if (g == 0) g_phase ^= 1;
+                if (++g == kGroups) {
+                    g = 0;
+                    g_phase ^= 1;
+                }
             }
         }
         if (stop) {
@@ -391,41 +433,42 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
             for (int k = 0; k < kMbarRounds; ++k)
                 if (mbar_try(drain + 8, 0)) break;
         }
-    } else if (warp < 10) {
-        // Scores to G: group g takes every other tile. After a wait that gave
-        // up the rest fail at once and the block runs out on what is there.
-        const int g = (warp - 2) / 4, quarter = warp & 3, in_tile = quarter * 32 + lane;
-        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-        const uint32_t s_addr = tmem + lanes + g * kStream;
-        const uint32_t g_addr = tmem + lanes + kGBase + g * (GP * (kStream / 2));
+    } else if (warp >= 4 && warp < 4 + 4 * kGroups) {
+        // Scores to G: group g takes every kGroups-th tile. After a wait that
+        // gave up the rest fail at once and the block runs out on what is there.
+        const int g = (warp - 4) / 4, quarter = warp & 3, in_tile = quarter * 32 + lane;
+        const uint32_t group = tmem + ((uint32_t)(quarter * 32) << 16) + g * kGroupColumns<PARTS>;
         const float c2 = p.scale * kLog2e;
-        int64_t i = 0;
-        int stage = 0;
+        int stage = 0, turn = 0;
         uint32_t phase = 0, stage_phase = 0;
-        for (int64_t u = blockIdx.x; u < p.units; u += gridDim.x) {
+        for (int u = blockIdx.x; u < p.units; u += gridDim.x) {
             const FusedWalk w = fused_unit(p, u);
-            const int64_t own = w.own0 + in_tile;
+            const int own = w.own0 + in_tile;
             int lab = kIgnored;
             float lse = kInf, r = 0.0f, at_label = 0.0f, own_bias = 0.0f, bias_sum = 0.0f;
             if (own < p.own) {
                 if constexpr (BY_CLASS) {
                     own_bias = p.class_bias[own];
                 } else {
-                    const float* v = p.row_values + own / kStream * (kRowValues * kStream) + own % kStream;
+                    const float* v = p.row_values + (int64_t)(own / kStream) * (kRowValues * kStream) + own % kStream;
                     lse = v[0];
                     r = v[kStream];
                     at_label = v[2 * kStream];
                     lab = __float_as_int(v[3 * kStream]);
                 }
             }
-            for (int64_t t = w.t0; t < w.t1; ++t, ++i) {
+            for (int t = w.t0; t < w.t1; ++t) {
                 const int at = stage;
                 const uint32_t at_phase = stage_phase;
                 if (++stage == p.stages) {
                     stage = 0;
                     stage_phase ^= 1;
                 }
-                if ((int)(i & 1) != g) continue;
+                if (turn++ != g) {
+                    if (turn == kGroups) turn = 0;
+                    continue;
+                }
+                if (turn == kGroups) turn = 0;
                 const uint32_t col = stream0 + at * stage_bytes + tile_bytes;
                 wait(full + 8 * at, at_phase);  // the columns' values
                 wait(s_full + 8 * g, phase);
@@ -434,17 +477,12 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
                 // to stay in the instruction cache of eight warps out of step
                 // (both halves of 32 unrolled: 38 % of the stalls were fetches)
 #pragma unroll 1
-                for (int k = 0; k < kStream; k += 16) {
-                    float z[16];
-                    tmem_load16(s_addr + k, z);
-                    if (k + 16 == kStream) {
-                        tmem_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(s_empty + 8 * g);
-                    }
+                for (int k = 0; k < kStream; k += kStep) {
+                    float z[kStep];
+                    tmem_load(group + k, z);
                     if constexpr (BY_CLASS) {
 #pragma unroll
-                        for (int j = 0; j < 16; j += 4) {
+                        for (int j = 0; j < kStep; j += 4) {
                             const float4 a = shared_float4(col + 4 * (k + j));
                             const float4 b = shared_float4(col + 4 * (kStream + k + j));
                             z[j] = exp2_fast(fmaf(z[j], c2, own_bias) - a.x) * b.x;
@@ -453,41 +491,36 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
                             z[j + 3] = exp2_fast(fmaf(z[j + 3], c2, own_bias) - a.w) * b.w;
                         }
                         // rows labelled with one of this warp's classes
-                        const int mine = shared_int(col + 4 * (3 * kStream + k + (lane & 15))) - (int)w.own0 - quarter * 32;
+                        const int mine = shared_int(col + 4 * (3 * kStream + k + (lane & (kStep - 1)))) - w.own0 - quarter * 32;
                         if (__any_sync(0xffffffffu, (unsigned)mine < 32u)) {
 #pragma unroll
-                            for (int j = 0; j < 16; ++j)
-                                if (shared_int(col + 4 * (3 * kStream + k + j)) == (int)own)
+                            for (int j = 0; j < kStep; ++j)
+                                if (shared_int(col + 4 * (3 * kStream + k + j)) == own)
                                     z[j] = __int_as_float(shared_int(col + 4 * (2 * kStream + k + j)));
                         }
                         if (p.part_bias != nullptr) {
                             float q[4] = {bias_sum, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) q[j % 4] += z[j];
+                            for (int j = 0; j < kStep; ++j) q[j % 4] += z[j];
                             bias_sum = (q[0] + q[1]) + (q[2] + q[3]);
                         }
                     } else {
 #pragma unroll
-                        for (int j = 0; j < 16; j += 4) {
+                        for (int j = 0; j < kStep; j += 4) {
                             const float4 b = shared_float4(col + 4 * (k + j));
                             z[j] = exp2_fast(fmaf(z[j], c2, b.x) - lse) * r;
                             z[j + 1] = exp2_fast(fmaf(z[j + 1], c2, b.y) - lse) * r;
                             z[j + 2] = exp2_fast(fmaf(z[j + 2], c2, b.z) - lse) * r;
                             z[j + 3] = exp2_fast(fmaf(z[j + 3], c2, b.w) - lse) * r;
                         }
-                        const int rel = lab - (int)(t * kStream) - k;
-                        if (__any_sync(0xffffffffu, (unsigned)rel < 16u)) {
+                        const int rel = lab - t * kStream - k;
+                        if (__any_sync(0xffffffffu, (unsigned)rel < (unsigned)kStep)) {
 #pragma unroll
-                            for (int j = 0; j < 16; ++j)
+                            for (int j = 0; j < kStep; ++j)
                                 if (j == rel) z[j] = at_label;
                         }
                     }
-                    // the G product of the tile before last has read this buffer
-                    if (k == 0) {
-                        wait(g_empty + 8 * g, phase ^ 1);
-                        tmem_fence_after();
-                    }
-                    store_parts<GP>(g_addr + k / 2, z);
+                    store_parts<GP>(group, k, z);
                 }
                 tmem_store_wait();
                 tmem_fence_before();
@@ -496,19 +529,19 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
                 phase ^= 1;
             }
             if (BY_CLASS && p.part_bias != nullptr && own < p.own)
-                p.part_bias[(int64_t)(w.split * 2 + g) * p.own + own] = bias_sum;
+                p.part_bias[(int64_t)(w.split * kGroups + g) * p.own + own] = bias_sum;
         }
-    } else {
+    } else if (warp != 3) {
         // acc: quarter of the rows, and every other 32 channels
-        const int quarter = warp & 3, half = (warp - 10) / 4;
+        const int quarter = warp & 3, half = (warp - 4 - 4 * kGroups) / 4;
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + kAccBase;
         const int n = (p.channels + 15) / 16 * 16;
         constexpr int kKept = PARTS == 3 ? 2 : 1;  // fp32: all (<= 128 channels) stay here
         int ab = 0;
         uint32_t ab_phase = 0;
-        for (int64_t u = blockIdx.x; u < p.units; u += gridDim.x) {
+        for (int u = blockIdx.x; u < p.units; u += gridDim.x) {
             const FusedWalk w = fused_unit(p, u);
-            const int64_t own = w.own0 + quarter * 32 + lane;
+            const int own = w.own0 + quarter * 32 + lane;
             float kept[kKept][32];
             if constexpr (PARTS == 3) {
 #pragma unroll
@@ -536,13 +569,13 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
                     }
                     return;
                 }
-                TypeOf<PARTS>* dst = static_cast<TypeOf<PARTS>*>(p.out) + own * p.channels + c;
+                TypeOf<PARTS>* dst = static_cast<TypeOf<PARTS>*>(p.out) + (int64_t)own * p.channels + c;
 #pragma unroll
                 for (int j = 0; j < 32; ++j)
                     if (c + j < p.channels) dst[j] = from_f32<TypeOf<PARTS>>(v[j] * p.scale);
             };
             bool first = true;
-            for (int64_t t = w.t0; t < w.t1; t += p.per_segment) {
+            for (int t = w.t0; t < w.t1; t += p.per_segment) {
                 wait(acc_full + 8 * ab, ab_phase);
                 tmem_fence_after();
                 if constexpr (PARTS == 3) {
@@ -551,9 +584,9 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
                         const int c = (2 * q + half) * 32;
                         if (c < n) {
 #pragma unroll
-                            for (int h = 0; h < 32; h += 16) {  // 16 at a time: 96 registers a thread
+                            for (int h = 0; h < 32; h += 16) {  // 16 at a time, for the registers' sake
                                 float v[16];
-                                tmem_load16(lanes + ab * n + c + h, v);
+                                tmem_load(lanes + ab * n + c + h, v);
 #pragma unroll
                                 for (int j = 0; j < 16; ++j) kept[q][h + j] += v[j];
                             }
@@ -598,13 +631,14 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
     }
 }
 
+inline int group_columns(int parts) { return kGroups * (kStream + (parts == 3 ? kStream / 2 : 0)); }
+
 // Whether the owning side, two streamed tiles and acc fit an SM: up to 128
 // channels of fp32, 192 of fp16, 256 of bf16.
 inline bool fused_fits(int parts, int channels) {
     const int chunks = (channels + 63) / 64, n = (channels + 15) / 16 * 16;
-    const int g_parts = parts == 1 ? 2 : parts;
     return parts * chunks * (kOwn * 128 + 2 * kStream * 128) + 2 * kColumnBytes <= kFusedShared - 1024 &&
-           2 * kStream + g_parts * kStream + n <= 512;
+           group_columns(parts) + n <= 512;
 }
 
 // Buffers for what is left: a second one for the owning side if four streamed
@@ -615,8 +649,7 @@ inline void fused_buffers(FusedArgs& p, int parts) {
     const int room = kFusedShared - 1024, n = (p.channels + 15) / 16 * 16;
     p.own_buffers = 2 * own + 4 * stage <= room ? 2 : 1;
     p.stages = std::min(kFusedStages, (room - p.own_buffers * own) / stage);
-    const int g_parts = parts == 1 ? 2 : parts;
-    p.acc_buffers = 2 * kStream + g_parts * kStream + 2 * n <= 512 ? 2 : 1;
+    p.acc_buffers = group_columns(parts) + 2 * n <= 512 ? 2 : 1;
 }
 
 }  // namespace

@@ -203,7 +203,10 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                     const int b0 = (S::kProduct ? w.first : w.first + t) * kN;
                     const int64_t c0 = S::kProduct ? w.c0 + (int64_t)t * p.per_segment : w.c0;
                     const int64_t c1 = S::kProduct ? min(w.c1, c0 + p.per_segment) : w.c1;
-                    const int n = min(kN, (p.columns - b0 + 15) / 16 * 16);
+                    // scores: every column that is read (32 at a time) has been written,
+                    // past the last class with zeros; tensor memory may hold NaNs
+                    constexpr int kRound = S::kProduct ? 16 : 32;
+                    const int n = min(kN, (p.columns - b0 + kRound - 1) / kRound * kRound);
                     const uint32_t idesc = uniform(mma_idesc(n, S::kAmn, S::kBmn));
                     const int chunks = (int)uniform((uint32_t)(c1 - c0));
                     // 16-entry steps of the last chunk

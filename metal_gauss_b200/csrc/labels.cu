@@ -338,7 +338,7 @@ struct BackwardScratch {
             class_bias = a.take<float>((size_t)up(n.classes, kOwn) * kOwn);
             row_part = a.take<float>(n.fused_direct() ? 0 : (size_t)rs.splits * n.rows * n.part_ld());
             class_part = a.take<float>((size_t)cs.splits * n.classes * n.part_ld());
-            bias_part = a.take<float>((size_t)cs.splits * 2 * n.classes);
+            bias_part = a.take<float>((size_t)cs.splits * kGroups * n.classes);
             bias_part2 = nullptr;
         } else {
             row_values = class_bias = nullptr;
@@ -469,7 +469,7 @@ mg_status launch_fused(FusedArgs& p, const Sizes& n, const CUtensorMap& own,
         ready[dev] = true;
     }
     fused_buffers(p, PARTS);
-    const int grid = (int)std::min<int64_t>(p.units, sm_count());
+    const int grid = std::min(p.units, sm_count());
     fused_kernel<BY_CLASS, PARTS><<<grid, kFusedThreads, kFusedShared, st>>>(p, own, stream);
     return check_launch(what);
 }
@@ -486,8 +486,6 @@ mg_status backward_fused(const Args& a, const RowGrad& rg, const float* stats, T
         return make_tensor_map(m, b, n.depth(), rows, PARTS, row, part, 64, box, true, "label_loss parts");
     };
     FusedArgs p{};
-    p.rows = n.rows;
-    p.classes = n.classes;
     p.channels = n.channels;
     p.chunks = (int)up(n.channels, 64);
     p.per_segment = n.fused_segment();
@@ -501,11 +499,11 @@ mg_status backward_fused(const Args& a, const RowGrad& rg, const float* stats, T
         const Shares sh = n.fused_by_row();
         MG_TRY(map(&own, f.xs, n.rows, kOwn));
         MG_TRY(map(&stream, f.ws, n.classes, kStream));
-        p.units = up(n.rows, kOwn) * sh.splits;
-        p.own = n.rows;
+        p.units = (int)(up(n.rows, kOwn) * sh.splits);
+        p.own = (int)n.rows;
         p.streamed = n.classes;
         p.splits = sh.splits;
-        p.per_split = sh.per_split;
+        p.per_split = (int)sh.per_split;
         p.part = n.fused_direct() ? nullptr : f.row_part;
         p.out = dx;
         MG_TRY((launch_fused<false, PARTS>(p, n, own, stream, a.st, "label_loss_backward rows")));
@@ -516,18 +514,18 @@ mg_status backward_fused(const Args& a, const RowGrad& rg, const float* stats, T
         const Shares sh = n.fused_by_class();
         MG_TRY(map(&own, f.ws, n.classes, kOwn));
         MG_TRY(map(&stream, f.xs, n.rows, kStream));
-        p.units = up(n.classes, kOwn) * sh.splits;
+        p.units = (int)(up(n.classes, kOwn) * sh.splits);
         p.own = n.classes;
-        p.streamed = n.rows;
+        p.streamed = (int)n.rows;
         p.splits = sh.splits;
-        p.per_split = sh.per_split;
+        p.per_split = (int)sh.per_split;
         p.part = f.class_part;
         p.part_bias = db != nullptr ? f.bias_part : nullptr;
         MG_TRY((launch_fused<true, PARTS>(p, n, own, stream, a.st, "label_loss_backward classes")));
         if (dw != nullptr)
             MG_TRY(join(f.class_part, sh.splits, n.classes, n.part_ld(), n.channels, a.scale, dw, a.st));
         if (db != nullptr)
-            MG_TRY(column_sum(f.bias_part, 2 * sh.splits, 2 * sh.splits, n.classes, db, a.st));
+            MG_TRY(column_sum(f.bias_part, kGroups * sh.splits, kGroups * sh.splits, n.classes, db, a.st));
     }
     return MG_OK;
 }

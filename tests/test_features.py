@@ -508,6 +508,20 @@ def test_label_loss_nan_features_spoil_their_row_alone(cuda):
     assert gx[9].isnan().all() and gx[keep].isfinite().all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_label_loss_after_a_loss_of_nans(cuda, dtype):
+    """What an earlier call left on the SMs (here NaN in every score) reaches
+    no later one, whatever its number of classes."""
+    bad = torch.full((148 * 128, 32), math.nan, dtype=dtype, device=cuda).requires_grad_(True)
+    wide = torch.randn(512, 32, generator=gen(30), device=cuda).to(dtype)
+    zeros = torch.zeros(148 * 128, dtype=torch.int64, device=cuda)
+    for v in (1, 5, 8, 17, 33, 63, 65, 130):
+        rows = label_loss(bad, wide, zeros, reduction="sum")
+        assert torch.autograd.grad(rows, bad)[0].isnan().all()
+        x, w, lab, bias, _ = label_case(31 + v, 300, 24, v, dtype)
+        check_label(x, w, lab, bias)
+
+
 def test_label_loss_confident_rows_keep_their_digits(cuda):
     """Rows whose class wins by 20 to 60: loss and gradient are e^-20 to e^-60
     and keep their relative precision (bounded by the logits' own)."""
