@@ -569,10 +569,17 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
                     }
                     return;
                 }
+                // 16 bytes at a time: the channels are a multiple of that here
+                constexpr int kVec = 16 / sizeof(TypeOf<PARTS>);
                 TypeOf<PARTS>* dst = static_cast<TypeOf<PARTS>*>(p.out) + (int64_t)own * p.channels + c;
 #pragma unroll
-                for (int j = 0; j < 32; ++j)
-                    if (c + j < p.channels) dst[j] = from_f32<TypeOf<PARTS>>(v[j] * p.scale);
+                for (int j = 0; j < 32; j += kVec) {
+                    if (c + j >= p.channels) continue;
+                    float o[kVec];
+#pragma unroll
+                    for (int i = 0; i < kVec; ++i) o[i] = v[j + i] * p.scale;
+                    store_row<TypeOf<PARTS>, kVec>(dst + j, o);
+                }
             };
             bool first = true;
             for (int t = w.t0; t < w.t1; t += p.per_segment) {

@@ -10,13 +10,16 @@ namespace {
 
 constexpr int kM = 128;        // rows of a tile
 constexpr int kN = 256;        // columns of a tile, at most
-constexpr int kThreads = 320;  // a copying warp, an issuing warp, 8 warps that take tiles out
 
 enum Mode { kStats, kLogitGrad, kProductRow, kProductClass };
 
 template <int MODE, int PARTS>
 struct Shape {
     static constexpr bool kProduct = MODE >= kProductRow;
+    // Sets of four warps that take tiles out, 32 columns at a time in turn: the
+    // exponentials of kStats wait on one another's latency and want many.
+    static constexpr int kSets = MODE == kStats ? 4 : 2;
+    static constexpr int kThreads = 64 + 128 * kSets;  // and a copying and an issuing warp
     static constexpr bool kAmn = MODE == kProductClass;  // A's row index runs fastest
     static constexpr bool kBmn = kProduct;
     static constexpr int kChunk = PARTS == 1 ? 64 : 32;  // contraction entries per stage
@@ -24,7 +27,7 @@ struct Shape {
     static constexpr int kB = kN * kChunk * 2;
     static constexpr int kStage = PARTS * (kA + kB);
     static constexpr int kStages = PARTS == 3 ? (MODE == kLogitGrad ? 2 : 3) : (MODE == kLogitGrad ? 3 : 4);
-    // G on its way out: 128 x 32 bf16 for each half of the taking warps, part and buffer
+    // G on its way out: 128 x 32 bf16 for each set of the taking warps, part and buffer
     static constexpr int kOutBuffers = PARTS == 3 ? 1 : 2;
     static constexpr int kOut = MODE == kLogitGrad ? 2 * PARTS * kOutBuffers * kM * 64 : 0;
     static constexpr int kDynamic = 1024 + kStages * kStage + kOut;
@@ -97,7 +100,7 @@ __device__ __forceinline__ Walk walk_unit(const TileArgs& p, int64_t u) {
 }
 
 template <int MODE, int PARTS>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__((Shape<MODE, PARTS>::kThreads), 1)
 tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensorMap map_a,
             const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_out) {
     using S = Shape<MODE, PARTS>;
@@ -119,7 +122,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(taken_full + 8 * i, 1);
-            mbar_init(taken_empty + 8 * i, 8);
+            mbar_init(taken_empty + 8 * i, 4 * S::kSets);
         }
         mbar_init(drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -257,13 +260,13 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
         }
     } else {
         // Takes tiles out: warp % 4 is the quarter of the rows it can reach,
-        // `half` the 32-column chunks it takes (even or odd ones). After a wait
+        // `set` the 32-column chunks it takes (every kSets-th). After a wait
         // that gave up the remaining waits fail at once and the block runs to
         // its end on whatever is there; the error word says so.
-        const int quarter = warp & 3, half = (warp - 2) / 4, et = threadIdx.x - 64;
+        const int quarter = warp & 3, set = (warp - 2) / 4, et = threadIdx.x - 64;
         const int in_tile = quarter * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-        const bool speaks = quarter == 0 && lane == 0;  // for its half's stores
+        const bool speaks = quarter == 0 && lane == 0;  // for its set's stores
         const float c2 = p.scale * kLog2e;
         int buf = 0, out_buf = 0;
         uint32_t buf_phase = 0;
@@ -281,15 +284,20 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                     lse = p.stats[row];
                     at_label = -p.stats[p.rows + row] * r;
                 }
+                const auto bias_of = [&](int v) {
+                    return p.bias != nullptr && et < kN && v < p.columns ? p.bias[v] : 0.0f;
+                };
+                float next_bias = bias_of(w.first * kN + et);
                 for (int t = 0; t < w.tiles; ++t) {
                     const int v0 = (w.first + t) * kN;
                     const int n = min(kN, p.columns - v0);
                     // bias times log2 e; classes past the end are taken out
-                    bias_s[buf][et] = et < n ? (p.bias != nullptr ? p.bias[v0 + et] * kLog2e : 0.0f) : -kInf;
-                    named_sync(1, 256);
+                    if (et < kN) bias_s[buf][et] = et < n ? next_bias * kLog2e : -kInf;
+                    named_sync(1, 128 * S::kSets);
+                    next_bias = bias_of(v0 + kN + et);  // of the next tile, while this one is taken
                     mbar_wait(taken_full + 8 * buf, buf_phase, &stop, p.error_word, DEV_ERR_TILE_WAIT);
                     tmem_fence_after();
-                    for (int k = half; k * 32 < n; k += 2) {
+                    for (int k = set; k * 32 < n; k += S::kSets) {
                         float z[32];
                         tmem_load32(lanes + buf * kN + k * 32, z);
 #pragma unroll
@@ -334,9 +342,9 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                             }
                             // staging is free again once the store before last has read it
                             const uint32_t stage0 = base + S::kStages * S::kStage +
-                                                    (half * S::kOutBuffers + out_buf) * (PARTS * kM * 64);
+                                                    (set * S::kOutBuffers + out_buf) * (PARTS * kM * 64);
                             if (speaks) tma_store_wait_read<S::kOutBuffers - 1>();
-                            named_sync(2 + half, 128);
+                            named_sync(2 + set, 128);
                             const uint32_t line = stage0 + in_tile * 64;
 #pragma unroll
                             for (int g = 0; g < 4; ++g) {
@@ -359,7 +367,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                                 }
                             }
                             fence_async_shared();
-                            named_sync(2 + half, 128);
+                            named_sync(2 + set, 128);
                             if (speaks) {
 #pragma unroll
                                 for (int i = 0; i < PARTS; ++i)
@@ -392,7 +400,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                     if (buf == 0) buf_phase ^= 1;
                 }
                 if (MODE == kStats && mine) {
-                    const int64_t at = (int64_t)(w.split * 2 + half) * p.rows + row;
+                    const int64_t at = (int64_t)(w.split * S::kSets + set) * p.rows + row;
                     p.part_m[at] = m;
                     p.part_s[at] = s;
                 }
@@ -409,9 +417,9 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                     tmem_fence_after();
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        if ((2 * q + half) * 32 < n) {
+                        if ((2 * q + set) * 32 < n) {
                             float v[32];
-                            tmem_load32(lanes + buf * kN + (2 * q + half) * 32, v);
+                            tmem_load32(lanes + buf * kN + (2 * q + set) * 32, v);
 #pragma unroll
                             for (int j = 0; j < 32; ++j) acc[q][j] += v[j];
                         }
@@ -425,7 +433,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                 if (mine) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        const int c = d0 + (2 * q + half) * 32;
+                        const int c = d0 + (2 * q + set) * 32;
                         if (c >= p.columns) continue;
                         if (p.part != nullptr) {
                             float* dst = p.part + ((int64_t)w.split * p.a_rows + a_row) * p.part_ld + c;

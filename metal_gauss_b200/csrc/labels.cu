@@ -285,9 +285,12 @@ struct Sizes {
     int fused_segment() const { return parts == 3 ? 1 : 4096 / kStream; }
     Shares fused_by_row() const { return split(up(classes, kStream), up(rows, kOwn)); }
     Shares fused_by_class() const { return split(up(rows, kStream), up(classes, kOwn)); }
-    bool fused_direct() const {  // dx in one visit: no shares to join
+    // dx in one visit, in rows of whole 16-byte stores: no shares to join.
+    // (Single elements, 32 rows apart in a warp, took 2 us of a unit.)
+    bool fused_direct() const {
         const Shares s = fused_by_row();
-        return s.splits == 1 && (parts == 3 || s.per_split <= fused_segment());
+        return s.splits == 1 && (parts == 3 || s.per_split <= fused_segment()) &&
+               channels % (parts == 3 ? 4 : 8) == 0;
     }
     int64_t row_blocks() const { return up(rows, 256); }
     // the bias's gradient: sums of 32 rows, then of up to kBiasLines of those
@@ -315,8 +318,8 @@ struct ForwardScratch {
         Scratch a{static_cast<char*>(base)};
         xs = a.take<__nv_bfloat16>((size_t)n.rows * n.parts * n.depth());
         ws = a.take<__nv_bfloat16>((size_t)n.classes * n.parts * n.depth());
-        m = a.take<float>((size_t)n.stats().splits * 2 * n.rows);
-        s = a.take<float>((size_t)n.stats().splits * 2 * n.rows);
+        m = a.take<float>((size_t)n.stats().splits * Shape<kStats, 1>::kSets * n.rows);
+        s = a.take<float>((size_t)n.stats().splits * Shape<kStats, 1>::kSets * n.rows);
         z = a.take<float>((size_t)n.rows);
         sums = a.take<double>(2 * (size_t)n.row_blocks());
         bytes = (size_t)(a.p - static_cast<char*>(base));
@@ -377,7 +380,7 @@ mg_status launch_tiles(const TileArgs& p, const CUtensorMap& a, const CUtensorMa
         ready[dev] = true;
     }
     const int grid = (int)std::min<int64_t>(p.units, sm_count());
-    tile_kernel<MODE, PARTS><<<grid, kThreads, bytes, st>>>(p, a, b, out);
+    tile_kernel<MODE, PARTS><<<grid, Shape<MODE, PARTS>::kThreads, bytes, st>>>(p, a, b, out);
     return check_launch(what);
 }
 
@@ -431,7 +434,7 @@ mg_status forward(const Args& a, int reduction, float* loss, float* stats, float
     p.error_word = device_error_word();
     MG_TRY((launch_tiles<kStats, PARTS>(p, mx, mw, mw, a.st, "label_loss_forward")));
     label_rows_kernel<<<(unsigned)a.n.row_blocks(), 256, 0, a.st>>>(
-        f.m, f.s, f.z, a.labels, sh.splits * 2, a.n.rows, stats,
+        f.m, f.s, f.z, a.labels, sh.splits * Shape<kStats, 1>::kSets, a.n.rows, stats,
         reduction == MG_REDUCE_NONE ? loss : nullptr, reduction == MG_REDUCE_NONE ? nullptr : f.sums,
         p.error_word);
     MG_TRY(check_launch("label_loss_forward rows"));
@@ -466,6 +469,12 @@ mg_status launch_fused(FusedArgs& p, const Sizes& n, const CUtensorMap& own,
         if (cudaFuncSetAttribute(fused_kernel<BY_CLASS, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  kFusedShared) != cudaSuccess)
             return check_launch(what);
+        // the registers that its warps hand on are those it is launched with
+        cudaFuncAttributes at{};
+        if (cudaFuncGetAttributes(&at, fused_kernel<BY_CLASS, PARTS>) != cudaSuccess)
+            return check_launch(what);
+        if ((at.numRegs + 7) / 8 * 8 * (kFusedThreads / 128) < kIssueRegs + kGroups * kScoreRegs + 2 * kAccRegs)
+            return fail(MG_ERR_CUDA, std::string(what) + ": built with too few registers");
         ready[dev] = true;
     }
     fused_buffers(p, PARTS);
@@ -726,6 +735,7 @@ extern "C" mg_status mg_label_loss_backward(
         return MG_OK;
     }
     if (d_features == nullptr && d_classes == nullptr && d_bias == nullptr) return MG_OK;
+    MG_REQUIRE(aligned16(d_features), "label_loss_backward: d_features must be 16-byte aligned");
     MG_REQUIRE(grad_loss && stats && (reduction != MG_REDUCE_MEAN || live),
                "label_loss_backward: null pointer");
     MG_REQUIRE(scratch != nullptr && (reinterpret_cast<uintptr_t>(scratch) & 255u) == 0u &&
