@@ -33,6 +33,12 @@ __device__ __forceinline__ int channel_of(int k, int warp, int lane) {
     return ((k * WARPS + warp) * 32 + lane) * VEC;
 }
 
+// Rows a team takes at once: enough loads in flight to cover HBM's latency
+// (about 40 KB an SM), 64 bytes a lane at most, and their reductions overlap.
+__host__ __device__ constexpr int rows_at_once(int bytes) {
+    return bytes >= 64 ? 1 : bytes >= 32 ? 2 : 4;
+}
+
 // Sum over the team that holds a row.
 template <int LPR, int WARPS>
 __device__ __forceinline__ float2 team_sum(float a, float b, float2* sh, int warp, int lane) {
@@ -85,65 +91,78 @@ norm_forward_kernel(const T* __restrict__ x, const void* __restrict__ weight,
     }
 
     // every lane of a warp takes every round: the reductions are warp-wide
-    const int64_t rounds = (rows + (int64_t)gridDim.x * kTeams - 1) / ((int64_t)gridDim.x * kTeams);
-    for (int64_t r = 0; r < rounds; ++r) {
-        const int64_t row = (r * gridDim.x + blockIdx.x) * kTeams + team;
-        const bool live = row < rows;
-        const T* xr = x + row * channels;
-        float v[NV * VEC];
-        float s = 0.0f;
+    constexpr int R = rows_at_once(NV * VEC * (int)sizeof(T));
+    const int64_t step = (int64_t)gridDim.x * kTeams * R;
+    const int64_t rounds = (rows + step - 1) / step;
+    for (int64_t it = 0; it < rounds; ++it) {
+        const int64_t row0 = (it * gridDim.x + blockIdx.x) * (kTeams * R) + team;
+        float v[R][NV * VEC];
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const int c = channel_of<VEC, LPR, WARPS>(k, warp, lane);
-            if (live && c < channels) {
-                load_row<T, VEC>(xr + c, v + k * VEC);
-            } else {
+        for (int r = 0; r < R; ++r) {
+            const int64_t row = row0 + r * kTeams;
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) v[k * VEC + i] = 0.0f;
-            }
+            for (int k = 0; k < NV; ++k) {
+                const int c = channel_of<VEC, LPR, WARPS>(k, warp, lane);
+                if (row < rows && c < channels) {
+                    load_row<T, VEC>(x + row * channels + c, v[r] + k * VEC);
+                } else {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) s += v[k * VEC + i];
-        }
-        const float mean = team_sum<LPR, WARPS>(s, 0.0f, sh, warp, lane).x * inv_n;
-        float q = 0.0f;
-#pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            if (channel_of<VEC, LPR, WARPS>(k, warp, lane) < channels) {
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    const float d = v[k * VEC + i] - mean;
-                    q = fmaf(d, d, q);
+                    for (int i = 0; i < VEC; ++i) v[r][k * VEC + i] = 0.0f;
                 }
             }
         }
-        const float var = team_sum<LPR, WARPS>(q, 0.0f, sh, warp, lane).x * inv_n;
-        const float rstd = 1.0f / sqrtf(var + eps);
-        if (codes != nullptr) {
-            // one scale per 128 channels, the maximum over the lanes that hold them
-            constexpr int kGroup = VEC == 8 ? (LPR < 16 ? LPR : 16) : LPR;
-            constexpr int kStep = VEC == 1 ? (NV < 4 ? NV : 4) : 1;
+        float mean[R], rstd[R];
 #pragma unroll
-            for (int k0 = 0; k0 < NV; k0 += kStep) {
-                float a = 0.0f;
+        for (int r = 0; r < R; ++r) {
+            float s = 0.0f;
 #pragma unroll
-                for (int i = 0; i < kStep * VEC; ++i) a = fmaxf(a, mag8(v[k0 * VEC + i]));
-                a = lanes_max<kGroup>(a);
-                const Scale8 s8 = scale8(a);
+            for (int i = 0; i < NV * VEC; ++i) s += v[r][i];
+            mean[r] = team_sum<LPR, WARPS>(s, 0.0f, sh, warp, lane).x * inv_n;
+        }
 #pragma unroll
-                for (int k = k0; k < k0 + kStep; ++k) {
-                    const int c = channel_of<VEC, LPR, WARPS>(k, warp, lane);
-                    if (live && c < channels) {
-                        int qv[VEC];
+        for (int r = 0; r < R; ++r) {
+            float q = 0.0f;
 #pragma unroll
-                        for (int i = 0; i < VEC; ++i) qv[i] = code8(v[k * VEC + i], s8.inv);
-                        store_codes<VEC>(codes + row * channels + c, qv);
-                        if (c % kBlock8 == 0) scales[row * nb + c / kBlock8] = s8.scale;
+            for (int k = 0; k < NV; ++k) {
+                if (channel_of<VEC, LPR, WARPS>(k, warp, lane) < channels) {
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) {
+                        const float d = v[r][k * VEC + i] - mean[r];
+                        q = fmaf(d, d, q);
                     }
                 }
             }
+            rstd[r] = 1.0f / sqrtf(team_sum<LPR, WARPS>(q, 0.0f, sh, warp, lane).x * inv_n + eps);
         }
-        if (live) {
-            T* yr = y + row * channels;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int64_t row = row0 + r * kTeams;
+            const bool live = row < rows;
+            if (codes != nullptr) {
+                // one scale per 128 channels, the maximum over the lanes that hold them
+                constexpr int kGroup = VEC == 8 ? (LPR < 16 ? LPR : 16) : LPR;
+                constexpr int kStep = VEC == 1 ? (NV < 4 ? NV : 4) : 1;
+#pragma unroll
+                for (int k0 = 0; k0 < NV; k0 += kStep) {
+                    float a = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < kStep * VEC; ++i) a = fmaxf(a, mag8(v[r][k0 * VEC + i]));
+                    a = lanes_max<kGroup>(a);
+                    const Scale8 s8 = scale8(a);
+#pragma unroll
+                    for (int k = k0; k < k0 + kStep; ++k) {
+                        const int c = channel_of<VEC, LPR, WARPS>(k, warp, lane);
+                        if (live && c < channels) {
+                            int qv[VEC];
+#pragma unroll
+                            for (int i = 0; i < VEC; ++i) qv[i] = code8(v[r][k * VEC + i], s8.inv);
+                            store_codes<VEC>(codes + row * channels + c, qv);
+                            if (c % kBlock8 == 0) scales[row * nb + c / kBlock8] = s8.scale;
+                        }
+                    }
+                }
+            }
+            if (!live) continue;
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
                 const int c = channel_of<VEC, LPR, WARPS>(k, warp, lane);
@@ -151,13 +170,13 @@ norm_forward_kernel(const T* __restrict__ x, const void* __restrict__ weight,
                     float o[VEC];
 #pragma unroll
                     for (int i = 0; i < VEC; ++i)
-                        o[i] = fmaf((v[k * VEC + i] - mean) * rstd, w[k * VEC + i], b[k * VEC + i]);
-                    store_row<T, VEC>(yr + c, o);
+                        o[i] = fmaf((v[r][k * VEC + i] - mean[r]) * rstd[r], w[k * VEC + i], b[k * VEC + i]);
+                    store_row<T, VEC>(y + row * channels + c, o);
                 }
             }
             if (mean_out != nullptr && lane == 0 && warp == 0) {
-                mean_out[row] = mean;
-                rstd_out[row] = rstd;
+                mean_out[row] = mean[r];
+                rstd_out[row] = rstd[r];
             }
         }
     }
@@ -190,48 +209,63 @@ norm_backward_kernel(const T* __restrict__ dy, const T* __restrict__ x,
         }
     }
 
-    const int64_t rounds = (rows + (int64_t)gridDim.x * kTeams - 1) / ((int64_t)gridDim.x * kTeams);
-    for (int64_t r = 0; r < rounds; ++r) {
-        const int64_t row = (r * gridDim.x + blockIdx.x) * kTeams + team;
-        const bool live = row < rows;
-        const float mean = live ? __ldg(mean_in + row) : 0.0f;
-        const float rstd = live ? __ldg(rstd_in + row) : 0.0f;
-        float h[NV * VEC], g[NV * VEC];
-        float sg = 0.0f, sgh = 0.0f;
+    constexpr int R = rows_at_once(2 * NV * VEC * (int)sizeof(T));
+    const int64_t step = (int64_t)gridDim.x * kTeams * R;
+    const int64_t rounds = (rows + step - 1) / step;
+    for (int64_t it = 0; it < rounds; ++it) {
+        const int64_t row0 = (it * gridDim.x + blockIdx.x) * (kTeams * R) + team;
+        float h[R][NV * VEC], g[R][NV * VEC], rstd[R];
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const int c = channel_of<VEC, LPR, WARPS>(k, warp, lane);
-            if (live && c < channels) {
-                load_row<T, VEC>(dy + row * channels + c, g + k * VEC);
-                if constexpr (HELD8) {
-                    load_codes<VEC>(codes + row * channels + c, h + k * VEC);
-                    const float sc = __ldg(scales + row * nb + c / kBlock8);
+        for (int r = 0; r < R; ++r) {
+            const int64_t row = row0 + r * kTeams;
+            const bool live = row < rows;
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i) h[k * VEC + i] = __fmul_rn(h[k * VEC + i], sc);
+            for (int k = 0; k < NV; ++k) {
+                const int c = channel_of<VEC, LPR, WARPS>(k, warp, lane);
+                if (live && c < channels) {
+                    load_row<T, VEC>(dy + row * channels + c, g[r] + k * VEC);
+                    if constexpr (HELD8) load_codes<VEC>(codes + row * channels + c, h[r] + k * VEC);
+                    else load_row<T, VEC>(x + row * channels + c, h[r] + k * VEC);
                 } else {
-                    load_row<T, VEC>(x + row * channels + c, h + k * VEC);
-                }
-            } else {
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    g[k * VEC + i] = 0.0f;
-                    h[k * VEC + i] = mean;
+                    for (int i = 0; i < VEC; ++i) g[r][k * VEC + i] = h[r][k * VEC + i] = 0.0f;
                 }
             }
         }
+        float2 sums[R];
 #pragma unroll
-        for (int i = 0; i < NV * VEC; ++i) {
-            h[i] = (h[i] - mean) * rstd;
-            dw[i] = fmaf(g[i], h[i], dw[i]);
-            db[i] += g[i];
-            g[i] *= w[i];
-            sg += g[i];
-            sgh = fmaf(g[i], h[i], sgh);
+        for (int r = 0; r < R; ++r) {
+            const int64_t row = row0 + r * kTeams;
+            const bool live = row < rows;
+            const float mean = live ? __ldg(mean_in + row) : 0.0f;
+            rstd[r] = live ? __ldg(rstd_in + row) : 0.0f;
+            float sg = 0.0f, sgh = 0.0f;
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const int c = channel_of<VEC, LPR, WARPS>(k, warp, lane);
+                const bool in = live && c < channels;
+                float scale = 1.0f;
+                if (HELD8 && in) scale = __ldg(scales + row * nb + c / kBlock8);
+#pragma unroll
+                for (int i = k * VEC; i < (k + 1) * VEC; ++i) {
+                    if constexpr (HELD8) h[r][i] = __fmul_rn(h[r][i], scale);
+                    h[r][i] = in ? (h[r][i] - mean) * rstd[r] : 0.0f;
+                    dw[i] = fmaf(g[r][i], h[r][i], dw[i]);
+                    db[i] += g[r][i];
+                    g[r][i] *= w[i];
+                    sg += g[r][i];
+                    sgh = fmaf(g[r][i], h[r][i], sgh);
+                }
+            }
+            sums[r] = make_float2(sg, sgh);
         }
         if (dx != nullptr) {
-            const float2 m = team_sum<LPR, WARPS>(sg, sgh, sh, warp, lane);
-            const float c1 = m.x * inv_n, c2 = m.y * inv_n;
-            if (live) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const int64_t row = row0 + r * kTeams;
+                const float2 m = team_sum<LPR, WARPS>(sums[r].x, sums[r].y, sh, warp, lane);
+                const float c1 = m.x * inv_n, c2 = m.y * inv_n;
+                if (row >= rows) continue;
 #pragma unroll
                 for (int k = 0; k < NV; ++k) {
                     const int c = channel_of<VEC, LPR, WARPS>(k, warp, lane);
@@ -239,7 +273,7 @@ norm_backward_kernel(const T* __restrict__ dy, const T* __restrict__ x,
                         float o[VEC];
 #pragma unroll
                         for (int i = 0; i < VEC; ++i)
-                            o[i] = rstd * (g[k * VEC + i] - c1 - h[k * VEC + i] * c2);
+                            o[i] = rstd[r] * (g[r][k * VEC + i] - c1 - h[r][k * VEC + i] * c2);
                         store_row<T, VEC>(dx + row * channels + c, o);
                     }
                 }
