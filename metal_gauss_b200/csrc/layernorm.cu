@@ -33,6 +33,40 @@ __device__ __forceinline__ int channel_of(int k, int warp, int lane) {
     return ((k * WARPS + warp) * 32 + lane) * VEC;
 }
 
+// weight or bias of a register group's channels: in shared memory (rows up to
+// 1024 channels, where registers hold rows in flight instead) or registers. At
+// 8 channels to a lane the two halves of each 8 are apart, so that the lanes'
+// 16-byte reads follow one another.
+template <int N, int VEC, int WARPS>
+struct Params {
+    float v[WARPS > 1 ? N : 1];
+    const float* sh;
+    int channels;
+
+    __device__ __forceinline__ static int place(int c, int channels) {
+        if constexpr (VEC == 8) return (c & 4 ? channels / 2 : 0) + (c >> 3) * 4 + (c & 3);
+        return c;
+    }
+    // the VEC values of group k, which starts at channel c
+    __device__ __forceinline__ void get(int k, int c, float (&o)[VEC]) const {
+        if constexpr (WARPS > 1) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) o[i] = v[k * VEC + i];
+        } else if constexpr (VEC == 1) {
+            o[0] = sh[c];
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC; i += 4) {
+                const float4 q = *reinterpret_cast<const float4*>(sh + place(c + i, channels));
+                o[i] = q.x;
+                o[i + 1] = q.y;
+                o[i + 2] = q.z;
+                o[i + 3] = q.w;
+            }
+        }
+    }
+};
+
 // Rows a team takes at once: enough loads in flight to cover HBM's latency
 // (about 40 KB an SM), 64 bytes a lane at most, and their reductions overlap.
 __host__ __device__ constexpr int rows_at_once(int bytes) {
@@ -79,15 +113,28 @@ norm_forward_kernel(const T* __restrict__ x, const void* __restrict__ weight,
     const float inv_n = 1.0f / (float)channels;
     const int nb = (channels + kBlock8 - 1) / kBlock8;
 
-    float w[NV * VEC], b[NV * VEC];
+    extern __shared__ float dynamic[];
+    using P = Params<NV * VEC, VEC, WARPS>;
+    P w, b;
+    w.sh = dynamic;
+    b.sh = dynamic + channels;
+    w.channels = b.channels = channels;
+    if constexpr (WARPS > 1) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        const int c = channel_of<VEC, LPR, WARPS>(k, warp, lane);
+        for (int k = 0; k < NV; ++k) {
+            const int c = channel_of<VEC, LPR, WARPS>(k, warp, lane);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            w[k * VEC + i] = (weight != nullptr && c < channels) ? param_at(weight, param_dtype, c + i) : 1.0f;
-            b[k * VEC + i] = (bias != nullptr && c < channels) ? param_at(bias, param_dtype, c + i) : 0.0f;
+            for (int i = 0; i < VEC; ++i) {
+                w.v[k * VEC + i] = (weight != nullptr && c < channels) ? param_at(weight, param_dtype, c + i) : 1.0f;
+                b.v[k * VEC + i] = (bias != nullptr && c < channels) ? param_at(bias, param_dtype, c + i) : 0.0f;
+            }
         }
+    } else {
+        for (int c = threadIdx.x; c < channels; c += kThreads) {
+            dynamic[P::place(c, channels)] = weight != nullptr ? param_at(weight, param_dtype, c) : 1.0f;
+            dynamic[channels + P::place(c, channels)] = bias != nullptr ? param_at(bias, param_dtype, c) : 0.0f;
+        }
+        __syncthreads();
     }
 
     // every lane of a warp takes every round: the reductions are warp-wide
@@ -96,7 +143,7 @@ norm_forward_kernel(const T* __restrict__ x, const void* __restrict__ weight,
     const int64_t rounds = (rows + step - 1) / step;
     for (int64_t it = 0; it < rounds; ++it) {
         const int64_t row0 = (it * gridDim.x + blockIdx.x) * (kTeams * R) + team;
-        float v[R][NV * VEC];
+        T v[R][NV * VEC];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int64_t row = row0 + r * kTeams;
@@ -104,10 +151,10 @@ norm_forward_kernel(const T* __restrict__ x, const void* __restrict__ weight,
             for (int k = 0; k < NV; ++k) {
                 const int c = channel_of<VEC, LPR, WARPS>(k, warp, lane);
                 if (row < rows && c < channels) {
-                    load_row<T, VEC>(x + row * channels + c, v[r] + k * VEC);
+                    load_raw<T, VEC>(x + row * channels + c, v[r] + k * VEC);
                 } else {
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i) v[r][k * VEC + i] = 0.0f;
+                    for (int i = 0; i < VEC; ++i) v[r][k * VEC + i] = from_f32<T>(0.0f);
                 }
             }
         }
@@ -116,7 +163,7 @@ norm_forward_kernel(const T* __restrict__ x, const void* __restrict__ weight,
         for (int r = 0; r < R; ++r) {
             float s = 0.0f;
 #pragma unroll
-            for (int i = 0; i < NV * VEC; ++i) s += v[r][i];
+            for (int i = 0; i < NV * VEC; ++i) s += to_f32<T>(v[r][i]);
             mean[r] = team_sum<LPR, WARPS>(s, 0.0f, sh, warp, lane).x * inv_n;
         }
 #pragma unroll
@@ -127,7 +174,7 @@ norm_forward_kernel(const T* __restrict__ x, const void* __restrict__ weight,
                 if (channel_of<VEC, LPR, WARPS>(k, warp, lane) < channels) {
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) {
-                        const float d = v[r][k * VEC + i] - mean[r];
+                        const float d = to_f32<T>(v[r][k * VEC + i]) - mean[r];
                         q = fmaf(d, d, q);
                     }
                 }
@@ -146,7 +193,7 @@ norm_forward_kernel(const T* __restrict__ x, const void* __restrict__ weight,
                 for (int k0 = 0; k0 < NV; k0 += kStep) {
                     float a = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < kStep * VEC; ++i) a = fmaxf(a, mag8(v[r][k0 * VEC + i]));
+                    for (int i = 0; i < kStep * VEC; ++i) a = fmaxf(a, mag8(to_f32<T>(v[r][k0 * VEC + i])));
                     a = lanes_max<kGroup>(a);
                     const Scale8 s8 = scale8(a);
 #pragma unroll
@@ -155,7 +202,7 @@ norm_forward_kernel(const T* __restrict__ x, const void* __restrict__ weight,
                         if (live && c < channels) {
                             int qv[VEC];
 #pragma unroll
-                            for (int i = 0; i < VEC; ++i) qv[i] = code8(v[r][k * VEC + i], s8.inv);
+                            for (int i = 0; i < VEC; ++i) qv[i] = code8(to_f32<T>(v[r][k * VEC + i]), s8.inv);
                             store_codes<VEC>(codes + row * channels + c, qv);
                             if (c % kBlock8 == 0) scales[row * nb + c / kBlock8] = s8.scale;
                         }
@@ -167,10 +214,12 @@ norm_forward_kernel(const T* __restrict__ x, const void* __restrict__ weight,
             for (int k = 0; k < NV; ++k) {
                 const int c = channel_of<VEC, LPR, WARPS>(k, warp, lane);
                 if (c < channels) {
-                    float o[VEC];
+                    float o[VEC], wk[VEC], bk[VEC];
+                    w.get(k, c, wk);
+                    b.get(k, c, bk);
 #pragma unroll
                     for (int i = 0; i < VEC; ++i)
-                        o[i] = fmaf((v[r][k * VEC + i] - mean[r]) * rstd[r], w[k * VEC + i], b[k * VEC + i]);
+                        o[i] = fmaf((to_f32<T>(v[r][k * VEC + i]) - mean[r]) * rstd[r], wk[i], bk[i]);
                     store_row<T, VEC>(y + row * channels + c, o);
                 }
             }
@@ -181,6 +230,11 @@ norm_forward_kernel(const T* __restrict__ x, const void* __restrict__ weight,
         }
     }
 }
+
+template <typename T, bool HELD8>
+struct HeldType { using type = T; };
+template <typename T>
+struct HeldType<T, true> { using type = int8_t; };
 
 template <typename T, int VEC, int LPR, int NV, int WARPS, bool HELD8>
 __global__ void __launch_bounds__(kThreads)
@@ -198,63 +252,91 @@ norm_backward_kernel(const T* __restrict__ dy, const T* __restrict__ x,
     const float inv_n = 1.0f / (float)channels;
     const int nb = (channels + kBlock8 - 1) / kBlock8;
 
-    float w[NV * VEC], dw[NV * VEC], db[NV * VEC];
+    extern __shared__ float dynamic[];  // weight, later 8 warps x channels
+    using P = Params<NV * VEC, VEC, WARPS>;
+    P w;
+    w.sh = dynamic;
+    w.channels = channels;
+    float dw[NV * VEC], db[NV * VEC];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         const int c = channel_of<VEC, LPR, WARPS>(k, warp, lane);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-            w[k * VEC + i] = (weight != nullptr && c < channels) ? param_at(weight, param_dtype, c + i) : 1.0f;
+            if constexpr (WARPS > 1)
+                w.v[k * VEC + i] = (weight != nullptr && c < channels) ? param_at(weight, param_dtype, c + i) : 1.0f;
             dw[k * VEC + i] = db[k * VEC + i] = 0.0f;
         }
     }
+    if constexpr (WARPS == 1) {
+        for (int c = threadIdx.x; c < channels; c += kThreads)
+            dynamic[P::place(c, channels)] = weight != nullptr ? param_at(weight, param_dtype, c) : 1.0f;
+        __syncthreads();
+    }
 
+    using Held = typename HeldType<T, HELD8>::type;
     constexpr int R = rows_at_once(2 * NV * VEC * (int)sizeof(T));
     const int64_t step = (int64_t)gridDim.x * kTeams * R;
     const int64_t rounds = (rows + step - 1) / step;
     for (int64_t it = 0; it < rounds; ++it) {
         const int64_t row0 = (it * gridDim.x + blockIdx.x) * (kTeams * R) + team;
-        float h[R][NV * VEC], g[R][NV * VEC], rstd[R];
+        T g[R][NV * VEC];
+        Held x_raw[R][NV * VEC];
+        float mean[R], rstd[R], scale[R][HELD8 ? NV : 1];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int64_t row = row0 + r * kTeams;
             const bool live = row < rows;
+            mean[r] = live ? __ldg(mean_in + row) : 0.0f;
+            rstd[r] = live ? __ldg(rstd_in + row) : 0.0f;
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
                 const int c = channel_of<VEC, LPR, WARPS>(k, warp, lane);
+                if (HELD8) scale[r][HELD8 ? k : 0] = 0.0f;
                 if (live && c < channels) {
-                    load_row<T, VEC>(dy + row * channels + c, g[r] + k * VEC);
-                    if constexpr (HELD8) load_codes<VEC>(codes + row * channels + c, h[r] + k * VEC);
-                    else load_row<T, VEC>(x + row * channels + c, h[r] + k * VEC);
+                    load_raw<T, VEC>(dy + row * channels + c, g[r] + k * VEC);
+                    if constexpr (HELD8) {
+                        load_codes_raw<VEC>(codes + row * channels + c, x_raw[r] + k * VEC);
+                        scale[r][k] = __ldg(scales + row * nb + c / kBlock8);
+                    } else {
+                        load_raw<T, VEC>(x + row * channels + c, x_raw[r] + k * VEC);
+                    }
                 } else {
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i) g[r][k * VEC + i] = h[r][k * VEC + i] = 0.0f;
+                    for (int i = 0; i < VEC; ++i) {
+                        g[r][k * VEC + i] = from_f32<T>(0.0f);
+                        x_raw[r][k * VEC + i] = Held(0.0f);
+                    }
                 }
             }
         }
+        // h of register i (of group k): only used where the row and channel exist
+        const auto hat = [&](int r, int k, int i) {
+            float v;
+            if constexpr (HELD8) v = __fmul_rn((float)x_raw[r][i], scale[r][k]);
+            else v = to_f32<T>(x_raw[r][i]);
+            return (v - mean[r]) * rstd[r];
+        };
         float2 sums[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const int64_t row = row0 + r * kTeams;
-            const bool live = row < rows;
-            const float mean = live ? __ldg(mean_in + row) : 0.0f;
-            rstd[r] = live ? __ldg(rstd_in + row) : 0.0f;
             float sg = 0.0f, sgh = 0.0f;
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
                 const int c = channel_of<VEC, LPR, WARPS>(k, warp, lane);
-                const bool in = live && c < channels;
-                float scale = 1.0f;
-                if (HELD8 && in) scale = __ldg(scales + row * nb + c / kBlock8);
+                if (row0 + r * kTeams < rows && c < channels) {
+                    float wk[VEC];
+                    w.get(k, c, wk);
 #pragma unroll
-                for (int i = k * VEC; i < (k + 1) * VEC; ++i) {
-                    if constexpr (HELD8) h[r][i] = __fmul_rn(h[r][i], scale);
-                    h[r][i] = in ? (h[r][i] - mean) * rstd[r] : 0.0f;
-                    dw[i] = fmaf(g[r][i], h[r][i], dw[i]);
-                    db[i] += g[r][i];
-                    g[r][i] *= w[i];
-                    sg += g[r][i];
-                    sgh = fmaf(g[r][i], h[r][i], sgh);
+                    for (int j = 0; j < VEC; ++j) {
+                        const int i = k * VEC + j;
+                        const float h = hat(r, k, i), d = to_f32<T>(g[r][i]);
+                        dw[i] = fmaf(d, h, dw[i]);
+                        db[i] += d;
+                        const float wg = d * wk[j];
+                        sg += wg;
+                        sgh = fmaf(wg, h, sgh);
+                    }
                 }
             }
             sums[r] = make_float2(sg, sgh);
@@ -270,10 +352,13 @@ norm_backward_kernel(const T* __restrict__ dy, const T* __restrict__ x,
                 for (int k = 0; k < NV; ++k) {
                     const int c = channel_of<VEC, LPR, WARPS>(k, warp, lane);
                     if (c < channels) {
-                        float o[VEC];
+                        float o[VEC], wk[VEC];
+                        w.get(k, c, wk);
 #pragma unroll
-                        for (int i = 0; i < VEC; ++i)
-                            o[i] = rstd[r] * (g[r][k * VEC + i] - c1 - h[r][k * VEC + i] * c2);
+                        for (int j = 0; j < VEC; ++j) {
+                            const int i = k * VEC + j;
+                            o[j] = rstd[r] * (to_f32<T>(g[r][i]) * wk[j] - c1 - hat(r, k, i) * c2);
+                        }
                         store_row<T, VEC>(dx + row * channels + c, o);
                     }
                 }
@@ -285,7 +370,7 @@ norm_backward_kernel(const T* __restrict__ dy, const T* __restrict__ x,
     // lanes of a warp that hold the same channels, then the block's warps
     float* out = partial + (int64_t)blockIdx.x * 2 * channels;
     if constexpr (WARPS == 1) {
-        extern __shared__ float join[];  // 8 warps x channels
+        float* join = dynamic;
         const int wid = threadIdx.x / 32;
 #pragma unroll
         for (int i = 0; i < NV * VEC; ++i) {
@@ -382,7 +467,8 @@ struct Forward {
         constexpr int kTeams = WARPS > 1 ? 1 : kThreads / LPR;
         const int64_t want = (rows + kTeams - 1) / kTeams;
         const int grid = (int)std::min<int64_t>(want, 8 * (int64_t)sm_count());
-        norm_forward_kernel<T, VEC, LPR, NV, WARPS><<<grid, kThreads, 0, st>>>(
+        const size_t smem = WARPS == 1 ? sizeof(float) * 2 * (size_t)channels : 0;
+        norm_forward_kernel<T, VEC, LPR, NV, WARPS><<<grid, kThreads, smem, st>>>(
             static_cast<const T*>(x), weight, bias, param_dtype, rows, channels, eps,
             static_cast<T*>(y), mean, rstd, codes, scales);
         return check_launch("layer_norm_forward");

@@ -62,6 +62,17 @@ __device__ __forceinline__ void store_row(T* __restrict__ p, const float* v) {
     }
 }
 
+// The same without the conversion: 16-bit rows wait in half the registers.
+template <typename T, int VEC>
+__device__ __forceinline__ void load_raw(const T* __restrict__ p, T* v) {
+    if constexpr (VEC == 1) {
+        v[0] = __ldg(p);
+    } else {
+        const uint4 r = __ldg(reinterpret_cast<const uint4*>(p));
+        memcpy(v, &r, 16);
+    }
+}
+
 // VEC codes (VEC 1, 4 or 8; p aligned to VEC bytes).
 template <int VEC>
 __device__ __forceinline__ void store_codes(int8_t* __restrict__ p, const int* q) {
@@ -89,6 +100,19 @@ __device__ __forceinline__ void load_codes(const int8_t* __restrict__ p, float* 
             const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(p) + k);
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[4 * k + i] = (float)(int8_t)(w >> (8 * i));
+        }
+    }
+}
+
+template <int VEC>
+__device__ __forceinline__ void load_codes_raw(const int8_t* __restrict__ p, int8_t* v) {
+    if constexpr (VEC == 1) {
+        v[0] = __ldg(p);
+    } else {
+#pragma unroll
+        for (int k = 0; k < VEC / 4; ++k) {
+            const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(p) + k);
+            memcpy(v + 4 * k, &w, 4);
         }
     }
 }
