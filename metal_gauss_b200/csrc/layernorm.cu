@@ -450,6 +450,19 @@ int64_t backward_blocks(int64_t rows, int64_t channels) {
     return std::max<int64_t>(1, std::min<int64_t>(want, 4 * (int64_t)sm_count()));
 }
 
+// Blocks of a kernel that an SM holds, asked once per device.
+template <typename K>
+int blocks_per_sm(K kernel, size_t smem, int (&known)[64]) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 2;
+    if (known[dev] == 0) {
+        int n = 0;
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kThreads, smem) != cudaSuccess || n < 1) n = 1;
+        known[dev] = n;
+    }
+    return known[dev];
+}
+
 struct Forward {
     const void *x, *weight, *bias;
     int param_dtype;
@@ -465,9 +478,12 @@ struct Forward {
     template <typename T, int VEC, int LPR, int NV, int WARPS>
     mg_status run() const {
         constexpr int kTeams = WARPS > 1 ? 1 : kThreads / LPR;
+        // one wave of blocks that stay: each reads the parameters once
         const int64_t want = (rows + kTeams - 1) / kTeams;
-        const int grid = (int)std::min<int64_t>(want, 8 * (int64_t)sm_count());
         const size_t smem = WARPS == 1 ? sizeof(float) * 2 * (size_t)channels : 0;
+        static int known[64] = {};
+        const int per_sm = blocks_per_sm(norm_forward_kernel<T, VEC, LPR, NV, WARPS>, smem, known);
+        const int grid = (int)std::min<int64_t>(want, per_sm * (int64_t)sm_count());
         norm_forward_kernel<T, VEC, LPR, NV, WARPS><<<grid, kThreads, smem, st>>>(
             static_cast<const T*>(x), weight, bias, param_dtype, rows, channels, eps,
             static_cast<T*>(y), mean, rstd, codes, scales);
@@ -486,12 +502,19 @@ struct Backward {
     int channels;
     void* dx;
     float* partial;
-    int grid;
+    int max_grid;
+    int* used;  // the grid that ran: rows of partial
     cudaStream_t st;
 
     template <typename T, int VEC, int LPR, int NV, int WARPS>
     mg_status run() const {
         const size_t smem = WARPS == 1 ? sizeof(float) * 8 * (size_t)channels : 0;
+        static int known[2][64] = {};
+        const int per_sm = codes != nullptr
+                               ? blocks_per_sm(norm_backward_kernel<T, VEC, LPR, NV, WARPS, true>, smem, known[0])
+                               : blocks_per_sm(norm_backward_kernel<T, VEC, LPR, NV, WARPS, false>, smem, known[1]);
+        const int grid = std::min(max_grid, per_sm * sm_count());
+        *used = grid;
         if (codes != nullptr)
             norm_backward_kernel<T, VEC, LPR, NV, WARPS, true><<<grid, kThreads, smem, st>>>(
                 static_cast<const T*>(dy), nullptr, codes, scales, weight, param_dtype, mean, rstd,
@@ -620,9 +643,9 @@ extern "C" mg_status mg_layer_norm_backward(const void* dy, const void* x, const
     MG_REQUIRE(!params || (scratch != nullptr &&
                            scratch_bytes >= mg_layer_norm_backward_scratch_bytes(rows, channels)),
                "layer_norm_backward: scratch too small");
-    const int grid = (int)backward_blocks(rows, channels);
+    int grid = 0;
     const Backward op{dy, x, codes, scales, weight, param_dtype, mean, rstd, rows, (int)channels,
-                      dx, params ? static_cast<float*>(scratch) : nullptr, grid, st};
+                      dx, params ? static_cast<float*>(scratch) : nullptr, (int)backward_blocks(rows, channels), &grid, st};
     MG_TRY(pick_type(op, dtype, (int)channels,
                      aligned16(dy) && (x == nullptr || aligned16(x)) && (dx == nullptr || aligned16(dx))));
     if (!params) return MG_OK;
