@@ -35,35 +35,6 @@ constexpr int kIssueRegs = 72, kScoreRegs = 64, kAccRegs = 88;
 constexpr int kFusedStages = 8;     // at most
 constexpr int kFusedShared = 226 * 1024;  // of it 1 KB to align
 
-// Parts of G: two also for bf16 features, whose gradients then carry no other
-// rounding than their own (one part would add its 2^-9 to theirs).
-template <int PARTS>
-constexpr int kGParts = PARTS == 1 ? 2 : PARTS;
-
-// Products (G part, stream part), smallest first.
-template <int PARTS>
-__device__ constexpr int g_pairs() { return PARTS == 1 ? 2 : PARTS == 2 ? 3 : 6; }
-template <int PARTS>
-__device__ constexpr int g_pair_a(int i) {
-    return PARTS == 1 ? 1 - i : pair_a<PARTS>(g_pairs<PARTS>(), i);
-}
-template <int PARTS>
-__device__ constexpr int g_pair_b(int i) {
-    return PARTS == 1 ? 0 : pair_b<PARTS>(g_pairs<PARTS>(), i);
-}
-
-// The features' type, by its parts.
-template <int PARTS>
-struct PartsType;
-template <>
-struct PartsType<1> { using type = __nv_bfloat16; };
-template <>
-struct PartsType<2> { using type = __half; };
-template <>
-struct PartsType<3> { using type = float; };
-template <int PARTS>
-using TypeOf = typename PartsType<PARTS>::type;
-
 struct FusedArgs {         // counts below 2^31: at most 2^30 rows
     int units;
     int own;               // items of the owning side
@@ -404,7 +375,7 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
                 const uint32_t a0 = uniform(tmem + g * kGroupColumns<PARTS>);
                 const uint32_t b0 = uniform(mn_major_lo(stream0 + stage * stage_bytes, kStreamChunk));
 #pragma unroll
-                for (int q = 0; q < g_pairs<PARTS>(); ++q) {
+                for (int q = 0; q < kGPairs<PARTS>; ++q) {
 #pragma unroll
                     for (int s = 0; s < kStream / 16; ++s)
                         mma_bf16_ta<kMnMajorHi>(d, a0 + g_column(g_pair_a<PARTS>(q), 16 * s),

@@ -25,14 +25,18 @@ struct Shape {
     static constexpr int kChunk = PARTS == 1 ? 64 : 32;  // contraction entries per stage
     static constexpr int kA = kM * kChunk * 2;           // bytes of one part
     static constexpr int kB = kN * kChunk * 2;
-    static constexpr int kStage = PARTS * (kA + kB);
-    static constexpr int kStages = PARTS == 3 ? (MODE == kLogitGrad ? 2 : 3) : (MODE == kLogitGrad ? 3 : 4);
+    static constexpr int kPartsA = kProduct ? kGParts<PARTS> : PARTS;
+    static constexpr int kPartsG = kGParts<PARTS>;
+    static constexpr int kStage = kPartsA * kA + PARTS * kB;
+    static constexpr int kStages = PARTS == 3 ? (MODE == kLogitGrad ? 2 : 3) : (MODE == kStats ? 4 : 3);
     // G on its way out: 128 x 32 bf16 for each set of the taking warps, part and buffer
     static constexpr int kOutBuffers = PARTS == 3 ? 1 : 2;
-    static constexpr int kOut = MODE == kLogitGrad ? 2 * PARTS * kOutBuffers * kM * 64 : 0;
+    static constexpr int kOut = MODE == kLogitGrad ? 2 * kPartsG * kOutBuffers * kM * 64 : 0;
     static constexpr int kDynamic = 1024 + kStages * kStage + kOut;
     // Products of parts (a, b), smallest first.
-    static constexpr int kPairs = PARTS == 1 ? 1 : PARTS == 3 ? 6 : kProduct ? 3 : 4;
+    static constexpr int kPairs = kProduct ? kGPairs<PARTS> : PARTS == 1 ? 1 : PARTS == 2 ? 4 : 6;
+    __device__ static constexpr int part_a(int i) { return kProduct ? g_pair_a<PARTS>(i) : pair_a<PARTS>(kPairs, i); }
+    __device__ static constexpr int part_b(int i) { return kProduct ? g_pair_b<PARTS>(i) : pair_b<PARTS>(kPairs, i); }
 };
 
 struct TileArgs {
@@ -56,7 +60,6 @@ struct TileArgs {
     int part_ld;
     int add;                // to what the share holds
     void* out;              // products: the result itself
-    int out_type;
     int32_t* error_word;
 };
 
@@ -150,28 +153,30 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                     const int64_t c1 = S::kProduct ? min(w.c1, c0 + p.per_segment) : w.c1;
                     const int blocks = S::kProduct ? (min(kN, p.columns - b0) + 63) / 64 : 0;
                     const uint32_t bytes =
-                        PARTS * (S::kA + (S::kProduct ? blocks * S::kChunk * 128 : S::kB));
+                        S::kPartsA * S::kA + PARTS * (S::kProduct ? blocks * S::kChunk * 128 : S::kB);
                     for (int64_t c = c0; c < c1; ++c) {
                         ok = mbar_wait_warp(empty + 8 * stage, phase ^ 1, &stop, p.error_word, DEV_ERR_TILE_WAIT);
                         if (!ok) break;
                         const uint32_t bar = full + 8 * stage;
                         mbar_expect(bar, bytes, on);
                         const int k = (int)(c * S::kChunk);
+                        const uint32_t a = base + stage * S::kStage, b = a + S::kPartsA * S::kA;
 #pragma unroll
-                        for (int i = 0; i < PARTS; ++i) {
-                            const uint32_t a = base + stage * S::kStage + i * S::kA;
-                            const uint32_t b = base + stage * S::kStage + PARTS * S::kA + i * S::kB;
+                        for (int i = 0; i < S::kPartsA; ++i) {
                             if (S::kAmn) {
                                 for (int q = 0; q < 2; ++q)
-                                    tma_load(a + q * S::kChunk * 128, &map_a, (int)w.a_row + 64 * q, k, i, bar, on);
+                                    tma_load(a + i * S::kA + q * S::kChunk * 128, &map_a, (int)w.a_row + 64 * q, k, i, bar, on);
                             } else {
-                                tma_load(a, &map_a, k, (int)w.a_row, i, bar, on);
+                                tma_load(a + i * S::kA, &map_a, k, (int)w.a_row, i, bar, on);
                             }
+                        }
+#pragma unroll
+                        for (int i = 0; i < PARTS; ++i) {
                             if (S::kBmn) {
                                 for (int q = 0; q < blocks; ++q)
-                                    tma_load(b + q * S::kChunk * 128, &map_b, b0 + 64 * q, k, i, bar, on);
+                                    tma_load(b + i * S::kB + q * S::kChunk * 128, &map_b, b0 + 64 * q, k, i, bar, on);
                             } else {
-                                tma_load(b, &map_b, k, b0, i, bar, on);
+                                tma_load(b + i * S::kB, &map_b, k, b0, i, bar, on);
                             }
                         }
                         ++issued;
@@ -223,7 +228,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                         if (!ok) break;
                         tmem_fence_after();
                         const int steps = c + 1 < chunks ? S::kChunk / 16 : tail;
-                        const uint32_t a_at = base + stage * S::kStage, b_at = a_at + PARTS * S::kA;
+                        const uint32_t a_at = base + stage * S::kStage, b_at = a_at + S::kPartsA * S::kA;
                         const uint32_t a = uniform(S::kAmn ? mn_major_lo(a_at, S::kChunk * 128) : k_major_lo(a_at));
                         const uint32_t b = uniform(S::kBmn ? mn_major_lo(b_at, S::kChunk * 128) : k_major_lo(b_at));
                         constexpr uint32_t a_hi = S::kAmn ? kMnMajorHi : k_major_hi(S::kChunk * 2);
@@ -235,8 +240,8 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                                 // 16 entries on: 32 bytes along a row, or 16 rows of 128 bytes
                                 if (s < steps)
                                     mma_bf16<a_hi, b_hi>(
-                                        d, a + pair_a<PARTS>(S::kPairs, i) * (S::kA / 16) + s * (S::kAmn ? 128 : 2),
-                                        b + pair_b<PARTS>(S::kPairs, i) * (S::kB / 16) + s * (S::kBmn ? 128 : 2), idesc,
+                                        d, a + S::part_a(i) * (S::kA / 16) + s * (S::kAmn ? 128 : 2),
+                                        b + S::part_b(i) * (S::kB / 16) + s * (S::kBmn ? 128 : 2), idesc,
                                         i > 0 || s > 0 ? true : c > 0, on);
                             }
                         }
@@ -342,23 +347,23 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                             }
                             // staging is free again once the store before last has read it
                             const uint32_t stage0 = base + S::kStages * S::kStage +
-                                                    (set * S::kOutBuffers + out_buf) * (PARTS * kM * 64);
+                                                    (set * S::kOutBuffers + out_buf) * (S::kPartsG * kM * 64);
                             if (speaks) tma_store_wait_read<S::kOutBuffers - 1>();
                             named_sync(2 + set, 128);
                             const uint32_t line = stage0 + in_tile * 64;
 #pragma unroll
                             for (int g = 0; g < 4; ++g) {
                                 const uint32_t at = line + ((g ^ ((in_tile >> 1) & 3)) * 16);
-                                __nv_bfloat16 o[PARTS][8];
+                                __nv_bfloat16 o[S::kPartsG][8];
 #pragma unroll
                                 for (int j = 0; j < 8; ++j) {
-                                    __nv_bfloat16 q[PARTS];
-                                    split_parts<PARTS>(z[8 * g + j], q);
+                                    __nv_bfloat16 q[S::kPartsG];
+                                    split_parts<S::kPartsG>(z[8 * g + j], q);
 #pragma unroll
-                                    for (int i = 0; i < PARTS; ++i) o[i][j] = q[i];
+                                    for (int i = 0; i < S::kPartsG; ++i) o[i][j] = q[i];
                                 }
 #pragma unroll
-                                for (int i = 0; i < PARTS; ++i) {
+                                for (int i = 0; i < S::kPartsG; ++i) {
                                     uint4 v;
                                     memcpy(&v, o[i], 16);
                                     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + i * kM * 64),
@@ -370,7 +375,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                             named_sync(2 + set, 128);
                             if (speaks) {
 #pragma unroll
-                                for (int i = 0; i < PARTS; ++i)
+                                for (int i = 0; i < S::kPartsG; ++i)
                                     tma_store(&map_out, v0 + k * 32, (int)w.a_row, i, stage0 + i * kM * 64);
                                 tma_store_commit();
                             }
@@ -452,14 +457,17 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                                 *d4 = o;
                             }
                         } else {
-                            const int64_t at = (p.row0 + a_row) * p.columns + c;
+                            // 16 bytes at a time: the channels are a multiple of that here
+                            using T = TypeOf<PARTS>;
+                            constexpr int kVec = 16 / sizeof(T);
+                            T* dst = static_cast<T*>(p.out) + (p.row0 + a_row) * p.columns + c;
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) {
+                            for (int j = 0; j < 32; j += kVec) {
                                 if (c + j >= p.columns) continue;
-                                const float v = acc[q][j] * p.scale;
-                                if (p.out_type == MG_F32) static_cast<float*>(p.out)[at + j] = v;
-                                else if (p.out_type == MG_BF16) static_cast<__nv_bfloat16*>(p.out)[at + j] = from_f32<__nv_bfloat16>(v);
-                                else static_cast<__half*>(p.out)[at + j] = from_f32<__half>(v);
+                                float o[kVec];
+#pragma unroll
+                                for (int i = 0; i < kVec; ++i) o[i] = acc[q][j + i] * p.scale;
+                                store_row<T, kVec>(dst + j, o);
                             }
                         }
                     }

@@ -269,8 +269,11 @@ struct Sizes {
     int64_t class_columns() const { return up(classes, kN); }
     int64_t channel_columns() const { return up(channels, kN); }
     int64_t g_ld() const { return up(classes, 64) * 64; }
+    int g_parts() const { return parts == 1 ? 2 : parts; }
+    // dx straight from the product, in rows of whole 16-byte stores
+    bool direct() const { return by_row().splits == 1 && channels % (parts == 3 ? 4 : 8) == 0; }
     int64_t piece() const {
-        const int64_t fit = kPieceBytes / (2 * parts * g_ld()) / kM * kM;
+        const int64_t fit = kPieceBytes / (2 * g_parts() * g_ld()) / kM * kM;
         return std::min(up(rows, kM) * kM, std::max(kPieceRows, fit));
     }
     Shares stats() const { return split(class_columns(), row_tiles()); }
@@ -345,9 +348,8 @@ struct BackwardScratch {
             bias_part2 = nullptr;
         } else {
             row_values = class_bias = nullptr;
-            g = a.take<__nv_bfloat16>((size_t)n.piece() * n.parts * n.g_ld());
-            const int rs = n.by_row().splits;
-            row_part = a.take<float>(rs > 1 ? (size_t)rs * n.piece() * n.part_ld() : 0);
+            g = a.take<__nv_bfloat16>((size_t)n.piece() * n.g_parts() * n.g_ld());
+            row_part = a.take<float>(n.direct() ? 0 : (size_t)n.by_row().splits * n.piece() * n.part_ld());
             class_part = a.take<float>((size_t)n.by_class().splits * n.classes * n.part_ld());
             bias_part = a.take<float>((size_t)n.bias_lines() * n.classes);
             bias_part2 = a.take<float>((size_t)(n.pieces() * n.bias_shares()) * n.classes);
@@ -556,7 +558,7 @@ mg_status backward(const Args& a, const RowGrad& rg, const float* stats, T* dx, 
         const __nv_bfloat16* xs = f.xs + row0 * PARTS * n.depth();
         CUtensorMap mx, mg_out;
         MG_TRY(parts_map(&mx, xs, n, rows, kM));
-        MG_TRY(make_tensor_map(&mg_out, f.g, n.classes, rows, PARTS, n.g_ld() * 2, g_part, 32, kM,
+        MG_TRY(make_tensor_map(&mg_out, f.g, n.classes, rows, kGParts<PARTS>, n.g_ld() * 2, g_part, 32, kM,
                                false, "label_loss G"));
         TileArgs p{};
         p.units = up(rows, kM) * n.class_columns();
@@ -584,25 +586,24 @@ mg_status backward(const Args& a, const RowGrad& rg, const float* stats, T* dx, 
         p.columns = n.channels;
         if (dx != nullptr) {
             CUtensorMap mg_in;
-            MG_TRY(make_tensor_map(&mg_in, f.g, n.classes, rows, PARTS, n.g_ld() * 2, g_part, n.chunk(),
+            MG_TRY(make_tensor_map(&mg_in, f.g, n.classes, rows, kGParts<PARTS>, n.g_ld() * 2, g_part, n.chunk(),
                                    kM, n.chunk() == 64, "label_loss G"));
             const Shares sh = n.by_row();
             p.units = up(rows, kM) * n.channel_columns() * sh.splits;
             p.depth = n.classes;
             p.splits = sh.splits;
             p.per_split = sh.per_split;
-            p.part = sh.splits > 1 ? f.row_part : nullptr;
+            p.part = n.direct() ? nullptr : f.row_part;
             p.part_ld = n.part_ld();
             p.out = dx;
-            p.out_type = a.dtype;
             MG_TRY((launch_tiles<kProductRow, PARTS>(p, mg_in, mw_prod, mw_prod, a.st, "label_loss_backward rows")));
-            if (sh.splits > 1)
+            if (!n.direct())
                 MG_TRY(join(f.row_part, sh.splits, rows, n.part_ld(), n.channels, a.scale,
                             dx + row0 * n.channels, a.st));
         }
         if (dw != nullptr) {
             CUtensorMap mg_in, mx_prod;
-            MG_TRY(make_tensor_map(&mg_in, f.g, n.classes, rows, PARTS, n.g_ld() * 2, g_part, 64,
+            MG_TRY(make_tensor_map(&mg_in, f.g, n.classes, rows, kGParts<PARTS>, n.g_ld() * 2, g_part, 64,
                                    n.chunk(), true, "label_loss G"));
             MG_TRY(parts_map(&mx_prod, xs, n, rows, 0));
             const Shares sh = n.by_class();

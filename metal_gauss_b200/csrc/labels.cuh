@@ -68,6 +68,12 @@ __device__ __forceinline__ void split_parts(float v, __nv_bfloat16 (&p)[PARTS]) 
     }
 }
 
+// Parts of the logits' gradient: two also for bf16 features, whose gradients
+// then carry no other rounding than their own (one part alone brings their
+// error from 0.0017 to 0.0028 of the norm).
+template <int PARTS>
+constexpr int kGParts = PARTS == 1 ? 2 : PARTS;
+
 // Products of parts (a, b), smallest first: of the 1, 3, 4 or 6 pairs that
 // matter at PARTS parts, the i-th.
 template <int PARTS>
@@ -82,5 +88,29 @@ __device__ constexpr int pair_b(int pairs, int i) {
     if (PARTS == 2) return (i + 4 - pairs) == 0 || (i + 4 - pairs) == 2 ? 1 : 0;
     return i == 2 ? 2 : i == 1 || i == 4 ? 1 : 0;
 }
+
+// The same for products of G's parts with a side's.
+template <int PARTS>
+constexpr int kGPairs = PARTS == 1 ? 2 : PARTS == 2 ? 3 : 6;
+template <int PARTS>
+__device__ constexpr int g_pair_a(int i) {
+    return PARTS == 1 ? 1 - i : pair_a<PARTS>(kGPairs<PARTS>, i);
+}
+template <int PARTS>
+__device__ constexpr int g_pair_b(int i) {
+    return PARTS == 1 ? 0 : pair_b<PARTS>(kGPairs<PARTS>, i);
+}
+
+// The features' type, by its parts.
+template <int PARTS>
+struct PartsType;
+template <>
+struct PartsType<1> { using type = __nv_bfloat16; };
+template <>
+struct PartsType<2> { using type = __half; };
+template <>
+struct PartsType<3> { using type = float; };
+template <int PARTS>
+using TypeOf = typename PartsType<PARTS>::type;
 
 }  // namespace mg
