@@ -18,7 +18,7 @@ struct Shape {
     static constexpr bool kProduct = MODE >= kProductRow;
     // Sets of four warps that take tiles out, 32 columns at a time in turn: the
     // exponentials of kStats wait on one another's latency and want many.
-    static constexpr int kSets = MODE == kStats ? 4 : 2;
+    static constexpr int kSets = MODE == kStats || (MODE == kLogitGrad && PARTS < 3) ? 4 : 2;
     static constexpr int kThreads = 64 + 128 * kSets;  // and a copying and an issuing warp
     static constexpr bool kAmn = MODE == kProductClass;  // A's row index runs fastest
     static constexpr bool kBmn = kProduct;
@@ -30,8 +30,8 @@ struct Shape {
     static constexpr int kStage = kPartsA * kA + PARTS * kB;
     static constexpr int kStages = PARTS == 3 ? (MODE == kLogitGrad ? 2 : 3) : (MODE == kStats ? 4 : 3);
     // G on its way out: 128 x 32 bf16 for each set of the taking warps, part and buffer
-    static constexpr int kOutBuffers = PARTS == 3 ? 1 : 2;
-    static constexpr int kOut = MODE == kLogitGrad ? 2 * kPartsG * kOutBuffers * kM * 64 : 0;
+    static constexpr int kOutBuffers = 1;
+    static constexpr int kOut = MODE == kLogitGrad ? kSets * kPartsG * kOutBuffers * kM * 64 : 0;
     static constexpr int kDynamic = 1024 + kStages * kStage + kOut;
     // Products of parts (a, b), smallest first.
     static constexpr int kPairs = kProduct ? kGPairs<PARTS> : PARTS == 1 ? 1 : PARTS == 2 ? 4 : 6;
@@ -100,6 +100,19 @@ __device__ __forceinline__ Walk walk_unit(const TileArgs& p, int64_t u) {
         w.tiles = (int)((w.c1 - w.c0 + p.per_segment - 1) / p.per_segment);
     }
     return w;
+}
+
+// Sums of products to logits in base 2: bias times log2 e from shared memory.
+template <int N>
+__device__ __forceinline__ void scores(float (&z)[N], float c2, const float* bias) {
+#pragma unroll
+    for (int j = 0; j < N; j += 4) {
+        const float4 b = *reinterpret_cast<const float4*>(bias + j);
+        z[j] = fmaf(z[j], c2, b.x);
+        z[j + 1] = fmaf(z[j + 1], c2, b.y);
+        z[j + 2] = fmaf(z[j + 2], c2, b.z);
+        z[j + 3] = fmaf(z[j + 3], c2, b.w);
+    }
 }
 
 template <int MODE, int PARTS>
@@ -303,21 +316,14 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                     mbar_wait(taken_full + 8 * buf, buf_phase, &stop, p.error_word, DEV_ERR_TILE_WAIT);
                     tmem_fence_after();
                     for (int k = set; k * 32 < n; k += S::kSets) {
-                        float z[32];
-                        tmem_load32(lanes + buf * kN + k * 32, z);
-#pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
-                            const float4 b = *reinterpret_cast<const float4*>(&bias_s[buf][k * 32 + j]);
-                            z[j] = fmaf(z[j], c2, b.x);
-                            z[j + 1] = fmaf(z[j + 1], c2, b.y);
-                            z[j + 2] = fmaf(z[j + 2], c2, b.z);
-                            z[j + 3] = fmaf(z[j + 3], c2, b.w);
-                        }
+                        const uint32_t at = lanes + buf * kN + k * 32;
                         const int rel = lab - v0 - k * 32;
-                        const bool here = (unsigned)rel < 32u;
-                        const bool any = __any_sync(0xffffffffu, here);
                         if constexpr (MODE == kStats) {
-                            if (any) {
+                            float z[32];
+                            tmem_load(at, z);
+                            scores<32>(z, c2, &bias_s[buf][k * 32]);
+                            const bool here = (unsigned)rel < 32u;
+                            if (__any_sync(0xffffffffu, here)) {
                                 float zl = 0.0f;
 #pragma unroll
                                 for (int j = 0; j < 32; ++j) {
@@ -338,37 +344,66 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                             s = (q[0] + q[1]) + (q[2] + q[3]);
                             m = top;
                         } else {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) z[j] = exp2_fast(z[j] - lse) * r;
-                            if (any) {
-#pragma unroll
-                                for (int j = 0; j < 32; ++j)
-                                    if (j == rel) z[j] = at_label;
-                            }
-                            // staging is free again once the store before last has read it
+                            // staging is free again once the store before has read it
                             const uint32_t stage0 = base + S::kStages * S::kStage +
                                                     (set * S::kOutBuffers + out_buf) * (S::kPartsG * kM * 64);
                             if (speaks) tma_store_wait_read<S::kOutBuffers - 1>();
                             named_sync(2 + set, 128);
-                            const uint32_t line = stage0 + in_tile * 64;
+                            // 16 columns at a time, the loop not unrolled: its code
+                            // has to stay in the instruction cache
+#pragma unroll 1
+                            for (int h = 0; h < 32; h += 16) {
+                                float z[16];
+                                tmem_load(at + h, z);
+                                scores<16>(z, c2, &bias_s[buf][k * 32 + h]);
 #pragma unroll
-                            for (int g = 0; g < 4; ++g) {
-                                const uint32_t at = line + ((g ^ ((in_tile >> 1) & 3)) * 16);
-                                __nv_bfloat16 o[S::kPartsG][8];
+                                for (int j = 0; j < 16; ++j) z[j] = exp2_fast(z[j] - lse) * r;
+                                if (__any_sync(0xffffffffu, (unsigned)(rel - h) < 16u)) {
 #pragma unroll
-                                for (int j = 0; j < 8; ++j) {
-                                    __nv_bfloat16 q[S::kPartsG];
-                                    split_parts<S::kPartsG>(z[8 * g + j], q);
-#pragma unroll
-                                    for (int i = 0; i < S::kPartsG; ++i) o[i][j] = q[i];
+                                    for (int j = 0; j < 16; ++j)
+                                        if (j == rel - h) z[j] = at_label;
                                 }
+                                if (p.part_bias != nullptr) {
+                                    // lanes c and c + 16 end with the sums of column c over
+                                    // half of the warp's 32 rows each
+                                    float q[16];
+#pragma unroll
+                                    for (int j = 0; j < 16; ++j) q[j] = z[j];
+#pragma unroll
+                                    for (int o = 8; o > 0; o >>= 1) {
+#pragma unroll
+                                        for (int j = 0; j < o; ++j) {
+                                            const bool up = (lane & o) != 0;
+                                            const float send = up ? q[j] : q[j + o];
+                                            const float keep = up ? q[j + o] : q[j];
+                                            q[j] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+                                        }
+                                    }
+                                    q[0] += __shfl_xor_sync(0xffffffffu, q[0], 16);
+                                    const int v = v0 + k * 32 + h + lane;
+                                    if (lane < 16 && v < p.columns)
+                                        p.part_bias[(w.a_row / 32 + quarter) * p.columns + v] = q[0];
+                                }
+                                // part i of 8 columns: 16 bytes of this row's 64, swizzled
 #pragma unroll
                                 for (int i = 0; i < S::kPartsG; ++i) {
-                                    uint4 v;
-                                    memcpy(&v, o[i], 16);
-                                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + i * kM * 64),
-                                                 "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
-                                                 : "memory");
+#pragma unroll
+                                    for (int g = 0; g < 2; ++g) {
+                                        uint32_t word[4];
+#pragma unroll
+                                        for (int j = 0; j < 4; ++j) {
+                                            float& lo = z[8 * g + 2 * j];
+                                            float& hi = z[8 * g + 2 * j + 1];
+                                            word[j] = pack_bf16(lo, hi);
+                                            lo -= __uint_as_float(word[j] << 16);
+                                            hi -= __uint_as_float(word[j] & 0xffff0000u);
+                                        }
+                                        const int piece = (h / 8 + g) ^ ((in_tile >> 1) & 3);
+                                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
+                                                         stage0 + i * kM * 64 + in_tile * 64 + piece * 16),
+                                                     "r"(word[0]), "r"(word[1]), "r"(word[2]), "r"(word[3])
+                                                     : "memory");
+                                    }
                                 }
                             }
                             fence_async_shared();
@@ -380,22 +415,6 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                                 tma_store_commit();
                             }
                             if (++out_buf == S::kOutBuffers) out_buf = 0;
-                            if (p.part_bias != nullptr) {
-                                // lane c ends with the sum of column c over the warp's 32 rows
-#pragma unroll
-                                for (int o = 16; o > 0; o >>= 1) {
-#pragma unroll
-                                    for (int j = 0; j < o; ++j) {
-                                        const bool up = (lane & o) != 0;
-                                        const float send = up ? z[j] : z[j + o];
-                                        const float keep = up ? z[j + o] : z[j];
-                                        z[j] = keep + __shfl_xor_sync(0xffffffffu, send, o);
-                                    }
-                                }
-                                const int v = v0 + k * 32 + lane;
-                                const int64_t line32 = w.a_row / 32 + quarter;
-                                if (v < p.columns) p.part_bias[line32 * p.columns + v] = z[0];
-                            }
                         }
                     }
                     tmem_fence_before();
@@ -424,7 +443,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                     for (int q = 0; q < 4; ++q) {
                         if ((2 * q + set) * 32 < n) {
                             float v[32];
-                            tmem_load32(lanes + buf * kN + (2 * q + set) * 32, v);
+                            tmem_load(lanes + buf * kN + (2 * q + set) * 32, v);
 #pragma unroll
                             for (int j = 0; j < 32; ++j) acc[q][j] += v[j];
                         }

@@ -68,6 +68,13 @@ __device__ __forceinline__ void split_parts(float v, __nv_bfloat16 (&p)[PARTS]) 
     }
 }
 
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    uint32_t r;
+    memcpy(&r, &v, 4);
+    return r;
+}
+
 // Parts of the logits' gradient: two also for bf16 features, whose gradients
 // then carry no other rounding than their own (one part alone brings their
 // error from 0.0017 to 0.0028 of the norm).
