@@ -55,9 +55,7 @@ struct FusedArgs {         // counts below 2^31: at most 2^30 rows
     int32_t* error_word;
 };
 
-// What the scores need of a row: log2 of its sum, r, G at its label, its label
-// (an int), each 64 in a row per block of 64 rows.
-constexpr int kRowValues = 4;
+static_assert(kStream == kRowBlock, "a streamed tile is a block of row values");
 constexpr int kColumnBytes = kRowValues * kStream * 4;  // of a streamed tile, beside its parts
 
 struct FusedWalk {

@@ -50,10 +50,9 @@ struct TileArgs {
     int64_t row0;           // the piece's first row
     int64_t rows;           // rows in all
     float scale;
-    const float* bias;
-    LabelSource labels;
-    RowGrad rg;
-    const float* stats;     // kLogitGrad: log2 of the sum, 1 - softmax(label)
+    const float* class_bias;   // bias times log2 e, -infinity past the last class
+    const int32_t* row_labels; // kStats
+    const float* row_values;   // kLogitGrad
     float *part_m, *part_s, *label_z;  // kStats
     float* part_bias;       // kLogitGrad: sums of 32 rows of G, or NULL
     float* part;            // products: fp32 shares (splits, a_rows, part_ld), or NULL
@@ -100,6 +99,29 @@ __device__ __forceinline__ Walk walk_unit(const TileArgs& p, int64_t u) {
         w.tiles = (int)((w.c1 - w.c0 + p.per_segment - 1) / p.per_segment);
     }
     return w;
+}
+
+// What a row's scores need.
+struct RowIn {
+    int lab = kIgnored;
+    float lse = kInf, r = 0.0f, at_label = 0.0f;
+};
+
+template <int MODE>
+__device__ __forceinline__ RowIn row_in(const TileArgs& p, int64_t a_row) {
+    RowIn in;
+    if (a_row >= p.a_rows) return in;
+    const int64_t row = p.row0 + a_row;
+    if constexpr (MODE == kStats) {
+        in.lab = p.row_labels[row];
+    } else {
+        const float* v = p.row_values + row / kRowBlock * (kRowValues * kRowBlock) + row % kRowBlock;
+        in.lse = v[0];
+        in.r = v[kRowBlock];
+        in.at_label = v[2 * kRowBlock];
+        in.lab = __float_as_int(v[3 * kRowBlock]);
+    }
+    return in;
 }
 
 // Sums of products to logits in base 2: bias times log2 e from shared memory.
@@ -288,31 +310,35 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
         const float c2 = p.scale * kLog2e;
         int buf = 0, out_buf = 0;
         uint32_t buf_phase = 0;
+        RowIn next_row;
+        float next_bias = 0.0f;
+        if constexpr (!S::kProduct) {
+            const Walk first = walk_unit<MODE, PARTS>(p, blockIdx.x);
+            next_row = row_in<MODE>(p, first.a_row + in_tile);
+            if (et < kN) next_bias = p.class_bias[first.first * kN + et];
+        }
         for (int64_t u = blockIdx.x; u < p.units; u += gridDim.x) {
             const Walk w = walk_unit<MODE, PARTS>(p, u);
             const int64_t a_row = w.a_row + in_tile;
             const bool mine = a_row < p.a_rows;
             if constexpr (!S::kProduct) {
                 const int64_t row = p.row0 + a_row;
-                const int lab = mine ? p.labels.at(row) : kIgnored;
+                const int lab = next_row.lab;
+                const float lse = next_row.lse, r = next_row.r, at_label = next_row.at_label;
                 float m = -kInf, s = 0.0f;
-                float lse = kInf, at_label = 0.0f, r = 0.0f;
-                if (MODE == kLogitGrad && lab >= 0) {
-                    r = p.rg.at(row, lab);
-                    lse = p.stats[row];
-                    at_label = -p.stats[p.rows + row] * r;
-                }
-                const auto bias_of = [&](int v) {
-                    return p.bias != nullptr && et < kN && v < p.columns ? p.bias[v] : 0.0f;
-                };
-                float next_bias = bias_of(w.first * kN + et);
                 for (int t = 0; t < w.tiles; ++t) {
                     const int v0 = (w.first + t) * kN;
                     const int n = min(kN, p.columns - v0);
-                    // bias times log2 e; classes past the end are taken out
-                    if (et < kN) bias_s[buf][et] = et < n ? next_bias * kLog2e : -kInf;
+                    if (et < kN) bias_s[buf][et] = next_bias;
                     named_sync(1, 128 * S::kSets);
-                    next_bias = bias_of(v0 + kN + et);  // of the next tile, while this one is taken
+                    // the next tile's values come while this one is taken
+                    if (t + 1 < w.tiles) {
+                        next_bias = et < kN ? p.class_bias[v0 + kN + et] : 0.0f;
+                    } else if (u + gridDim.x < p.units) {
+                        const Walk next = walk_unit<MODE, PARTS>(p, u + gridDim.x);
+                        next_bias = et < kN ? p.class_bias[next.first * kN + et] : 0.0f;
+                        next_row = row_in<MODE>(p, next.a_row + in_tile);
+                    }
                     mbar_wait(taken_full + 8 * buf, buf_phase, &stop, p.error_word, DEV_ERR_TILE_WAIT);
                     tmem_fence_after();
                     for (int k = set; k * 32 < n; k += S::kSets) {

@@ -37,12 +37,14 @@ namespace mg {
 
 namespace {
 
-// What the backward pass's scores need beside the parts (label_fused.cuh).
+// What the scores need beside the parts: labels (forward) or the row values
+// (backward), and the bias.
 struct ColumnValues {
     RowGrad rg;
     const float* stats;
     const float* bias;
-    float* row_values;  // NULL in the forward pass
+    int32_t* row_labels;
+    float* row_values;
     float* class_bias;
 };
 
@@ -58,7 +60,8 @@ split_kernel(const T* __restrict__ x, const T* __restrict__ w, LabelSource label
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int64_t all = i / groups;
     const int c = (int)(i - all * groups) * 8;
-    if (cv.row_values != nullptr && i < (rows + kStream - 1) / kStream * kStream) {
+    if (cv.row_labels != nullptr && i < rows) cv.row_labels[i] = labels.at(i);
+    if (cv.row_values != nullptr && i < (rows + kRowBlock - 1) / kRowBlock * kRowBlock) {
         float v[kRowValues] = {kInf, 0.0f, 0.0f, __int_as_float(kIgnored)};
         if (i < rows) {
             const int lab = labels.at(i);
@@ -71,9 +74,9 @@ split_kernel(const T* __restrict__ x, const T* __restrict__ w, LabelSource label
         }
 #pragma unroll
         for (int k = 0; k < kRowValues; ++k)
-            cv.row_values[i / kStream * (kRowValues * kStream) + k * kStream + i % kStream] = v[k];
+            cv.row_values[i / kRowBlock * (kRowValues * kRowBlock) + k * kRowBlock + i % kRowBlock] = v[k];
     }
-    if (cv.class_bias != nullptr && i < (classes + kOwn - 1) / kOwn * kOwn)
+    if (i < (classes + kClassPad - 1) / kClassPad * kClassPad)
         cv.class_bias[i] = i < classes ? (cv.bias != nullptr ? cv.bias[i] * kLog2e : 0.0f) : -kInf;
     if (all >= rows + classes) return;
     const bool feature = all < rows;
@@ -295,6 +298,7 @@ struct Sizes {
         return s.splits == 1 && (parts == 3 || s.per_split <= fused_segment()) &&
                channels % (parts == 3 ? 4 : 8) == 0;
     }
+    int64_t class_pad() const { return up(classes, kClassPad) * kClassPad; }
     int64_t row_blocks() const { return up(rows, 256); }
     // the bias's gradient: sums of 32 rows, then of up to kBiasLines of those
     int64_t pieces() const { return up(rows, piece()); }
@@ -314,13 +318,16 @@ struct Scratch {
 
 struct ForwardScratch {
     __nv_bfloat16 *xs, *ws;
-    float *m, *s, *z;
+    int32_t* row_labels;
+    float *class_bias, *m, *s, *z;
     double* sums;
     size_t bytes;
     ForwardScratch(void* base, const Sizes& n) {
         Scratch a{static_cast<char*>(base)};
         xs = a.take<__nv_bfloat16>((size_t)n.rows * n.parts * n.depth());
         ws = a.take<__nv_bfloat16>((size_t)n.classes * n.parts * n.depth());
+        row_labels = a.take<int32_t>((size_t)n.rows);
+        class_bias = a.take<float>((size_t)n.class_pad());
         m = a.take<float>((size_t)n.stats().splits * Shape<kStats, 1>::kSets * n.rows);
         s = a.take<float>((size_t)n.stats().splits * Shape<kStats, 1>::kSets * n.rows);
         z = a.take<float>((size_t)n.rows);
@@ -337,17 +344,16 @@ struct BackwardScratch {
         Scratch a{static_cast<char*>(base)};
         xs = a.take<__nv_bfloat16>((size_t)n.rows * n.parts * n.depth());
         ws = a.take<__nv_bfloat16>((size_t)n.classes * n.parts * n.depth());
+        row_values = a.take<float>((size_t)up(n.rows, kRowBlock) * kRowBlock * kRowValues);
+        class_bias = a.take<float>((size_t)n.class_pad());
         if (n.fused()) {
             const Shares rs = n.fused_by_row(), cs = n.fused_by_class();
             g = nullptr;
-            row_values = a.take<float>((size_t)up(n.rows, kStream) * kStream * kRowValues);
-            class_bias = a.take<float>((size_t)up(n.classes, kOwn) * kOwn);
             row_part = a.take<float>(n.fused_direct() ? 0 : (size_t)rs.splits * n.rows * n.part_ld());
             class_part = a.take<float>((size_t)cs.splits * n.classes * n.part_ld());
             bias_part = a.take<float>((size_t)cs.splits * kGroups * n.classes);
             bias_part2 = nullptr;
         } else {
-            row_values = class_bias = nullptr;
             g = a.take<__nv_bfloat16>((size_t)n.piece() * n.g_parts() * n.g_ld());
             row_part = a.take<float>(n.direct() ? 0 : (size_t)n.by_row().splits * n.piece() * n.part_ld());
             class_part = a.take<float>((size_t)n.by_class().splits * n.classes * n.part_ld());
@@ -388,10 +394,10 @@ mg_status launch_tiles(const TileArgs& p, const CUtensorMap& a, const CUtensorMa
 
 template <typename T>
 mg_status split_inputs(const Args& a, __nv_bfloat16* xs, __nv_bfloat16* ws,
-                       const ColumnValues& cv = {}) {
+                       const ColumnValues& cv) {
     // a thread for each 8 channels, and for each of the padded rows and classes
     const int64_t threads = std::max({(a.n.rows + a.n.classes) * (a.n.depth() / 8),
-                                      up(a.n.rows, kStream) * kStream, up(a.n.classes, kOwn) * kOwn});
+                                      up(a.n.rows, kRowBlock) * kRowBlock, a.n.class_pad()});
     split_kernel<T><<<(unsigned)up(threads, 256), 256, 0, a.st>>>(
         static_cast<const T*>(a.x), static_cast<const T*>(a.w), a.labels, a.n.rows, a.n.classes,
         a.n.channels, a.n.depth(), cv, xs, ws);
@@ -415,7 +421,7 @@ mg_status forward(const Args& a, int reduction, float* loss, float* stats, float
                   void* scratch) {
     constexpr int PARTS = kPartsOf<T>;
     const ForwardScratch f(scratch, a.n);
-    MG_TRY((split_inputs<T>(a, f.xs, f.ws)));
+    MG_TRY((split_inputs<T>(a, f.xs, f.ws, ColumnValues{{}, nullptr, a.bias, f.row_labels, nullptr, f.class_bias})));
     CUtensorMap mx, mw;
     MG_TRY(parts_map(&mx, f.xs, a.n, a.n.rows, kM));
     MG_TRY(parts_map(&mw, f.ws, a.n, a.n.classes, kN));
@@ -428,8 +434,8 @@ mg_status forward(const Args& a, int reduction, float* loss, float* stats, float
     p.splits = sh.splits;
     p.per_split = sh.per_split;
     p.scale = a.scale;
-    p.bias = a.bias;
-    p.labels = a.labels;
+    p.class_bias = f.class_bias;
+    p.row_labels = f.row_labels;
     p.part_m = f.m;
     p.part_s = f.s;
     p.label_z = f.z;
@@ -491,7 +497,7 @@ mg_status backward_fused(const Args& a, const RowGrad& rg, const float* stats, T
     constexpr int PARTS = kPartsOf<T>;
     const Sizes& n = a.n;
     const BackwardScratch f(scratch, n);
-    MG_TRY((split_inputs<T>(a, f.xs, f.ws, ColumnValues{rg, stats, a.bias, f.row_values, f.class_bias})));
+    MG_TRY((split_inputs<T>(a, f.xs, f.ws, ColumnValues{rg, stats, a.bias, nullptr, f.row_values, f.class_bias})));
     const int64_t part = 2 * (int64_t)n.depth(), row = n.parts * part;
     const auto map = [&](CUtensorMap* m, const __nv_bfloat16* b, int64_t rows, int box) {
         return make_tensor_map(m, b, n.depth(), rows, PARTS, row, part, 64, box, true, "label_loss parts");
@@ -548,7 +554,7 @@ mg_status backward(const Args& a, const RowGrad& rg, const float* stats, T* dx, 
     const Sizes& n = a.n;
     if (n.fused()) return backward_fused<T>(a, rg, stats, dx, dw, db, scratch);
     const BackwardScratch f(scratch, n);
-    MG_TRY((split_inputs<T>(a, f.xs, f.ws)));
+    MG_TRY((split_inputs<T>(a, f.xs, f.ws, ColumnValues{rg, stats, a.bias, nullptr, f.row_values, f.class_bias})));
     CUtensorMap mw_score, mw_prod;
     MG_TRY(parts_map(&mw_score, f.ws, n, n.classes, kN));
     MG_TRY(parts_map(&mw_prod, f.ws, n, n.classes, 0));
@@ -569,10 +575,8 @@ mg_status backward(const Args& a, const RowGrad& rg, const float* stats, T* dx, 
         p.columns = n.classes;
         p.splits = 1;
         p.scale = a.scale;
-        p.bias = a.bias;
-        p.labels = a.labels;
-        p.rg = rg;
-        p.stats = stats;
+        p.class_bias = f.class_bias;
+        p.row_values = f.row_values;
         p.part_bias = db != nullptr ? f.bias_part : nullptr;
         p.error_word = device_error_word();
         MG_TRY((launch_tiles<kLogitGrad, PARTS>(p, mx, mw_score, mg_out, a.st, "label_loss_backward logits")));

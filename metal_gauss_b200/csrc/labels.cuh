@@ -41,6 +41,12 @@ struct RowGrad {
     }
 };
 
+// What the backward pass's scores need of a row: log2 of its sum, r, G at its
+// label, its label (an int), each kRowBlock in a row per block of rows.
+constexpr int kRowValues = 4;
+constexpr int kRowBlock = 64;
+constexpr int kClassPad = 256;  // class_bias is padded to a multiple of this
+
 constexpr float kInf = __builtin_huge_valf();
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
