@@ -131,14 +131,25 @@ __device__ __forceinline__ void store_parts(uint32_t group, int k, float (&z)[kS
         uint32_t r[kStep / 2];
 #pragma unroll
         for (int j = 0; j < kStep / 2; ++j) {
-            r[j] = pack_bf16(z[2 * j], z[2 * j + 1]);
-            if (i + 1 < GP) {
-                z[2 * j] -= __uint_as_float(r[j] << 16);
-                z[2 * j + 1] -= __uint_as_float(r[j] & 0xffff0000u);
-            }
+            if (i + 1 < GP) r[j] = take_part(z[2 * j], z[2 * j + 1]);
+            else r[j] = pack_bf16(z[2 * j], z[2 * j + 1]);
         }
         tmem_store(group + g_column(i, k), r);
     }
+}
+
+// Four sums of products to r softmax: logits in base 2 (scale, bias), minus the
+// log of the row's sum, exponential, times r.
+__device__ __forceinline__ void gradients(float* z, float c2, float2 bias0, float2 bias1, float2 lse0,
+                                          float2 lse1, float2 r0, float2 r1) {
+    const float2 a = add2(fma2(make_float2(z[0], z[1]), both(c2), bias0), lse0);
+    const float2 b = add2(fma2(make_float2(z[2], z[3]), both(c2), bias1), lse1);
+    const float2 e = mul2(make_float2(exp2_fast(a.x), exp2_fast(a.y)), r0);
+    const float2 f = mul2(make_float2(exp2_fast(b.x), exp2_fast(b.y)), r1);
+    z[0] = e.x;
+    z[1] = e.y;
+    z[2] = f.x;
+    z[3] = f.y;
 }
 
 template <bool BY_CLASS, int PARTS>
@@ -423,10 +434,8 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
                         for (int j = 0; j < kStep; j += 4) {
                             const float4 a = shared_float4(col + 4 * (k + j));
                             const float4 b = shared_float4(col + 4 * (kStream + k + j));
-                            z[j] = exp2_fast(fmaf(z[j], c2, own_bias) - a.x) * b.x;
-                            z[j + 1] = exp2_fast(fmaf(z[j + 1], c2, own_bias) - a.y) * b.y;
-                            z[j + 2] = exp2_fast(fmaf(z[j + 2], c2, own_bias) - a.z) * b.z;
-                            z[j + 3] = exp2_fast(fmaf(z[j + 3], c2, own_bias) - a.w) * b.w;
+                            gradients(z + j, c2, both(own_bias), both(own_bias), make_float2(-a.x, -a.y),
+                                      make_float2(-a.z, -a.w), make_float2(b.x, b.y), make_float2(b.z, b.w));
                         }
                         // rows labelled with one of this warp's classes
                         const int mine = shared_int(col + 4 * (3 * kStream + k + (lane & (kStep - 1)))) - w.own0 - quarter * 32;
@@ -446,10 +455,8 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
 #pragma unroll
                         for (int j = 0; j < kStep; j += 4) {
                             const float4 b = shared_float4(col + 4 * (k + j));
-                            z[j] = exp2_fast(fmaf(z[j], c2, b.x) - lse) * r;
-                            z[j + 1] = exp2_fast(fmaf(z[j + 1], c2, b.y) - lse) * r;
-                            z[j + 2] = exp2_fast(fmaf(z[j + 2], c2, b.z) - lse) * r;
-                            z[j + 3] = exp2_fast(fmaf(z[j + 3], c2, b.w) - lse) * r;
+                            gradients(z + j, c2, make_float2(b.x, b.y), make_float2(b.z, b.w), both(-lse), both(-lse),
+                                      both(r), both(r));
                         }
                         const int rel = lab - t * kStream - k;
                         if (__any_sync(0xffffffffu, (unsigned)rel < (unsigned)kStep)) {

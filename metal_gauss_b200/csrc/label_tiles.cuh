@@ -124,16 +124,19 @@ __device__ __forceinline__ RowIn row_in(const TileArgs& p, int64_t a_row) {
     return in;
 }
 
-// Sums of products to logits in base 2: bias times log2 e from shared memory.
+// Sums of products to logits in base 2; `bias`, the same for all lanes, is
+// read through L1 (no barrier between the warps of a tile).
 template <int N>
-__device__ __forceinline__ void scores(float (&z)[N], float c2, const float* bias) {
+__device__ __forceinline__ void scores(float (&z)[N], float c2, const float* __restrict__ bias) {
 #pragma unroll
     for (int j = 0; j < N; j += 4) {
-        const float4 b = *reinterpret_cast<const float4*>(bias + j);
-        z[j] = fmaf(z[j], c2, b.x);
-        z[j + 1] = fmaf(z[j + 1], c2, b.y);
-        z[j + 2] = fmaf(z[j + 2], c2, b.z);
-        z[j + 3] = fmaf(z[j + 3], c2, b.w);
+        const float4 b = __ldg(reinterpret_cast<const float4*>(bias + j));
+        const float2 lo = fma2(make_float2(z[j], z[j + 1]), both(c2), make_float2(b.x, b.y));
+        const float2 hi = fma2(make_float2(z[j + 2], z[j + 3]), both(c2), make_float2(b.z, b.w));
+        z[j] = lo.x;
+        z[j + 1] = lo.y;
+        z[j + 2] = hi.x;
+        z[j + 3] = hi.y;
     }
 }
 
@@ -143,7 +146,6 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
             const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_out) {
     using S = Shape<MODE, PARTS>;
     extern __shared__ uint8_t dynamic[];
-    __shared__ alignas(16) float bias_s[2][kN];
     __shared__ uint64_t bars[2 * S::kStages + 5];
     __shared__ uint32_t tmem_s;
     __shared__ volatile int stop;
@@ -303,7 +305,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
         // `set` the 32-column chunks it takes (every kSets-th). After a wait
         // that gave up the remaining waits fail at once and the block runs to
         // its end on whatever is there; the error word says so.
-        const int quarter = warp & 3, set = (warp - 2) / 4, et = threadIdx.x - 64;
+        const int quarter = warp & 3, set = (warp - 2) / 4;
         const int in_tile = quarter * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
         const bool speaks = quarter == 0 && lane == 0;  // for its set's stores
@@ -311,12 +313,8 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
         int buf = 0, out_buf = 0;
         uint32_t buf_phase = 0;
         RowIn next_row;
-        float next_bias = 0.0f;
-        if constexpr (!S::kProduct) {
-            const Walk first = walk_unit<MODE, PARTS>(p, blockIdx.x);
-            next_row = row_in<MODE>(p, first.a_row + in_tile);
-            if (et < kN) next_bias = p.class_bias[first.first * kN + et];
-        }
+        if constexpr (!S::kProduct)
+            next_row = row_in<MODE>(p, walk_unit<MODE, PARTS>(p, blockIdx.x).a_row + in_tile);
         for (int64_t u = blockIdx.x; u < p.units; u += gridDim.x) {
             const Walk w = walk_unit<MODE, PARTS>(p, u);
             const int64_t a_row = w.a_row + in_tile;
@@ -329,16 +327,8 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                 for (int t = 0; t < w.tiles; ++t) {
                     const int v0 = (w.first + t) * kN;
                     const int n = min(kN, p.columns - v0);
-                    if (et < kN) bias_s[buf][et] = next_bias;
-                    named_sync(1, 128 * S::kSets);
-                    // the next tile's values come while this one is taken
-                    if (t + 1 < w.tiles) {
-                        next_bias = et < kN ? p.class_bias[v0 + kN + et] : 0.0f;
-                    } else if (u + gridDim.x < p.units) {
-                        const Walk next = walk_unit<MODE, PARTS>(p, u + gridDim.x);
-                        next_bias = et < kN ? p.class_bias[next.first * kN + et] : 0.0f;
-                        next_row = row_in<MODE>(p, next.a_row + in_tile);
-                    }
+                    if (t + 1 == w.tiles && u + gridDim.x < p.units)  // while this tile is taken
+                        next_row = row_in<MODE>(p, walk_unit<MODE, PARTS>(p, u + gridDim.x).a_row + in_tile);
                     mbar_wait(taken_full + 8 * buf, buf_phase, &stop, p.error_word, DEV_ERR_TILE_WAIT);
                     tmem_fence_after();
                     for (int k = set; k * 32 < n; k += S::kSets) {
@@ -347,27 +337,41 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                         if constexpr (MODE == kStats) {
                             float z[32];
                             tmem_load(at, z);
-                            scores<32>(z, c2, &bias_s[buf][k * 32]);
-                            const bool here = (unsigned)rel < 32u;
-                            if (__any_sync(0xffffffffu, here)) {
-                                float zl = 0.0f;
+                            scores<32>(z, c2, p.class_bias + v0 + k * 32);
+                            // the label's logit goes apart, 8 columns at a time: most
+                            // have no row's label
 #pragma unroll
-                                for (int j = 0; j < 32; ++j) {
-                                    if (j == rel) {
-                                        zl = z[j];
-                                        z[j] = -kInf;
+                            for (int h = 0; h < 32; h += 8) {
+                                const bool here = (unsigned)(rel - h) < 8u;
+                                if (__any_sync(0xffffffffu, here)) {
+                                    float zl = 0.0f;
+#pragma unroll
+                                    for (int j = h; j < h + 8; ++j) {
+                                        if (j == rel) {
+                                            zl = z[j];
+                                            z[j] = -kInf;
+                                        }
                                     }
+                                    if (here) p.label_z[row] = zl;
                                 }
-                                if (here) p.label_z[row] = zl;
                             }
-                            float top = m;
+                            float t0 = m, t1 = -kInf;
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) top = fmaxf(top, z[j]);
+                            for (int j = 0; j < 32; j += 4) {
+                                t0 = max3(t0, z[j], z[j + 1]);
+                                t1 = max3(t1, z[j + 2], z[j + 3]);
+                            }
+                            const float top = fmaxf(t0, t1);
                             const float ref = top == -kInf ? 0.0f : top;
-                            float q[4] = {s * exp2_fast(m - ref), 0.0f, 0.0f, 0.0f};
+                            float2 q0 = make_float2(s * exp2_fast(m - ref), 0.0f), q1 = make_float2(0.0f, 0.0f);
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) q[j % 4] += exp2_fast(z[j] - ref);
-                            s = (q[0] + q[1]) + (q[2] + q[3]);
+                            for (int j = 0; j < 32; j += 4) {
+                                const float2 a = add2(make_float2(z[j], z[j + 1]), both(-ref));
+                                const float2 b = add2(make_float2(z[j + 2], z[j + 3]), both(-ref));
+                                q0 = add2(q0, make_float2(exp2_fast(a.x), exp2_fast(a.y)));
+                                q1 = add2(q1, make_float2(exp2_fast(b.x), exp2_fast(b.y)));
+                            }
+                            s = (q0.x + q0.y) + (q1.x + q1.y);
                             m = top;
                         } else {
                             // staging is free again once the store before has read it
@@ -381,9 +385,14 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                             for (int h = 0; h < 32; h += 16) {
                                 float z[16];
                                 tmem_load(at + h, z);
-                                scores<16>(z, c2, &bias_s[buf][k * 32 + h]);
+                                scores<16>(z, c2, p.class_bias + v0 + k * 32 + h);
 #pragma unroll
-                                for (int j = 0; j < 16; ++j) z[j] = exp2_fast(z[j] - lse) * r;
+                                for (int j = 0; j < 16; j += 2) {
+                                    const float2 d = add2(make_float2(z[j], z[j + 1]), both(-lse));
+                                    const float2 e = mul2(make_float2(exp2_fast(d.x), exp2_fast(d.y)), both(r));
+                                    z[j] = e.x;
+                                    z[j + 1] = e.y;
+                                }
                                 if (__any_sync(0xffffffffu, (unsigned)(rel - h) < 16u)) {
 #pragma unroll
                                     for (int j = 0; j < 16; ++j)
@@ -418,11 +427,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                                         uint32_t word[4];
 #pragma unroll
                                         for (int j = 0; j < 4; ++j) {
-                                            float& lo = z[8 * g + 2 * j];
-                                            float& hi = z[8 * g + 2 * j + 1];
-                                            word[j] = pack_bf16(lo, hi);
-                                            lo -= __uint_as_float(word[j] << 16);
-                                            hi -= __uint_as_float(word[j] & 0xffff0000u);
+                                            word[j] = take_part(z[8 * g + 2 * j], z[8 * g + 2 * j + 1]);
                                         }
                                         const int piece = (h / 8 + g) ^ ((in_tile >> 1) & 3);
                                         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(

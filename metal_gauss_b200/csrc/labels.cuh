@@ -56,6 +56,39 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
+// Two fp32 operations in one instruction, each rounded as its scalar form.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n.reg .b64 x, y, z, w;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmov.b64 z, {%6, %7};\n"
+        "fma.rn.f32x2 w, x, y, z;\nmov.b64 {%0, %1}, w;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n.reg .b64 x, y, w;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\n"
+        "add.rn.f32x2 w, x, y;\nmov.b64 {%0, %1}, w;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n.reg .b64 x, y, w;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\n"
+        "mul.rn.f32x2 w, x, y;\nmov.b64 {%0, %1}, w;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+// The largest of three; NaNs drop out as with fmaxf.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 // --------------------------------------------------------------------- parts
 
 // The number of bf16 parts of a type.
@@ -79,6 +112,15 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     uint32_t r;
     memcpy(&r, &v, 4);
     return r;
+}
+
+// One part of (lo, hi) as a word; lo and hi keep what it leaves over.
+__device__ __forceinline__ uint32_t take_part(float& lo, float& hi) {
+    const uint32_t w = pack_bf16(lo, hi);
+    const float2 rest = add2(make_float2(lo, hi), make_float2(-__uint_as_float(w << 16), -__uint_as_float(w & 0xffff0000u)));
+    lo = rest.x;
+    hi = rest.y;
+    return w;
 }
 
 // Parts of the logits' gradient: two also for bf16 features, whose gradients
