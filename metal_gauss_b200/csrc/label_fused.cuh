@@ -45,6 +45,7 @@ struct FusedArgs {         // counts below 2^31: at most 2^30 rows
     int channels;
     int chunks;            // of 64 channels
     int stages, own_buffers, acc_buffers;
+    int resident;          // the streamed tiles, all the same for every unit, stay: one stage each
     float scale;
     const float* row_values;   // kRowValues per row, in blocks of 64 rows
     const float* class_bias;   // bias times log2 e, -infinity past the last class
@@ -205,6 +206,8 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
     __syncthreads();
     tmem_fence_after();
     constexpr uint32_t tmem = kTmemBase;
+    // tiles that stay are waited for in their one and only phase
+    const uint32_t flip = p.resident ? 0 : 1;
     const auto wait = [&](uint32_t bar, uint32_t parity) {
         return mbar_wait(bar, parity, &stop, p.error_word, DEV_ERR_TILE_WAIT);
     };
@@ -238,6 +241,7 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
                     ob = 0;
                     ob_phase ^= 1;
                 }
+                if (p.resident && u != (int)blockIdx.x) continue;
                 for (int t = w.t0; t < w.t1; ++t) {
                     ok = wait_warp(empty + 8 * stage, phase ^ 1);
                     if (!ok) break;
@@ -313,7 +317,7 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
                 mma_commit(s_full + 8 * g, on);
                 if (++stage == p.stages) {
                     stage = 0;
-                    phase ^= 1;
+                    phase ^= flip;
                 }
                 if (++g == kGroups) {
                     g = 0;
@@ -411,7 +415,7 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
                 const uint32_t at_phase = stage_phase;
                 if (++stage == p.stages) {
                     stage = 0;
-                    stage_phase ^= 1;
+                    stage_phase ^= flip;
                 }
                 if (turn++ != g) {
                     if (turn == kGroups) turn = 0;
@@ -602,6 +606,10 @@ inline void fused_buffers(FusedArgs& p, int parts) {
     p.own_buffers = 2 * own + 4 * stage <= room ? 2 : 1;
     p.stages = std::min(kFusedStages, (room - p.own_buffers * own) / stage);
     p.acc_buffers = group_columns(parts) + 2 * n <= 512 ? 2 : 1;
+    // few streamed items and no shares of them: each unit streams the same tiles
+    const int tiles = (p.streamed + kStream - 1) / kStream;
+    p.resident = p.splits == 1 && tiles <= p.stages;
+    if (p.resident) p.stages = tiles;
 }
 
 }  // namespace

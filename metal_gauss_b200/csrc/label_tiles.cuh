@@ -33,6 +33,7 @@ struct Shape {
     static constexpr int kOutBuffers = 1;
     static constexpr int kOut = MODE == kLogitGrad ? kSets * kPartsG * kOutBuffers * kM * 64 : 0;
     static constexpr int kDynamic = 1024 + kStages * kStage + kOut;
+    static constexpr int kBars = MODE == kStats ? 8 : kStages;  // stages at most
     // Products of parts (a, b), smallest first.
     static constexpr int kPairs = kProduct ? kGPairs<PARTS> : PARTS == 1 ? 1 : PARTS == 2 ? 4 : 6;
     __device__ static constexpr int part_a(int i) { return kProduct ? g_pair_a<PARTS>(i) : pair_a<PARTS>(kPairs, i); }
@@ -54,6 +55,8 @@ struct TileArgs {
     const int32_t* row_labels; // kStats
     const float* row_values;   // kLogitGrad
     float *part_m, *part_s, *label_z;  // kStats
+    int resident;           // kStats: B chunks that stay in shared memory for good, or 0
+    int resident_stages;    // and the stages, of A alone, beside them
     float* part_bias;       // kLogitGrad: sums of 32 rows of G, or NULL
     float* part;            // products: fp32 shares (splits, a_rows, part_ld), or NULL
     int part_ld;
@@ -146,17 +149,24 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
             const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_out) {
     using S = Shape<MODE, PARTS>;
     extern __shared__ uint8_t dynamic[];
-    __shared__ uint64_t bars[2 * S::kStages + 5];
+    __shared__ uint64_t bars[2 * S::kBars + 6];
     __shared__ uint32_t tmem_s;
     __shared__ volatile int stop;
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x / 32, 0), lane = threadIdx.x % 32;
     const uint32_t base = (smem_u32(dynamic) + 1023u) & ~1023u;
-    const uint32_t full = smem_u32(bars), empty = full + 8 * S::kStages;
-    const uint32_t taken_full = empty + 8 * S::kStages, taken_empty = taken_full + 16;
-    const uint32_t drain = taken_empty + 16;
+    const uint32_t full = smem_u32(bars), empty = full + 8 * S::kBars;
+    const uint32_t taken_full = empty + 8 * S::kBars, taken_empty = taken_full + 16;
+    const uint32_t drain = taken_empty + 16, resident_full = drain + 8;
+    // Few classes: every unit's B side is the same, and stays. (Each SM
+    // fetching it for each tile, 24 KB at 256 classes of 16 channels, made the
+    // copies the bound: 7200 cycles a tile.)
+    const int resident = MODE == kStats ? p.resident : 0;
+    const int stages = resident > 0 ? p.resident_stages : S::kStages;
+    const uint32_t stage_bytes = resident > 0 ? S::kPartsA * S::kA : S::kStage;
+    const uint32_t ring = base + resident * (PARTS * S::kB);
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < S::kStages; ++i) {
+        for (int i = 0; i < S::kBars; ++i) {
             mbar_init(full + 8 * i, 1);
             mbar_init(empty + 8 * i, 1);
         }
@@ -165,6 +175,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
             mbar_init(taken_empty + 8 * i, 4 * S::kSets);
         }
         mbar_init(drain, 1);
+        mbar_init(resident_full, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_shared();
         stop = 0;
@@ -182,6 +193,14 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
             uint32_t phase = 0;
             int64_t issued = 0;
             bool ok = true;
+            if (MODE == kStats && resident > 0) {
+                const int chunks = (int)((p.depth + S::kChunk - 1) / S::kChunk);
+                mbar_expect(resident_full, resident * PARTS * S::kB, on);
+                for (int c = 0; c < resident; ++c)
+                    for (int i = 0; i < PARTS; ++i)
+                        tma_load(base + (c * PARTS + i) * S::kB, &map_b, c % chunks * S::kChunk, c / chunks * kN, i,
+                                 resident_full, on);
+            }
             for (int64_t u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
                 const Walk w = walk_unit<MODE, PARTS>(p, u);
                 for (int t = 0; ok && t < w.tiles; ++t) {
@@ -190,14 +209,15 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                     const int64_t c1 = S::kProduct ? min(w.c1, c0 + p.per_segment) : w.c1;
                     const int blocks = S::kProduct ? (min(kN, p.columns - b0) + 63) / 64 : 0;
                     const uint32_t bytes =
-                        S::kPartsA * S::kA + PARTS * (S::kProduct ? blocks * S::kChunk * 128 : S::kB);
+                        S::kPartsA * S::kA +
+                        (resident > 0 ? 0 : PARTS * (S::kProduct ? blocks * S::kChunk * 128 : S::kB));
                     for (int64_t c = c0; c < c1; ++c) {
                         ok = mbar_wait_warp(empty + 8 * stage, phase ^ 1, &stop, p.error_word, DEV_ERR_TILE_WAIT);
                         if (!ok) break;
                         const uint32_t bar = full + 8 * stage;
                         mbar_expect(bar, bytes, on);
                         const int k = (int)(c * S::kChunk);
-                        const uint32_t a = base + stage * S::kStage, b = a + S::kPartsA * S::kA;
+                        const uint32_t a = ring + stage * stage_bytes, b = a + S::kPartsA * S::kA;
 #pragma unroll
                         for (int i = 0; i < S::kPartsA; ++i) {
                             if (S::kAmn) {
@@ -209,6 +229,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                         }
 #pragma unroll
                         for (int i = 0; i < PARTS; ++i) {
+                            if (resident > 0) break;
                             if (S::kBmn) {
                                 for (int q = 0; q < blocks; ++q)
                                     tma_load(b + i * S::kB + q * S::kChunk * 128, &map_b, b0 + 64 * q, k, i, bar, on);
@@ -217,7 +238,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                             }
                         }
                         ++issued;
-                        if (++stage == S::kStages) {
+                        if (++stage == stages) {
                             stage = 0;
                             phase ^= 1;
                         }
@@ -225,10 +246,13 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                 }
             }
             if (stop) {  // this block gave up: its copies in flight land before it ends
-                const int n = (int)min(issued, (int64_t)S::kStages);
+                if (MODE == kStats && resident > 0)
+                    for (int i = 0; i < kMbarRounds; ++i)
+                        if (mbar_try(resident_full, 0)) break;
+                const int n = (int)min(issued, (int64_t)stages);
                 for (int j = 0; j < n; ++j) {
                     if (--stage < 0) {
-                        stage = S::kStages - 1;
+                        stage = stages - 1;
                         phase ^= 1;
                     }
                     for (int i = 0; i < kMbarRounds; ++i)
@@ -241,7 +265,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
             const uint32_t on = elect_lane();
             int stage = 0, buf = 0;
             uint32_t phase = 0, buf_phase = 0;
-            bool ok = true;
+            bool ok = resident == 0 || mbar_wait_warp(resident_full, 0, &stop, p.error_word, DEV_ERR_TILE_WAIT);
             for (int64_t u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
                 const Walk w = walk_unit<MODE, PARTS>(p, u);
                 for (int t = 0; ok && t < w.tiles; ++t) {
@@ -265,7 +289,8 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                         if (!ok) break;
                         tmem_fence_after();
                         const int steps = c + 1 < chunks ? S::kChunk / 16 : tail;
-                        const uint32_t a_at = base + stage * S::kStage, b_at = a_at + S::kPartsA * S::kA;
+                        const uint32_t a_at = ring + stage * stage_bytes;
+                        const uint32_t b_at = resident > 0 ? base + (t * chunks + c) * (PARTS * S::kB) : a_at + S::kPartsA * S::kA;
                         const uint32_t a = uniform(S::kAmn ? mn_major_lo(a_at, S::kChunk * 128) : k_major_lo(a_at));
                         const uint32_t b = uniform(S::kBmn ? mn_major_lo(b_at, S::kChunk * 128) : k_major_lo(b_at));
                         constexpr uint32_t a_hi = S::kAmn ? kMnMajorHi : k_major_hi(S::kChunk * 2);
@@ -283,7 +308,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                             }
                         }
                         mma_commit(empty + 8 * stage, on);
-                        if (++stage == S::kStages) {
+                        if (++stage == stages) {
                             stage = 0;
                             phase ^= 1;
                         }

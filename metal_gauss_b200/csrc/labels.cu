@@ -440,6 +440,14 @@ mg_status forward(const Args& a, int reduction, float* loss, float* stats, float
     p.part_s = f.s;
     p.label_z = f.z;
     p.error_word = device_error_word();
+    // every class's chunks stay in shared memory where they leave two stages
+    using S = Shape<kStats, PARTS>;
+    const int64_t chunks = a.n.class_columns() * up(p.depth, S::kChunk);
+    const int64_t room = S::kStages * S::kStage - chunks * PARTS * S::kB;
+    if (sh.splits == 1 && room >= 2 * PARTS * S::kA) {
+        p.resident = (int)chunks;
+        p.resident_stages = (int)std::min<int64_t>(S::kBars, room / (PARTS * S::kA));
+    }
     MG_TRY((launch_tiles<kStats, PARTS>(p, mx, mw, mw, a.st, "label_loss_forward")));
     label_rows_kernel<<<(unsigned)a.n.row_blocks(), 256, 0, a.st>>>(
         f.m, f.s, f.z, a.labels, sh.splits * Shape<kStats, 1>::kSets, a.n.rows, stats,
