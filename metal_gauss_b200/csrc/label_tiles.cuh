@@ -40,13 +40,13 @@ struct Shape {
     __device__ static constexpr int part_b(int i) { return kProduct ? g_pair_b<PARTS>(i) : pair_b<PARTS>(kPairs, i); }
 };
 
-struct TileArgs {
-    int64_t units;
-    int64_t a_rows;         // rows of the A side (of the piece, or classes)
-    int64_t depth;          // contraction entries
+struct TileArgs {           // counts below 2^31: at most 2^30 rows
+    int units;
+    int a_rows;             // rows of the A side (of the piece, or classes)
+    int depth;              // contraction entries
     int columns;            // columns of the B side in all (classes, or channels)
     int splits;             // shares of the classes (kStats) or of the contraction
-    int64_t per_split;      // column tiles, or chunks, per share
+    int per_split;          // column tiles, or chunks, per share
     int per_segment;        // chunks between visits to the registers
     int64_t row0;           // the piece's first row
     int64_t rows;           // rows in all
@@ -69,37 +69,36 @@ struct TileArgs {
 // tiles (kStats) or one column tile (kLogitGrad). Products: a unit is a row
 // tile, a column tile and a share of the contraction, in segments.
 struct Walk {
-    int64_t a_row, c0, c1;
-    int b_row, split, tiles, first;
+    int a_row, c0, c1, split, tiles, first;
 };
 
 template <int MODE, int PARTS>
-__device__ __forceinline__ Walk walk_unit(const TileArgs& p, int64_t u) {
+__device__ __forceinline__ Walk walk_unit(const TileArgs& p, int u) {
     Walk w;
     const int col_tiles = (p.columns + kN - 1) / kN;
+    const int chunks = (p.depth + Shape<MODE, PARTS>::kChunk - 1) / Shape<MODE, PARTS>::kChunk;
     if (MODE == kStats) {
-        w.a_row = u / p.splits * kM;
-        w.split = (int)(u % p.splits);
-        w.first = (int)(w.split * p.per_split);
-        w.tiles = (int)min((int64_t)col_tiles, w.first + p.per_split) - w.first;
+        w.a_row = p.splits == 1 ? u * kM : u / p.splits * kM;
+        w.split = p.splits == 1 ? 0 : u % p.splits;
+        w.first = w.split * p.per_split;
+        w.tiles = min(col_tiles, w.first + p.per_split) - w.first;
         w.c0 = 0;
-        w.c1 = (p.depth + Shape<MODE, PARTS>::kChunk - 1) / Shape<MODE, PARTS>::kChunk;
+        w.c1 = chunks;
     } else if (MODE == kLogitGrad) {
         w.a_row = u / col_tiles * kM;
-        w.first = (int)(u % col_tiles);
+        w.first = u % col_tiles;
         w.tiles = 1;
         w.split = 0;
         w.c0 = 0;
-        w.c1 = (p.depth + Shape<MODE, PARTS>::kChunk - 1) / Shape<MODE, PARTS>::kChunk;
+        w.c1 = chunks;
     } else {
-        const int64_t chunks = (p.depth + Shape<MODE, PARTS>::kChunk - 1) / Shape<MODE, PARTS>::kChunk;
-        w.split = (int)(u % p.splits);
-        const int64_t t = u / p.splits;
-        w.first = (int)(t % col_tiles);
+        w.split = u % p.splits;
+        const int t = u / p.splits;
+        w.first = t % col_tiles;
         w.a_row = t / col_tiles * kM;
         w.c0 = w.split * p.per_split;
         w.c1 = min(chunks, w.c0 + p.per_split);
-        w.tiles = (int)((w.c1 - w.c0 + p.per_segment - 1) / p.per_segment);
+        w.tiles = (w.c1 - w.c0 + p.per_segment - 1) / p.per_segment;
     }
     return w;
 }
@@ -111,7 +110,7 @@ struct RowIn {
 };
 
 template <int MODE>
-__device__ __forceinline__ RowIn row_in(const TileArgs& p, int64_t a_row) {
+__device__ __forceinline__ RowIn row_in(const TileArgs& p, int a_row) {
     RowIn in;
     if (a_row >= p.a_rows) return in;
     const int64_t row = p.row0 + a_row;
@@ -191,7 +190,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
             const uint32_t on = elect_lane();
             int stage = 0;
             uint32_t phase = 0;
-            int64_t issued = 0;
+            int issued = 0;
             bool ok = true;
             if (MODE == kStats && resident > 0) {
                 const int chunks = (int)((p.depth + S::kChunk - 1) / S::kChunk);
@@ -201,30 +200,30 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                         tma_load(base + (c * PARTS + i) * S::kB, &map_b, c % chunks * S::kChunk, c / chunks * kN, i,
                                  resident_full, on);
             }
-            for (int64_t u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
+            for (int u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
                 const Walk w = walk_unit<MODE, PARTS>(p, u);
                 for (int t = 0; ok && t < w.tiles; ++t) {
                     const int b0 = (S::kProduct ? w.first : w.first + t) * kN;
-                    const int64_t c0 = S::kProduct ? w.c0 + (int64_t)t * p.per_segment : w.c0;
-                    const int64_t c1 = S::kProduct ? min(w.c1, c0 + p.per_segment) : w.c1;
+                    const int c0 = S::kProduct ? w.c0 + t * p.per_segment : w.c0;
+                    const int c1 = S::kProduct ? min(w.c1, c0 + p.per_segment) : w.c1;
                     const int blocks = S::kProduct ? (min(kN, p.columns - b0) + 63) / 64 : 0;
                     const uint32_t bytes =
                         S::kPartsA * S::kA +
                         (resident > 0 ? 0 : PARTS * (S::kProduct ? blocks * S::kChunk * 128 : S::kB));
-                    for (int64_t c = c0; c < c1; ++c) {
+                    for (int c = c0; c < c1; ++c) {
                         ok = mbar_wait_warp(empty + 8 * stage, phase ^ 1, &stop, p.error_word, DEV_ERR_TILE_WAIT);
                         if (!ok) break;
                         const uint32_t bar = full + 8 * stage;
                         mbar_expect(bar, bytes, on);
-                        const int k = (int)(c * S::kChunk);
+                        const int k = c * S::kChunk;
                         const uint32_t a = ring + stage * stage_bytes, b = a + S::kPartsA * S::kA;
 #pragma unroll
                         for (int i = 0; i < S::kPartsA; ++i) {
                             if (S::kAmn) {
                                 for (int q = 0; q < 2; ++q)
-                                    tma_load(a + i * S::kA + q * S::kChunk * 128, &map_a, (int)w.a_row + 64 * q, k, i, bar, on);
+                                    tma_load(a + i * S::kA + q * S::kChunk * 128, &map_a, w.a_row + 64 * q, k, i, bar, on);
                             } else {
-                                tma_load(a + i * S::kA, &map_a, k, (int)w.a_row, i, bar, on);
+                                tma_load(a + i * S::kA, &map_a, k, w.a_row, i, bar, on);
                             }
                         }
 #pragma unroll
@@ -237,7 +236,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                                 tma_load(b + i * S::kB, &map_b, k, b0, i, bar, on);
                             }
                         }
-                        ++issued;
+                        issued = min(issued + 1, stages);
                         if (++stage == stages) {
                             stage = 0;
                             phase ^= 1;
@@ -249,8 +248,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                 if (MODE == kStats && resident > 0)
                     for (int i = 0; i < kMbarRounds; ++i)
                         if (mbar_try(resident_full, 0)) break;
-                const int n = (int)min(issued, (int64_t)stages);
-                for (int j = 0; j < n; ++j) {
+                for (int j = 0; j < issued; ++j) {
                     if (--stage < 0) {
                         stage = stages - 1;
                         phase ^= 1;
@@ -266,12 +264,12 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
             int stage = 0, buf = 0;
             uint32_t phase = 0, buf_phase = 0;
             bool ok = resident == 0 || mbar_wait_warp(resident_full, 0, &stop, p.error_word, DEV_ERR_TILE_WAIT);
-            for (int64_t u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
+            for (int u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
                 const Walk w = walk_unit<MODE, PARTS>(p, u);
                 for (int t = 0; ok && t < w.tiles; ++t) {
                     const int b0 = (S::kProduct ? w.first : w.first + t) * kN;
-                    const int64_t c0 = S::kProduct ? w.c0 + (int64_t)t * p.per_segment : w.c0;
-                    const int64_t c1 = S::kProduct ? min(w.c1, c0 + p.per_segment) : w.c1;
+                    const int c0 = S::kProduct ? w.c0 + t * p.per_segment : w.c0;
+                    const int c1 = S::kProduct ? min(w.c1, c0 + p.per_segment) : w.c1;
                     // scores: every column that is read (32 at a time) has been written,
                     // past the last class with zeros; tensor memory may hold NaNs
                     constexpr int kRound = S::kProduct ? 16 : 32;
@@ -279,7 +277,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                     const uint32_t idesc = uniform(mma_idesc(n, S::kAmn, S::kBmn));
                     const int chunks = (int)uniform((uint32_t)(c1 - c0));
                     // 16-entry steps of the last chunk
-                    const int tail = (int)uniform((uint32_t)min((int64_t)(S::kChunk / 16), (p.depth - (c1 - 1) * S::kChunk + 15) / 16));
+                    const int tail = (int)uniform((uint32_t)min(S::kChunk / 16, (p.depth - (c1 - 1) * S::kChunk + 15) / 16));
                     ok = mbar_wait_warp(taken_empty + 8 * buf, buf_phase ^ 1, &stop, p.error_word, DEV_ERR_TILE_WAIT);
                     if (!ok) break;
                     tmem_fence_after();
@@ -340,9 +338,9 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
         RowIn next_row;
         if constexpr (!S::kProduct)
             next_row = row_in<MODE>(p, walk_unit<MODE, PARTS>(p, blockIdx.x).a_row + in_tile);
-        for (int64_t u = blockIdx.x; u < p.units; u += gridDim.x) {
+        for (int u = blockIdx.x; u < p.units; u += gridDim.x) {
             const Walk w = walk_unit<MODE, PARTS>(p, u);
-            const int64_t a_row = w.a_row + in_tile;
+            const int a_row = w.a_row + in_tile;
             const bool mine = a_row < p.a_rows;
             if constexpr (!S::kProduct) {
                 const int64_t row = p.row0 + a_row;
@@ -352,8 +350,8 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                 for (int t = 0; t < w.tiles; ++t) {
                     const int v0 = (w.first + t) * kN;
                     const int n = min(kN, p.columns - v0);
-                    if (t + 1 == w.tiles && u + gridDim.x < p.units)  // while this tile is taken
-                        next_row = row_in<MODE>(p, walk_unit<MODE, PARTS>(p, u + gridDim.x).a_row + in_tile);
+                    if (t + 1 == w.tiles && u + (int)gridDim.x < p.units)  // while this tile is taken
+                        next_row = row_in<MODE>(p, walk_unit<MODE, PARTS>(p, u + (int)gridDim.x).a_row + in_tile);
                     mbar_wait(taken_full + 8 * buf, buf_phase, &stop, p.error_word, DEV_ERR_TILE_WAIT);
                     tmem_fence_after();
                     for (int k = set; k * 32 < n; k += S::kSets) {
@@ -442,7 +440,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                                     q[0] += __shfl_xor_sync(0xffffffffu, q[0], 16);
                                     const int v = v0 + k * 32 + h + lane;
                                     if (lane < 16 && v < p.columns)
-                                        p.part_bias[(w.a_row / 32 + quarter) * p.columns + v] = q[0];
+                                        p.part_bias[(int64_t)(w.a_row / 32 + quarter) * p.columns + v] = q[0];
                                 }
                                 // part i of 8 columns: 16 bytes of this row's 64, swizzled
 #pragma unroll
@@ -467,7 +465,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                             if (speaks) {
 #pragma unroll
                                 for (int i = 0; i < S::kPartsG; ++i)
-                                    tma_store(&map_out, v0 + k * 32, (int)w.a_row, i, stage0 + i * kM * 64);
+                                    tma_store(&map_out, v0 + k * 32, w.a_row, i, stage0 + i * kM * 64);
                                 tma_store_commit();
                             }
                             if (++out_buf == S::kOutBuffers) out_buf = 0;

@@ -387,7 +387,7 @@ mg_status launch_tiles(const TileArgs& p, const CUtensorMap& a, const CUtensorMa
             return check_launch(what);
         ready[dev] = true;
     }
-    const int grid = (int)std::min<int64_t>(p.units, sm_count());
+    const int grid = std::min(p.units, sm_count());
     tile_kernel<MODE, PARTS><<<grid, Shape<MODE, PARTS>::kThreads, bytes, st>>>(p, a, b, out);
     return check_launch(what);
 }
@@ -427,12 +427,13 @@ mg_status forward(const Args& a, int reduction, float* loss, float* stats, float
     MG_TRY(parts_map(&mw, f.ws, a.n, a.n.classes, kN));
     const Shares sh = a.n.stats();
     TileArgs p{};
-    p.units = a.n.row_tiles() * sh.splits;
-    p.a_rows = p.rows = a.n.rows;
+    p.units = (int)(a.n.row_tiles() * sh.splits);
+    p.a_rows = (int)a.n.rows;
+    p.rows = a.n.rows;
     p.depth = a.n.depth();
     p.columns = a.n.classes;
     p.splits = sh.splits;
-    p.per_split = sh.per_split;
+    p.per_split = (int)sh.per_split;
     p.scale = a.scale;
     p.class_bias = f.class_bias;
     p.row_labels = f.row_labels;
@@ -575,8 +576,8 @@ mg_status backward(const Args& a, const RowGrad& rg, const float* stats, T* dx, 
         MG_TRY(make_tensor_map(&mg_out, f.g, n.classes, rows, kGParts<PARTS>, n.g_ld() * 2, g_part, 32, kM,
                                false, "label_loss G"));
         TileArgs p{};
-        p.units = up(rows, kM) * n.class_columns();
-        p.a_rows = rows;
+        p.units = (int)(up(rows, kM) * n.class_columns());
+        p.a_rows = (int)rows;
         p.rows = n.rows;
         p.row0 = row0;
         p.depth = n.depth();
@@ -601,10 +602,10 @@ mg_status backward(const Args& a, const RowGrad& rg, const float* stats, T* dx, 
             MG_TRY(make_tensor_map(&mg_in, f.g, n.classes, rows, kGParts<PARTS>, n.g_ld() * 2, g_part, n.chunk(),
                                    kM, n.chunk() == 64, "label_loss G"));
             const Shares sh = n.by_row();
-            p.units = up(rows, kM) * n.channel_columns() * sh.splits;
+            p.units = (int)(up(rows, kM) * n.channel_columns() * sh.splits);
             p.depth = n.classes;
             p.splits = sh.splits;
-            p.per_split = sh.per_split;
+            p.per_split = (int)sh.per_split;
             p.part = n.direct() ? nullptr : f.row_part;
             p.part_ld = n.part_ld();
             p.out = dx;
@@ -619,11 +620,11 @@ mg_status backward(const Args& a, const RowGrad& rg, const float* stats, T* dx, 
                                    n.chunk(), true, "label_loss G"));
             MG_TRY(parts_map(&mx_prod, xs, n, rows, 0));
             const Shares sh = n.by_class();
-            p.units = up(n.classes, kM) * n.channel_columns() * sh.splits;
+            p.units = (int)(up(n.classes, kM) * n.channel_columns() * sh.splits);
             p.a_rows = n.classes;
-            p.depth = rows;
+            p.depth = (int)rows;
             p.splits = sh.splits;
-            p.per_split = sh.per_split;
+            p.per_split = (int)sh.per_split;
             p.part = f.class_part;
             p.part_ld = n.part_ld();
             p.add = row0 > 0;
