@@ -301,17 +301,18 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
                 tmem_fence_after();
                 const uint32_t b0 = uniform(k_major_lo(stream0 + stage * stage_bytes));
                 const uint32_t d = uniform(tmem + g * kGroupColumns<PARTS>);
-                for (int c = 0; c < p.chunks; ++c) {
-                    const uint32_t a1 = a0 + c * (kOwnChunk / 16), b1 = b0 + c * (kStreamChunk / 16);
+                // the small products first: the tensor cores truncate the running
+                // sum at each step, and only the large ones' steps weigh
 #pragma unroll
-                    for (int q = 0; q < kScorePairs; ++q) {
+                for (int q = 0; q < kScorePairs; ++q) {
+                    for (int c = 0; c < p.chunks; ++c) {
+                        const uint32_t a1 = a0 + pair_a<PARTS>(kScorePairs, q) * a_part + c * (kOwnChunk / 16);
+                        const uint32_t b1 = b0 + pair_b<PARTS>(kScorePairs, q) * b_part + c * (kStreamChunk / 16);
 #pragma unroll
                         for (int s = 0; s < 4; ++s)
                             if (64 * c + 16 * s < p.channels)
-                                mma_bf16<k_major_hi(128), k_major_hi(128)>(
-                                    d, a1 + pair_a<PARTS>(kScorePairs, q) * a_part + 2 * s,
-                                    b1 + pair_b<PARTS>(kScorePairs, q) * b_part + 2 * s, idesc,
-                                    q > 0 || s > 0 ? true : c > 0, on);
+                                mma_bf16<k_major_hi(128), k_major_hi(128)>(d, a1 + 2 * s, b1 + 2 * s, idesc,
+                                                                           q > 0 || s > 0 ? true : c > 0, on);
                     }
                 }
                 mma_commit(s_full + 8 * g, on);

@@ -33,6 +33,11 @@ struct Shape {
     static constexpr int kOutBuffers = 1;
     static constexpr int kOut = MODE == kLogitGrad ? kSets * kPartsG * kOutBuffers * kM * 64 : 0;
     static constexpr int kDynamic = 1024 + kStages * kStage + kOut;
+    // Scores of more than one chunk go over them twice: the small products of all
+    // of them, then the large one (with its parts fetched again). The tensor
+    // cores truncate the running sum at each step, and only steps that come when
+    // it is large weigh: 32 of 192 at 512 fp32 channels.
+    static constexpr bool kTwice = !kProduct && PARTS > 1;
     static constexpr int kBars = MODE == kStats ? 8 : kStages;  // stages at most
     // Products of parts (a, b), smallest first.
     static constexpr int kPairs = kProduct ? kGPairs<PARTS> : PARTS == 1 ? 1 : PARTS == 2 ? 4 : 6;
@@ -210,30 +215,34 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                     const uint32_t bytes =
                         S::kPartsA * S::kA +
                         (resident > 0 ? 0 : PARTS * (S::kProduct ? blocks * S::kChunk * 128 : S::kB));
-                    for (int c = c0; c < c1; ++c) {
+                    const int passes = S::kTwice && c1 - c0 > 1 ? 2 : 1;
+                    for (int i = 0; i < passes * (c1 - c0); ++i) {
+                        const bool again = i >= c1 - c0;  // the first part alone
+                        const int c = again ? i - (c1 - c0) + c0 : i + c0;
                         ok = mbar_wait_warp(empty + 8 * stage, phase ^ 1, &stop, p.error_word, DEV_ERR_TILE_WAIT);
                         if (!ok) break;
                         const uint32_t bar = full + 8 * stage;
-                        mbar_expect(bar, bytes, on);
+                        mbar_expect(bar, again ? S::kA + (resident > 0 ? 0 : S::kB) : bytes, on);
                         const int k = c * S::kChunk;
                         const uint32_t a = ring + stage * stage_bytes, b = a + S::kPartsA * S::kA;
 #pragma unroll
-                        for (int i = 0; i < S::kPartsA; ++i) {
+                        for (int j = 0; j < S::kPartsA; ++j) {
+                            if (again && j > 0) break;
                             if (S::kAmn) {
                                 for (int q = 0; q < 2; ++q)
-                                    tma_load(a + i * S::kA + q * S::kChunk * 128, &map_a, w.a_row + 64 * q, k, i, bar, on);
+                                    tma_load(a + j * S::kA + q * S::kChunk * 128, &map_a, w.a_row + 64 * q, k, j, bar, on);
                             } else {
-                                tma_load(a + i * S::kA, &map_a, k, w.a_row, i, bar, on);
+                                tma_load(a + j * S::kA, &map_a, k, w.a_row, j, bar, on);
                             }
                         }
 #pragma unroll
-                        for (int i = 0; i < PARTS; ++i) {
-                            if (resident > 0) break;
+                        for (int j = 0; j < PARTS; ++j) {
+                            if (resident > 0 || (again && j > 0)) break;
                             if (S::kBmn) {
                                 for (int q = 0; q < blocks; ++q)
-                                    tma_load(b + i * S::kB + q * S::kChunk * 128, &map_b, b0 + 64 * q, k, i, bar, on);
+                                    tma_load(b + j * S::kB + q * S::kChunk * 128, &map_b, b0 + 64 * q, k, j, bar, on);
                             } else {
-                                tma_load(b + i * S::kB, &map_b, k, b0, i, bar, on);
+                                tma_load(b + j * S::kB, &map_b, k, b0, j, bar, on);
                             }
                         }
                         issued = min(issued + 1, stages);
@@ -282,10 +291,12 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                     if (!ok) break;
                     tmem_fence_after();
                     const uint32_t d = uniform(tmem + buf * kN);
-                    for (int c = 0; c < chunks; ++c) {
+                    const int passes = S::kTwice && chunks > 1 ? 2 : 1;
+                    for (int v = 0; v < passes * chunks; ++v) {
                         ok = mbar_wait_warp(full + 8 * stage, phase, &stop, p.error_word, DEV_ERR_TILE_WAIT);
                         if (!ok) break;
                         tmem_fence_after();
+                        const int c = v < chunks ? v : v - chunks;
                         const int steps = c + 1 < chunks ? S::kChunk / 16 : tail;
                         const uint32_t a_at = ring + stage * stage_bytes;
                         const uint32_t b_at = resident > 0 ? base + (t * chunks + c) * (PARTS * S::kB) : a_at + S::kPartsA * S::kA;
@@ -295,6 +306,8 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                         constexpr uint32_t b_hi = S::kBmn ? kMnMajorHi : k_major_hi(S::kChunk * 2);
 #pragma unroll
                         for (int i = 0; i < S::kPairs; ++i) {
+                            // of two passes the first leaves the last, large product out
+                            if (S::kTwice && passes == 2 && (i + 1 < S::kPairs) != (v < chunks)) continue;
 #pragma unroll
                             for (int s = 0; s < S::kChunk / 16; ++s) {
                                 // 16 entries on: 32 bytes along a row, or 16 rows of 128 bytes
@@ -302,7 +315,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                                     mma_bf16<a_hi, b_hi>(
                                         d, a + S::part_a(i) * (S::kA / 16) + s * (S::kAmn ? 128 : 2),
                                         b + S::part_b(i) * (S::kB / 16) + s * (S::kBmn ? 128 : 2), idesc,
-                                        i > 0 || s > 0 ? true : c > 0, on);
+                                        i > 0 || s > 0 ? true : v > 0, on);
                             }
                         }
                         mma_commit(empty + 8 * stage, on);

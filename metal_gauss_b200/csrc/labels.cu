@@ -263,9 +263,9 @@ struct Sizes {
     int channels, classes, parts;
 
     int chunk() const { return parts == 1 ? 64 : 32; }
-    // fp32: 256 entries between visits to the registers; the others round their
+    // fp32: 32 entries between visits to the registers; the others round their
     // result to 11 bits or fewer and go 4096
-    int segment() const { return (parts == 3 ? 64 : 4096) / chunk(); }
+    int segment() const { return (parts == 3 ? 32 : 4096) / chunk(); }
     int depth() const { return (int)up(channels, 8) * 8; }
     int part_ld() const { return (int)up(channels, 4) * 4; }
     int64_t row_tiles() const { return up(rows, kM); }
