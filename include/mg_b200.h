@@ -786,7 +786,7 @@ mg_status mg_label_loss_forward(const void* features, const void* classes, int32
                                 void* scratch, size_t scratch_bytes, mg_stream_t stream);
 
 /* Its adjoint: d_features, d_classes (of `dtype`) and d_bias (fp32), each
- * OVERWRITTEN, each NULL to leave it out (d_features 16-byte aligned).
+ * OVERWRITTEN, each NULL to leave it out (both 16-byte aligned).
  * grad_loss: one float, or one per row with MG_REDUCE_NONE. The scratch (backward = 1) holds pieces of the
  * logits' gradient, never all of it when it is large. Sums run in a fixed
  * order: equal calls give equal bits. */

@@ -15,6 +15,8 @@ so a value comes back within a / 254 of itself.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
@@ -27,6 +29,19 @@ DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # MG_F32, MG_
 
 def wants_grad(*tensors: torch.Tensor | None) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def once(backward):
+    """The backward of an autograd function that has no second derivative:
+    torch's own guard where a graph of it is being built, none of its cost
+    where not."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+    return run
 
 
 def dtype_code(t: torch.Tensor, what: str) -> int:
@@ -100,7 +115,7 @@ class _Checkpoint8(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once
     def backward(ctx, grad):
         codes, scales, *tensors = ctx.saved_tensors
         need = ctx.needs_input_grad[1:]

@@ -27,8 +27,8 @@
 //   kProductClass  dw += G^T x of the piece
 //
 // Products that sum over more than a few hundred entries leave the tensor
-// cores' accumulator for registers after every kSegment entries (fp32), since
-// its additions truncate. Classes or rows are split over blocks when there are
+// cores' accumulator for registers after every few entries (fp32), since its
+// additions truncate. Classes or rows are split over blocks when there are
 // few of the others; shares are joined in a fixed order.
 #include "label_fused.cuh"
 #include "label_tiles.cuh"
@@ -119,12 +119,16 @@ __device__ __forceinline__ void join_stats(float& m, float& s, float m2, float s
 // Per row: the shares' join, the loss, and what the backward pass needs
 // (stats: log2 of the sum, then 1 - softmax(label)); per block the sum of the losses and
 // the count of live rows.
+template <int L>
 __global__ void __launch_bounds__(256)
 label_rows_kernel(const float* __restrict__ part_m, const float* __restrict__ part_s,
                   const float* __restrict__ label_z, LabelSource labels, int splits, int64_t rows,
                   float* __restrict__ stats, float* __restrict__ row_loss,
-                  double* __restrict__ block_sum, int32_t* __restrict__ error_word) {
-    const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
+                  double* __restrict__ block_sum, float* __restrict__ total, int mean,
+                  float* __restrict__ live_out, int32_t* __restrict__ error_word) {
+    const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+    const int lane = threadIdx.x % L;
+    const uint32_t lanes = L == 32 ? 0xffffffffu : 1u << (threadIdx.x & 31);
     float loss = 0.0f;
     int live = 0;
     if (row < rows) {
@@ -133,9 +137,14 @@ label_rows_kernel(const float* __restrict__ part_m, const float* __restrict__ pa
         if (lab >= 0) {
             live = 1;
             float m = -kInf, s = 0.0f;
-            for (int k = 0; k < splits; ++k) {
+            for (int k = lane; k < splits; k += L) {
                 const float m2 = part_m[(int64_t)k * rows + row];
                 const float s2 = part_s[(int64_t)k * rows + row];
+                join_stats(m, s, m2, s2);
+            }
+#pragma unroll
+            for (int o = 1; o < L; o <<= 1) {  // the row's lanes are in step: all have its label
+                const float m2 = __shfl_xor_sync(lanes, m, o), s2 = __shfl_xor_sync(lanes, s, o);
                 join_stats(m, s, m2, s2);
             }
             const float z = label_z[row];
@@ -154,15 +163,18 @@ label_rows_kernel(const float* __restrict__ part_m, const float* __restrict__ pa
         } else if (lab == kBadLabel) {
             live = 1;
             loss = __int_as_float(0x7fc00000);
-            record_device_error(error_word, DEV_ERR_LABEL);
+            if (lane == 0) record_device_error(error_word, DEV_ERR_LABEL);
         }
-        if (stats != nullptr) {
+        if (lane != 0) {
+            loss = 0.0f;
+            live = 0;
+        } else if (stats != nullptr) {
             stats[row] = lse;
             stats[rows + row] = miss;
         }
-        if (row_loss != nullptr) row_loss[row] = loss;
+        if (row_loss != nullptr && lane == 0) row_loss[row] = loss;
     }
-    if (block_sum == nullptr) return;
+    if (block_sum == nullptr && total == nullptr) return;
     __shared__ double sh[256];
     sh[threadIdx.x] = (double)loss;
     const int count = __syncthreads_count(live);
@@ -170,7 +182,11 @@ label_rows_kernel(const float* __restrict__ part_m, const float* __restrict__ pa
         if (threadIdx.x < o) sh[threadIdx.x] += sh[threadIdx.x + o];
         __syncthreads();
     }
-    if (threadIdx.x == 0) {
+    if (threadIdx.x != 0) return;
+    if (total != nullptr) {  // the only block
+        total[0] = (float)(mean ? sh[0] / fmax((double)count, 1.0) : sh[0]);
+        if (live_out != nullptr) live_out[0] = (float)count;
+    } else {
         block_sum[2 * blockIdx.x] = sh[0];
         block_sum[2 * blockIdx.x + 1] = (double)count;
     }
@@ -274,6 +290,9 @@ struct Sizes {
     int64_t g_ld() const { return up(classes, 64) * 64; }
     int g_parts() const { return parts == 1 ? 2 : parts; }
     // dx straight from the product, in rows of whole 16-byte stores
+    bool class_direct() const {
+        return pieces() == 1 && by_class().splits == 1 && channels % (parts == 3 ? 4 : 8) == 0;
+    }
     bool direct() const { return by_row().splits == 1 && channels % (parts == 3 ? 4 : 8) == 0; }
     int64_t piece() const {
         const int64_t fit = kPieceBytes / (2 * g_parts() * g_ld()) / kM * kM;
@@ -299,7 +318,9 @@ struct Sizes {
                channels % (parts == 3 ? 4 : 8) == 0;
     }
     int64_t class_pad() const { return up(classes, kClassPad) * kClassPad; }
-    int64_t row_blocks() const { return up(rows, 256); }
+    // the forward's join: a warp to a row where the classes are in many shares
+    bool wide_rows() const { return stats().splits >= 8; }
+    int64_t row_blocks() const { return up(rows, wide_rows() ? 8 : 256); }
     // the bias's gradient: sums of 32 rows, then of up to kBiasLines of those
     int64_t pieces() const { return up(rows, piece()); }
     int64_t bias_lines() const { return piece() / 32; }
@@ -450,14 +471,15 @@ mg_status forward(const Args& a, int reduction, float* loss, float* stats, float
         p.resident_stages = (int)std::min<int64_t>(S::kBars, room / (PARTS * S::kA));
     }
     MG_TRY((launch_tiles<kStats, PARTS>(p, mx, mw, mw, a.st, "label_loss_forward")));
-    label_rows_kernel<<<(unsigned)a.n.row_blocks(), 256, 0, a.st>>>(
-        f.m, f.s, f.z, a.labels, sh.splits * Shape<kStats, 1>::kSets, a.n.rows, stats,
-        reduction == MG_REDUCE_NONE ? loss : nullptr, reduction == MG_REDUCE_NONE ? nullptr : f.sums,
-        p.error_word);
+    const int shares = sh.splits * S::kSets, mean = reduction == MG_REDUCE_MEAN;
+    const bool none = reduction == MG_REDUCE_NONE, single = a.n.row_blocks() == 1;
+    const auto rows_kernel = a.n.wide_rows() ? label_rows_kernel<32> : label_rows_kernel<1>;
+    rows_kernel<<<(unsigned)a.n.row_blocks(), 256, 0, a.st>>>(
+        f.m, f.s, f.z, a.labels, shares, a.n.rows, stats, none ? loss : nullptr,
+        none || single ? nullptr : f.sums, none || !single ? nullptr : loss, mean, live, p.error_word);
     MG_TRY(check_launch("label_loss_forward rows"));
-    if (reduction == MG_REDUCE_NONE) return MG_OK;
-    label_total_kernel<<<1, 1024, 0, a.st>>>(f.sums, (int)a.n.row_blocks(),
-                                             reduction == MG_REDUCE_MEAN, loss, live);
+    if (none || single) return MG_OK;
+    label_total_kernel<<<1, 1024, 0, a.st>>>(f.sums, (int)a.n.row_blocks(), mean, loss, live);
     return check_launch("label_loss_forward total");
 }
 
@@ -625,13 +647,15 @@ mg_status backward(const Args& a, const RowGrad& rg, const float* stats, T* dx, 
             p.depth = (int)rows;
             p.splits = sh.splits;
             p.per_split = (int)sh.per_split;
-            p.part = f.class_part;
+            p.part = n.class_direct() ? nullptr : f.class_part;
             p.part_ld = n.part_ld();
             p.add = row0 > 0;
+            p.row0 = 0;
+            p.out = dw;
             MG_TRY((launch_tiles<kProductClass, PARTS>(p, mg_in, mx_prod, mx_prod, a.st, "label_loss_backward classes")));
         }
     }
-    if (dw != nullptr)
+    if (dw != nullptr && !n.class_direct())
         MG_TRY(join(f.class_part, n.by_class().splits, n.classes, n.part_ld(), n.channels, a.scale, dw, a.st));
     if (db != nullptr && n.pieces() * n.bias_shares() > 1) {
         const int64_t shares = n.pieces() * n.bias_shares();
@@ -749,7 +773,8 @@ extern "C" mg_status mg_label_loss_backward(
         return MG_OK;
     }
     if (d_features == nullptr && d_classes == nullptr && d_bias == nullptr) return MG_OK;
-    MG_REQUIRE(aligned16(d_features), "label_loss_backward: d_features must be 16-byte aligned");
+    MG_REQUIRE(aligned16(d_features) && aligned16(d_classes),
+               "label_loss_backward: d_features and d_classes must be 16-byte aligned");
     MG_REQUIRE(grad_loss && stats && (reduction != MG_REDUCE_MEAN || live),
                "label_loss_backward: null pointer");
     MG_REQUIRE(scratch != nullptr && (reinterpret_cast<uintptr_t>(scratch) & 255u) == 0u &&

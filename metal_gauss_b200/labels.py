@@ -17,7 +17,7 @@ import torch
 
 from . import _lib
 from ._lib import ptr
-from .activations import DTYPES, check_cuda, dtype_code, wants_grad
+from .activations import DTYPES, check_cuda, dtype_code, once, wants_grad
 
 MAX_CHANNELS, MAX_CLASSES = 512, 1 << 20      # MG_LABEL_MAX_CHANNELS, MG_LABEL_MAX_CLASSES
 REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
@@ -66,7 +66,7 @@ class _LabelLoss(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once
     def backward(ctx, grad):
         x, w, lab, b, stats = ctx.saved_tensors
         scale, ignore_index, reduction = ctx.meta

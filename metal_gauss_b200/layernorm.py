@@ -15,7 +15,7 @@ import torch
 
 from . import _lib
 from ._lib import ptr
-from .activations import BLOCK, DTYPES, check_cuda, dtype_code, wants_grad
+from .activations import BLOCK, DTYPES, check_cuda, dtype_code, once, wants_grad
 
 MAX_CHANNELS = 8192      # MG_LAYER_NORM_MAX_CHANNELS
 _FORWARD = _lib.Launcher("mg_layer_norm_forward")
@@ -60,7 +60,7 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once
     def backward(ctx, dy):
         x, codes, scales, w, stats = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]

@@ -118,7 +118,7 @@ def test_c_entry_points_refuse():
         g=one, stats=one, live=one, dx=one, dw=one, db=None, scr=one, nb=1 << 30, st=s0),
         **k}.values())
     assert [gb(dtype=5), gb(lb=3), gb(red=-1), gb(g=None), gb(stats=None), gb(live=None),
-            gb(scr=None), gb(scr=128), gb(nb=8), gb(dx=264)] == [bad] * 10
+            gb(scr=None), gb(scr=128), gb(nb=8), gb(dx=264), gb(dw=264)] == [bad] * 11
     assert L.mg_label_loss_scratch_bytes(0, 8, 8, 0, 0) == 0
     assert L.mg_label_loss_scratch_bytes(8, 600, 8, 0, 0) == 0
     assert b"label_loss" in L.mg_last_error()

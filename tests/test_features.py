@@ -579,6 +579,21 @@ def test_label_gradient_against_differences(cuda):
     assert abs(got - slope) <= 1e-6 + 200 * U * size
 
 
+def test_second_derivatives_are_refused(cuda):
+    """A first derivative may be part of a graph; asking for the second of
+    these operators raises."""
+    x, w, lab, bias, _ = label_case(21, 20, 8, 6, F32)
+    for f in (lambda t: label_loss(t, w, lab), lambda t: layer_norm(t).square().sum(),
+              lambda t: layer_norm(t, saved="int8").square().sum(),
+              lambda t: checkpoint8(lambda u: label_loss(u, w, lab), t)):
+        xl = x.clone().requires_grad_(True)
+        (plain,) = torch.autograd.grad(f(xl), xl)
+        (g,) = torch.autograd.grad(f(xl), xl, create_graph=True)
+        assert torch.equal(g, plain)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(g.sum(), xl)
+
+
 # ------------------------------------------------------------------ as a user's program runs them
 
 def head(x, lw, lb, c, lab, cb):
