@@ -177,7 +177,71 @@ __device__ __forceinline__ Scale8 scale8(float a) {
 // A NaN or infinite x times inv = 0 is NaN, which converts to code 0.
 __device__ __forceinline__ int code8(float x, float inv) { return __float2int_rn(__fmul_rn(x, inv)); }
 
+// ------------------------------------------------- rows of any length, staged
+//
+// Rows whose length is no multiple of 16 bytes start anywhere, but a chunk of
+// rows is one stretch of memory: a block copies it to shared memory in 16-byte
+// pieces (asynchronous, the next chunk while this one is worked on), works on
+// it there by rows or columns, and writes the result back the same way. Chunks
+// of stage_rows rows start on 16-byte boundaries when the tensor does.
+
+constexpr int kStageMaxChannels = 1024;
+
+// Rows of a chunk: about 16 KB, a multiple of 16 rows while that allows (so
+// that rows of single bytes keep the boundary too), at least 8.
+__host__ __device__ inline int stage_rows(int channels, int elem_bytes) {
+    const int fit = 16384 / (channels * elem_bytes);
+    return fit >= 16 ? fit / 16 * 16 : 8;
+}
+
+// `bytes` from global to shared memory by a whole block; src and dst 16-byte
+// aligned unless `aligned` is false. Ends with the copies committed as one
+// cp.async group (plain copies are done at the next barrier).
+__device__ __forceinline__ void stage_in(uint8_t* dst, const uint8_t* __restrict__ src, int bytes,
+                                         bool aligned) {
+    const int whole = aligned ? bytes / 16 * 16 : 0;
+    const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+    for (int i = threadIdx.x * 16; i < whole; i += blockDim.x * 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d + i), "l"(src + i) : "memory");
+    for (int i = whole + threadIdx.x; i < bytes; i += blockDim.x) dst[i] = __ldg(src + i);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int PENDING>
+__device__ __forceinline__ void stage_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
+}
+
+__device__ __forceinline__ void stage_out(uint8_t* __restrict__ dst, const uint8_t* src, int bytes,
+                                          bool aligned) {
+    const int whole = aligned ? bytes / 16 * 16 : 0;
+    for (int i = threadIdx.x * 16; i < whole; i += blockDim.x * 16)
+        *reinterpret_cast<uint4*>(dst + i) = *reinterpret_cast<const uint4*>(src + i);
+    for (int i = whole + threadIdx.x; i < bytes; i += blockDim.x) dst[i] = src[i];
+}
+
+__host__ __device__ inline int align16(int bytes) { return (bytes + 15) & ~15; }
+
 inline int blocks8(int64_t channels) { return (int)((channels + kBlock8 - 1) / kBlock8); }
+
+// Codes and scales of a row in shared memory by a team of LPR lanes (32 for
+// rows over 128 channels): element j * LPR + lane is this lane's, and a scale's
+// 128 channels are 4 steps of 32 lanes or the whole row.
+template <typename T, int LPR>
+__device__ __forceinline__ void row_to_codes(const T* row, int channels, int lane, bool live,
+                                             int8_t* codes, float* scales) {
+    for (int c0 = 0; c0 < channels; c0 += kBlock8) {
+        const int end = min(channels, c0 + kBlock8);
+        float a = 0.0f;
+        if (live)
+            for (int c = c0 + lane; c < end; c += LPR) a = fmaxf(a, mag8(to_f32<T>(row[c])));
+        a = lanes_max<LPR>(a);
+        const Scale8 s = scale8(a);
+        if (live) {
+            for (int c = c0 + lane; c < end; c += LPR) codes[c] = (int8_t)code8(to_f32<T>(row[c]), s.inv);
+            if (lane == 0) scales[c0 / kBlock8] = s.scale;
+        }
+    }
+}
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0u; }
 
