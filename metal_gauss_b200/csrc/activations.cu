@@ -30,8 +30,12 @@ pack8_kernel(const T* __restrict__ x, int64_t units, int nb, int channels,
 #pragma unroll
     for (int j = 0; j < kUnits; ++j) {
         const int64_t u = u0 + j * kTeams;
-        const int64_t row = nb == 1 ? u : u / nb;
-        const int c0 = nb == 1 ? 0 : (int)(u - row * nb) * kBlock8;
+        int64_t row = u;
+        int c0 = 0;
+        if (nb > 1) {  // 32-bit division where it does: the 64-bit one costs more than the block
+            row = u <= 0xffffffffll ? (int64_t)((uint32_t)u / (uint32_t)nb) : u / nb;
+            c0 = (int)(u - row * nb) * kBlock8;
+        }
         base[j] = row * channels + c0;
         len[j] = u < units ? min(kBlock8, channels - c0) : 0;
 #pragma unroll
@@ -47,16 +51,16 @@ pack8_kernel(const T* __restrict__ x, int64_t units, int nb, int channels,
     }
 #pragma unroll
     for (int j = 0; j < kUnits; ++j) {
-        float a = 0.0f;
+        uint32_t a = 0u;
 #pragma unroll
-        for (int i = 0; i < NV * VEC; ++i) a = fmaxf(a, mag8(v[j][i]));
+        for (int i = 0; i < NV * VEC; ++i) a = max(a, mag8(v[j][i]));
         a = lanes_max<LPR>(a);
         const Scale8 s = scale8(a);
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int c = (k * LPR + lane) * VEC;
             if (c < len[j]) {
-                int q[VEC];
+                uint32_t q[VEC];
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) q[i] = code8(v[j][k * VEC + i], s.inv);
                 store_codes<VEC>(codes + base[j] + c, q);
@@ -104,51 +108,63 @@ pack8_staged_kernel(const T* __restrict__ x, int64_t rows, int channels, int chu
     }
 }
 
-// x = code * scale over the flat tensor, 8 elements to a thread wherever rows
-// and blocks end (VEC 1 for what is left, or tensors off the boundaries).
+// x = code * scale over the flat tensor, kFlat groups of VEC elements to a
+// thread wherever rows and blocks end (VEC 1 for what is left, or tensors off
+// the boundaries).
+constexpr int kFlat = 2;
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads)
 unpack8_kernel(const int8_t* __restrict__ codes, const float* __restrict__ scales, int64_t first,
                int64_t count, int nb, int channels, T* __restrict__ x) {
-    const int64_t v = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (v >= count) return;
-    const int64_t e = first + v * VEC;
-    int64_t row;
-    int c;
-    if (e <= 0xffffffffll) {
-        const uint32_t q = (uint32_t)e / (uint32_t)channels;
-        row = q;
-        c = (int)((uint32_t)e - q * (uint32_t)channels);
-    } else {
-        row = e / channels;
-        c = (int)(e - row * channels);
-    }
-    int8_t q[VEC];
-    if constexpr (VEC == 8) {
-        const uint2 w = __ldg(reinterpret_cast<const uint2*>(codes + e));
-        memcpy(q, &w, 8);
-    } else {
-        q[0] = __ldg(codes + e);
-    }
-    const float* s = scales + row * nb + c / kBlock8;
-    float scale = __ldg(s);
-    T o[VEC];
+    const int64_t v0 = (int64_t)blockIdx.x * (kThreads * kFlat) + threadIdx.x;
+    int8_t q[kFlat][VEC];
+    const float* s[kFlat];
+    float scale[kFlat];
+    int c[kFlat];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-        o[i] = from_f32<T>(__fmul_rn((float)q[i], scale));
-        ++c;
-        if (i + 1 < VEC && (c == channels || c % kBlock8 == 0)) {
-            if (c == channels) c = 0;
-            scale = __ldg(++s);  // the next block, of this row or the next
+    for (int j = 0; j < kFlat; ++j) {
+        const int64_t v = v0 + j * kThreads, e = first + v * VEC;
+        if (v >= count) continue;
+        if constexpr (VEC == 8) {
+            const uint2 w = __ldg(reinterpret_cast<const uint2*>(codes + e));
+            memcpy(q[j], &w, 8);
+        } else {
+            q[j][0] = __ldg(codes + e);
         }
+        int64_t row;
+        if (e <= 0xffffffffll) {
+            const uint32_t r = (uint32_t)e / (uint32_t)channels;
+            row = r;
+            c[j] = (int)((uint32_t)e - r * (uint32_t)channels);
+        } else {
+            row = e / channels;
+            c[j] = (int)(e - row * channels);
+        }
+        s[j] = scales + row * nb + c[j] / kBlock8;
+        scale[j] = __ldg(s[j]);
     }
-    if constexpr (VEC == 8) {
-        uint4 w[sizeof(o) / 16];
-        memcpy(w, o, sizeof(o));
 #pragma unroll
-        for (int i = 0; i < (int)(sizeof(o) / 16); ++i) reinterpret_cast<uint4*>(x + e)[i] = w[i];
-    } else {
-        x[e] = o[0];
+    for (int j = 0; j < kFlat; ++j) {
+        const int64_t v = v0 + j * kThreads, e = first + v * VEC;
+        if (v >= count) continue;
+        T o[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            o[i] = from_f32<T>(__fmul_rn((float)q[j][i], scale[j]));
+            ++c[j];
+            if (i + 1 < VEC && (c[j] == channels || c[j] % kBlock8 == 0)) {
+                if (c[j] == channels) c[j] = 0;
+                scale[j] = __ldg(++s[j]);  // the next block, of this row or the next
+            }
+        }
+        if constexpr (VEC == 8) {
+            uint4 w[sizeof(o) / 16];
+            memcpy(w, o, sizeof(o));
+#pragma unroll
+            for (int i = 0; i < (int)(sizeof(o) / 16); ++i) reinterpret_cast<uint4*>(x + e)[i] = w[i];
+        } else {
+            x[e] = o[0];
+        }
     }
 }
 
@@ -229,12 +245,12 @@ mg_status unpack(const int8_t* codes, const float* scales, int64_t rows, int cha
     const int nb = blocks8(channels);
     const int64_t vectors = aligned16(x) ? n / 8 : 0, left = n - 8 * vectors;
     if (vectors > 0) {
-        unpack8_kernel<T, 8><<<(unsigned)((vectors + kThreads - 1) / kThreads), kThreads, 0, st>>>(
+        unpack8_kernel<T, 8><<<(unsigned)((vectors + kThreads * kFlat - 1) / (kThreads * kFlat)), kThreads, 0, st>>>(
             codes, scales, 0, vectors, nb, channels, x);
         MG_TRY(check_launch("unpack8"));
     }
     if (left == 0) return MG_OK;
-    unpack8_kernel<T, 1><<<(unsigned)((left + kThreads - 1) / kThreads), kThreads, 0, st>>>(
+    unpack8_kernel<T, 1><<<(unsigned)((left + kThreads * kFlat - 1) / (kThreads * kFlat)), kThreads, 0, st>>>(
         codes, scales, 8 * vectors, left, nb, channels, x);
     return check_launch("unpack8");
 }

@@ -191,16 +191,16 @@ norm_forward_kernel(const T* __restrict__ x, const void* __restrict__ weight,
                 constexpr int kStep = VEC == 1 ? (NV < 4 ? NV : 4) : 1;
 #pragma unroll
                 for (int k0 = 0; k0 < NV; k0 += kStep) {
-                    float a = 0.0f;
+                    uint32_t a = 0u;
 #pragma unroll
-                    for (int i = 0; i < kStep * VEC; ++i) a = fmaxf(a, mag8(to_f32<T>(v[r][k0 * VEC + i])));
+                    for (int i = 0; i < kStep * VEC; ++i) a = max(a, mag8(to_f32<T>(v[r][k0 * VEC + i])));
                     a = lanes_max<kGroup>(a);
                     const Scale8 s8 = scale8(a);
 #pragma unroll
                     for (int k = k0; k < k0 + kStep; ++k) {
                         const int c = channel_of<VEC, LPR, WARPS>(k, warp, lane);
                         if (live && c < channels) {
-                            int qv[VEC];
+                            uint32_t qv[VEC];
 #pragma unroll
                             for (int i = 0; i < VEC; ++i) qv[i] = code8(to_f32<T>(v[r][k * VEC + i]), s8.inv);
                             store_codes<VEC>(codes + row * channels + c, qv);

@@ -73,34 +73,17 @@ __device__ __forceinline__ void load_raw(const T* __restrict__ p, T* v) {
     }
 }
 
-// VEC codes (VEC 1, 4 or 8; p aligned to VEC bytes).
+// VEC codes, the low bytes of q (VEC 1, 4 or 8; p aligned to VEC bytes).
 template <int VEC>
-__device__ __forceinline__ void store_codes(int8_t* __restrict__ p, const int* q) {
+__device__ __forceinline__ void store_codes(int8_t* __restrict__ p, const uint32_t* q) {
     if constexpr (VEC == 1) {
         p[0] = (int8_t)q[0];
     } else {
 #pragma unroll
-        for (int k = 0; k < VEC / 4; ++k) {
-            const uint32_t w = (uint32_t)(uint8_t)q[4 * k] | (uint32_t)(uint8_t)q[4 * k + 1] << 8 |
-                               (uint32_t)(uint8_t)q[4 * k + 2] << 16 |
-                               (uint32_t)(uint8_t)q[4 * k + 3] << 24;
-            if constexpr (VEC == 4) *reinterpret_cast<uint32_t*>(p) = w;
-            else reinterpret_cast<uint32_t*>(p)[k] = w;
-        }
-    }
-}
-
-template <int VEC>
-__device__ __forceinline__ void load_codes(const int8_t* __restrict__ p, float* v) {
-    if constexpr (VEC == 1) {
-        v[0] = (float)__ldg(p);
-    } else {
-#pragma unroll
-        for (int k = 0; k < VEC / 4; ++k) {
-            const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(p) + k);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[4 * k + i] = (float)(int8_t)(w >> (8 * i));
-        }
+        for (int k = 0; k < VEC / 4; ++k)
+            reinterpret_cast<uint32_t*>(p)[k] =
+                __byte_perm(__byte_perm(q[4 * k], q[4 * k + 1], 0x0040),
+                            __byte_perm(q[4 * k + 2], q[4 * k + 3], 0x0040), 0x5410);
     }
 }
 
@@ -127,9 +110,10 @@ __device__ __forceinline__ float lanes_sum(float v) {
 }
 
 template <int L>
-__device__ __forceinline__ float lanes_max(float v) {
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+    if constexpr (L == 32) return __reduce_max_sync(0xffffffffu, v);
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    for (int o = L / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
 
@@ -149,14 +133,12 @@ struct Scale8 {
     float inv, scale;
 };
 
-// fmaxf drops NaNs, so the caller's maximum is over |x| with NaN mapped to
-// infinity (mag8).
-__device__ __forceinline__ float mag8(float x) {
-    const float a = fabsf(x);
-    return a <= 3.402823466e38f ? a : __int_as_float(0x7f800000);
-}
+// |x| as an integer, whose order is that of the magnitudes with infinity and
+// then NaN above them: the maximum of these misses no NaN, as fmaxf would.
+__device__ __forceinline__ uint32_t mag8(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-__device__ __forceinline__ Scale8 scale8(float a) {
+__device__ __forceinline__ Scale8 scale8(uint32_t magnitude) {
+    const float a = __uint_as_float(magnitude);
     Scale8 s;
     if (!(a <= 3.402823466e38f)) {
         s.inv = 0.0f;
@@ -174,8 +156,12 @@ __device__ __forceinline__ Scale8 scale8(float a) {
     return s;
 }
 
-// A NaN or infinite x times inv = 0 is NaN, which converts to code 0.
-__device__ __forceinline__ int code8(float x, float inv) { return __float2int_rn(__fmul_rn(x, inv)); }
+// The code in the low byte: adding 1.5 * 2^23 rounds a product of at most 127
+// to an integer, half to even, in the sum's last bits. (In a block with a NaN
+// or an infinity the byte means nothing: its scale is NaN.)
+__device__ __forceinline__ uint32_t code8(float x, float inv) {
+    return __float_as_uint(__fadd_rn(__fmul_rn(x, inv), 12582912.0f));
+}
 
 // ------------------------------------------------- rows of any length, staged
 //
@@ -231,9 +217,9 @@ __device__ __forceinline__ void row_to_codes(const T* row, int channels, int lan
                                              int8_t* codes, float* scales) {
     for (int c0 = 0; c0 < channels; c0 += kBlock8) {
         const int end = min(channels, c0 + kBlock8);
-        float a = 0.0f;
+        uint32_t a = 0u;
         if (live)
-            for (int c = c0 + lane; c < end; c += LPR) a = fmaxf(a, mag8(to_f32<T>(row[c])));
+            for (int c = c0 + lane; c < end; c += LPR) a = max(a, mag8(to_f32<T>(row[c])));
         a = lanes_max<LPR>(a);
         const Scale8 s = scale8(a);
         if (live) {
