@@ -49,24 +49,33 @@ pack8_kernel(const T* __restrict__ x, int64_t units, int nb, int channels,
             }
         }
     }
+    // The two quotients of unit j are lane j's to compute: two divisions for all
+    // kUnits blocks, where each lane doing them for its own cost more than all else.
+    static_assert(kUnits <= LPR, "a lane for each unit");
+    uint32_t mine = 0u;
 #pragma unroll
     for (int j = 0; j < kUnits; ++j) {
         uint32_t a = 0u;
 #pragma unroll
         for (int i = 0; i < NV * VEC; ++i) a = max(a, mag8(v[j][i]));
         a = lanes_max<LPR>(a);
-        const Scale8 s = scale8(a);
+        if (lane == j) mine = a;
+    }
+    const Scale8 s = scale8(mine);
+    if (lane < kUnits && u0 + lane * kTeams < units) scales[u0 + lane * kTeams] = s.scale;
+#pragma unroll
+    for (int j = 0; j < kUnits; ++j) {
+        const float inv = __shfl_sync(0xffffffffu, s.inv, j, LPR);
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int c = (k * LPR + lane) * VEC;
             if (c < len[j]) {
                 uint32_t q[VEC];
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) q[i] = code8(v[j][k * VEC + i], s.inv);
+                for (int i = 0; i < VEC; ++i) q[i] = code8(v[j][k * VEC + i], inv);
                 store_codes<VEC>(codes + base[j] + c, q);
             }
         }
-        if (lane == 0 && len[j] > 0) scales[u0 + j * kTeams] = s.scale;
     }
 }
 

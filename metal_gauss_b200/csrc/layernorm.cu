@@ -181,34 +181,50 @@ norm_forward_kernel(const T* __restrict__ x, const void* __restrict__ weight,
             }
             rstd[r] = 1.0f / sqrtf(team_sum<LPR, WARPS>(q, 0.0f, sh, warp, lane).x * inv_n + eps);
         }
+        if (codes != nullptr) {
+            // one scale per 128 channels, the maximum over the kGroup lanes that hold
+            // them; the quotients of block q (of a row and kStep register groups)
+            // are lane q's to compute
+            constexpr int kGroup = VEC == 8 ? (LPR < 16 ? LPR : 16) : LPR;
+            constexpr int kStep = VEC == 1 ? (NV < 4 ? NV : 4) : 1;
+            constexpr int kBlocks = R * (NV / kStep);
+            static_assert(kBlocks <= kGroup, "a lane for each block");
+            const int member = lane % kGroup;
+            uint32_t mine = 0u;
+#pragma unroll
+            for (int q = 0; q < kBlocks; ++q) {
+                uint32_t a = 0u;
+#pragma unroll
+                for (int i = 0; i < kStep * VEC; ++i)
+                    a = max(a, mag8(to_f32<T>(v[q / (NV / kStep)][q % (NV / kStep) * kStep * VEC + i])));
+                a = lanes_max<kGroup>(a);
+                if (member == q) mine = a;
+            }
+            const Scale8 s8 = scale8(mine);
+#pragma unroll
+            for (int q = 0; q < kBlocks; ++q) {
+                const int r = q / (NV / kStep), k0 = q % (NV / kStep) * kStep;
+                const int64_t row = row0 + r * kTeams;
+                const float inv = __shfl_sync(0xffffffffu, s8.inv, q, kGroup);
+                if (row >= rows) continue;
+                const int block = channel_of<VEC, LPR, WARPS>(k0, warp, lane) / kBlock8;
+                if (member == q && block < nb) scales[row * nb + block] = s8.scale;
+#pragma unroll
+                for (int k = k0; k < k0 + kStep; ++k) {
+                    const int c = channel_of<VEC, LPR, WARPS>(k, warp, lane);
+                    if (c < channels) {
+                        uint32_t qv[VEC];
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) qv[i] = code8(to_f32<T>(v[r][k * VEC + i]), inv);
+                        store_codes<VEC>(codes + row * channels + c, qv);
+                    }
+                }
+            }
+        }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int64_t row = row0 + r * kTeams;
             const bool live = row < rows;
-            if (codes != nullptr) {
-                // one scale per 128 channels, the maximum over the lanes that hold them
-                constexpr int kGroup = VEC == 8 ? (LPR < 16 ? LPR : 16) : LPR;
-                constexpr int kStep = VEC == 1 ? (NV < 4 ? NV : 4) : 1;
-#pragma unroll
-                for (int k0 = 0; k0 < NV; k0 += kStep) {
-                    uint32_t a = 0u;
-#pragma unroll
-                    for (int i = 0; i < kStep * VEC; ++i) a = max(a, mag8(to_f32<T>(v[r][k0 * VEC + i])));
-                    a = lanes_max<kGroup>(a);
-                    const Scale8 s8 = scale8(a);
-#pragma unroll
-                    for (int k = k0; k < k0 + kStep; ++k) {
-                        const int c = channel_of<VEC, LPR, WARPS>(k, warp, lane);
-                        if (live && c < channels) {
-                            uint32_t qv[VEC];
-#pragma unroll
-                            for (int i = 0; i < VEC; ++i) qv[i] = code8(to_f32<T>(v[r][k * VEC + i]), s8.inv);
-                            store_codes<VEC>(codes + row * channels + c, qv);
-                            if (c % kBlock8 == 0) scales[row * nb + c / kBlock8] = s8.scale;
-                        }
-                    }
-                }
-            }
             if (!live) continue;
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
