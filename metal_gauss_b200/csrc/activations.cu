@@ -24,7 +24,7 @@ pack8_kernel(const T* __restrict__ x, int64_t units, int nb, int channels,
     constexpr int kTeams = kThreads / LPR;
     const int lane = threadIdx.x % LPR;
     const int64_t u0 = (int64_t)blockIdx.x * kTeams * kUnits + threadIdx.x / LPR;
-    float v[kUnits][NV * VEC];
+    T v[kUnits][NV * VEC];
     int64_t base[kUnits];
     int len[kUnits];
 #pragma unroll
@@ -42,10 +42,10 @@ pack8_kernel(const T* __restrict__ x, int64_t units, int nb, int channels,
         for (int k = 0; k < NV; ++k) {
             const int c = (k * LPR + lane) * VEC;
             if (c < len[j]) {
-                load_row<T, VEC>(x + base[j] + c, &v[j][k * VEC]);
+                load_raw<T, VEC>(x + base[j] + c, &v[j][k * VEC]);
             } else {
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) v[j][k * VEC + i] = 0.0f;
+                for (int i = 0; i < VEC; ++i) v[j][k * VEC + i] = from_f32<T>(0.0f);
             }
         }
     }
@@ -55,10 +55,7 @@ pack8_kernel(const T* __restrict__ x, int64_t units, int nb, int channels,
     uint32_t mine = 0u;
 #pragma unroll
     for (int j = 0; j < kUnits; ++j) {
-        uint32_t a = 0u;
-#pragma unroll
-        for (int i = 0; i < NV * VEC; ++i) a = max(a, mag8(v[j][i]));
-        a = lanes_max<LPR>(a);
+        const uint32_t a = lanes_max<LPR>(largest8<T, NV * VEC>(v[j]));
         if (lane == j) mine = a;
     }
     const Scale8 s = scale8(mine);
@@ -72,7 +69,7 @@ pack8_kernel(const T* __restrict__ x, int64_t units, int nb, int channels,
             if (c < len[j]) {
                 uint32_t q[VEC];
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) q[i] = code8(v[j][k * VEC + i], inv);
+                for (int i = 0; i < VEC; ++i) q[i] = code8(to_f32<T>(v[j][k * VEC + i]), inv);
                 store_codes<VEC>(codes + base[j] + c, q);
             }
         }

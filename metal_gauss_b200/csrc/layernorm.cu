@@ -193,11 +193,8 @@ norm_forward_kernel(const T* __restrict__ x, const void* __restrict__ weight,
             uint32_t mine = 0u;
 #pragma unroll
             for (int q = 0; q < kBlocks; ++q) {
-                uint32_t a = 0u;
-#pragma unroll
-                for (int i = 0; i < kStep * VEC; ++i)
-                    a = max(a, mag8(to_f32<T>(v[q / (NV / kStep)][q % (NV / kStep) * kStep * VEC + i])));
-                a = lanes_max<kGroup>(a);
+                const uint32_t a = lanes_max<kGroup>(
+                    largest8<T, kStep * VEC>(v[q / (NV / kStep)] + q % (NV / kStep) * kStep * VEC));
                 if (member == q) mine = a;
             }
             const Scale8 s8 = scale8(mine);

@@ -137,6 +137,29 @@ struct Scale8 {
 // then NaN above them: the maximum of these misses no NaN, as fmaxf would.
 __device__ __forceinline__ uint32_t mag8(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
+// The largest of N elements' magnitudes; 16-bit types two at a time.
+template <typename T, int N>
+__device__ __forceinline__ uint32_t largest8(const T* v) {
+    if constexpr (sizeof(T) == 2 && N % 2 == 0) {
+        uint32_t a = 0u;
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            uint32_t w;
+            memcpy(&w, v + i, 4);
+            a = __vmaxu2(a, w & 0x7fff7fffu);
+        }
+        const uint16_t top = (uint16_t)max(a & 0xffffu, a >> 16);
+        T t;
+        memcpy(&t, &top, 2);
+        return __float_as_uint(to_f32<T>(t));
+    } else {
+        uint32_t a = 0u;
+#pragma unroll
+        for (int i = 0; i < N; ++i) a = max(a, mag8(to_f32<T>(v[i])));
+        return a;
+    }
+}
+
 __device__ __forceinline__ Scale8 scale8(uint32_t magnitude) {
     const float a = __uint_as_float(magnitude);
     Scale8 s;
