@@ -79,17 +79,19 @@ pack8_kernel(const T* __restrict__ x, int64_t units, int nb, int channels,
 // Rows of a length that is no multiple of 16 bytes, a staged chunk at a time.
 template <typename T, int LPR>
 __global__ void __launch_bounds__(kThreads)
-pack8_staged_kernel(const T* __restrict__ x, int64_t rows, int channels, int chunk, bool aligned,
-                    bool codes_aligned, int8_t* __restrict__ codes, float* __restrict__ scales) {
+pack8_staged_kernel(const T* __restrict__ x, int64_t rows, int channels, int chunk, int width,
+                    int codes_width, int8_t* __restrict__ codes, float* __restrict__ scales) {
     extern __shared__ __align__(16) uint8_t staged[];
     const int row_bytes = channels * (int)sizeof(T), nb = (channels + kBlock8 - 1) / kBlock8;
     const int buffer = align16(chunk * row_bytes);
     int8_t* out = reinterpret_cast<int8_t*>(staged + 2 * buffer);
+    float* work = reinterpret_cast<float*>(staged + 2 * buffer + align16(chunk * channels));
     const int64_t chunks = (rows + chunk - 1) / chunk;
     const auto rows_of = [&](int64_t i) { return (int)min((int64_t)chunk, rows - i * chunk); };
     const auto fetch = [&](int64_t i, int b) {
         stage_in(staged + b * buffer, reinterpret_cast<const uint8_t*>(x + i * chunk * channels),
-                 rows_of(i) * row_bytes, aligned);
+                 rows_of(i) * row_bytes, width);
+        stage_commit();
     };
     int b = 0;
     if (blockIdx.x < chunks) fetch(blockIdx.x, 0);
@@ -101,15 +103,11 @@ pack8_staged_kernel(const T* __restrict__ x, int64_t rows, int channels, int chu
             stage_wait<0>();
         }
         __syncthreads();
-        const int n = rows_of(i), lane = threadIdx.x % LPR;
-        for (int r0 = 0; r0 < n; r0 += kThreads / LPR) {
-            const int r = r0 + threadIdx.x / LPR;
-            row_to_codes<T, LPR>(reinterpret_cast<const T*>(staged + b * buffer) + r * channels, channels, lane,
-                                 r < n, out + r * channels, scales + (i * chunk + r) * nb);
-        }
-        __syncthreads();
+        const int n = rows_of(i);
+        staged_codes<T, LPR>(reinterpret_cast<const T*>(staged + b * buffer), n, channels, work, out,
+                             scales + i * chunk * nb);
         stage_out(reinterpret_cast<uint8_t*>(codes + i * chunk * channels), reinterpret_cast<uint8_t*>(out),
-                  n * channels, codes_aligned);
+                  n * channels, codes_width);
         __syncthreads();
     }
 }
@@ -212,35 +210,27 @@ mg_status pick_team(const Op& op, int channels) {
 
 template <typename T, int LPR>
 mg_status pack_staged(const Pack& p) {
-    const int chunk = stage_rows(p.channels, (int)sizeof(T));
-    const size_t smem = 2 * align16(chunk * p.channels * (int)sizeof(T)) + align16(chunk * p.channels);
-    static int per_sm[64] = {};
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
-    if (per_sm[dev] == 0) {
-        // the most a chunk can take: 8 rows of 1024 channels
-        if (cudaFuncSetAttribute(pack8_staged_kernel<T, LPR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 80 * 1024) != cudaSuccess)
-            return check_launch("pack8");
-        per_sm[dev] = 4;
-    }
+    const int chunk = stage_rows(p.channels, (int)sizeof(T)), nb = blocks8(p.channels);
+    const int bytes = chunk * p.channels * (int)sizeof(T);
+    const int smem = 2 * align16(bytes) + align16(chunk * p.channels) + 4 * chunk * nb;
+    static int known[64] = {};
+    int per_sm = 0;
+    MG_TRY(staged_launch(pack8_staged_kernel<T, LPR>, kThreads, smem, known, &per_sm, "pack8"));
     const int64_t chunks = (p.rows + chunk - 1) / chunk;
-    const int grid = (int)std::min<int64_t>(chunks, per_sm[dev] * (int64_t)sm_count());
+    const int grid = (int)std::min<int64_t>(chunks, per_sm * (int64_t)sm_count());
     pack8_staged_kernel<T, LPR><<<grid, kThreads, smem, p.st>>>(
-        static_cast<const T*>(p.x), p.rows, p.channels, chunk, aligned16(p.x),
-        aligned16(p.codes) && (int64_t)chunk * p.channels % 16 == 0, p.codes, p.scales);
+        static_cast<const T*>(p.x), p.rows, p.channels, chunk, stage_width(p.x, bytes),
+        stage_width(p.codes, chunk * p.channels), p.codes, p.scales);
     return check_launch("pack8");
 }
 
-// Whole 16-byte vectors by row where the length allows, staged chunks of rows
-// where not (up to 1024 channels: 2.3 times the single elements' rate at 77
-// fp32 channels), single elements above.
+// Whole 16-byte vectors by row where the length allows; where not, staged chunks
+// of short rows (2000000 x 19 fp32: 100 us against 176 by single elements; at 77
+// channels they are level) and single elements of longer ones.
 template <typename T, int VEC>
 mg_status pack(const Pack& p) {
     if (aligned16(p.x) && p.channels % VEC == 0) return pick_team<T, VEC>(p, p.channels);
-    if (p.channels <= 32) return pack_staged<T, 8>(p);
-    if (p.channels <= kBlock8) return pack_staged<T, 16>(p);
-    if (p.channels <= kStageMaxChannels) return pack_staged<T, 32>(p);
+    if (p.channels <= 64) return p.channels <= 32 ? pack_staged<T, 8>(p) : pack_staged<T, 16>(p);
     return pick_team<T, 1>(p, p.channels);
 }
 

@@ -430,6 +430,210 @@ norm_backward_kernel(const T* __restrict__ dy, const T* __restrict__ x,
     }
 }
 
+// ------------------------------------------------------ rows of any length
+//
+// Rows that do not come in 16-byte vectors (or start off their boundary): where
+// it pays (staged() below), chunks of rows staged in shared memory (rows.cuh),
+// a team of LPR lanes to a row, and for dw and db a thread to a column.
+
+template <typename T, int LPR>
+__global__ void __launch_bounds__(kThreads)
+norm_forward_staged_kernel(const T* __restrict__ x, const void* __restrict__ weight,
+                           const void* __restrict__ bias, int param_dtype, int64_t rows,
+                           int channels, float eps, int chunk, int width, int width_y, int width_codes,
+                           T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out,
+                           int8_t* __restrict__ codes, float* __restrict__ scales) {
+    extern __shared__ __align__(16) uint8_t staged[];
+    const int row_bytes = channels * (int)sizeof(T), nb = (channels + kBlock8 - 1) / kBlock8;
+    const int buffer = align16(chunk * row_bytes);
+    float* w = reinterpret_cast<float*>(staged + 2 * buffer);
+    float* b = w + channels;
+    float* work = b + channels;  // with codes: chunk * nb floats, then the codes
+    int8_t* out8 = reinterpret_cast<int8_t*>(staged + 2 * buffer + align16(4 * (2 * channels + chunk * nb)));
+    for (int c = threadIdx.x; c < channels; c += kThreads) {
+        w[c] = weight != nullptr ? param_at(weight, param_dtype, c) : 1.0f;
+        b[c] = bias != nullptr ? param_at(bias, param_dtype, c) : 0.0f;
+    }
+    const float inv_n = 1.0f / (float)channels;
+    const int64_t chunks = (rows + chunk - 1) / chunk;
+    const auto rows_of = [&](int64_t i) { return (int)min((int64_t)chunk, rows - i * chunk); };
+    const auto fetch = [&](int64_t i, int q) {
+        stage_in(staged + q * buffer, reinterpret_cast<const uint8_t*>(x + i * chunk * channels),
+                 rows_of(i) * row_bytes, width);
+        stage_commit();
+    };
+    const int lane = threadIdx.x % LPR, team = threadIdx.x / LPR;
+    constexpr int kTeams = kThreads / LPR;
+    int q = 0;
+    if (blockIdx.x < chunks) fetch(blockIdx.x, 0);
+    for (int64_t i = blockIdx.x; i < chunks; i += gridDim.x, q ^= 1) {
+        if (i + gridDim.x < chunks) {
+            fetch(i + gridDim.x, q ^ 1);
+            stage_wait<1>();
+        } else {
+            stage_wait<0>();
+        }
+        __syncthreads();
+        const int n = rows_of(i);
+        T* in = reinterpret_cast<T*>(staged + q * buffer);
+        if (codes != nullptr) {
+            staged_codes<T, LPR>(in, n, channels, work, out8, scales + i * chunk * nb);
+            stage_out(reinterpret_cast<uint8_t*>(codes + i * chunk * channels), reinterpret_cast<uint8_t*>(out8),
+                      n * channels, width_codes);
+        }
+        for (int r0 = 0; r0 < n; r0 += kTeams) {
+            const int r = r0 + team, length = r < n ? channels : 0;
+            T* row = in + r * channels;
+            float s = 0.0f;
+            for (int c = lane; c < length; c += LPR) s += to_f32<T>(row[c]);
+            const float mean = lanes_sum<LPR>(s) * inv_n;
+            float v = 0.0f;
+            for (int c = lane; c < length; c += LPR) {
+                const float d = to_f32<T>(row[c]) - mean;
+                v = fmaf(d, d, v);
+            }
+            const float rstd = 1.0f / sqrtf(lanes_sum<LPR>(v) * inv_n + eps);
+            if (r < n) {
+                for (int c = lane; c < channels; c += LPR)
+                    row[c] = from_f32<T>(fmaf((to_f32<T>(row[c]) - mean) * rstd, w[c], b[c]));
+                if (mean_out != nullptr && lane == 0) {
+                    mean_out[i * chunk + r] = mean;
+                    rstd_out[i * chunk + r] = rstd;
+                }
+            }
+        }
+        __syncthreads();
+        stage_out(reinterpret_cast<uint8_t*>(y + i * chunk * channels), staged + q * buffer, n * row_bytes, width_y);
+        __syncthreads();
+    }
+}
+
+constexpr int kColumns = kStageMaxChannels / kThreads;  // of a thread, at most
+
+template <typename T, int LPR, bool HELD8>
+__global__ void __launch_bounds__(kThreads)
+norm_backward_staged_kernel(const T* __restrict__ dy, const T* __restrict__ x,
+                            const int8_t* __restrict__ codes, const float* __restrict__ scales,
+                            const void* __restrict__ weight, int param_dtype,
+                            const float* __restrict__ mean_in, const float* __restrict__ rstd_in,
+                            int64_t rows, int channels, int chunk, int width_dy, int width_x, int width_dx,
+                            T* __restrict__ dx, float* __restrict__ partial) {
+    using Held = typename HeldType<T, HELD8>::type;
+    extern __shared__ __align__(16) uint8_t staged[];
+    const int row_bytes = channels * (int)sizeof(T), held_bytes = channels * (int)sizeof(Held);
+    const int nb = (channels + kBlock8 - 1) / kBlock8;
+    const int size_g = align16(chunk * row_bytes), size_x = align16(chunk * held_bytes);
+    const int buffer = size_g + size_x;
+    float* w = reinterpret_cast<float*>(staged + 2 * buffer);
+    float2* stat = reinterpret_cast<float2*>(w + (channels + 1) / 2 * 2);  // mean, rstd of the chunk
+    for (int c = threadIdx.x; c < channels; c += kThreads)
+        w[c] = weight != nullptr ? param_at(weight, param_dtype, c) : 1.0f;
+    const float inv_n = 1.0f / (float)channels;
+    const int64_t chunks = (rows + chunk - 1) / chunk;
+    const auto rows_of = [&](int64_t i) { return (int)min((int64_t)chunk, rows - i * chunk); };
+    const auto fetch = [&](int64_t i, int q) {
+        stage_in(staged + q * buffer, reinterpret_cast<const uint8_t*>(dy + i * chunk * channels),
+                 rows_of(i) * row_bytes, width_dy);
+        const uint8_t* held = HELD8 ? reinterpret_cast<const uint8_t*>(codes + i * chunk * channels)
+                                    : reinterpret_cast<const uint8_t*>(x + i * chunk * channels);
+        stage_in(staged + q * buffer + size_g, held, rows_of(i) * held_bytes, width_x);
+        stage_commit();
+    };
+    const int lane = threadIdx.x % LPR, team = threadIdx.x / LPR;
+    constexpr int kTeams = kThreads / LPR;
+    // columns: fewer than the threads leave several row groups to each column
+    const int groups = channels < kThreads ? kThreads / channels : 1;
+    const int group = channels < kThreads ? (int)threadIdx.x / channels : 0;
+    const int column = channels < kThreads ? (int)threadIdx.x % channels : (int)threadIdx.x;
+    float dw[kColumns] = {}, db[kColumns] = {};
+    int q = 0;
+    if (blockIdx.x < chunks) fetch(blockIdx.x, 0);
+    for (int64_t i = blockIdx.x; i < chunks; i += gridDim.x, q ^= 1) {
+        const int n = rows_of(i);
+        for (int r = threadIdx.x; r < n; r += kThreads)
+            stat[r] = make_float2(__ldg(mean_in + i * chunk + r), __ldg(rstd_in + i * chunk + r));
+        if (i + gridDim.x < chunks) {
+            fetch(i + gridDim.x, q ^ 1);
+            stage_wait<1>();
+        } else {
+            stage_wait<0>();
+        }
+        __syncthreads();
+        T* g = reinterpret_cast<T*>(staged + q * buffer);
+        const Held* h = reinterpret_cast<const Held*>(staged + q * buffer + size_g);
+        const float* sc = HELD8 ? scales + i * chunk * nb : nullptr;
+        const auto hat = [&](int r, int c, float2 st) {
+            float v;
+            if constexpr (HELD8) v = __fmul_rn((float)h[r * channels + c], __ldg(sc + r * nb + c / kBlock8));
+            else v = to_f32<T>(h[r * channels + c]);
+            return (v - st.x) * st.y;
+        };
+        if (partial != nullptr && group < groups) {
+            for (int r = group; r < n; r += groups) {
+                const float2 st = stat[r];
+#pragma unroll
+                for (int k = 0; k < kColumns; ++k) {
+                    const int c = column + k * kThreads;
+                    if (c < channels) {
+                        const float d = to_f32<T>(g[r * channels + c]);
+                        dw[k] = fmaf(d, hat(r, c, st), dw[k]);
+                        db[k] += d;
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        if (dx != nullptr) {
+            for (int r0 = 0; r0 < n; r0 += kTeams) {
+                const int r = r0 + team;
+                float sg = 0.0f, sgh = 0.0f;
+                if (r < n) {
+                    const float2 st = stat[r];
+                    for (int c = lane; c < channels; c += LPR) {
+                        const float wg = to_f32<T>(g[r * channels + c]) * w[c];
+                        sg += wg;
+                        sgh = fmaf(wg, hat(r, c, st), sgh);
+                    }
+                }
+                const float c1 = lanes_sum<LPR>(sg) * inv_n, c2 = lanes_sum<LPR>(sgh) * inv_n;
+                if (r < n) {
+                    const float2 st = stat[r];
+                    for (int c = lane; c < channels; c += LPR)
+                        g[r * channels + c] = from_f32<T>(
+                            st.y * (to_f32<T>(g[r * channels + c]) * w[c] - c1 - hat(r, c, st) * c2));
+                }
+            }
+            __syncthreads();
+            stage_out(reinterpret_cast<uint8_t*>(dx + i * chunk * channels), staged + q * buffer, n * row_bytes,
+                      width_dx);
+        }
+        __syncthreads();
+    }
+    if (partial == nullptr) return;
+    // the row groups' sums of a column, in order (the buffers are free now)
+    float* join = reinterpret_cast<float*>(staged);
+    float* out = partial + (int64_t)blockIdx.x * 2 * channels;
+#pragma unroll
+    for (int pass = 0; pass < 2; ++pass) {
+        if (groups > 1) {
+            if (group < groups) join[group * channels + column] = pass == 0 ? dw[0] : db[0];
+            __syncthreads();
+            if ((int)threadIdx.x < channels) {
+                float s = 0.0f;
+                for (int k = 0; k < groups; ++k) s += join[k * channels + threadIdx.x];
+                out[pass * channels + threadIdx.x] = s;
+            }
+            __syncthreads();
+        } else {
+#pragma unroll
+            for (int k = 0; k < kColumns; ++k) {
+                const int c = column + k * kThreads;
+                if (group < groups && c < channels) out[pass * channels + c] = pass == 0 ? dw[k] : db[k];
+            }
+        }
+    }
+}
+
 // Column sums of the blocks' partial rows: 32 columns and 32 row groups to a
 // block; columns [0, channels) are dw, the rest db.
 __global__ void __launch_bounds__(1024)
@@ -540,6 +744,63 @@ struct Backward {
     }
 };
 
+template <typename T, int LPR>
+mg_status forward_staged(const Forward& f) {
+    const int chunk = stage_rows(f.channels, (int)sizeof(T)), nb = blocks8(f.channels);
+    const int bytes = chunk * f.channels * (int)sizeof(T);
+    int smem = 2 * align16(bytes) + align16(4 * (2 * f.channels + chunk * nb));
+    if (f.codes != nullptr) smem += align16(chunk * f.channels);
+    static int known[64] = {};
+    int per_sm = 0;
+    MG_TRY(staged_launch(norm_forward_staged_kernel<T, LPR>, kThreads, smem, known, &per_sm, "layer_norm_forward"));
+    const int grid = (int)std::min<int64_t>((f.rows + chunk - 1) / chunk, per_sm * (int64_t)sm_count());
+    norm_forward_staged_kernel<T, LPR><<<grid, kThreads, smem, f.st>>>(
+        static_cast<const T*>(f.x), f.weight, f.bias, f.param_dtype, f.rows, f.channels, f.eps, chunk,
+        stage_width(f.x, bytes), stage_width(f.y, bytes), stage_width(f.codes, chunk * f.channels),
+        static_cast<T*>(f.y), f.mean, f.rstd, f.codes, f.scales);
+    return check_launch("layer_norm_forward");
+}
+
+template <typename T, int LPR, bool HELD8>
+mg_status backward_staged(const Backward& f) {
+    const int chunk = stage_rows(f.channels, (int)sizeof(T));
+    const int bytes = chunk * f.channels * (int)sizeof(T);
+    const int held = HELD8 ? chunk * f.channels : bytes;
+    // the join at the end takes the buffers' place: 256 floats, or 1 KB a group
+    const int smem = std::max(2 * (align16(bytes) + align16(held)), 4 * kThreads) + 4 * (f.channels + 1) + 8 * chunk;
+    static int known[64] = {};
+    int per_sm = 0;
+    MG_TRY(staged_launch(norm_backward_staged_kernel<T, LPR, HELD8>, kThreads, smem, known, &per_sm, "layer_norm_backward"));
+    const int grid = (int)std::min<int64_t>((f.rows + chunk - 1) / chunk,
+                                            std::min(f.max_grid, per_sm * sm_count()));
+    *f.used = grid;
+    norm_backward_staged_kernel<T, LPR, HELD8><<<grid, kThreads, smem, f.st>>>(
+        static_cast<const T*>(f.dy), static_cast<const T*>(f.x), f.codes, f.scales, f.weight, f.param_dtype,
+        f.mean, f.rstd, f.rows, f.channels, chunk, stage_width(f.dy, bytes),
+        HELD8 ? stage_width(f.codes, held) : stage_width(f.x, bytes), stage_width(f.dx, bytes),
+        static_cast<T*>(f.dx), f.partial);
+    return check_launch("layer_norm_backward");
+}
+
+// Where staging wins over single elements by row. Forward: up to 128 channels
+// (500000 x 77 fp32: 93 us against 135, 2000000 x 19: 135 against 324) and above
+// 512, where a team's row fills its registers (100000 x 1001 fp16: 150 us against
+// 356). The adjoint: above 512, where its sums for dw and db do (the same rows:
+// 247 us against 445; but 500000 x 77 fp32: 163 against 150).
+template <typename T>
+bool staged(const Forward& f, mg_status* s) {
+    if (f.channels > kStageMaxChannels || (f.channels > kBlock8 && f.channels <= 512)) return false;
+    *s = f.channels <= 32 ? forward_staged<T, 8>(f)
+         : f.channels <= kBlock8 ? forward_staged<T, 16>(f) : forward_staged<T, 32>(f);
+    return true;
+}
+template <typename T>
+bool staged(const Backward& f, mg_status* s) {
+    if (f.channels <= 512 || f.channels > kStageMaxChannels) return false;
+    *s = f.codes != nullptr ? backward_staged<T, 32, true>(f) : backward_staged<T, 32, false>(f);
+    return true;
+}
+
 // The team for a row length: the fewest lanes that hold the row with one
 // vector each, then more vectors per lane, then a block.
 template <typename T, int VEC, typename Op>
@@ -566,16 +827,19 @@ mg_status pick_team(const Op& op, int channels) {
     }
 }
 
+// Whole vectors, staged chunks, or single elements.
+template <typename T, int VEC, typename Op>
+mg_status pick_path(const Op& op, int channels, bool aligned) {
+    if (aligned && channels % VEC == 0) return pick_team<T, VEC>(op, channels);
+    mg_status s = MG_OK;
+    return staged<T>(op, &s) ? s : pick_team<T, 1>(op, channels);
+}
+
 template <typename Op>
 mg_status pick_type(const Op& op, int dtype, int channels, bool aligned) {
-    if (dtype == MG_F32)
-        return aligned && channels % 4 == 0 ? pick_team<float, 4>(op, channels)
-                                            : pick_team<float, 1>(op, channels);
-    if (dtype == MG_BF16)
-        return aligned && channels % 8 == 0 ? pick_team<__nv_bfloat16, 8>(op, channels)
-                                            : pick_team<__nv_bfloat16, 1>(op, channels);
-    return aligned && channels % 8 == 0 ? pick_team<__half, 8>(op, channels)
-                                        : pick_team<__half, 1>(op, channels);
+    if (dtype == MG_F32) return pick_path<float, 4>(op, channels, aligned);
+    if (dtype == MG_BF16) return pick_path<__nv_bfloat16, 8>(op, channels, aligned);
+    return pick_path<__half, 8>(op, channels, aligned);
 }
 
 bool known_dtype(int d) { return d == MG_F32 || d == MG_BF16 || d == MG_F16; }

@@ -203,28 +203,50 @@ __host__ __device__ inline int stage_rows(int channels, int elem_bytes) {
     return fit >= 16 ? fit / 16 * 16 : 8;
 }
 
-// `bytes` from global to shared memory by a whole block; src and dst 16-byte
-// aligned unless `aligned` is false. Ends with the copies committed as one
-// cp.async group (plain copies are done at the next barrier).
-__device__ __forceinline__ void stage_in(uint8_t* dst, const uint8_t* __restrict__ src, int bytes,
-                                         bool aligned) {
-    const int whole = aligned ? bytes / 16 * 16 : 0;
-    const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
-    for (int i = threadIdx.x * 16; i < whole; i += blockDim.x * 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d + i), "l"(src + i) : "memory");
-    for (int i = whole + threadIdx.x; i < bytes; i += blockDim.x) dst[i] = __ldg(src + i);
-    asm volatile("cp.async.commit_group;" ::: "memory");
+// The pieces (16, 8, 4 bytes or single ones) that a tensor's chunks of
+// chunk_bytes allow.
+inline int stage_width(const void* base, int64_t chunk_bytes) {
+    const uintptr_t all = reinterpret_cast<uintptr_t>(base) | (uintptr_t)chunk_bytes;
+    return all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : 1;
 }
+
+// `bytes` from global to 16-byte aligned shared memory by a whole block, in
+// pieces of `width` (asynchronous from 4 up). The caller commits the group.
+__device__ __forceinline__ void stage_in(uint8_t* dst, const uint8_t* __restrict__ src, int bytes,
+                                         int width) {
+    const int whole = width > 1 ? bytes / width * width : 0;
+    const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+    if (width == 16) {
+        for (int i = threadIdx.x * 16; i < whole; i += blockDim.x * 16)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d + i), "l"(src + i) : "memory");
+    } else if (width == 8) {
+        for (int i = threadIdx.x * 8; i < whole; i += blockDim.x * 8)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(d + i), "l"(src + i) : "memory");
+    } else if (width == 4) {
+        for (int i = threadIdx.x * 4; i < whole; i += blockDim.x * 4)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(d + i), "l"(src + i) : "memory");
+    }
+    for (int i = whole + threadIdx.x; i < bytes; i += blockDim.x) dst[i] = __ldg(src + i);
+}
+__device__ __forceinline__ void stage_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int PENDING>
 __device__ __forceinline__ void stage_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
 }
 
 __device__ __forceinline__ void stage_out(uint8_t* __restrict__ dst, const uint8_t* src, int bytes,
-                                          bool aligned) {
-    const int whole = aligned ? bytes / 16 * 16 : 0;
-    for (int i = threadIdx.x * 16; i < whole; i += blockDim.x * 16)
-        *reinterpret_cast<uint4*>(dst + i) = *reinterpret_cast<const uint4*>(src + i);
+                                          int width) {
+    const int whole = width > 1 ? bytes / width * width : 0;
+    if (width == 16) {
+        for (int i = threadIdx.x * 16; i < whole; i += blockDim.x * 16)
+            *reinterpret_cast<uint4*>(dst + i) = *reinterpret_cast<const uint4*>(src + i);
+    } else if (width == 8) {
+        for (int i = threadIdx.x * 8; i < whole; i += blockDim.x * 8)
+            *reinterpret_cast<uint2*>(dst + i) = *reinterpret_cast<const uint2*>(src + i);
+    } else if (width == 4) {
+        for (int i = threadIdx.x * 4; i < whole; i += blockDim.x * 4)
+            *reinterpret_cast<uint32_t*>(dst + i) = *reinterpret_cast<const uint32_t*>(src + i);
+    }
     for (int i = whole + threadIdx.x; i < bytes; i += blockDim.x) dst[i] = src[i];
 }
 
@@ -232,29 +254,59 @@ __host__ __device__ inline int align16(int bytes) { return (bytes + 15) & ~15; }
 
 inline int blocks8(int64_t channels) { return (int)((channels + kBlock8 - 1) / kBlock8); }
 
-// Codes and scales of a row in shared memory by a team of LPR lanes (32 for
-// rows over 128 channels): element j * LPR + lane is this lane's, and a scale's
-// 128 channels are 4 steps of 32 lanes or the whole row.
+// The 8-bit form of n staged rows by the whole block (kThreads of it, LPR lanes
+// to a row): maxima, then one thread for each block's two quotients, then codes.
+// work: n * blocks floats. Ends with a barrier.
 template <typename T, int LPR>
-__device__ __forceinline__ void row_to_codes(const T* row, int channels, int lane, bool live,
-                                             int8_t* codes, float* scales) {
-    for (int c0 = 0; c0 < channels; c0 += kBlock8) {
-        const int end = min(channels, c0 + kBlock8);
-        uint32_t a = 0u;
-        if (live)
-            for (int c = c0 + lane; c < end; c += LPR) a = max(a, mag8(to_f32<T>(row[c])));
-        a = lanes_max<LPR>(a);
-        const Scale8 s = scale8(a);
-        if (live) {
-            for (int c = c0 + lane; c < end; c += LPR) codes[c] = (int8_t)code8(to_f32<T>(row[c]), s.inv);
-            if (lane == 0) scales[c0 / kBlock8] = s.scale;
+__device__ __forceinline__ void staged_codes(const T* rows, int n, int channels, float* work,
+                                             int8_t* codes, float* __restrict__ scales) {
+    const int nb = (channels + kBlock8 - 1) / kBlock8, lane = threadIdx.x % LPR;
+    const int teams = blockDim.x / LPR, team = threadIdx.x / LPR;
+    for (int r0 = 0; r0 < n; r0 += teams) {
+        const int r = r0 + team;
+        for (int q = 0; q < nb; ++q) {
+            uint32_t a = 0u;
+            if (r < n)
+                for (int c = q * kBlock8 + lane; c < min(channels, (q + 1) * kBlock8); c += LPR)
+                    a = max(a, mag8(to_f32<T>(rows[r * channels + c])));
+            a = lanes_max<LPR>(a);
+            if (lane == 0 && r < n) work[r * nb + q] = __uint_as_float(a);
         }
     }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n * nb; i += blockDim.x) {
+        const Scale8 s = scale8(__float_as_uint(work[i]));
+        scales[i] = s.scale;
+        work[i] = s.inv;
+    }
+    __syncthreads();
+    for (int r = team; r < n; r += teams)
+        for (int c = lane; c < channels; c += LPR)
+            codes[r * channels + c] = (int8_t)code8(to_f32<T>(rows[r * channels + c]), work[r * nb + c / kBlock8]);
+    __syncthreads();
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0u; }
 
 // SMs of the current device (cached per device).
 int sm_count();
+
+// Readies a staged kernel for `smem` bytes of dynamic shared memory and gives
+// the blocks of one wave on an SM (by shared memory: 227 KB, 1 KB a block kept
+// back, and 2048 threads).
+constexpr int kStageMaxShared = 160 * 1024;
+template <typename K>
+mg_status staged_launch(K kernel, int threads, int smem, int (&known)[64], int* per_sm, const char* what) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+    if (known[dev] == 0) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kStageMaxShared) !=
+            cudaSuccess)
+            return check_launch(what);
+        known[dev] = 1;
+    }
+    *per_sm = std::max(1, std::min(2048 / threads, 227 * 1024 / (smem + 1024)));
+    return MG_OK;
+}
 
 }  // namespace mg
