@@ -287,6 +287,7 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
         const uint32_t idesc = mma_idesc(kStream, false, false);
         const uint32_t a_part = uniform(p.chunks * kOwnChunk / 16);
         const uint32_t b_part = uniform(p.chunks * kStreamChunk / 16);
+        const int steps = (int)uniform((uint32_t)(p.channels + 15) / 16);
         int stage = 0, ob = 0, g = 0;
         uint32_t phase = 0, ob_phase = 0, g_phase = 0;
         bool ok = true;
@@ -303,16 +304,27 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
                 const uint32_t d = uniform(tmem + g * kGroupColumns<PARTS>);
                 // the small products first: the tensor cores truncate the running
                 // sum at each step, and only the large ones' steps weigh
+                if (steps <= 4) {  // 16 channels each, of one chunk: no loop to run
 #pragma unroll
-                for (int q = 0; q < kScorePairs; ++q) {
-                    for (int c = 0; c < p.chunks; ++c) {
-                        const uint32_t a1 = a0 + pair_a<PARTS>(kScorePairs, q) * a_part + c * (kOwnChunk / 16);
-                        const uint32_t b1 = b0 + pair_b<PARTS>(kScorePairs, q) * b_part + c * (kStreamChunk / 16);
+                    for (int q = 0; q < kScorePairs; ++q) {
 #pragma unroll
-                        for (int s = 0; s < 4; ++s)
-                            if (64 * c + 16 * s < p.channels)
-                                mma_bf16<k_major_hi(128), k_major_hi(128)>(d, a1 + 2 * s, b1 + 2 * s, idesc,
-                                                                           q > 0 || s > 0 ? true : c > 0, on);
+                        for (int k = 0; k < 4; ++k)
+                            if (k < steps)
+                                mma_bf16<k_major_hi(128), k_major_hi(128)>(
+                                    d, a0 + pair_a<PARTS>(kScorePairs, q) * a_part + 2 * k,
+                                    b0 + pair_b<PARTS>(kScorePairs, q) * b_part + 2 * k, idesc,
+                                    q > 0 || k > 0, on);
+                    }
+                } else {
+#pragma unroll
+                    for (int q = 0; q < kScorePairs; ++q) {
+                        uint32_t a = uniform(a0 + pair_a<PARTS>(kScorePairs, q) * a_part);
+                        uint32_t b = uniform(b0 + pair_b<PARTS>(kScorePairs, q) * b_part);
+                        for (int k = 0; k < steps; ++k) {
+                            mma_bf16<k_major_hi(128), k_major_hi(128)>(d, a, b, idesc, q > 0 ? true : k > 0, on);
+                            a += (k & 3) == 3 ? kOwnChunk / 16 - 6 : 2;
+                            b += (k & 3) == 3 ? kStreamChunk / 16 - 6 : 2;
+                        }
                     }
                 }
                 mma_commit(s_full + 8 * g, on);
