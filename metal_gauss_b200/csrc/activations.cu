@@ -271,7 +271,7 @@ mg_status check_sizes(int32_t dtype, int64_t rows, int64_t channels, const int8_
 using namespace mg;
 
 extern "C" mg_status mg_pack8(const void* x, int32_t dtype, int64_t rows, int64_t channels,
-                              int8_t* codes, float* scales, mg_stream_t stream) {
+                              int8_t* codes, float* scales, mg_stream_t stream) try {
     MG_TRY(check_sizes(dtype, rows, channels, codes, "pack8"));
     if (rows == 0) return MG_OK;
     MG_REQUIRE(x && codes && scales, "pack8: null pointer");
@@ -279,10 +279,12 @@ extern "C" mg_status mg_pack8(const void* x, int32_t dtype, int64_t rows, int64_
     if (dtype == MG_F32) return pack<float, 4>(op);
     if (dtype == MG_BF16) return pack<__nv_bfloat16, 8>(op);
     return pack<__half, 8>(op);
+} catch (...) {
+    return caught("pack8");
 }
 
 extern "C" mg_status mg_unpack8(const int8_t* codes, const float* scales, int64_t rows,
-                                int64_t channels, int32_t dtype, void* x, mg_stream_t stream) {
+                                int64_t channels, int32_t dtype, void* x, mg_stream_t stream) try {
     MG_TRY(check_sizes(dtype, rows, channels, codes, "unpack8"));
     if (rows == 0) return MG_OK;
     MG_REQUIRE(x && codes && scales, "unpack8: null pointer");
@@ -290,4 +292,6 @@ extern "C" mg_status mg_unpack8(const int8_t* codes, const float* scales, int64_
     if (dtype == MG_F32) return unpack(codes, scales, rows, (int)channels, static_cast<float*>(x), st);
     if (dtype == MG_BF16) return unpack(codes, scales, rows, (int)channels, static_cast<__nv_bfloat16*>(x), st);
     return unpack(codes, scales, rows, (int)channels, static_cast<__half*>(x), st);
+} catch (...) {
+    return caught("unpack8");
 }

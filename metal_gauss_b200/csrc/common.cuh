@@ -25,6 +25,16 @@ inline mg_status fail(mg_status s, const std::string& msg) {
     return s;
 }
 
+// For a C entry point's catch: nothing is thrown across it (the message's own
+// allocation is the one thing that can fail on the host side).
+inline mg_status caught(const char* who) noexcept {
+    try {
+        set_error(std::string(who) + ": an exception on the host (out of memory)");
+    } catch (...) {
+    }
+    return MG_ERR_CUDA;
+}
+
 #define MG_REQUIRE(cond, msg)                                          \
     do {                                                               \
         if (!(cond)) return ::mg::fail(MG_ERR_INVALID_ARGUMENT, (msg)); \

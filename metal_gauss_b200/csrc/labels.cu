@@ -731,7 +731,7 @@ extern "C" mg_status mg_label_loss_forward(const void* features, const void* cla
                                            int64_t channels, int64_t n_classes, float scale,
                                            int32_t reduction, float* loss, float* stats,
                                            float* live, void* scratch, size_t scratch_bytes,
-                                           mg_stream_t stream) {
+                                           mg_stream_t stream) try {
     MG_TRY(check_args("label_loss_forward", features, classes, dtype, labels, label_bytes, rows,
                       channels, n_classes, reduction));
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
@@ -754,6 +754,8 @@ extern "C" mg_status mg_label_loss_forward(const void* features, const void* cla
     if (dtype == MG_F32) return forward<float>(a, reduction, loss, stats, live, scratch);
     if (dtype == MG_BF16) return forward<__nv_bfloat16>(a, reduction, loss, stats, live, scratch);
     return forward<__half>(a, reduction, loss, stats, live, scratch);
+} catch (...) {
+    return caught("label_loss_forward");
 }
 
 extern "C" mg_status mg_label_loss_backward(
@@ -761,7 +763,7 @@ extern "C" mg_status mg_label_loss_backward(
     const void* labels, int32_t label_bytes, int64_t ignore_index, int64_t rows, int64_t channels,
     int64_t n_classes, float scale, int32_t reduction, const float* grad_loss, const float* stats,
     const float* live, void* d_features, void* d_classes, float* d_bias, void* scratch,
-    size_t scratch_bytes, mg_stream_t stream) {
+    size_t scratch_bytes, mg_stream_t stream) try {
     MG_TRY(check_args("label_loss_backward", features, classes, dtype, labels, label_bytes, rows,
                       channels, n_classes, reduction));
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
@@ -792,4 +794,6 @@ extern "C" mg_status mg_label_loss_backward(
         return backward(a, rg, stats, static_cast<__nv_bfloat16*>(d_features),
                         static_cast<__nv_bfloat16*>(d_classes), d_bias, scratch);
     return backward(a, rg, stats, static_cast<__half*>(d_features), static_cast<__half*>(d_classes), d_bias, scratch);
+} catch (...) {
+    return caught("label_loss_backward");
 }

@@ -867,7 +867,7 @@ extern "C" mg_status mg_layer_norm_forward(const void* x, int32_t dtype, const v
                                            const void* bias, int32_t param_dtype, int64_t rows,
                                            int64_t channels, float eps, void* y, float* mean,
                                            float* rstd, int8_t* codes, float* scales,
-                                           mg_stream_t stream) {
+                                           mg_stream_t stream) try {
     MG_REQUIRE(known_dtype(dtype) && known_dtype(param_dtype), "layer_norm_forward: unknown dtype");
     MG_REQUIRE(rows >= 0, "layer_norm_forward: negative row count");
     MG_REQUIRE(channels >= 1 && channels <= MG_LAYER_NORM_MAX_CHANNELS,
@@ -882,6 +882,8 @@ extern "C" mg_status mg_layer_norm_forward(const void* x, int32_t dtype, const v
     const Forward op{x, weight, bias, param_dtype, rows, (int)channels, eps, y, mean, rstd,
                      codes, scales, reinterpret_cast<cudaStream_t>(stream)};
     return pick_type(op, dtype, (int)channels, aligned16(x) && aligned16(y));
+} catch (...) {
+    return caught("layer_norm_forward");
 }
 
 extern "C" size_t mg_layer_norm_backward_scratch_bytes(int64_t rows, int64_t channels) {
@@ -894,7 +896,7 @@ extern "C" mg_status mg_layer_norm_backward(const void* dy, const void* x, const
                                             int32_t param_dtype, const float* mean,
                                             const float* rstd, int64_t rows, int64_t channels,
                                             void* dx, void* dweight, void* dbias, void* scratch,
-                                            size_t scratch_bytes, mg_stream_t stream) {
+                                            size_t scratch_bytes, mg_stream_t stream) try {
     MG_REQUIRE(known_dtype(dtype) && known_dtype(param_dtype), "layer_norm_backward: unknown dtype");
     MG_REQUIRE(rows >= 0, "layer_norm_backward: negative row count");
     MG_REQUIRE(channels >= 1 && channels <= MG_LAYER_NORM_MAX_CHANNELS,
@@ -929,4 +931,6 @@ extern "C" mg_status mg_layer_norm_backward(const void* dy, const void* x, const
     norm_join_kernel<<<ceil_div(2 * channels, 32), dim3(32, 32), 0, st>>>(
         static_cast<const float*>(scratch), grid, (int)channels, param_dtype, dweight, dbias);
     return check_launch("layer_norm_backward join");
+} catch (...) {
+    return caught("layer_norm_backward");
 }

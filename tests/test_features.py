@@ -100,6 +100,14 @@ def test_layer_norm(cuda, n, d, dtype, saved):
         within(got, ref, t + half(dtype) * (ref.abs() + t) + 2.0 ** -25 * (dtype == F16), what)
 
 
+@pytest.mark.parametrize("saved", ["full", "int8"])
+@pytest.mark.parametrize("n,d,dtype", [(200_001, 19, F32), (60_000, 77, BF16), (30_001, 601, F16),
+                                       (100_003, 64, F32), (20_000, 1000, BF16), (12_000, 1025, F32)])
+def test_layer_norm_of_many_rows(cuda, n, d, dtype, saved):
+    """Blocks that take several chunks or rounds of rows each."""
+    test_layer_norm(cuda, n, d, dtype, saved)
+
+
 @pytest.mark.parametrize("dtype,wdtype", [(BF16, F32), (F16, F32), (F32, F32)])
 def test_layer_norm_parameter_types_and_absent_parameters(cuda, dtype, wdtype):
     g = gen(3)
@@ -231,6 +239,12 @@ def test_pack8_equals_its_definition(cuda, n, d, dtype):
     off = (unpack8(codes, scales).double() - x.double()).abs().cpu()
     step = s.double().repeat_interleave(128, 1)[:, :d]
     assert (off <= step * (0.5 + 256 * U)).all()
+
+
+@pytest.mark.parametrize("n,d,dtype", [(300_000, 19, F32), (40_000, 200, BF16), (20_000, 333, F32),
+                                       (200_000, 64, F16)])
+def test_pack8_of_many_rows(cuda, n, d, dtype):
+    test_pack8_equals_its_definition(cuda, n, d, dtype)
 
 
 def test_pack8_ties_non_finite_tiny_and_views(cuda):
@@ -389,6 +403,36 @@ LABELS = [(1, 1, 1), (1, 3, 2), (2, 16, 5), (63, 8, 64), (64, 16, 65), (65, 17, 
 def test_label_loss(cuda, n, d, v, dtype):
     x, w, lab, bias, _ = label_case(n + 7 * d + 31 * v, n, d, v, dtype)
     check_label(x, w, lab, bias)
+
+
+@pytest.mark.parametrize("n,d,v,dtype", [
+    (40_000, 16, 200, F32),      # classes that stay in shared memory, several row tiles to a block
+    (40_000, 100, 129, F32),     # the same with two chunks of channels
+    (20_000, 24, 4_300, BF16),   # more than one visit of the accumulator to memory
+    (25_000, 140, 300, F32),     # wide features: the logits' gradient through scratch
+    (5_000, 300, 16_500, BF16),  # in more than one piece
+    (2_500, 200, 20_000, F16),
+    (300, 300, 40_000, F32),     # few rows: the classes in shares
+    (50_000, 128, 2_000, F32),   # two streamed tiles are all that fits
+])
+def test_label_loss_of_many(cuda, n, d, v, dtype):
+    x, w, lab, bias, _ = label_case(n + d + v, n, d, v, dtype)
+    check_label(x, w, lab, bias)
+
+
+def test_label_loss_off_the_boundaries(cuda):
+    """Contiguous tensors that start 2 or 4 bytes off a 16-byte boundary."""
+    for dtype in (F32, BF16):
+        x, w, lab, bias, g = label_case(22, 90, 32, 50, dtype)
+
+        def off(t):
+            flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=cuda)
+            flat[1:] = t.flatten()
+            return flat[1:].view(t.shape)
+
+        a, ga = check_label(x, w, lab, bias)
+        b, gb = check_label(off(x), off(w), off(lab), off(bias))
+        assert torch.equal(a, b) and all(torch.equal(p, q) for p, q in zip(ga, gb))
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
@@ -577,6 +621,51 @@ def test_label_gradient_against_differences(cuda):
     size = sum(float((q.double().abs() * v.abs()).sum()) for q, v in zip(grads, dirs))
     # third derivatives of order |direction|^3 ~ 10^3 times step^2 = 10^-10; fp32 work
     assert abs(got - slope) <= 1e-6 + 200 * U * size
+
+
+@pytest.mark.parametrize("d", [1030, 1032])
+def test_more_than_2_to_the_32_elements(cuda, d):
+    """Offsets past 32 bits: the last rows of a 8.6 GB map come out as they do
+    alone."""
+    n = 2 ** 32 // d + 3
+    x = torch.zeros(n, d, dtype=BF16, device=cuda)
+    tail = torch.randn(4, d, generator=gen(40), device=cuda).to(BF16)
+    x[-4:] = tail
+    codes, scales = pack8(x)
+    one = pack8(tail)
+    assert torch.equal(codes[-4:], one[0]) and torch.equal(scales[-4:], one[1])
+    back = unpack8(codes, scales, dtype=BF16)
+    assert torch.equal(back[-4:], unpack8(*one, dtype=BF16)) and not back[-8:-4].any()
+    del codes, scales, back
+    x.requires_grad_(True)
+    w = torch.randn(d, generator=gen(41), device=cuda).to(BF16).requires_grad_(True)
+    y = layer_norm(x, w, saved="int8")
+    dy = torch.zeros_like(x)
+    dy[-4:] = tail.flip(0)
+    gx, gw = torch.autograd.grad(y, (x, w), dy)
+    tl = tail.clone().requires_grad_(True)
+    want = layer_norm(tl, w, saved="int8")
+    wx, ww = torch.autograd.grad(want, (tl, w), tail.flip(0))
+    assert torch.equal(y[-4:], want) and torch.equal(gx[-4:], wx)
+    # the same four rows summed in another order
+    assert float((gw - ww).abs().max()) <= 2 * half(BF16) * float(ww.abs().max())
+
+
+def test_label_loss_past_2_to_the_32_elements(cuda):
+    n, d = 2 ** 26 + 200, 64
+    x = torch.zeros(n, d, dtype=BF16, device=cuda)
+    xt, w, lab_t, _, _ = label_case(42, 150, d, 20, BF16)
+    x[-150:] = xt
+    lab = torch.full((n,), 255, dtype=torch.uint8, device=cuda)
+    lab[-150:] = torch.where(lab_t == -100, 255, lab_t).to(torch.uint8)
+    x.requires_grad_(True)
+    loss = label_loss(x, w, lab, ignore_index=255, reduction="none")
+    (gx,) = torch.autograd.grad(loss, x, torch.ones_like(loss))
+    tl = xt.clone().requires_grad_(True)
+    want = label_loss(tl, w, lab[-150:], ignore_index=255, reduction="none")
+    (wx,) = torch.autograd.grad(want, tl, torch.ones_like(want))
+    assert torch.equal(loss[-150:], want) and not loss[:-150].any()
+    assert torch.equal(gx[-150:], wx) and not gx[-1000:-150].any()
 
 
 def test_second_derivatives_are_refused(cuda):
