@@ -35,8 +35,9 @@ constexpr int kStream = 64;
 constexpr int kGroups = 4;          // of four warps that turn scores into G
 // copy, issue scores, issue G products, (none); the groups; 8 warps for acc
 constexpr int kFusedThreads = 128 * (1 + kGroups + 2);
-// Registers a thread: 72 at launch; the first four warps give up 32 and the
-// groups 8 each for the acc warps' 32 more: 40 + 4 * 64 + 2 * 104 = 7 * 72.
+// Registers a thread: 72 at launch, and the issuing warps keep them; the groups
+// give up 8 each for the acc warps' 16 more: 72 + 4 * 64 + 2 * 88 = 7 * 72. (Other
+// splits, 40 to 120 for the issuing warps, measured level or worse.)
 constexpr int kIssueRegs = 72, kScoreRegs = 64, kAccRegs = 88;
 constexpr int kFusedStages = 8;     // at most
 constexpr int kFusedShared = 226 * 1024;  // of it 1 KB to align
@@ -147,10 +148,10 @@ __device__ __forceinline__ void store_parts(uint32_t group, int k, float (&z)[kS
 
 // Four sums of products to r softmax: logits in base 2 (scale, bias), minus the
 // log of the row's sum, exponential, times r.
-__device__ __forceinline__ void gradients(float* z, float c2, float2 bias0, float2 bias1, float2 lse0,
-                                          float2 lse1, float2 r0, float2 r1) {
-    const float2 a = add2(fma2(make_float2(z[0], z[1]), both(c2), bias0), lse0);
-    const float2 b = add2(fma2(make_float2(z[2], z[3]), both(c2), bias1), lse1);
+__device__ __forceinline__ void gradients(float* z, float c2, float2 bias0, float2 bias1, float2 minus_lse0,
+                                          float2 minus_lse1, float2 r0, float2 r1) {
+    const float2 a = add2(fma2(make_float2(z[0], z[1]), both(c2), bias0), minus_lse0);
+    const float2 b = add2(fma2(make_float2(z[2], z[3]), both(c2), bias1), minus_lse1);
     const float2 e = mul2(make_float2(exp2_fast(a.x), exp2_fast(a.y)), r0);
     const float2 f = mul2(make_float2(exp2_fast(b.x), exp2_fast(b.y)), r1);
     z[0] = e.x;
@@ -222,9 +223,8 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
         return mbar_wait_warp(bar, parity, &stop, p.error_word, DEV_ERR_TILE_WAIT);
     };
 
-    if (warp < 4) registers_down<kIssueRegs>();
-    else if (warp < 4 + 4 * kGroups) registers_down<kScoreRegs>();
-    else registers_up<kAccRegs>();
+    if (warp >= 4 + 4 * kGroups) registers_up<kAccRegs>();
+    else if (warp >= 4) registers_down<kScoreRegs>();
 
     if (warp == 0) {
         {  // copies tiles in
@@ -417,13 +417,13 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
             const FusedWalk w = fused_unit(p, u);
             const int own = w.own0 + in_tile;
             int lab = kIgnored;
-            float lse = kInf, r = 0.0f, at_label = 0.0f, own_bias = 0.0f, bias_sum = 0.0f;
+            float minus_lse = -kInf, r = 0.0f, at_label = 0.0f, own_bias = 0.0f, bias_sum = 0.0f;
             if (own < p.own) {
                 if constexpr (BY_CLASS) {
                     own_bias = p.class_bias[own];
                 } else {
                     const float* v = p.row_values + (int64_t)(own / kStream) * (kRowValues * kStream) + own % kStream;
-                    lse = v[0];
+                    minus_lse = v[0];
                     r = v[kStream];
                     at_label = v[2 * kStream];
                     lab = __float_as_int(v[3 * kStream]);
@@ -457,8 +457,8 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
                         for (int j = 0; j < kStep; j += 4) {
                             const float4 a = shared_float4(col + 4 * (k + j));
                             const float4 b = shared_float4(col + 4 * (kStream + k + j));
-                            gradients(z + j, c2, both(own_bias), both(own_bias), make_float2(-a.x, -a.y),
-                                      make_float2(-a.z, -a.w), make_float2(b.x, b.y), make_float2(b.z, b.w));
+                            gradients(z + j, c2, both(own_bias), both(own_bias), make_float2(a.x, a.y),
+                                      make_float2(a.z, a.w), make_float2(b.x, b.y), make_float2(b.z, b.w));
                         }
                         // rows labelled with one of this warp's classes
                         const int mine = shared_int(col + 4 * (3 * kStream + k + (lane & (kStep - 1)))) - w.own0 - quarter * 32;
@@ -478,7 +478,7 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
 #pragma unroll
                         for (int j = 0; j < kStep; j += 4) {
                             const float4 b = shared_float4(col + 4 * (k + j));
-                            gradients(z + j, c2, make_float2(b.x, b.y), make_float2(b.z, b.w), both(-lse), both(-lse),
+                            gradients(z + j, c2, make_float2(b.x, b.y), make_float2(b.z, b.w), both(minus_lse), both(minus_lse),
                                       both(r), both(r));
                         }
                         const int rel = lab - t * kStream - k;
@@ -560,6 +560,7 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
                         if (c < n) {
 #pragma unroll
                             for (int h = 0; h < 32; h += 16) {  // 16 at a time, for the registers' sake
+                                if (c + h >= n) break;
                                 float v[16];
                                 tmem_load(lanes + ab * n + c + h, v);
 #pragma unroll

@@ -120,7 +120,7 @@ __device__ __forceinline__ Walk walk_unit(const TileArgs& p, int u) {
 // What a row's scores need.
 struct RowIn {
     int lab = kIgnored;
-    float lse = kInf, r = 0.0f, at_label = 0.0f;
+    float minus_lse = -kInf, r = 0.0f, at_label = 0.0f;
 };
 
 template <int MODE>
@@ -132,7 +132,7 @@ __device__ __forceinline__ RowIn row_in(const TileArgs& p, int a_row) {
         in.lab = p.row_labels[row];
     } else {
         const float* v = p.row_values + row / kRowBlock * (kRowValues * kRowBlock) + row % kRowBlock;
-        in.lse = v[0];
+        in.minus_lse = v[0];
         in.r = v[kRowBlock];
         in.at_label = v[2 * kRowBlock];
         in.lab = __float_as_int(v[3 * kRowBlock]);
@@ -367,7 +367,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
             if constexpr (!S::kProduct) {
                 const int64_t row = p.row0 + a_row;
                 const int lab = next_row.lab;
-                const float lse = next_row.lse, r = next_row.r, at_label = next_row.at_label;
+                const float minus_lse = next_row.minus_lse, r = next_row.r, at_label = next_row.at_label;
                 float m = -kInf, s = 0.0f;
                 for (int t = 0; t < w.tiles; ++t) {
                     const int v0 = (w.first + t) * kN;
@@ -433,7 +433,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                                 scores<16>(z, c2, p.class_bias + v0 + k * 32 + h);
 #pragma unroll
                                 for (int j = 0; j < 16; j += 2) {
-                                    const float2 d = add2(make_float2(z[j], z[j + 1]), both(-lse));
+                                    const float2 d = add2(make_float2(z[j], z[j + 1]), both(minus_lse));
                                     const float2 e = mul2(make_float2(exp2_fast(d.x), exp2_fast(d.y)), both(r));
                                     z[j] = e.x;
                                     z[j + 1] = e.y;

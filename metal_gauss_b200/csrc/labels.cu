@@ -68,11 +68,11 @@ split_kernel(const T* __restrict__ x, const T* __restrict__ w, LabelSource label
     const int c = (int)(i - all * groups) * 8;
     if (cv.row_labels != nullptr && i < rows) cv.row_labels[i] = labels.at(i);
     if (cv.row_values != nullptr && i < (rows + kRowBlock - 1) / kRowBlock * kRowBlock) {
-        float v[kRowValues] = {kInf, 0.0f, 0.0f, __int_as_float(kIgnored)};
+        float v[kRowValues] = {-kInf, 0.0f, 0.0f, __int_as_float(kIgnored)};
         if (i < rows) {
             const int lab = labels.at(i);
             if (lab >= 0) {
-                v[0] = cv.stats[i];
+                v[0] = -cv.stats[i];
                 v[1] = cv.rg.at(i, lab);
                 v[2] = -cv.stats[rows + i] * v[1];
                 v[3] = __int_as_float(lab);

@@ -41,8 +41,8 @@ struct RowGrad {
     }
 };
 
-// What the backward pass's scores need of a row: log2 of its sum, r, G at its
-// label, its label (an int), each kRowBlock in a row per block of rows.
+// What the backward pass's scores need of a row: minus log2 of its sum, r, G at
+// its label, its label (an int), each kRowBlock in a row per block of rows.
 constexpr int kRowValues = 4;
 constexpr int kRowBlock = 64;
 constexpr int kClassPad = 256;  // class_bias is padded to a multiple of this
@@ -117,7 +117,8 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 // One part of (lo, hi) as a word; lo and hi keep what it leaves over.
 __device__ __forceinline__ uint32_t take_part(float& lo, float& hi) {
     const uint32_t w = pack_bf16(lo, hi);
-    const float2 rest = add2(make_float2(lo, hi), make_float2(-__uint_as_float(w << 16), -__uint_as_float(w & 0xffff0000u)));
+    const float2 rest = fma2(make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)), both(-1.0f),
+                             make_float2(lo, hi));
     lo = rest.x;
     hi = rest.y;
     return w;
