@@ -227,62 +227,61 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
     else if (warp >= 4) registers_down<kScoreRegs>();
 
     if (warp == 0) {
-        {  // copies tiles in
-            const uint32_t on = elect_lane();
-            int stage = 0, ob = 0;
-            uint32_t phase = 0, ob_phase = 0;
-            int issued = 0, owns = 0;  // of the last ring, for a stop
-            bool ok = true;
-            for (int u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
-                const FusedWalk w = fused_unit(p, u);
-                ok = wait_warp(own_empty + 8 * ob, ob_phase ^ 1);
+        // copies tiles in
+        const uint32_t on = elect_lane();
+        int stage = 0, ob = 0;
+        uint32_t phase = 0, ob_phase = 0;
+        int issued = 0, owns = 0;  // of the last ring, for a stop
+        bool ok = true;
+        for (int u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
+            const FusedWalk w = fused_unit(p, u);
+            ok = wait_warp(own_empty + 8 * ob, ob_phase ^ 1);
+            if (!ok) break;
+            mbar_expect(own_full + 8 * ob, own_bytes, on);
+            for (int i = 0; i < PARTS; ++i)
+                for (int c = 0; c < p.chunks; ++c)
+                    tma_load(base + ob * own_bytes + (i * p.chunks + c) * kOwnChunk, &map_own,
+                             c * 64, w.own0, i, own_full + 8 * ob, on);
+            owns = min(owns + 1, p.own_buffers);
+            if (++ob == p.own_buffers) {
+                ob = 0;
+                ob_phase ^= 1;
+            }
+            if (p.resident && u != (int)blockIdx.x) continue;
+            for (int t = w.t0; t < w.t1; ++t) {
+                ok = wait_warp(empty + 8 * stage, phase ^ 1);
                 if (!ok) break;
-                mbar_expect(own_full + 8 * ob, own_bytes, on);
+                mbar_expect(full + 8 * stage, tile_bytes + column_bytes, on);
+                bulk_load(stream0 + stage * stage_bytes + tile_bytes,
+                          (BY_CLASS ? p.row_values : p.class_bias) + (int64_t)t * (column_bytes / 4), column_bytes,
+                          full + 8 * stage, on);
                 for (int i = 0; i < PARTS; ++i)
                     for (int c = 0; c < p.chunks; ++c)
-                        tma_load(base + ob * own_bytes + (i * p.chunks + c) * kOwnChunk, &map_own,
-                                 c * 64, w.own0, i, own_full + 8 * ob, on);
-                owns = min(owns + 1, p.own_buffers);
-                if (++ob == p.own_buffers) {
-                    ob = 0;
-                    ob_phase ^= 1;
-                }
-                if (p.resident && u != (int)blockIdx.x) continue;
-                for (int t = w.t0; t < w.t1; ++t) {
-                    ok = wait_warp(empty + 8 * stage, phase ^ 1);
-                    if (!ok) break;
-                    mbar_expect(full + 8 * stage, tile_bytes + column_bytes, on);
-                    bulk_load(stream0 + stage * stage_bytes + tile_bytes,
-                              (BY_CLASS ? p.row_values : p.class_bias) + (int64_t)t * (column_bytes / 4), column_bytes,
-                              full + 8 * stage, on);
-                    for (int i = 0; i < PARTS; ++i)
-                        for (int c = 0; c < p.chunks; ++c)
-                            tma_load(stream0 + stage * stage_bytes + (i * p.chunks + c) * kStreamChunk,
-                                     &map_stream, c * 64, t * kStream, i, full + 8 * stage, on);
-                    issued = min(issued + 1, p.stages);
-                    if (++stage == p.stages) {
-                        stage = 0;
-                        phase ^= 1;
-                    }
+                        tma_load(stream0 + stage * stage_bytes + (i * p.chunks + c) * kStreamChunk,
+                                 &map_stream, c * 64, t * kStream, i, full + 8 * stage, on);
+                issued = min(issued + 1, p.stages);
+                if (++stage == p.stages) {
+                    stage = 0;
+                    phase ^= 1;
                 }
             }
-            if (stop) {  // this block gave up: its copies in flight land before it ends
-                for (int j = issued; j > 0; --j) {
-                    if (--stage < 0) {
-                        stage = p.stages - 1;
-                        phase ^= 1;
-                    }
-                    for (int i = 0; i < kMbarRounds; ++i)
-                        if (mbar_try(full + 8 * stage, phase)) break;
+        }
+        if (stop) {  // this block gave up: its copies in flight land before it ends
+            for (int j = issued; j > 0; --j) {
+                if (--stage < 0) {
+                    stage = p.stages - 1;
+                    phase ^= 1;
                 }
-                for (int j = owns; j > 0; --j) {
-                    if (--ob < 0) {
-                        ob = p.own_buffers - 1;
-                        ob_phase ^= 1;
-                    }
-                    for (int i = 0; i < kMbarRounds; ++i)
-                        if (mbar_try(own_full + 8 * ob, ob_phase)) break;
+                for (int i = 0; i < kMbarRounds; ++i)
+                    if (mbar_try(full + 8 * stage, phase)) break;
+            }
+            for (int j = owns; j > 0; --j) {
+                if (--ob < 0) {
+                    ob = p.own_buffers - 1;
+                    ob_phase ^= 1;
                 }
+                for (int i = 0; i < kMbarRounds; ++i)
+                    if (mbar_try(own_full + 8 * ob, ob_phase)) break;
             }
         }
     } else if (warp == 1) {

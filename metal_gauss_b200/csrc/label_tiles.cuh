@@ -200,150 +200,148 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
     constexpr uint32_t tmem = kTmemBase;
 
     if (warp == 0) {
-        {  // copies tiles in
-            const uint32_t on = elect_lane();
-            int stage = 0;
-            uint32_t phase = 0;
-            int issued = 0;
-            bool ok = true;
-            if (MODE == kStats && resident > 0) {
-                const int chunks = (int)((p.depth + S::kChunk - 1) / S::kChunk);
-                mbar_expect(resident_full, resident * PARTS * S::kB, on);
-                for (int c = 0; c < resident; ++c)
-                    for (int i = 0; i < PARTS; ++i)
-                        tma_load(base + (c * PARTS + i) * S::kB, &map_b, c % chunks * S::kChunk, c / chunks * kN, i,
-                                 resident_full, on);
-            }
-            for (int u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
-                const Walk w = walk_unit<MODE, PARTS>(p, u);
-                for (int t = 0; ok && t < w.tiles; ++t) {
-                    const int b0 = (S::kProduct ? w.first : w.first + t) * kN;
-                    const int c0 = S::kProduct ? w.c0 + t * p.per_segment : w.c0;
-                    const int c1 = S::kProduct ? min(w.c1, c0 + p.per_segment) : w.c1;
-                    const int blocks = S::kProduct ? (min(kN, p.columns - b0) + 63) / 64 : 0;
-                    const uint32_t bytes =
-                        S::kPartsA * S::kA +
-                        (resident > 0 ? 0 : PARTS * (S::kProduct ? blocks * S::kChunk * 128 : S::kB));
-                    const int passes = S::kTwice && c1 - c0 > 1 ? 2 : 1;
-                    for (int i = 0; i < passes * (c1 - c0); ++i) {
-                        const bool again = i >= c1 - c0;  // the first part alone
-                        const int c = again ? i - (c1 - c0) + c0 : i + c0;
-                        ok = mbar_wait_warp(empty + 8 * stage, phase ^ 1, &stop, p.error_word, DEV_ERR_TILE_WAIT);
-                        if (!ok) break;
-                        const uint32_t bar = full + 8 * stage;
-                        mbar_expect(bar, again ? S::kA + (resident > 0 ? 0 : S::kB) : bytes, on);
-                        const int k = c * S::kChunk;
-                        const uint32_t a = ring + stage * stage_bytes, b = a + S::kPartsA * S::kA;
+        // copies tiles in
+        const uint32_t on = elect_lane();
+        int stage = 0;
+        uint32_t phase = 0;
+        int issued = 0;
+        bool ok = true;
+        if (MODE == kStats && resident > 0) {
+            const int chunks = (int)((p.depth + S::kChunk - 1) / S::kChunk);
+            mbar_expect(resident_full, resident * PARTS * S::kB, on);
+            for (int c = 0; c < resident; ++c)
+                for (int i = 0; i < PARTS; ++i)
+                    tma_load(base + (c * PARTS + i) * S::kB, &map_b, c % chunks * S::kChunk, c / chunks * kN, i,
+                             resident_full, on);
+        }
+        for (int u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
+            const Walk w = walk_unit<MODE, PARTS>(p, u);
+            for (int t = 0; ok && t < w.tiles; ++t) {
+                const int b0 = (S::kProduct ? w.first : w.first + t) * kN;
+                const int c0 = S::kProduct ? w.c0 + t * p.per_segment : w.c0;
+                const int c1 = S::kProduct ? min(w.c1, c0 + p.per_segment) : w.c1;
+                const int blocks = S::kProduct ? (min(kN, p.columns - b0) + 63) / 64 : 0;
+                const uint32_t bytes =
+                    S::kPartsA * S::kA +
+                    (resident > 0 ? 0 : PARTS * (S::kProduct ? blocks * S::kChunk * 128 : S::kB));
+                const int passes = S::kTwice && c1 - c0 > 1 ? 2 : 1;
+                for (int i = 0; i < passes * (c1 - c0); ++i) {
+                    const bool again = i >= c1 - c0;  // the first part alone
+                    const int c = again ? i - (c1 - c0) + c0 : i + c0;
+                    ok = mbar_wait_warp(empty + 8 * stage, phase ^ 1, &stop, p.error_word, DEV_ERR_TILE_WAIT);
+                    if (!ok) break;
+                    const uint32_t bar = full + 8 * stage;
+                    mbar_expect(bar, again ? S::kA + (resident > 0 ? 0 : S::kB) : bytes, on);
+                    const int k = c * S::kChunk;
+                    const uint32_t a = ring + stage * stage_bytes, b = a + S::kPartsA * S::kA;
 #pragma unroll
-                        for (int j = 0; j < S::kPartsA; ++j) {
-                            if (again && j > 0) break;
-                            if (S::kAmn) {
-                                for (int q = 0; q < 2; ++q)
-                                    tma_load(a + j * S::kA + q * S::kChunk * 128, &map_a, w.a_row + 64 * q, k, j, bar, on);
-                            } else {
-                                tma_load(a + j * S::kA, &map_a, k, w.a_row, j, bar, on);
-                            }
-                        }
-#pragma unroll
-                        for (int j = 0; j < PARTS; ++j) {
-                            if (resident > 0 || (again && j > 0)) break;
-                            if (S::kBmn) {
-                                for (int q = 0; q < blocks; ++q)
-                                    tma_load(b + j * S::kB + q * S::kChunk * 128, &map_b, b0 + 64 * q, k, j, bar, on);
-                            } else {
-                                tma_load(b + j * S::kB, &map_b, k, b0, j, bar, on);
-                            }
-                        }
-                        issued = min(issued + 1, stages);
-                        if (++stage == stages) {
-                            stage = 0;
-                            phase ^= 1;
+                    for (int j = 0; j < S::kPartsA; ++j) {
+                        if (again && j > 0) break;
+                        if (S::kAmn) {
+                            for (int q = 0; q < 2; ++q)
+                                tma_load(a + j * S::kA + q * S::kChunk * 128, &map_a, w.a_row + 64 * q, k, j, bar, on);
+                        } else {
+                            tma_load(a + j * S::kA, &map_a, k, w.a_row, j, bar, on);
                         }
                     }
-                }
-            }
-            if (stop) {  // this block gave up: its copies in flight land before it ends
-                if (MODE == kStats && resident > 0)
-                    for (int i = 0; i < kMbarRounds; ++i)
-                        if (mbar_try(resident_full, 0)) break;
-                for (int j = 0; j < issued; ++j) {
-                    if (--stage < 0) {
-                        stage = stages - 1;
+#pragma unroll
+                    for (int j = 0; j < PARTS; ++j) {
+                        if (resident > 0 || (again && j > 0)) break;
+                        if (S::kBmn) {
+                            for (int q = 0; q < blocks; ++q)
+                                tma_load(b + j * S::kB + q * S::kChunk * 128, &map_b, b0 + 64 * q, k, j, bar, on);
+                        } else {
+                            tma_load(b + j * S::kB, &map_b, k, b0, j, bar, on);
+                        }
+                    }
+                    issued = min(issued + 1, stages);
+                    if (++stage == stages) {
+                        stage = 0;
                         phase ^= 1;
                     }
-                    for (int i = 0; i < kMbarRounds; ++i)
-                        if (mbar_try(full + 8 * stage, phase)) break;
                 }
             }
         }
+        if (stop) {  // this block gave up: its copies in flight land before it ends
+            if (MODE == kStats && resident > 0)
+                for (int i = 0; i < kMbarRounds; ++i)
+                    if (mbar_try(resident_full, 0)) break;
+            for (int j = 0; j < issued; ++j) {
+                if (--stage < 0) {
+                    stage = stages - 1;
+                    phase ^= 1;
+                }
+                for (int i = 0; i < kMbarRounds; ++i)
+                    if (mbar_try(full + 8 * stage, phase)) break;
+            }
+        }
     } else if (warp == 1) {
-        {  // issues products
-            const uint32_t on = elect_lane();
-            int stage = 0, buf = 0;
-            uint32_t phase = 0, buf_phase = 0;
-            bool ok = resident == 0 || mbar_wait_warp(resident_full, 0, &stop, p.error_word, DEV_ERR_TILE_WAIT);
-            for (int u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
-                const Walk w = walk_unit<MODE, PARTS>(p, u);
-                for (int t = 0; ok && t < w.tiles; ++t) {
-                    const int b0 = (S::kProduct ? w.first : w.first + t) * kN;
-                    const int c0 = S::kProduct ? w.c0 + t * p.per_segment : w.c0;
-                    const int c1 = S::kProduct ? min(w.c1, c0 + p.per_segment) : w.c1;
-                    // scores: every column that is read (32 at a time) has been written,
-                    // past the last class with zeros; tensor memory may hold NaNs
-                    constexpr int kRound = S::kProduct ? 16 : 32;
-                    const int n = min(kN, (p.columns - b0 + kRound - 1) / kRound * kRound);
-                    const uint32_t idesc = uniform(mma_idesc(n, S::kAmn, S::kBmn));
-                    const int chunks = (int)uniform((uint32_t)(c1 - c0));
-                    // 16-entry steps of the last chunk
-                    const int tail = (int)uniform((uint32_t)min(S::kChunk / 16, (p.depth - (c1 - 1) * S::kChunk + 15) / 16));
-                    ok = mbar_wait_warp(taken_empty + 8 * buf, buf_phase ^ 1, &stop, p.error_word, DEV_ERR_TILE_WAIT);
+        // issues products
+        const uint32_t on = elect_lane();
+        int stage = 0, buf = 0;
+        uint32_t phase = 0, buf_phase = 0;
+        bool ok = resident == 0 || mbar_wait_warp(resident_full, 0, &stop, p.error_word, DEV_ERR_TILE_WAIT);
+        for (int u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
+            const Walk w = walk_unit<MODE, PARTS>(p, u);
+            for (int t = 0; ok && t < w.tiles; ++t) {
+                const int b0 = (S::kProduct ? w.first : w.first + t) * kN;
+                const int c0 = S::kProduct ? w.c0 + t * p.per_segment : w.c0;
+                const int c1 = S::kProduct ? min(w.c1, c0 + p.per_segment) : w.c1;
+                // scores: every column that is read (32 at a time) has been written,
+                // past the last class with zeros; tensor memory may hold NaNs
+                constexpr int kRound = S::kProduct ? 16 : 32;
+                const int n = min(kN, (p.columns - b0 + kRound - 1) / kRound * kRound);
+                const uint32_t idesc = uniform(mma_idesc(n, S::kAmn, S::kBmn));
+                const int chunks = (int)uniform((uint32_t)(c1 - c0));
+                // 16-entry steps of the last chunk
+                const int tail = (int)uniform((uint32_t)min(S::kChunk / 16, (p.depth - (c1 - 1) * S::kChunk + 15) / 16));
+                ok = mbar_wait_warp(taken_empty + 8 * buf, buf_phase ^ 1, &stop, p.error_word, DEV_ERR_TILE_WAIT);
+                if (!ok) break;
+                tmem_fence_after();
+                const uint32_t d = uniform(tmem + buf * kN);
+                const int passes = S::kTwice && chunks > 1 ? 2 : 1;
+                for (int v = 0; v < passes * chunks; ++v) {
+                    ok = mbar_wait_warp(full + 8 * stage, phase, &stop, p.error_word, DEV_ERR_TILE_WAIT);
                     if (!ok) break;
                     tmem_fence_after();
-                    const uint32_t d = uniform(tmem + buf * kN);
-                    const int passes = S::kTwice && chunks > 1 ? 2 : 1;
-                    for (int v = 0; v < passes * chunks; ++v) {
-                        ok = mbar_wait_warp(full + 8 * stage, phase, &stop, p.error_word, DEV_ERR_TILE_WAIT);
-                        if (!ok) break;
-                        tmem_fence_after();
-                        const int c = v < chunks ? v : v - chunks;
-                        const int steps = c + 1 < chunks ? S::kChunk / 16 : tail;
-                        const uint32_t a_at = ring + stage * stage_bytes;
-                        const uint32_t b_at = resident > 0 ? base + (t * chunks + c) * (PARTS * S::kB) : a_at + S::kPartsA * S::kA;
-                        const uint32_t a = uniform(S::kAmn ? mn_major_lo(a_at, S::kChunk * 128) : k_major_lo(a_at));
-                        const uint32_t b = uniform(S::kBmn ? mn_major_lo(b_at, S::kChunk * 128) : k_major_lo(b_at));
-                        constexpr uint32_t a_hi = S::kAmn ? kMnMajorHi : k_major_hi(S::kChunk * 2);
-                        constexpr uint32_t b_hi = S::kBmn ? kMnMajorHi : k_major_hi(S::kChunk * 2);
+                    const int c = v < chunks ? v : v - chunks;
+                    const int steps = c + 1 < chunks ? S::kChunk / 16 : tail;
+                    const uint32_t a_at = ring + stage * stage_bytes;
+                    const uint32_t b_at = resident > 0 ? base + (t * chunks + c) * (PARTS * S::kB) : a_at + S::kPartsA * S::kA;
+                    const uint32_t a = uniform(S::kAmn ? mn_major_lo(a_at, S::kChunk * 128) : k_major_lo(a_at));
+                    const uint32_t b = uniform(S::kBmn ? mn_major_lo(b_at, S::kChunk * 128) : k_major_lo(b_at));
+                    constexpr uint32_t a_hi = S::kAmn ? kMnMajorHi : k_major_hi(S::kChunk * 2);
+                    constexpr uint32_t b_hi = S::kBmn ? kMnMajorHi : k_major_hi(S::kChunk * 2);
 #pragma unroll
-                        for (int i = 0; i < S::kPairs; ++i) {
-                            // of two passes the first leaves the last, large product out
-                            if (S::kTwice && passes == 2 && (i + 1 < S::kPairs) != (v < chunks)) continue;
+                    for (int i = 0; i < S::kPairs; ++i) {
+                        // of two passes the first leaves the last, large product out
+                        if (S::kTwice && passes == 2 && (i + 1 < S::kPairs) != (v < chunks)) continue;
 #pragma unroll
-                            for (int s = 0; s < S::kChunk / 16; ++s) {
-                                // 16 entries on: 32 bytes along a row, or 16 rows of 128 bytes
-                                if (s < steps)
-                                    mma_bf16<a_hi, b_hi>(
-                                        d, a + S::part_a(i) * (S::kA / 16) + s * (S::kAmn ? 128 : 2),
-                                        b + S::part_b(i) * (S::kB / 16) + s * (S::kBmn ? 128 : 2), idesc,
-                                        i > 0 || s > 0 ? true : v > 0, on);
-                            }
-                        }
-                        mma_commit(empty + 8 * stage, on);
-                        if (++stage == stages) {
-                            stage = 0;
-                            phase ^= 1;
+                        for (int s = 0; s < S::kChunk / 16; ++s) {
+                            // 16 entries on: 32 bytes along a row, or 16 rows of 128 bytes
+                            if (s < steps)
+                                mma_bf16<a_hi, b_hi>(
+                                    d, a + S::part_a(i) * (S::kA / 16) + s * (S::kAmn ? 128 : 2),
+                                    b + S::part_b(i) * (S::kB / 16) + s * (S::kBmn ? 128 : 2), idesc,
+                                    i > 0 || s > 0 ? true : v > 0, on);
                         }
                     }
-                    if (!ok) break;
-                    mma_commit(taken_full + 8 * buf, on);
-                    buf ^= 1;
-                    if (buf == 0) buf_phase ^= 1;
+                    mma_commit(empty + 8 * stage, on);
+                    if (++stage == stages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
                 }
+                if (!ok) break;
+                mma_commit(taken_full + 8 * buf, on);
+                buf ^= 1;
+                if (buf == 0) buf_phase ^= 1;
             }
-            if (stop) {
-                mma_commit(drain, on);
-                for (int i = 0; i < kMbarRounds; ++i)
-                    if (mbar_try(drain, 0)) break;
-            }
+        }
+        if (stop) {
+            mma_commit(drain, on);
+            for (int i = 0; i < kMbarRounds; ++i)
+                if (mbar_try(drain, 0)) break;
         }
     } else {
         // Takes tiles out: warp % 4 is the quarter of the rows it can reach,

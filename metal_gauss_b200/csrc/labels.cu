@@ -296,11 +296,10 @@ struct Sizes {
     int64_t channel_columns() const { return up(channels, kN); }
     int64_t g_ld() const { return up(classes, 64) * 64; }
     int g_parts() const { return parts == 1 ? 2 : parts; }
-    // dx straight from the product, in rows of whole 16-byte stores
-    bool class_direct() const {
-        return pieces() == 1 && by_class().splits == 1 && channels % (parts == 3 ? 4 : 8) == 0;
-    }
-    bool direct() const { return by_row().splits == 1 && channels % (parts == 3 ? 4 : 8) == 0; }
+    // dx and dw straight from the product: one share, in rows of whole 16-byte stores
+    bool whole_stores() const { return channels % (parts == 3 ? 4 : 8) == 0; }
+    bool direct() const { return by_row().splits == 1 && whole_stores(); }
+    bool class_direct() const { return pieces() == 1 && by_class().splits == 1 && whole_stores(); }
     int64_t piece() const {
         const int64_t fit = kPieceBytes / (2 * g_parts() * g_ld()) / kM * kM;
         return std::min(up(rows, kM) * kM, std::max(kPieceRows, fit));
@@ -321,8 +320,7 @@ struct Sizes {
     // (Single elements, 32 rows apart in a warp, took 2 us of a unit.)
     bool fused_direct() const {
         const Shares s = fused_by_row();
-        return s.splits == 1 && (parts == 3 || s.per_split <= fused_segment()) &&
-               channels % (parts == 3 ? 4 : 8) == 0;
+        return s.splits == 1 && (parts == 3 || s.per_split <= fused_segment()) && whole_stores();
     }
     int64_t class_pad() const { return up(classes, kClassPad) * kClassPad; }
     // the forward's join: a warp to a row where the classes are in many shares
