@@ -253,14 +253,20 @@ struct HeldType { using type = T; };
 template <typename T>
 struct HeldType<T, true> { using type = int8_t; };
 
+// Threads of the adjoint's block: half as many where a row has one warp, so that
+// blocks of 98 registers a thread (16 channels a lane) leave fewer registers over.
+template <int WARPS>
+constexpr int kBackThreads = WARPS > 1 ? kThreads : 128;
+
 template <typename T, int VEC, int LPR, int NV, int WARPS, bool HELD8>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kBackThreads<WARPS>)
 norm_backward_kernel(const T* __restrict__ dy, const T* __restrict__ x,
                      const int8_t* __restrict__ codes, const float* __restrict__ scales,
                      const void* __restrict__ weight, int param_dtype,
                      const float* __restrict__ mean_in, const float* __restrict__ rstd_in,
                      int64_t rows, int channels, T* __restrict__ dx,
                      float* __restrict__ partial) {
+    constexpr int kThreads = kBackThreads<WARPS>;
     __shared__ float2 sh[WARPS > 1 ? WARPS : 1];
     constexpr int kTeams = WARPS > 1 ? 1 : kThreads / LPR;
     const int lane = WARPS > 1 ? threadIdx.x % 32 : threadIdx.x % LPR;
@@ -269,7 +275,7 @@ norm_backward_kernel(const T* __restrict__ dy, const T* __restrict__ x,
     const float inv_n = 1.0f / (float)channels;
     const int nb = (channels + kBlock8 - 1) / kBlock8;
 
-    extern __shared__ float dynamic[];  // weight, later 8 warps x channels
+    extern __shared__ float dynamic[];  // weight, later a row of sums per warp
     using P = Params<NV * VEC, VEC, WARPS>;
     P w;
     w.sh = dynamic;
@@ -666,19 +672,19 @@ norm_join_kernel(const float* __restrict__ partial, int blocks, int channels, in
 // Blocks of the adjoint: enough to fill the device, few enough that the join
 // stays short. Depends on the sizes only, so scratch and launch agree.
 int64_t backward_blocks(int64_t rows, int64_t channels) {
-    const int64_t teams = channels > 1024 ? 1 : std::max<int64_t>(8, 256 / std::max<int64_t>(1, channels));
+    const int64_t teams = channels > 1024 ? 1 : std::max<int64_t>(4, 128 / std::max<int64_t>(1, channels));
     const int64_t want = (rows + teams - 1) / teams;
-    return std::max<int64_t>(1, std::min<int64_t>(want, 4 * (int64_t)sm_count()));
+    return std::max<int64_t>(1, std::min<int64_t>(want, (channels > 1024 ? 4 : 8) * (int64_t)sm_count()));
 }
 
 // Blocks of a kernel that an SM holds, asked once per device.
 template <typename K>
-int blocks_per_sm(K kernel, size_t smem, int (&known)[64]) {
+int blocks_per_sm(K kernel, size_t smem, int (&known)[64], int threads = kThreads) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 2;
     if (known[dev] == 0) {
         int n = 0;
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kThreads, smem) != cudaSuccess || n < 1) n = 1;
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess || n < 1) n = 1;
         known[dev] = n;
     }
     return known[dev];
@@ -729,19 +735,20 @@ struct Backward {
 
     template <typename T, int VEC, int LPR, int NV, int WARPS>
     mg_status run() const {
-        const size_t smem = WARPS == 1 ? sizeof(float) * 8 * (size_t)channels : 0;
+        const size_t smem = WARPS == 1 ? sizeof(float) * (kBackThreads<1> / 32) * (size_t)channels : 0;
+        constexpr int threads = kBackThreads<WARPS>;
         static int known[2][64] = {};
         const int per_sm = codes != nullptr
-                               ? blocks_per_sm(norm_backward_kernel<T, VEC, LPR, NV, WARPS, true>, smem, known[0])
-                               : blocks_per_sm(norm_backward_kernel<T, VEC, LPR, NV, WARPS, false>, smem, known[1]);
+                               ? blocks_per_sm(norm_backward_kernel<T, VEC, LPR, NV, WARPS, true>, smem, known[0], threads)
+                               : blocks_per_sm(norm_backward_kernel<T, VEC, LPR, NV, WARPS, false>, smem, known[1], threads);
         const int grid = std::min(max_grid, per_sm * sm_count());
         *used = grid;
         if (codes != nullptr)
-            norm_backward_kernel<T, VEC, LPR, NV, WARPS, true><<<grid, kThreads, smem, st>>>(
+            norm_backward_kernel<T, VEC, LPR, NV, WARPS, true><<<grid, threads, smem, st>>>(
                 static_cast<const T*>(dy), nullptr, codes, scales, weight, param_dtype, mean, rstd,
                 rows, channels, static_cast<T*>(dx), partial);
         else
-            norm_backward_kernel<T, VEC, LPR, NV, WARPS, false><<<grid, kThreads, smem, st>>>(
+            norm_backward_kernel<T, VEC, LPR, NV, WARPS, false><<<grid, threads, smem, st>>>(
                 static_cast<const T*>(dy), static_cast<const T*>(x), nullptr, nullptr, weight,
                 param_dtype, mean, rstd, rows, channels, static_cast<T*>(dx), partial);
         return check_launch("layer_norm_backward");
