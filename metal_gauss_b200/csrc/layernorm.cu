@@ -12,9 +12,9 @@
 // short), the 8 warps of a block above that. The variance is the mean of
 // (x - mean)^2 from those registers, never E[x^2] - mean^2.
 // Measured (of 6.55 TB/s copied): 640000 x 64 fp32 58 us forward (86 %), 77 us
-// adjoint (98 %); with the 8-bit form 80 and 73 us (70, 73 %); 262144 x 512 bf16
-// 103 and 180 us (80, 68 %: a lane's 32 sums for dw and db leave room for 16
-// warps on an SM).
+// adjoint (98 %); with the 8-bit form 80 and 75 us (73, 74 %); 262144 x 512 bf16
+// 103 and 160 us (80, 77 %: a lane's 32 sums for dw and db leave room for 20
+// warps on an SM). Odd lengths: 500000 x 77 fp32 94 and 149 us (50, 47 %).
 // dw and db: a lane owns the same channels of every row its team takes, so
 // the sums over rows stay in its registers; teams of a block join in shared
 // memory, blocks through one fp32 row each in scratch, summed in a fixed order
