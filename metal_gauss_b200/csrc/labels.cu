@@ -326,10 +326,15 @@ struct Sizes {
     // the forward's join: a warp to a row where the classes are in many shares
     bool wide_rows() const { return stats().splits >= 8; }
     int64_t row_blocks() const { return up(rows, wide_rows() ? 8 : 256); }
-    // the bias's gradient: sums of 32 rows, then of up to kBiasLines of those
+    // the bias's gradient: sums of 32 rows, then of up to kBiasLines of those; the
+    // pieces' shares follow one another, and those of the last, short one are fewer
     int64_t pieces() const { return up(rows, piece()); }
     int64_t bias_lines() const { return piece() / 32; }
-    int64_t bias_shares() const { return up(bias_lines(), kBiasLines); }
+    int64_t bias_shares(int64_t piece_rows) const { return up(up(piece_rows, kM) * 4, kBiasLines); }
+    int64_t all_bias_shares() const {
+        const int64_t whole = pieces() - 1;
+        return whole * bias_shares(piece()) + bias_shares(rows - whole * piece());
+    }
 };
 
 struct Scratch {
@@ -384,7 +389,7 @@ struct BackwardScratch {
             row_part = a.take<float>(n.direct() ? 0 : (size_t)n.by_row().splits * n.piece() * n.part_ld());
             class_part = a.take<float>((size_t)n.by_class().splits * n.classes * n.part_ld());
             bias_part = a.take<float>((size_t)n.bias_lines() * n.classes);
-            bias_part2 = a.take<float>((size_t)(n.pieces() * n.bias_shares()) * n.classes);
+            bias_part2 = a.take<float>((size_t)n.all_bias_shares() * n.classes);
         }
         bytes = (size_t)(a.p - static_cast<char*>(base));
     }
@@ -617,9 +622,9 @@ mg_status backward(const Args& a, const RowGrad& rg, const float* stats, T* dx, 
         p.error_word = device_error_word();
         MG_TRY((launch_tiles<kLogitGrad, PARTS>(p, mx, mw_score, mg_out, a.st, "label_loss_backward logits")));
         if (db != nullptr) {
-            float* sums = f.bias_part2 + row0 / n.piece() * n.bias_shares() * n.classes;
+            float* sums = f.bias_part2 + row0 / n.piece() * n.bias_shares(n.piece()) * n.classes;
             MG_TRY(column_sum(f.bias_part, up(rows, kM) * 4, kBiasLines, n.classes,
-                              n.pieces() * n.bias_shares() > 1 ? sums : db, a.st));
+                              n.all_bias_shares() > 1 ? sums : db, a.st));
         }
         p.part_bias = nullptr;
         p.per_segment = n.segment();
@@ -662,8 +667,8 @@ mg_status backward(const Args& a, const RowGrad& rg, const float* stats, T* dx, 
     }
     if (dw != nullptr && !n.class_direct())
         MG_TRY(join(f.class_part, n.by_class().splits, n.classes, n.part_ld(), n.channels, a.scale, dw, a.st));
-    if (db != nullptr && n.pieces() * n.bias_shares() > 1) {
-        const int64_t shares = n.pieces() * n.bias_shares();
+    if (db != nullptr && n.all_bias_shares() > 1) {
+        const int64_t shares = n.all_bias_shares();
         MG_TRY(column_sum(f.bias_part2, shares, shares, n.classes, db, a.st));
     }
     return MG_OK;
