@@ -18,6 +18,7 @@ from __future__ import annotations
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import ptr
@@ -28,6 +29,11 @@ DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # MG_F32, MG_
 
 
 def wants_grad(*tensors: torch.Tensor | None) -> bool:
+    """Whether an operator on these goes through its autograd function: one of
+    them needs a gradient, or a forward-mode level is open (the function then
+    refuses an input that carries a tangent, which a detached one would lose)."""
+    if forward_ad._current_level >= 0:
+        return True
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
