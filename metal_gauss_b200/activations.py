@@ -106,14 +106,46 @@ def unpack8(codes: torch.Tensor, scales: torch.Tensor,
     return x
 
 
+def _parameters(fn) -> tuple[torch.Tensor, ...]:
+    """The parameters that a module (or a module's method, or a partial of
+    either) trains."""
+    while isinstance(fn, functools.partial):
+        fn = fn.func
+    module = fn if isinstance(fn, torch.nn.Module) else getattr(fn, "__self__", None)
+    if not isinstance(module, torch.nn.Module):
+        return ()
+    return tuple(p for p in module.parameters() if p.requires_grad)
+
+
+def _refuse_other_leaves(out: torch.Tensor, leaves: list[torch.Tensor]) -> None:
+    """Raises when out's graph ends in a tensor that is none of leaves."""
+    known = {id(t) for t in leaves}
+    seen, todo = set(), [out.grad_fn]
+    while todo:
+        node = todo.pop()
+        if node is None or node in seen:
+            continue
+        seen.add(node)
+        leaf = getattr(node, "variable", None)
+        if leaf is not None and id(leaf) not in known:
+            raise RuntimeError(f"checkpoint8: fn uses a tensor {tuple(leaf.shape)} that needs a "
+                               "gradient and is none of its arguments: pass it as an argument, "
+                               "or detach it")
+        todo.extend(n for n, _ in node.next_functions)
+
+
 class _Checkpoint8(torch.autograd.Function):
+    """Inputs: fn, the number of its arguments after x, x, those, and the
+    parameters that fn brings along."""
+
     @staticmethod
-    def forward(ctx, fn, x, *args):
-        ctx.fn, ctx.dtype = fn, x.dtype
+    def forward(ctx, fn, count, x, *rest):
+        args = rest[:count]
+        ctx.fn, ctx.count, ctx.dtype = fn, count, x.dtype
         ctx.where = [i for i, a in enumerate(args) if torch.is_tensor(a)]
         ctx.others = [None if torch.is_tensor(a) else a for a in args]
         codes, scales = pack8(x)
-        ctx.save_for_backward(codes, scales, *(args[i] for i in ctx.where))
+        ctx.save_for_backward(codes, scales, *(args[i] for i in ctx.where), *rest[count:])
         with torch.no_grad():
             out = fn(x, *args)
         if not torch.is_tensor(out):
@@ -124,7 +156,7 @@ class _Checkpoint8(torch.autograd.Function):
     @once
     def backward(ctx, grad):
         codes, scales, *tensors = ctx.saved_tensors
-        need = ctx.needs_input_grad[1:]
+        need = ctx.needs_input_grad[2:]
         x = unpack8(codes, scales, ctx.dtype)
         args = list(ctx.others)
         with torch.enable_grad():
@@ -132,19 +164,26 @@ class _Checkpoint8(torch.autograd.Function):
             for i, t in zip(ctx.where, tensors):
                 args[i] = t.detach().requires_grad_(need[1 + i])
             out = ctx.fn(x, *args)
-        leaves = [t for t, k in zip([x] + args, need) if k]
-        found = iter(torch.autograd.grad(out, leaves, grad, allow_unused=True))
-        return (None,) + tuple(next(found) if k else None for k in need)
+        inputs = [x, *args, *tensors[len(ctx.where):]]
+        leaves = [t for t, k in zip(inputs, need) if k]
+        _refuse_other_leaves(out, leaves)
+        if out.requires_grad:
+            found = iter(torch.autograd.grad(out, leaves, grad, allow_unused=True))
+        else:      # none of them was used
+            found = iter([None] * len(leaves))
+        return (None, None) + tuple(next(found) if k else None for k in need)
 
 
 def checkpoint8(fn, x: torch.Tensor, *args) -> torch.Tensor:
-    """fn(x, *args), differentiable in x and the tensors among args, holding
-    x in 8 bits and nothing that fn computes: the backward pass reads x back
-    and runs fn again. The result is fn's own; the gradients are those of fn
-    at the x that was read back. fn must return one tensor, do the same work
-    both times, and take every tensor that needs a gradient as an argument
-    (one that it closes over gets none)."""
+    """fn(x, *args), differentiable in x, the tensors among args and, where fn
+    is a module or a module's method, the module's parameters; it holds x in 8
+    bits and nothing that fn computes: the backward pass reads x back and runs
+    fn again. The result is fn's own; the gradients are those of fn at the x
+    that was read back. fn must return one tensor and do the same work both
+    times (no random numbers, no running statistics). Every other tensor that
+    needs a gradient has to be an argument: one that fn closes over, or that
+    sits in a list among args, makes the backward pass raise."""
     dtype_code(x, "checkpoint8: x")
     _rows(x, "checkpoint8: x")
     check_cuda(x, "checkpoint8: x")
-    return _Checkpoint8.apply(fn, x, *args)
+    return _Checkpoint8.apply(fn, len(args), x, *args, *_parameters(fn))
