@@ -15,6 +15,7 @@ so a value comes back within a / 254 of itself.
 
 from __future__ import annotations
 
+import contextlib
 import functools
 
 import torch
@@ -134,6 +135,20 @@ def _refuse_other_leaves(out: torch.Tensor, leaves: list[torch.Tensor]) -> None:
         todo.extend(n for n, _ in node.next_functions)
 
 
+def _autocast_state() -> tuple[bool, torch.dtype]:
+    return torch.is_autocast_enabled("cuda"), torch.get_autocast_dtype("cuda")
+
+
+def _autocast(state: tuple[bool, torch.dtype]):
+    """The mixed precision of state, without the cache of cast parameters: one
+    cast without a graph must not serve a later use that needs it, nor one from
+    outside a segment's own graph."""
+    enabled, dtype = state
+    if not enabled and not torch.is_autocast_enabled("cuda"):
+        return contextlib.nullcontext()
+    return torch.autocast("cuda", dtype=dtype, enabled=enabled, cache_enabled=False)
+
+
 class _Checkpoint8(torch.autograd.Function):
     """Inputs: fn, the number of its arguments after x, x, those, and the
     parameters that fn brings along."""
@@ -146,7 +161,8 @@ class _Checkpoint8(torch.autograd.Function):
         ctx.others = [None if torch.is_tensor(a) else a for a in args]
         codes, scales = pack8(x)
         ctx.save_for_backward(codes, scales, *(args[i] for i in ctx.where), *rest[count:])
-        with torch.no_grad():
+        ctx.autocast = _autocast_state()
+        with torch.no_grad(), _autocast(ctx.autocast):
             out = fn(x, *args)
         if not torch.is_tensor(out):
             raise TypeError(f"checkpoint8: fn must return one tensor, got {type(out).__name__}")
@@ -159,7 +175,7 @@ class _Checkpoint8(torch.autograd.Function):
         need = ctx.needs_input_grad[2:]
         x = unpack8(codes, scales, ctx.dtype)
         args = list(ctx.others)
-        with torch.enable_grad():
+        with torch.enable_grad(), _autocast(ctx.autocast):
             x.requires_grad_(need[0])
             for i, t in zip(ctx.where, tensors):
                 args[i] = t.detach().requires_grad_(need[1 + i])
@@ -180,7 +196,8 @@ def checkpoint8(fn, x: torch.Tensor, *args) -> torch.Tensor:
     bits and nothing that fn computes: the backward pass reads x back and runs
     fn again. The result is fn's own; the gradients are those of fn at the x
     that was read back. fn must return one tensor and do the same work both
-    times (no random numbers, no running statistics). Every other tensor that
+    times (no random numbers, no running statistics); it runs under the forward
+    pass's autocast state both times. Every other tensor that
     needs a gradient has to be an argument: one that fn closes over, or that
     sits in a list among args, makes the backward pass raise."""
     dtype_code(x, "checkpoint8: x")

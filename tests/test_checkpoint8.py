@@ -97,3 +97,41 @@ def test_a_segment_that_uses_no_input(cuda):
     assert got is None
     (got,) = torch.autograd.grad(checkpoint8(lambda t: t, x), x, torch.full_like(x, 3.0))
     assert torch.equal(got, torch.full_like(x, 3.0))
+
+
+@pytest.mark.parametrize("inside", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_the_segment_runs_again_in_the_forward_passs_precision(cuda, dtype, inside):
+    """Mixed precision in the forward pass, the backward pass outside it or in
+    another one; the same parameter used beside the segment keeps its own
+    gradient."""
+    g = gen(5)
+    x = torch.randn(64, 48, generator=g, device=cuda, requires_grad=True)
+    w = torch.randn(32, 48, generator=g, device=cuda, requires_grad=True)
+    seen = []
+
+    def segment(t, u):
+        y = torch.nn.functional.linear(t, u)
+        seen.append(y.dtype)
+        return y.float().square().mean()
+
+    def step(run, t):
+        with torch.autocast("cuda", dtype=dtype):
+            loss = run(segment, t, w) + torch.nn.functional.linear(x.detach(), w).float().mean()
+        with torch.autocast("cuda", dtype=torch.bfloat16, enabled=inside):
+            return loss.detach(), *torch.autograd.grad(loss, (t, w))
+
+    got = step(checkpoint8, x)
+    assert seen == [dtype, dtype]
+    xr = held8(x).requires_grad_(True)
+    want = step(lambda f, *a: f(*a), xr)
+    assert torch.equal(got[1], want[1])
+    # the two uses of w in one sum: half a step of dtype for each cast gradient
+    eps = torch.finfo(dtype).eps
+    assert float((got[2] - want[2]).abs().max()) <= 2 * eps * float(want[2].abs().max())
+    # and without mixed precision the segment never enters it
+    seen.clear()
+    loss = checkpoint8(segment, x, w)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        torch.autograd.grad(loss, x)
+    assert seen == [torch.float32, torch.float32]
