@@ -149,6 +149,12 @@ def _autocast(state: tuple[bool, torch.dtype]):
     return torch.autocast("cuda", dtype=dtype, enabled=enabled, cache_enabled=False)
 
 
+def _one_tensor(out) -> torch.Tensor:
+    if not torch.is_tensor(out):
+        raise TypeError(f"checkpoint8: fn must return one tensor, got {type(out).__name__}")
+    return out
+
+
 class _Checkpoint8(torch.autograd.Function):
     """Inputs: fn, the number of its arguments after x, x, those, and the
     parameters that fn brings along."""
@@ -163,10 +169,7 @@ class _Checkpoint8(torch.autograd.Function):
         ctx.save_for_backward(codes, scales, *(args[i] for i in ctx.where), *rest[count:])
         ctx.autocast = _autocast_state()
         with torch.no_grad(), _autocast(ctx.autocast):
-            out = fn(x, *args)
-        if not torch.is_tensor(out):
-            raise TypeError(f"checkpoint8: fn must return one tensor, got {type(out).__name__}")
-        return out
+            return _one_tensor(fn(x, *args))
 
     @staticmethod
     @once
@@ -199,8 +202,12 @@ def checkpoint8(fn, x: torch.Tensor, *args) -> torch.Tensor:
     times (no random numbers, no running statistics); it runs under the forward
     pass's autocast state both times. Every other tensor that
     needs a gradient has to be an argument: one that fn closes over, or that
-    sits in a list among args, makes the backward pass raise."""
+    sits in a list among args, makes the backward pass raise. Where no
+    gradient of those inputs is wanted, fn runs by itself and nothing is held."""
     dtype_code(x, "checkpoint8: x")
     _rows(x, "checkpoint8: x")
     check_cuda(x, "checkpoint8: x")
-    return _Checkpoint8.apply(fn, len(args), x, *args, *_parameters(fn))
+    params = _parameters(fn)
+    if not wants_grad(x, *(a for a in args if torch.is_tensor(a)), *params):
+        return _one_tensor(fn(x, *args))
+    return _Checkpoint8.apply(fn, len(args), x, *args, *params)

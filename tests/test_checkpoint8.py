@@ -5,7 +5,8 @@ import functools
 import pytest
 import torch
 
-from metal_gauss_b200.activations import checkpoint8
+from metal_gauss_b200 import activations
+from metal_gauss_b200.activations import checkpoint8, pack8
 from metal_gauss_b200.labels import label_loss
 from metal_gauss_b200.layernorm import layer_norm
 from test_features import gen, held8
@@ -135,3 +136,26 @@ def test_the_segment_runs_again_in_the_forward_passs_precision(cuda, dtype, insi
     with torch.autocast("cuda", dtype=torch.bfloat16):
         torch.autograd.grad(loss, x)
     assert seen == [torch.float32, torch.float32]
+
+
+def test_nothing_is_packed_where_no_gradient_is_wanted(cuda, monkeypatch):
+    x, lab, head = case(6)
+    calls = []
+
+    def counted(t):
+        calls.append(t.shape)
+        return pack8(t)
+
+    monkeypatch.setattr(activations, "pack8", counted)
+    with torch.no_grad():
+        assert torch.equal(checkpoint8(head, x, lab), head(x, lab))
+    d = x.detach()
+    assert torch.equal(checkpoint8(lambda t, k: t * k, d, 2.0), d * 2)
+    assert not calls
+    # a closure over a module then trains it as it would by itself
+    (got,) = torch.autograd.grad(checkpoint8(lambda t: head(t, lab), d), head.classes)
+    (want,) = torch.autograd.grad(head(d, lab), head.classes)
+    assert torch.equal(got, want) and not calls
+    with pytest.raises(TypeError, match="one tensor"):
+        checkpoint8(lambda t: (t, t), d)
+    assert checkpoint8(head, x, lab).requires_grad and len(calls) == 1
