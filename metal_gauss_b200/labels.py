@@ -96,9 +96,10 @@ def label_loss(features: torch.Tensor, classes: torch.Tensor, labels: torch.Tens
     labels, differentiable in features, classes and bias.
 
     features (..., channels), up to 512 channels; classes (n_classes,
-    channels) of the same type (float32, bfloat16 or float16); labels (...)
-    uint8, int32 or int64; bias (n_classes,) float32 or of the features' type,
-    -infinity taking a class out. Pixels labelled ignore_index have loss 0 and
+    channels) of the same type (float32, bfloat16 or float16); scale a number
+    (a tensor that needs a gradient is refused); labels (...) uint8, int32 or
+    int64; bias (n_classes,) float32 or of the features' type, -infinity taking
+    a class out. Pixels labelled ignore_index have loss 0 and
     no gradient whatever their features hold, and do not count in a mean. The
     result is float32: one value for reduction "mean" (0 when no pixel takes
     part) or "sum", labels' shape for "none". Another label outside
@@ -132,6 +133,9 @@ def label_loss(features: torch.Tensor, classes: torch.Tensor, labels: torch.Tens
     if reduction not in REDUCTIONS:
         raise ValueError(f"label_loss: reduction must be one of {tuple(REDUCTIONS)}, got "
                          f"{reduction!r}")
+    if torch.is_tensor(scale) and wants_grad(scale):
+        raise TypeError("label_loss: scale is a number and has no gradient; to learn it, multiply "
+                        "the features or the classes by it")
     check_cuda(features, "label_loss: features")
     args = (features, classes, labels, bias, float(scale), int(ignore_index),
             REDUCTIONS[reduction])

@@ -98,6 +98,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
                          f"channels, got {tuple(x.shape)}")
     if saved not in ("full", "int8"):
         raise ValueError(f"layer_norm: saved must be 'full' or 'int8', got {saved!r}")
+    if torch.is_tensor(eps) and wants_grad(eps):
+        raise TypeError("layer_norm: eps is a number and has no gradient")
     if not eps >= 0:
         raise ValueError(f"layer_norm: eps must not be negative, got {eps}")
     for t, what in ((weight, "weight"), (bias, "bias")):

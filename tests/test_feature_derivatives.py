@@ -23,6 +23,24 @@ def test_an_open_forward_mode_level_goes_through_the_autograd_function():
     assert not wants_grad(x)
 
 
+def test_numbers_that_need_a_gradient_are_refused():
+    """A learned temperature would get none. (What passes goes on to the next
+    refusal, of CPU tensors.)"""
+    x, c, lab = torch.zeros(4, 8), torch.zeros(3, 8), torch.zeros(4, dtype=torch.int64)
+    k = torch.tensor(0.5, requires_grad=True)
+    with pytest.raises(TypeError, match="scale"):
+        label_loss(x, c, lab, scale=k)
+    with pytest.raises(TypeError, match="eps"):
+        layer_norm(x, eps=k)
+    for ok in (0.5, torch.tensor(0.5)):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            label_loss(x, c, lab, scale=ok)
+        with pytest.raises(RuntimeError, match="CUDA"):
+            layer_norm(x, eps=ok)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+        label_loss(x, c, lab, scale=k)
+
+
 @pytest.mark.gpu
 def test_forward_mode_derivatives_are_refused(cuda):
     g = torch.Generator(device=cuda).manual_seed(3)
