@@ -72,7 +72,7 @@ def _rows(t: torch.Tensor, what: str) -> tuple[int, int]:
 
 def pack8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """x (..., channels) in 8 bits: codes int8 (..., channels) and scales
-    float32 (..., ceil(channels / 128)). 128 channels with an infinity or a
+    float32 (..., ceil(channels / 128)), neither differentiable in x. 128 channels with an infinity or a
     NaN among them read back as NaN; below 1e-30 they read back as 0."""
     code, (n, d) = dtype_code(x, "pack8: x"), _rows(x, "pack8: x")
     check_cuda(x, "pack8: x")
@@ -85,7 +85,10 @@ def pack8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 def unpack8(codes: torch.Tensor, scales: torch.Tensor,
             dtype: torch.dtype = torch.float32) -> torch.Tensor:
-    """The tensor that `pack8` gave codes and scales for, as `dtype`."""
+    """The tensor that `pack8` gave codes and scales for, as `dtype`. It has no
+    gradient: scales that need one are refused."""
+    if scales.requires_grad and torch.is_grad_enabled():
+        raise TypeError("unpack8: scales need a gradient, and unpack8 has none")
     if codes.dtype != torch.int8 or scales.dtype != torch.float32:
         raise TypeError(f"unpack8 takes int8 codes and float32 scales, got {codes.dtype} and "
                         f"{scales.dtype}")

@@ -5,7 +5,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from metal_gauss_b200.activations import checkpoint8, wants_grad
+from metal_gauss_b200.activations import checkpoint8, unpack8, wants_grad
 from metal_gauss_b200.labels import label_loss
 from metal_gauss_b200.layernorm import layer_norm
 
@@ -39,6 +39,16 @@ def test_numbers_that_need_a_gradient_are_refused():
             layer_norm(x, eps=ok)
     with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
         label_loss(x, c, lab, scale=k)
+
+
+def test_scales_that_need_a_gradient_are_refused():
+    codes, scales = torch.zeros(4, 8, dtype=torch.int8), torch.zeros(4, 1, requires_grad=True)
+    with pytest.raises(TypeError, match="gradient"):
+        unpack8(codes, scales)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+        unpack8(codes, scales)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        unpack8(codes, scales.detach())
 
 
 @pytest.mark.gpu
