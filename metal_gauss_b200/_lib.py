@@ -223,6 +223,32 @@ class Launcher:
             check(status, self.name)
 
 
+class SizeOf:
+    """An mg_*_scratch_bytes function whose result depends on the device (on
+    its number of SMs): asked with the device current that the tensors are on,
+    and remembered for it and the sizes."""
+
+    __slots__ = ("name", "known")
+
+    def __init__(self, name: str):
+        self.name, self.known = name, {}
+
+    def __call__(self, device: int, *sizes: int) -> int:
+        key = (device, *sizes)
+        n = self.known.get(key)
+        if n is None:
+            fn = getattr(load(), self.name)
+            if torch._C._cuda_getDevice() == device:
+                n = fn(*sizes)
+            else:
+                with torch.cuda.device(device):
+                    n = fn(*sizes)
+            if len(self.known) >= 256:
+                self.known.clear()
+            self.known[key] = n
+        return n
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 

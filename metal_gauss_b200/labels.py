@@ -11,8 +11,6 @@ again (`mg_label_loss_forward`, `mg_label_loss_backward`).
 
 from __future__ import annotations
 
-from functools import lru_cache
-
 import torch
 
 from . import _lib
@@ -26,11 +24,7 @@ LABEL_BYTES = {torch.uint8: 1, torch.int32: 4, torch.int64: 8}
 
 _FORWARD = _lib.Launcher("mg_label_loss_forward")
 _BACKWARD = _lib.Launcher("mg_label_loss_backward")
-
-
-@lru_cache(maxsize=256)
-def _scratch_bytes(n: int, d: int, v: int, code: int, backward: int) -> int:
-    return _lib.load().mg_label_loss_scratch_bytes(n, d, v, code, backward)
+_SCRATCH = _lib.SizeOf("mg_label_loss_scratch_bytes")
 
 
 def _forward(features, classes, labels, bias, scale, ignore_index, reduction, train):
@@ -47,7 +41,7 @@ def _forward(features, classes, labels, bias, scale, ignore_index, reduction, tr
                        device=x.device)
     stats = torch.empty(2 * n + 1, dtype=torch.float32, device=x.device) if train else None
     at = ptr(stats)
-    nbytes = _scratch_bytes(n, d, v, code, 0)
+    nbytes = _SCRATCH(x.get_device(), n, d, v, code, 0)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
     _FORWARD(x.get_device(), ptr(x), ptr(w), code, ptr(b), ptr(lab), LABEL_BYTES[lab.dtype],
              ignore_index, n, d, v, scale, reduction, ptr(loss), at,
@@ -77,7 +71,7 @@ class _LabelLoss(torch.autograd.Function):
         dx = torch.empty_like(x) if need_x else None
         dw = torch.empty_like(w) if need_w else None
         db = torch.empty(v, dtype=torch.float32, device=x.device) if need_b else None
-        nbytes = _scratch_bytes(n, d, v, code, 1)
+        nbytes = _SCRATCH(x.get_device(), n, d, v, code, 1)
         scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
         at = stats.data_ptr()
         _BACKWARD(x.get_device(), ptr(x), ptr(w), code, ptr(b), ptr(lab), LABEL_BYTES[lab.dtype],

@@ -9,8 +9,6 @@ fp32 in a fixed order, so equal calls give equal bits.
 
 from __future__ import annotations
 
-from functools import lru_cache
-
 import torch
 
 from . import _lib
@@ -20,11 +18,7 @@ from .activations import BLOCK, DTYPES, check_cuda, dtype_code, once, wants_grad
 MAX_CHANNELS = 8192      # MG_LAYER_NORM_MAX_CHANNELS
 _FORWARD = _lib.Launcher("mg_layer_norm_forward")
 _BACKWARD = _lib.Launcher("mg_layer_norm_backward")
-
-
-@lru_cache(maxsize=256)
-def _scratch_bytes(n: int, d: int) -> int:
-    return _lib.load().mg_layer_norm_backward_scratch_bytes(n, d)
+_SCRATCH = _lib.SizeOf("mg_layer_norm_backward_scratch_bytes")
 
 
 def _forward(x, weight, bias, eps, train, saved):
@@ -73,7 +67,7 @@ class _LayerNorm(torch.autograd.Function):
         db = torch.empty(d, dtype=pdtype, device=dy.device) if need_b else None
         scratch, nbytes = None, 0
         if need_w or need_b:
-            nbytes = _scratch_bytes(n, d)
+            nbytes = _SCRATCH(dy.get_device(), n, d)
             scratch = torch.empty(nbytes, dtype=torch.uint8, device=dy.device)
         mean = stats.data_ptr()
         _BACKWARD(dy.get_device(), ptr(dy), ptr(x), ptr(codes), ptr(scales), DTYPES[dy.dtype],
