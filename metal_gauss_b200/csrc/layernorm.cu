@@ -677,7 +677,9 @@ int64_t backward_blocks(int64_t rows, int64_t channels) {
     return std::max<int64_t>(1, std::min<int64_t>(want, (channels > 1024 ? 4 : 8) * (int64_t)sm_count()));
 }
 
-// Blocks of a kernel that an SM holds, asked once per device.
+// Blocks of a kernel that an SM holds, asked once per device, with the shared
+// memory of the kernel's longest rows: the grid, and with it the order of the
+// adjoint's sums, depends on a call's own sizes and not on those of the first.
 template <typename K>
 int blocks_per_sm(K kernel, size_t smem, int (&known)[64], int threads = kThreads) {
     int dev = 0;
@@ -708,8 +710,9 @@ struct Forward {
         // one wave of blocks that stay: each reads the parameters once
         const int64_t want = (rows + kTeams - 1) / kTeams;
         const size_t smem = WARPS == 1 ? sizeof(float) * 2 * (size_t)channels : 0;
+        constexpr size_t most = WARPS == 1 ? sizeof(float) * 2 * VEC * LPR * NV : 0;
         static int known[64] = {};
-        const int per_sm = blocks_per_sm(norm_forward_kernel<T, VEC, LPR, NV, WARPS>, smem, known);
+        const int per_sm = blocks_per_sm(norm_forward_kernel<T, VEC, LPR, NV, WARPS>, most, known);
         const int grid = (int)std::min<int64_t>(want, per_sm * (int64_t)sm_count());
         norm_forward_kernel<T, VEC, LPR, NV, WARPS><<<grid, kThreads, smem, st>>>(
             static_cast<const T*>(x), weight, bias, param_dtype, rows, channels, eps,
@@ -736,11 +739,12 @@ struct Backward {
     template <typename T, int VEC, int LPR, int NV, int WARPS>
     mg_status run() const {
         const size_t smem = WARPS == 1 ? sizeof(float) * (kBackThreads<1> / 32) * (size_t)channels : 0;
+        constexpr size_t most = WARPS == 1 ? sizeof(float) * (kBackThreads<1> / 32) * VEC * LPR * NV : 0;
         constexpr int threads = kBackThreads<WARPS>;
         static int known[2][64] = {};
         const int per_sm = codes != nullptr
-                               ? blocks_per_sm(norm_backward_kernel<T, VEC, LPR, NV, WARPS, true>, smem, known[0], threads)
-                               : blocks_per_sm(norm_backward_kernel<T, VEC, LPR, NV, WARPS, false>, smem, known[1], threads);
+                               ? blocks_per_sm(norm_backward_kernel<T, VEC, LPR, NV, WARPS, true>, most, known[0], threads)
+                               : blocks_per_sm(norm_backward_kernel<T, VEC, LPR, NV, WARPS, false>, most, known[1], threads);
         const int grid = std::min(max_grid, per_sm * sm_count());
         *used = grid;
         if (codes != nullptr)
