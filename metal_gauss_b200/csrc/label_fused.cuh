@@ -223,6 +223,13 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
         return mbar_wait_warp(bar, parity, &stop, p.error_word, DEV_ERR_TILE_WAIT);
     };
 
+    // For the end of every warp: once all are past their last wait `stop` changes
+    // no more, and what is in flight then is drained or has been waited for.
+    const auto gave_up = [&] {
+        named_sync(1, kFusedThreads);
+        return stop != 0;
+    };
+
     if (warp >= 4 + 4 * kGroups) registers_up<kAccRegs>();
     else if (warp >= 4) registers_down<kScoreRegs>();
 
@@ -266,7 +273,7 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
                 }
             }
         }
-        if (stop) {  // this block gave up: its copies in flight land before it ends
+        if (gave_up()) {  // its copies in flight land before the block ends
             for (int j = issued; j > 0; --j) {
                 if (--stage < 0) {
                     stage = p.stages - 1;
@@ -348,7 +355,7 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
                 ob_phase ^= 1;
             }
         }
-        if (stop) {
+        if (gave_up()) {
             mma_commit(drain, on);
             for (int k = 0; k < kMbarRounds; ++k)
                 if (mbar_try(drain, 0)) break;
@@ -399,7 +406,7 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
                 }
             }
         }
-        if (stop) {
+        if (gave_up()) {
             mma_commit(drain + 8, on);
             for (int k = 0; k < kMbarRounds; ++k)
                 if (mbar_try(drain + 8, 0)) break;
@@ -598,6 +605,7 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
             }
         }
     }
+    if (warp > 2) gave_up();
     tmem_fence_before();
     __syncthreads();
     if (warp == 1) {

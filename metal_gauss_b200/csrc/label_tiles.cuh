@@ -198,6 +198,12 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
     __syncthreads();
     tmem_fence_after();
     constexpr uint32_t tmem = kTmemBase;
+    // For the end of every warp: once all are past their last wait `stop` changes
+    // no more, and what is in flight then is drained or has been waited for.
+    const auto gave_up = [&] {
+        named_sync(1, S::kThreads);
+        return stop != 0;
+    };
 
     if (warp == 0) {
         // copies tiles in
@@ -262,7 +268,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                 }
             }
         }
-        if (stop) {  // this block gave up: its copies in flight land before it ends
+        if (gave_up()) {  // its copies in flight land before the block ends
             if (MODE == kStats && resident > 0)
                 for (int i = 0; i < kMbarRounds; ++i)
                     if (mbar_try(resident_full, 0)) break;
@@ -338,7 +344,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                 if (buf == 0) buf_phase ^= 1;
             }
         }
-        if (stop) {
+        if (gave_up()) {
             mma_commit(drain, on);
             for (int i = 0; i < kMbarRounds; ++i)
                 if (mbar_try(drain, 0)) break;
@@ -568,6 +574,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
             }
         }
         if (MODE == kLogitGrad && speaks) tma_store_wait_all();
+        gave_up();
     }
     tmem_fence_before();
     __syncthreads();
