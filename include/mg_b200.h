@@ -799,6 +799,19 @@ mg_status mg_label_loss_backward(const void* features, const void* classes, int3
                                  float* d_bias, void* scratch, size_t scratch_bytes,
                                  mg_stream_t stream);
 
+/* Failure detection: the forward pass (grad_loss NULL) or the backward pass of
+ * mg_label_loss_* with MG_REDUCE_NONE, no bias and ignore_index -100, whose
+ * tensor-core tiles wait for at most `rounds` rounds and get only their first
+ * `units` units' tiles (0: none), so that the other waits run out. The kernels
+ * return, code 4 is in the device error word, and what such a wait was for is
+ * NaN. rounds in [1, 4096], rows in [1, 2^20]. */
+mg_status mg_label_loss_wait_selftest(int32_t rounds, int32_t units, const void* features,
+                                      const void* classes, int32_t dtype, const int64_t* labels,
+                                      int64_t rows, int64_t channels, int64_t n_classes, float* loss,
+                                      float* stats, const float* grad_loss, void* d_features,
+                                      void* d_classes, float* d_bias, void* scratch,
+                                      size_t scratch_bytes, mg_stream_t stream);
+
 /* ------------------------------------------------------------------------ */
 /* Device error word                                                        */
 /* ------------------------------------------------------------------------ */

@@ -148,6 +148,8 @@ SIGNATURES = {
                                     vp, vp, sz, vp]),
     "mg_label_loss_backward": (i32, [vp, vp, i32, vp, vp, i32, i64, i64, i64, i64, f32, i32, vp,
                                      vp, vp, vp, vp, vp, vp, sz, vp]),
+    "mg_label_loss_wait_selftest": (i32, [i32, i32, vp, vp, i32, vp, i64, i64, i64, vp, vp, vp, vp,
+                                          vp, vp, vp, sz, vp]),
     "mg_read_device_error": (i32, [C.POINTER(i32), vp]),
     "mg_peek_device_error": (i32, [vp, vp]),
     "mg_sort_lookback_selftest_scratch_bytes": (sz, []),

@@ -44,6 +44,8 @@ constexpr int kFusedShared = 226 * 1024;  // of it 1 KB to align
 
 struct FusedArgs {         // counts below 2^31: at most 2^30 rows
     int units;
+    int copied;            // units whose tiles are copied in: all, but for the self-test
+    int rounds;            // of the issuing and copying warps' waits, at most
     int own;               // items of the owning side
     int streamed;          // items of the streaming side
     int per_split;         // tiles of a share
@@ -216,11 +218,11 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
     // tiles that stay are waited for in their one and only phase
     const uint32_t flip = p.resident ? 0 : 1;
     const auto wait = [&](uint32_t bar, uint32_t parity) {
-        return mbar_wait(bar, parity, &stop, p.error_word, DEV_ERR_TILE_WAIT);
+        return mbar_wait(bar, parity, kMbarRounds, &stop, p.error_word, DEV_ERR_TILE_WAIT);
     };
 
     const auto wait_warp = [&](uint32_t bar, uint32_t parity) {
-        return mbar_wait_warp(bar, parity, &stop, p.error_word, DEV_ERR_TILE_WAIT);
+        return mbar_wait_warp(bar, parity, p.rounds, &stop, p.error_word, DEV_ERR_TILE_WAIT);
     };
 
     // For the end of every warp: once all are past their last wait `stop` changes
@@ -240,7 +242,7 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
         uint32_t phase = 0, ob_phase = 0;
         int issued = 0, owns = 0;  // of the last ring, for a stop
         bool ok = true;
-        for (int u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
+        for (int u = blockIdx.x; ok && u < p.copied; u += gridDim.x) {
             const FusedWalk w = fused_unit(p, u);
             ok = wait_warp(own_empty + 8 * ob, ob_phase ^ 1);
             if (!ok) break;
@@ -413,7 +415,8 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
         }
     } else if (warp >= 4 && warp < 4 + 4 * kGroups) {
         // Scores to G: group g takes every kGroups-th tile. After a wait that
-        // gave up the rest fail at once and the block runs out on what is there.
+        // gave up the rest fail at once and the block runs out on what is there,
+        // storing NaN (`stop`).
         const int g = (warp - 4) / 4, quarter = warp & 3, in_tile = quarter * 32 + lane;
         const uint32_t group = tmem + ((uint32_t)(quarter * 32) << 16) + g * kGroupColumns<PARTS>;
         const float c2 = p.scale * kLog2e;
@@ -503,7 +506,7 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
                 phase ^= 1;
             }
             if (BY_CLASS && p.part_bias != nullptr && own < p.own)
-                p.part_bias[(int64_t)(w.split * kGroups + g) * p.own + own] = bias_sum;
+                p.part_bias[(int64_t)(w.split * kGroups + g) * p.own + own] = stop ? kNaN : bias_sum;
         }
     } else if (warp != 3) {
         // acc: quarter of the rows, and every other 32 channels
@@ -602,6 +605,12 @@ fused_kernel(const __grid_constant__ FusedArgs p, const __grid_constant__ CUtens
                     const int c = (2 * q + half) * 32;
                     if (c < n) write(kept[q], c, false);
                 }
+            }
+            if (stop && own < p.own) {
+                if (p.part != nullptr)
+                    store_nan(p.part + ((int64_t)w.split * p.own + own) * p.part_ld, p.part_ld);
+                else
+                    store_nan(static_cast<TypeOf<PARTS>*>(p.out) + (int64_t)own * p.channels, p.channels);
             }
         }
     }

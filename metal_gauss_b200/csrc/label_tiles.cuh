@@ -56,6 +56,8 @@ struct Shape {
 
 struct TileArgs {           // counts below 2^31: at most 2^30 rows
     int units;
+    int copied;             // units whose tiles are copied in: all, but for the self-test
+    int rounds;             // of the issuing and copying warps' waits, at most
     int a_rows;             // rows of the A side (of the piece, or classes)
     int depth;              // contraction entries
     int columns;            // columns of the B side in all (classes, or channels)
@@ -220,7 +222,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                     tma_load(base + (c * PARTS + i) * S::kB, &map_b, c % chunks * S::kChunk, c / chunks * kN, i,
                              resident_full, on);
         }
-        for (int u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
+        for (int u = blockIdx.x; ok && u < p.copied; u += gridDim.x) {
             const Walk w = walk_unit<MODE, PARTS>(p, u);
             for (int t = 0; ok && t < w.tiles; ++t) {
                 const int b0 = (S::kProduct ? w.first : w.first + t) * kN;
@@ -234,7 +236,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                 for (int i = 0; i < passes * (c1 - c0); ++i) {
                     const bool again = i >= c1 - c0;  // the first part alone
                     const int c = again ? i - (c1 - c0) + c0 : i + c0;
-                    ok = mbar_wait_warp(empty + 8 * stage, phase ^ 1, &stop, p.error_word, DEV_ERR_TILE_WAIT);
+                    ok = mbar_wait_warp(empty + 8 * stage, phase ^ 1, p.rounds, &stop, p.error_word, DEV_ERR_TILE_WAIT);
                     if (!ok) break;
                     const uint32_t bar = full + 8 * stage;
                     mbar_expect(bar, again ? S::kA + (resident > 0 ? 0 : S::kB) : bytes, on);
@@ -286,7 +288,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
         const uint32_t on = elect_lane();
         int stage = 0, buf = 0;
         uint32_t phase = 0, buf_phase = 0;
-        bool ok = resident == 0 || mbar_wait_warp(resident_full, 0, &stop, p.error_word, DEV_ERR_TILE_WAIT);
+        bool ok = resident == 0 || mbar_wait_warp(resident_full, 0, p.rounds, &stop, p.error_word, DEV_ERR_TILE_WAIT);
         for (int u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
             const Walk w = walk_unit<MODE, PARTS>(p, u);
             for (int t = 0; ok && t < w.tiles; ++t) {
@@ -301,13 +303,13 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                 const int chunks = (int)uniform((uint32_t)(c1 - c0));
                 // 16-entry steps of the last chunk
                 const int tail = (int)uniform((uint32_t)min(S::kChunk / 16, (p.depth - (c1 - 1) * S::kChunk + 15) / 16));
-                ok = mbar_wait_warp(taken_empty + 8 * buf, buf_phase ^ 1, &stop, p.error_word, DEV_ERR_TILE_WAIT);
+                ok = mbar_wait_warp(taken_empty + 8 * buf, buf_phase ^ 1, p.rounds, &stop, p.error_word, DEV_ERR_TILE_WAIT);
                 if (!ok) break;
                 tmem_fence_after();
                 const uint32_t d = uniform(tmem + buf * kN);
                 const int passes = S::kTwice && chunks > 1 ? 2 : 1;
                 for (int v = 0; v < passes * chunks; ++v) {
-                    ok = mbar_wait_warp(full + 8 * stage, phase, &stop, p.error_word, DEV_ERR_TILE_WAIT);
+                    ok = mbar_wait_warp(full + 8 * stage, phase, p.rounds, &stop, p.error_word, DEV_ERR_TILE_WAIT);
                     if (!ok) break;
                     tmem_fence_after();
                     const int c = v < chunks ? v : v - chunks;
@@ -353,7 +355,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
         // Takes tiles out: warp % 4 is the quarter of the rows it can reach,
         // `set` the 32-column chunks it takes (every kSets-th). After a wait
         // that gave up the remaining waits fail at once and the block runs to
-        // its end on whatever is there; the error word says so.
+        // its end on whatever is there, storing NaN (`stop`).
         const int quarter = warp & 3, set = (warp - 2) / 4;
         const int in_tile = quarter * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
@@ -378,7 +380,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                     const int n = min(kN, p.columns - v0);
                     if (t + 1 == w.tiles && u + (int)gridDim.x < p.units)  // while this tile is taken
                         next_row = row_in<MODE>(p, walk_unit<MODE, PARTS>(p, u + (int)gridDim.x).a_row + in_tile);
-                    mbar_wait(taken_full + 8 * buf, buf_phase, &stop, p.error_word, DEV_ERR_TILE_WAIT);
+                    mbar_wait(taken_full + 8 * buf, buf_phase, kMbarRounds, &stop, p.error_word, DEV_ERR_TILE_WAIT);
                     tmem_fence_after();
                     for (int k = set; k * 32 < n; k += S::kSets) {
                         const uint32_t at = lanes + buf * kN + k * 32;
@@ -447,6 +449,10 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                                     for (int j = 0; j < 16; ++j)
                                         if (j == rel - h) z[j] = at_label;
                                 }
+                                if (stop) {
+#pragma unroll
+                                    for (int j = 0; j < 16; ++j) z[j] = kNaN;
+                                }
                                 if (p.part_bias != nullptr) {
                                     // lanes c and c + 16 end with the sums of column c over
                                     // half of the warp's 32 rows each
@@ -506,7 +512,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                 if (MODE == kStats && mine) {
                     const int64_t at = (int64_t)(w.split * S::kSets + set) * p.rows + row;
                     p.part_m[at] = m;
-                    p.part_s[at] = s;
+                    p.part_s[at] = stop ? kNaN : s;
                 }
             } else {
                 const int d0 = w.first * kN;
@@ -517,7 +523,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
 #pragma unroll
                     for (int j = 0; j < 32; ++j) acc[q][j] = 0.0f;
                 for (int t = 0; t < w.tiles; ++t) {
-                    mbar_wait(taken_full + 8 * buf, buf_phase, &stop, p.error_word, DEV_ERR_TILE_WAIT);
+                    mbar_wait(taken_full + 8 * buf, buf_phase, kMbarRounds, &stop, p.error_word, DEV_ERR_TILE_WAIT);
                     tmem_fence_after();
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
@@ -569,6 +575,12 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                                 store_row<T, kVec>(dst + j, o);
                             }
                         }
+                    }
+                    if (stop) {
+                        if (p.part != nullptr)
+                            store_nan(p.part + ((int64_t)w.split * p.a_rows + a_row) * p.part_ld + d0, min(n, p.part_ld - d0));
+                        else
+                            store_nan(static_cast<TypeOf<PARTS>*>(p.out) + (p.row0 + a_row) * p.columns + d0, n);
                     }
                 }
             }

@@ -395,6 +395,12 @@ struct BackwardScratch {
     }
 };
 
+// What the tile kernels' waits are held to.
+struct Waits {
+    int rounds = kMbarRounds;
+    int units = INT32_MAX;  // that are copied in; the self-test starves the others
+};
+
 struct Args {
     const void *x, *w;
     int dtype;
@@ -403,11 +409,12 @@ struct Args {
     Sizes n;
     float scale;
     cudaStream_t st;
+    Waits waits = {};
 };
 
 template <int MODE, int PARTS>
-mg_status launch_tiles(const TileArgs& p, const CUtensorMap& a, const CUtensorMap& b,
-                       const CUtensorMap& out, cudaStream_t st, const char* what) {
+mg_status launch_tiles(TileArgs& p, const CUtensorMap& a, const CUtensorMap& b,
+                       const CUtensorMap& out, const Args& args, const char* what) {
     constexpr int bytes = Shape<MODE, PARTS>::kDynamic;
     static bool ready[64] = {};
     int dev = 0;
@@ -419,7 +426,9 @@ mg_status launch_tiles(const TileArgs& p, const CUtensorMap& a, const CUtensorMa
         ready[dev] = true;
     }
     const int grid = std::min(p.units, sm_count());
-    tile_kernel<MODE, PARTS><<<grid, Shape<MODE, PARTS>::kThreads, bytes, st>>>(p, a, b, out);
+    p.copied = std::min(p.units, args.waits.units);
+    p.rounds = args.waits.rounds;
+    tile_kernel<MODE, PARTS><<<grid, Shape<MODE, PARTS>::kThreads, bytes, args.st>>>(p, a, b, out);
     return check_launch(what);
 }
 
@@ -480,7 +489,7 @@ mg_status forward(const Args& a, int reduction, float* loss, float* stats, float
         p.resident = (int)chunks;
         p.resident_stages = (int)std::min<int64_t>(S::kBars, room / (PARTS * S::kA));
     }
-    MG_TRY((launch_tiles<kStats, PARTS>(p, mx, mw, mw, a.st, "label_loss_forward")));
+    MG_TRY((launch_tiles<kStats, PARTS>(p, mx, mw, mw, a, "label_loss_forward")));
     const int shares = sh.splits * S::kSets, mean = reduction == MG_REDUCE_MEAN;
     const bool none = reduction == MG_REDUCE_NONE, single = a.n.row_blocks() == 1;
     const auto rows_kernel = a.n.wide_rows() ? label_rows_kernel<32> : label_rows_kernel<1>;
@@ -510,7 +519,7 @@ mg_status column_sum(const float* in, int64_t lines, int64_t per_block, int colu
 
 template <bool BY_CLASS, int PARTS>
 mg_status launch_fused(FusedArgs& p, const Sizes& n, const CUtensorMap& own,
-                       const CUtensorMap& stream, cudaStream_t st, const char* what) {
+                       const CUtensorMap& stream, const Args& args, const char* what) {
     static bool ready[64] = {};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
@@ -528,7 +537,9 @@ mg_status launch_fused(FusedArgs& p, const Sizes& n, const CUtensorMap& own,
     }
     fused_buffers(p, PARTS);
     const int grid = std::min(p.units, sm_count());
-    fused_kernel<BY_CLASS, PARTS><<<grid, kFusedThreads, kFusedShared, st>>>(p, own, stream);
+    p.copied = std::min(p.units, args.waits.units);
+    p.rounds = args.waits.rounds;
+    fused_kernel<BY_CLASS, PARTS><<<grid, kFusedThreads, kFusedShared, args.st>>>(p, own, stream);
     return check_launch(what);
 }
 
@@ -564,7 +575,7 @@ mg_status backward_fused(const Args& a, const RowGrad& rg, const float* stats, T
         p.per_split = (int)sh.per_split;
         p.part = n.fused_direct() ? nullptr : f.row_part;
         p.out = dx;
-        MG_TRY((launch_fused<false, PARTS>(p, n, own, stream, a.st, "label_loss_backward rows")));
+        MG_TRY((launch_fused<false, PARTS>(p, n, own, stream, a, "label_loss_backward rows")));
         if (!n.fused_direct())
             MG_TRY(join(f.row_part, sh.splits, n.rows, n.part_ld(), n.channels, a.scale, dx, a.st));
     }
@@ -579,7 +590,7 @@ mg_status backward_fused(const Args& a, const RowGrad& rg, const float* stats, T
         p.per_split = (int)sh.per_split;
         p.part = f.class_part;
         p.part_bias = db != nullptr ? f.bias_part : nullptr;
-        MG_TRY((launch_fused<true, PARTS>(p, n, own, stream, a.st, "label_loss_backward classes")));
+        MG_TRY((launch_fused<true, PARTS>(p, n, own, stream, a, "label_loss_backward classes")));
         if (dw != nullptr)
             MG_TRY(join(f.class_part, sh.splits, n.classes, n.part_ld(), n.channels, a.scale, dw, a.st));
         if (db != nullptr)
@@ -620,7 +631,7 @@ mg_status backward(const Args& a, const RowGrad& rg, const float* stats, T* dx, 
         p.row_values = f.row_values;
         p.part_bias = db != nullptr ? f.bias_part : nullptr;
         p.error_word = device_error_word();
-        MG_TRY((launch_tiles<kLogitGrad, PARTS>(p, mx, mw_score, mg_out, a.st, "label_loss_backward logits")));
+        MG_TRY((launch_tiles<kLogitGrad, PARTS>(p, mx, mw_score, mg_out, a, "label_loss_backward logits")));
         if (db != nullptr) {
             float* sums = f.bias_part2 + row0 / n.piece() * n.bias_shares(n.piece()) * n.classes;
             MG_TRY(column_sum(f.bias_part, up(rows, kM) * 4, kBiasLines, n.classes,
@@ -641,7 +652,7 @@ mg_status backward(const Args& a, const RowGrad& rg, const float* stats, T* dx, 
             p.part = n.direct() ? nullptr : f.row_part;
             p.part_ld = n.part_ld();
             p.out = dx;
-            MG_TRY((launch_tiles<kProductRow, PARTS>(p, mg_in, mw_prod, mw_prod, a.st, "label_loss_backward rows")));
+            MG_TRY((launch_tiles<kProductRow, PARTS>(p, mg_in, mw_prod, mw_prod, a, "label_loss_backward rows")));
             if (!n.direct())
                 MG_TRY(join(f.row_part, sh.splits, rows, n.part_ld(), n.channels, a.scale,
                             dx + row0 * n.channels, a.st));
@@ -662,7 +673,7 @@ mg_status backward(const Args& a, const RowGrad& rg, const float* stats, T* dx, 
             p.add = row0 > 0;
             p.row0 = 0;
             p.out = dw;
-            MG_TRY((launch_tiles<kProductClass, PARTS>(p, mg_in, mx_prod, mx_prod, a.st, "label_loss_backward classes")));
+            MG_TRY((launch_tiles<kProductClass, PARTS>(p, mg_in, mx_prod, mx_prod, a, "label_loss_backward classes")));
         }
     }
     if (dw != nullptr && !n.class_direct())
@@ -735,6 +746,25 @@ extern "C" size_t mg_label_loss_scratch_bytes(int64_t rows, int64_t channels, in
     return backward ? BackwardScratch(nullptr, n).bytes : ForwardScratch(nullptr, n).bytes;
 }
 
+namespace {
+
+mg_status run_forward(const Args& a, int reduction, float* loss, float* stats, float* live, void* scratch) {
+    if (a.dtype == MG_F32) return forward<float>(a, reduction, loss, stats, live, scratch);
+    if (a.dtype == MG_BF16) return forward<__nv_bfloat16>(a, reduction, loss, stats, live, scratch);
+    return forward<__half>(a, reduction, loss, stats, live, scratch);
+}
+
+mg_status run_backward(const Args& a, const RowGrad& rg, const float* stats, void* dx, void* dw, float* db,
+                       void* scratch) {
+    if (a.dtype == MG_F32)
+        return backward(a, rg, stats, static_cast<float*>(dx), static_cast<float*>(dw), db, scratch);
+    if (a.dtype == MG_BF16)
+        return backward(a, rg, stats, static_cast<__nv_bfloat16*>(dx), static_cast<__nv_bfloat16*>(dw), db, scratch);
+    return backward(a, rg, stats, static_cast<__half*>(dx), static_cast<__half*>(dw), db, scratch);
+}
+
+}  // namespace
+
 extern "C" mg_status mg_label_loss_forward(const void* features, const void* classes, int32_t dtype,
                                            const float* class_bias, const void* labels,
                                            int32_t label_bytes, int64_t ignore_index, int64_t rows,
@@ -761,9 +791,7 @@ extern "C" mg_status mg_label_loss_forward(const void* features, const void* cla
     const Args a{features, classes, dtype, class_bias,
                  LabelSource{labels, label_bytes, ignore_index, (int)n_classes},
                  Sizes{rows, (int)channels, (int)n_classes, parts_of_dtype(dtype)}, scale, st};
-    if (dtype == MG_F32) return forward<float>(a, reduction, loss, stats, live, scratch);
-    if (dtype == MG_BF16) return forward<__nv_bfloat16>(a, reduction, loss, stats, live, scratch);
-    return forward<__half>(a, reduction, loss, stats, live, scratch);
+    return run_forward(a, reduction, loss, stats, live, scratch);
 } catch (...) {
     return caught("label_loss_forward");
 }
@@ -798,12 +826,34 @@ extern "C" mg_status mg_label_loss_backward(
                  Sizes{rows, (int)channels, (int)n_classes, parts_of_dtype(dtype)}, scale, st};
     const RowGrad rg{grad_loss, reduction == MG_REDUCE_MEAN ? live : nullptr,
                      reduction == MG_REDUCE_NONE};
-    if (dtype == MG_F32)
-        return backward(a, rg, stats, static_cast<float*>(d_features), static_cast<float*>(d_classes), d_bias, scratch);
-    if (dtype == MG_BF16)
-        return backward(a, rg, stats, static_cast<__nv_bfloat16*>(d_features),
-                        static_cast<__nv_bfloat16*>(d_classes), d_bias, scratch);
-    return backward(a, rg, stats, static_cast<__half*>(d_features), static_cast<__half*>(d_classes), d_bias, scratch);
+    return run_backward(a, rg, stats, d_features, d_classes, d_bias, scratch);
 } catch (...) {
     return caught("label_loss_backward");
+}
+
+extern "C" mg_status mg_label_loss_wait_selftest(
+    int32_t rounds, int32_t units, const void* features, const void* classes, int32_t dtype,
+    const int64_t* labels, int64_t rows, int64_t channels, int64_t n_classes, float* loss,
+    float* stats, const float* grad_loss, void* d_features, void* d_classes, float* d_bias,
+    void* scratch, size_t scratch_bytes, mg_stream_t stream) try {
+    const bool back = grad_loss != nullptr;
+    MG_TRY(check_args("label_loss_wait_selftest", features, classes, dtype, labels, 8, rows, channels,
+                      n_classes, MG_REDUCE_NONE));
+    MG_REQUIRE(rounds >= 1 && rounds <= 1 << 12, "label_loss_wait_selftest: rounds must be 1..4096");
+    MG_REQUIRE(units >= 0, "label_loss_wait_selftest: units must not be negative");
+    MG_REQUIRE(rows >= 1 && rows <= 1 << 20, "label_loss_wait_selftest: rows must be 1..2^20");
+    MG_REQUIRE(stats && (back ? d_features && d_classes && d_bias : loss != nullptr),
+               "label_loss_wait_selftest: null pointer");
+    MG_REQUIRE(aligned16(d_features) && aligned16(d_classes),
+               "label_loss_wait_selftest: d_features and d_classes must be 16-byte aligned");
+    MG_REQUIRE(scratch != nullptr && (reinterpret_cast<uintptr_t>(scratch) & 255u) == 0u &&
+                   scratch_bytes >= mg_label_loss_scratch_bytes(rows, channels, n_classes, dtype, back),
+               "label_loss_wait_selftest: scratch too small or not 256-byte aligned");
+    const Args a{features, classes, dtype, nullptr, LabelSource{labels, 8, -100, (int)n_classes},
+                 Sizes{rows, (int)channels, (int)n_classes, parts_of_dtype(dtype)}, 1.0f,
+                 reinterpret_cast<cudaStream_t>(stream), Waits{rounds, units}};
+    if (!back) return run_forward(a, MG_REDUCE_NONE, loss, stats, nullptr, scratch);
+    return run_backward(a, RowGrad{grad_loss, nullptr, 1}, stats, d_features, d_classes, d_bias, scratch);
+} catch (...) {
+    return caught("label_loss_wait_selftest");
 }

@@ -48,6 +48,7 @@ constexpr int kRowBlock = 64;
 constexpr int kClassPad = 256;  // class_bias is padded to a multiple of this
 
 constexpr float kInf = __builtin_huge_valf();
+constexpr float kNaN = __builtin_nanf("");
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -155,6 +156,13 @@ __device__ constexpr int g_pair_a(int i) {
 template <int PARTS>
 __device__ constexpr int g_pair_b(int i) {
     return PARTS == 1 ? 0 : pair_b<PARTS>(kGPairs<PARTS>, i);
+}
+
+// What a wait that gave up leaves of n results.
+template <typename T>
+__device__ __forceinline__ void store_nan(T* dst, int n) {
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) dst[i] = from_f32<T>(kNaN);
 }
 
 // The features' type, by its parts.

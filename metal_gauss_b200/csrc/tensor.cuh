@@ -54,25 +54,30 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
     return ok != 0;
 }
 
-// Every wait ends: after kMbarRounds rounds it gives up, records `code` in the
-// device error word and raises the block's stop flag, which ends the block's
-// other waits too. A round is one try_wait, which the hardware may suspend.
+// Every wait ends: after `rounds` rounds (kMbarRounds outside the self-test, some
+// 4 s at the 3.7 us that one takes when nothing arrives) it gives up, records
+// `code` in the device error word and raises the block's stop flag, which ends
+// the block's other waits too. A round is one try_wait, which the hardware may
+// suspend. Nothing that is not valid is read before the flag is up, so who stores
+// results looks at it after the last read: NaN if it is.
 constexpr int kMbarRounds = 1 << 20;
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* stop,
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int rounds, volatile int* stop,
                                           int32_t* error_word, int32_t code) {
-    for (int i = 0; i < kMbarRounds; ++i) {
-        if (mbar_try(bar, parity)) return true;
+    if (mbar_try(bar, parity)) return true;
+    for (int i = 1; i < rounds; ++i) {
         if (*stop) return false;
+        if (mbar_try(bar, parity)) return true;
     }
+    if (*stop) return false;
     *stop = 1;
     record_device_error(error_word, code);
     return false;
 }
 
 // The same for a whole warp, which agrees on the answer (and stays in step).
-__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* stop,
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, int rounds, volatile int* stop,
                                                int32_t* error_word, int32_t code) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, stop, error_word, code));
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, rounds, stop, error_word, code));
 }
 
 // ------------------------------------------------------------------------ TMA
