@@ -156,7 +156,8 @@ label_rows_kernel(const float* __restrict__ part_m, const float* __restrict__ pa
             const float z = label_z[row];
             // all in base 2; others = sum over the other classes of exp2(z_v - top)
             const float top = fmaxf(m, z);
-            if (top == -kInf || z != z || s != s) {
+            // no finite logit, an infinite one (inf - inf) or a NaN
+            if (fabsf(top) == kInf || z != z || s != s) {
                 lse = loss = miss = __int_as_float(0x7fc00000);
             } else {
                 const float others = m == -kInf ? 0.0f : s * exp2f(m - top);

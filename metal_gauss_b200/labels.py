@@ -96,7 +96,8 @@ def label_loss(features: torch.Tensor, classes: torch.Tensor, labels: torch.Tens
     a class out. Pixels labelled ignore_index have loss 0 and
     no gradient whatever their features hold, and do not count in a mean. The
     result is float32: one value for reduction "mean" (0 when no pixel takes
-    part) or "sum", labels' shape for "none". Another label outside
+    part) or "sum", labels' shape for "none". A row with an infinite logit has
+    loss NaN; logits have to stay within float32's range. Another label outside
     [0, n_classes) makes the loss NaN and is recorded in the device error word
     (`_lib.check_device_error`)."""
     dtype_code(features, "label_loss: features")

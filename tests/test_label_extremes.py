@@ -1,0 +1,33 @@
+"""label_loss at the ends of the floating range."""
+
+import math
+
+import pytest
+import torch
+
+from metal_gauss_b200.labels import label_loss
+from test_features import BF16, F32, label_case
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("v", [1, 40, 300])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_an_infinite_logit_gives_nan(cuda, dtype, v):
+    """log sum exp(z) - z[label] is infinity - infinity where the label's logit
+    is infinite: a NaN loss and gradient, as for another class's."""
+    x, w, lab, bias, _ = label_case(50 + v, 60, 24, v, dtype, share=0.0)
+    bias[0] = math.inf
+    xl = x.clone().requires_grad_(True)
+    rows = label_loss(xl, w, lab, bias=bias, reduction="none")
+    (gx,) = torch.autograd.grad(rows, xl, torch.ones_like(rows))
+    assert rows.isnan().all() and gx.isnan().all()
+    # by a product that overflows, in its own row alone
+    x, w, lab, bias, _ = label_case(51 + v, 60, 24, v, BF16, share=0.0)
+    clean = label_loss(x, w, lab, bias=bias, reduction="none")
+    w[:, 0] = 0.0
+    w[lab[7], 0] = 3e38
+    x[:, 0], x[7, 0] = 0.0, 3e38
+    rows = label_loss(x, w, lab, bias=bias, reduction="none")
+    keep = torch.arange(60, device=cuda) != 7
+    assert rows[7].isnan() and rows[keep].isfinite().all() and clean.isfinite().all()
