@@ -98,9 +98,12 @@ constexpr int kPartsOf = sizeof(T) == 4 ? 3 : 2;
 template <>
 constexpr int kPartsOf<__nv_bfloat16> = 1;
 
+// An fp32 value past bf16's largest (by less than half a step of it, the type's
+// lowest among them) takes that as its first part; rounded, it would be infinite.
 template <int PARTS>
 __device__ __forceinline__ void split_parts(float v, __nv_bfloat16 (&p)[PARTS]) {
-    p[0] = __float2bfloat16_rn(v);
+    constexpr float kMost = 3.38953138925153547e38f;
+    p[0] = __float2bfloat16_rn(PARTS == 3 && fabsf(v) < kInf ? fminf(fmaxf(v, -kMost), kMost) : v);
 #pragma unroll
     for (int i = 1; i < PARTS; ++i) {
         v -= __bfloat162float(p[i - 1]);

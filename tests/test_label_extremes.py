@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from metal_gauss_b200.labels import label_loss
-from test_features import BF16, F32, label_case
+from test_features import BF16, F16, F32, check_label, label_case
 
 pytestmark = pytest.mark.gpu
 
@@ -31,3 +31,18 @@ def test_an_infinite_logit_gives_nan(cuda, dtype, v):
     rows = label_loss(x, w, lab, bias=bias, reduction="none")
     keep = torch.arange(60, device=cuda) != 7
     assert rows[7].isnan() and rows[keep].isfinite().all() and clean.isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("n,d,v", [(70, 24, 50), (60, 150, 70), (40, 300, 50)])
+def test_the_types_ends_where_the_other_side_is_zero(cuda, n, d, v, dtype):
+    """The largest and the lowest finite value in an embedding or a feature
+    whose partner is 0: products of 0, and gradients that large."""
+    ends = torch.finfo(dtype)
+    x, w, lab, bias, _ = label_case(n + d + v, n, d, v, dtype)
+    x[:, 0] = 0.0
+    w[3, 0], w[5, 0] = ends.min, ends.max
+    w[:, d - 1] = 0.0
+    live = (lab != -100).nonzero()[:, 0]
+    x[live[2], d - 1], x[live[4], d - 1] = ends.max, ends.min
+    check_label(x, w, lab, bias)
