@@ -710,7 +710,8 @@ mg_status mg_mcmc_add_noise(float* means, const float* quats, const float* log_s
 /* Operators on rows of per-pixel features (no reference counterpart)       */
 /* ------------------------------------------------------------------------ */
 
-/* Element types of the entry points below. */
+/* Element types of the entry points below. An address off its element's
+ * boundary is refused. */
 #define MG_F32 0
 #define MG_BF16 1
 #define MG_F16 2

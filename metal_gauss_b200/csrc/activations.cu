@@ -277,6 +277,8 @@ extern "C" mg_status mg_pack8(const void* x, int32_t dtype, int64_t rows, int64_
     MG_TRY(check_sizes(dtype, rows, channels, codes, "pack8"));
     if (rows == 0) return MG_OK;
     MG_REQUIRE(x && codes && scales, "pack8: null pointer");
+    MG_REQUIRE(on_boundary(elem_bytes(dtype), {x}) && on_boundary(4, {scales}),
+               "pack8: a pointer off its element's boundary");
     const Pack op{x, rows, (int)channels, codes, scales, reinterpret_cast<cudaStream_t>(stream)};
     if (dtype == MG_F32) return pack<float, 4>(op);
     if (dtype == MG_BF16) return pack<__nv_bfloat16, 8>(op);
@@ -290,6 +292,8 @@ extern "C" mg_status mg_unpack8(const int8_t* codes, const float* scales, int64_
     MG_TRY(check_sizes(dtype, rows, channels, codes, "unpack8"));
     if (rows == 0) return MG_OK;
     MG_REQUIRE(x && codes && scales, "unpack8: null pointer");
+    MG_REQUIRE(on_boundary(elem_bytes(dtype), {x}) && on_boundary(4, {scales}),
+               "unpack8: a pointer off its element's boundary");
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (dtype == MG_F32) return unpack(codes, scales, rows, (int)channels, static_cast<float*>(x), st);
     if (dtype == MG_BF16) return unpack(codes, scales, rows, (int)channels, static_cast<__nv_bfloat16*>(x), st);

@@ -789,6 +789,9 @@ extern "C" mg_status mg_label_loss_forward(const void* features, const void* cla
                    scratch_bytes >=
                        mg_label_loss_scratch_bytes(rows, channels, n_classes, dtype, 0),
                "label_loss_forward: scratch too small or not 256-byte aligned");
+    MG_REQUIRE(on_boundary(elem_bytes(dtype), {features, classes}) && on_boundary(label_bytes, {labels}) &&
+                   on_boundary(4, {class_bias, loss, stats, live}),
+               "label_loss_forward: a pointer off its element's boundary");
     const Args a{features, classes, dtype, class_bias,
                  LabelSource{labels, label_bytes, ignore_index, (int)n_classes},
                  Sizes{rows, (int)channels, (int)n_classes, parts_of_dtype(dtype)}, scale, st};
@@ -822,6 +825,9 @@ extern "C" mg_status mg_label_loss_backward(
                    scratch_bytes >=
                        mg_label_loss_scratch_bytes(rows, channels, n_classes, dtype, 1),
                "label_loss_backward: scratch too small or not 256-byte aligned");
+    MG_REQUIRE(on_boundary(elem_bytes(dtype), {features, classes}) && on_boundary(label_bytes, {labels}) &&
+                   on_boundary(4, {class_bias, grad_loss, stats, live, d_bias}),
+               "label_loss_backward: a pointer off its element's boundary");
     const Args a{features, classes, dtype, class_bias,
                  LabelSource{labels, label_bytes, ignore_index, (int)n_classes},
                  Sizes{rows, (int)channels, (int)n_classes, parts_of_dtype(dtype)}, scale, st};
@@ -850,6 +856,9 @@ extern "C" mg_status mg_label_loss_wait_selftest(
     MG_REQUIRE(scratch != nullptr && (reinterpret_cast<uintptr_t>(scratch) & 255u) == 0u &&
                    scratch_bytes >= mg_label_loss_scratch_bytes(rows, channels, n_classes, dtype, back),
                "label_loss_wait_selftest: scratch too small or not 256-byte aligned");
+    MG_REQUIRE(on_boundary(elem_bytes(dtype), {features, classes}) && on_boundary(8, {labels}) &&
+                   on_boundary(4, {loss, stats, grad_loss, d_bias}),
+               "label_loss_wait_selftest: a pointer off its element's boundary");
     const Args a{features, classes, dtype, nullptr, LabelSource{labels, 8, -100, (int)n_classes},
                  Sizes{rows, (int)channels, (int)n_classes, parts_of_dtype(dtype)}, 1.0f,
                  reinterpret_cast<cudaStream_t>(stream), Waits{rounds, units}};

@@ -894,6 +894,9 @@ extern "C" mg_status mg_layer_norm_forward(const void* x, int32_t dtype, const v
     MG_REQUIRE(x && y, "layer_norm_forward: null pointer");
     MG_REQUIRE(codes == nullptr || (reinterpret_cast<uintptr_t>(codes) & 7u) == 0u,
                "layer_norm_forward: codes must be 8-byte aligned");
+    MG_REQUIRE(on_boundary(elem_bytes(dtype), {x, y}) && on_boundary(elem_bytes(param_dtype), {weight, bias}) &&
+                   on_boundary(4, {mean, rstd, scales}),
+               "layer_norm_forward: a pointer off its element's boundary");
     const Forward op{x, weight, bias, param_dtype, rows, (int)channels, eps, y, mean, rstd,
                      codes, scales, reinterpret_cast<cudaStream_t>(stream)};
     return pick_type(op, dtype, (int)channels, aligned16(x) && aligned16(y));
@@ -934,6 +937,9 @@ extern "C" mg_status mg_layer_norm_backward(const void* dy, const void* x, const
     MG_REQUIRE(dy && mean && rstd, "layer_norm_backward: null pointer");
     MG_REQUIRE(codes == nullptr || (reinterpret_cast<uintptr_t>(codes) & 7u) == 0u,
                "layer_norm_backward: codes must be 8-byte aligned");
+    MG_REQUIRE(on_boundary(elem_bytes(dtype), {dy, x, dx}) && on_boundary(4, {mean, rstd, scales, scratch}) &&
+                   on_boundary(elem_bytes(param_dtype), {weight, dweight, dbias}),
+               "layer_norm_backward: a pointer off its element's boundary");
     MG_REQUIRE(!params || (scratch != nullptr &&
                            scratch_bytes >= mg_layer_norm_backward_scratch_bytes(rows, channels)),
                "layer_norm_backward: scratch too small");

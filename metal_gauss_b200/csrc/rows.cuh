@@ -6,6 +6,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <initializer_list>
+
 #include "common.cuh"
 
 namespace mg {
@@ -287,6 +289,16 @@ __device__ __forceinline__ void staged_codes(const T* rows, int n, int channels,
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0u; }
+
+inline int elem_bytes(int32_t dtype) { return dtype == MG_F32 ? 4 : 2; }
+
+// Whether all of these are on a boundary of `bytes` (NULL is). An address off its
+// element's boundary would fault on the device.
+inline bool on_boundary(int bytes, std::initializer_list<const void*> pointers) {
+    uintptr_t all = 0;
+    for (const void* p : pointers) all |= reinterpret_cast<uintptr_t>(p);
+    return all % (uintptr_t)bytes == 0;
+}
 
 // SMs of the current device (cached per device).
 int sm_count();
