@@ -38,9 +38,8 @@ struct Shape {
     static constexpr int kPartsG = kGParts<PARTS>;
     static constexpr int kStage = kPartsA * kA + PARTS * kB;
     static constexpr int kStages = PARTS == 3 ? (MODE == kLogitGrad ? 2 : 3) : (MODE == kStats ? 4 : 3);
-    // G on its way out: 128 x 32 bf16 for each set of the taking warps, part and buffer
-    static constexpr int kOutBuffers = 1;
-    static constexpr int kOut = MODE == kLogitGrad ? kSets * kPartsG * kOutBuffers * kM * 64 : 0;
+    // G on its way out: 128 x 32 bf16 for each set of the taking warps and part
+    static constexpr int kOut = MODE == kLogitGrad ? kSets * kPartsG * kM * 64 : 0;
     static constexpr int kDynamic = 1024 + kStages * kStage + kOut;
     // Scores of more than one chunk go over them twice: the small products of all
     // of them, then the large one (with its parts fetched again). The tensor
@@ -361,7 +360,7 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
         const bool speaks = quarter == 0 && lane == 0;  // for its set's stores
         const float c2 = p.scale * kLog2e;
-        int buf = 0, out_buf = 0;
+        int buf = 0;
         uint32_t buf_phase = 0;
         RowIn next_row;
         if constexpr (!S::kProduct)
@@ -426,9 +425,8 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                             m = top;
                         } else {
                             // staging is free again once the store before has read it
-                            const uint32_t stage0 = base + S::kStages * S::kStage +
-                                                    (set * S::kOutBuffers + out_buf) * (S::kPartsG * kM * 64);
-                            if (speaks) tma_store_wait_read<S::kOutBuffers - 1>();
+                            const uint32_t stage0 = base + S::kStages * S::kStage + set * (S::kPartsG * kM * 64);
+                            if (speaks) tma_store_wait_read();
                             named_sync(2 + set, 128);
                             // 16 columns at a time, the loop not unrolled: its code
                             // has to stay in the instruction cache
@@ -500,7 +498,6 @@ tile_kernel(const __grid_constant__ TileArgs p, const __grid_constant__ CUtensor
                                     tma_store(&map_out, v0 + k * 32, w.a_row, i, stage0 + i * kM * 64);
                                 tma_store_commit();
                             }
-                            if (++out_buf == S::kOutBuffers) out_buf = 0;
                         }
                     }
                     tmem_fence_before();

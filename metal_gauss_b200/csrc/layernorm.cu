@@ -551,10 +551,6 @@ norm_backward_staged_kernel(const T* __restrict__ dy, const T* __restrict__ x,
     };
     const int lane = threadIdx.x % LPR, team = threadIdx.x / LPR;
     constexpr int kTeams = kThreads / LPR;
-    // columns: fewer than the threads leave several row groups to each column
-    const int groups = channels < kThreads ? kThreads / channels : 1;
-    const int group = channels < kThreads ? (int)threadIdx.x / channels : 0;
-    const int column = channels < kThreads ? (int)threadIdx.x % channels : (int)threadIdx.x;
     float dw[kColumns] = {}, db[kColumns] = {};
     int q = 0;
     if (blockIdx.x < chunks) fetch(blockIdx.x, 0);
@@ -578,12 +574,13 @@ norm_backward_staged_kernel(const T* __restrict__ dy, const T* __restrict__ x,
             else v = to_f32<T>(h[r * channels + c]);
             return (v - st.x) * st.y;
         };
-        if (partial != nullptr && group < groups) {
-            for (int r = group; r < n; r += groups) {
+        if (partial != nullptr) {
+#pragma unroll 4
+            for (int r = 0; r < n; ++r) {
                 const float2 st = stat[r];
 #pragma unroll
                 for (int k = 0; k < kColumns; ++k) {
-                    const int c = column + k * kThreads;
+                    const int c = threadIdx.x + k * kThreads;
                     if (c < channels) {
                         const float d = to_f32<T>(g[r * channels + c]);
                         dw[k] = fmaf(d, hat(r, c, st), dw[k]);
@@ -620,26 +617,13 @@ norm_backward_staged_kernel(const T* __restrict__ dy, const T* __restrict__ x,
         __syncthreads();
     }
     if (partial == nullptr) return;
-    // the row groups' sums of a column, in order (the buffers are free now)
-    float* join = reinterpret_cast<float*>(staged);
     float* out = partial + (int64_t)blockIdx.x * 2 * channels;
 #pragma unroll
-    for (int pass = 0; pass < 2; ++pass) {
-        if (groups > 1) {
-            if (group < groups) join[group * channels + column] = pass == 0 ? dw[0] : db[0];
-            __syncthreads();
-            if ((int)threadIdx.x < channels) {
-                float s = 0.0f;
-                for (int k = 0; k < groups; ++k) s += join[k * channels + threadIdx.x];
-                out[pass * channels + threadIdx.x] = s;
-            }
-            __syncthreads();
-        } else {
-#pragma unroll
-            for (int k = 0; k < kColumns; ++k) {
-                const int c = column + k * kThreads;
-                if (group < groups && c < channels) out[pass * channels + c] = pass == 0 ? dw[k] : db[k];
-            }
+    for (int k = 0; k < kColumns; ++k) {
+        const int c = threadIdx.x + k * kThreads;
+        if (c < channels) {
+            out[c] = dw[k];
+            out[channels + c] = db[k];
         }
     }
 }
@@ -781,8 +765,7 @@ mg_status backward_staged(const Backward& f) {
     const int chunk = stage_rows(f.channels, (int)sizeof(T));
     const int bytes = chunk * f.channels * (int)sizeof(T);
     const int held = HELD8 ? chunk * f.channels : bytes;
-    // the join at the end takes the buffers' place: 256 floats, or 1 KB a group
-    const int smem = std::max(2 * (align16(bytes) + align16(held)), 4 * kThreads) + 4 * (f.channels + 1) + 8 * chunk;
+    const int smem = 2 * (align16(bytes) + align16(held)) + 4 * (f.channels + 1) + 8 * chunk;
     static int known[64] = {};
     int per_sm = 0;
     MG_TRY(staged_launch(norm_backward_staged_kernel<T, LPR, HELD8>, kThreads, smem, known, &per_sm, "layer_norm_backward"));

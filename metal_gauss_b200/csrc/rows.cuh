@@ -34,22 +34,8 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
-// VEC elements at p as fp32; VEC * sizeof(T) is 16 bytes (p aligned to it) or
-// VEC is 1. Read-once data: past L1.
-template <typename T, int VEC>
-__device__ __forceinline__ void load_row(const T* __restrict__ p, float* v) {
-    if constexpr (VEC == 1) {
-        v[0] = to_f32<T>(__ldg(p));
-    } else {
-        static_assert(VEC * sizeof(T) == 16, "16-byte vectors");
-        const uint4 r = __ldg(reinterpret_cast<const uint4*>(p));
-        T e[VEC];
-        memcpy(e, &r, 16);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) v[i] = to_f32<T>(e[i]);
-    }
-}
-
+// VEC elements at p from fp32; VEC * sizeof(T) is 16 bytes (p aligned to it) or
+// VEC is 1.
 template <typename T, int VEC>
 __device__ __forceinline__ void store_row(T* __restrict__ p, const float* v) {
     if constexpr (VEC == 1) {
@@ -64,7 +50,8 @@ __device__ __forceinline__ void store_row(T* __restrict__ p, const float* v) {
     }
 }
 
-// The same without the conversion: 16-bit rows wait in half the registers.
+// VEC elements at p as they are: 16-bit rows wait in half the registers.
+// Read-once data: past L1.
 template <typename T, int VEC>
 __device__ __forceinline__ void load_raw(const T* __restrict__ p, T* v) {
     if constexpr (VEC == 1) {
