@@ -130,11 +130,10 @@ def _refuse_other_leaves(out: torch.Tensor, leaves: list[torch.Tensor]) -> None:
         if node is None or node in seen:
             continue
         seen.add(node)
-        leaf = getattr(node, "variable", None)
-        if leaf is not None and id(leaf) not in known:
-            raise RuntimeError(f"checkpoint8: fn uses a tensor {tuple(leaf.shape)} that needs a "
-                               "gradient and is none of its arguments: pass it as an argument, "
-                               "or detach it")
+        if node.name() == "torch::autograd::AccumulateGrad" and id(node.variable) not in known:
+            raise RuntimeError(f"checkpoint8: fn uses a tensor {tuple(node.variable.shape)} that "
+                               "needs a gradient and is none of its arguments: pass it as an "
+                               "argument, or detach it")
         todo.extend(n for n, _ in node.next_functions)
 
 

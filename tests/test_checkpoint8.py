@@ -159,3 +159,38 @@ def test_nothing_is_packed_where_no_gradient_is_wanted(cuda, monkeypatch):
     with pytest.raises(TypeError, match="one tensor"):
         checkpoint8(lambda t: (t, t), d)
     assert checkpoint8(head, x, lab).requires_grad and len(calls) == 1
+
+
+class Doubled(torch.autograd.Function):
+    """A user's function with an attribute called variable."""
+
+    @staticmethod
+    def forward(ctx, t):
+        ctx.variable = torch.zeros(1)
+        return t * 2
+
+    @staticmethod
+    def backward(ctx, grad):
+        return grad * 2
+
+
+def test_users_functions_and_segments_within_segments(cuda):
+    x, lab, head = case(7)
+    (got,) = torch.autograd.grad(checkpoint8(lambda t: Doubled.apply(t), x).sum(), x)
+    assert torch.equal(got, torch.full_like(x, 2.0))
+    # a segment within a segment: both inputs are read back from 8 bits
+    params = (head.weight, head.classes)
+
+    class Outer(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.head = head
+
+        def forward(self, t):
+            return checkpoint8(self.head, t * 1.5, lab)
+
+    got = torch.autograd.grad(checkpoint8(Outer(), x), (x, *params))
+    xr = held8(x).requires_grad_(True)
+    inner = held8(xr.detach() * 1.5).requires_grad_(True)
+    di, *want = torch.autograd.grad(head(inner, lab), (inner, *params))
+    assert all(torch.equal(a, b) for a, b in zip(got, (di * 1.5, *want)))
