@@ -766,8 +766,9 @@ mg_status mg_unpack8(const int8_t* codes, const float* scales, int64_t rows, int
  * label equals ignore_index has loss 0, takes no part in a mean and gets and
  * gives no gradient, whatever its features hold. A label outside [0,
  * n_classes) makes the loss NaN, records code 3 in the device error word, and
- * gives no gradient. reduction: MG_REDUCE_NONE writes `rows` losses,
- * MG_REDUCE_SUM and MG_REDUCE_MEAN one; the mean of no live rows is 0.
+ * gives no gradient. A row with an infinite or NaN logit has loss NaN.
+ * reduction: MG_REDUCE_NONE writes `rows` losses, MG_REDUCE_SUM and
+ * MG_REDUCE_MEAN one; the mean of no live rows is 0.
  * For the backward pass stats (2, rows) and live (1,) are written when not
  * NULL (live: sum and mean only): the log of the sum, 1 - softmax(label), and
  * the count of rows that take part. */

@@ -1,11 +1,13 @@
 """Activation checkpoints in 8 bits.
 
-The feature maps of a step's views are the largest tensors its backward pass
-holds. `pack8` puts a map into one byte per element and one fp32 scale per 128
-channels (`mg_pack8`), `unpack8` reads it back, and `checkpoint8(fn, x, ...)`
-runs a segment of the graph whose input is held in that form and computed
-again in the backward pass. `layernorm.layer_norm(saved="int8")` uses the same
-form without the second forward pass.
+What follows a feature map in the graph (normalisation, products, a loss) holds
+it and its own intermediate maps for the backward pass. `pack8` puts a map into
+one byte per element and one fp32 scale per 128 channels (`mg_pack8`), `unpack8`
+reads it back, and `checkpoint8(fn, x, ...)` runs a segment of the graph whose
+input is held in that form and computed again in the backward pass.
+`layernorm.layer_norm(saved="int8")` uses the same form without the second
+forward pass. What the rasteriser itself holds for the map's own gradient is
+untouched by this.
 
     a = largest magnitude of 128 channels of a row (fewer at its end)
     scale = a / 127,  code = round half even(x * (127 / a)),  value = code * scale

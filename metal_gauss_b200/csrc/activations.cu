@@ -226,8 +226,11 @@ mg_status pack_staged(const Pack& p) {
 }
 
 // Whole 16-byte vectors by row where the length allows; where not, staged chunks
-// of short rows (2000000 x 19 fp32: 100 us against 176 by single elements; at 77
-// channels they are level) and single elements of longer ones.
+// of short rows and single elements of longer ones. In us, staged and by elements:
+//   1766022 x 19 fp32 92 and 96, fp16 88 and 94; 400000 x 61 55 and 35, 53 and 35
+//   435771 x 77 fp32 68 and 47; 260111 x 129 76 and 70; 111476 x 301 72 and 49
+//   5000 x 19 8 and 6, 110000 x 19 12 and 10, 160000 x 19 14 and 14
+// So the border of 64 channels is too high (61 channels lose), by up to 20 us.
 template <typename T, int VEC>
 mg_status pack(const Pack& p) {
     if (aligned16(p.x) && p.channels % VEC == 0) return pick_team<T, VEC>(p, p.channels);

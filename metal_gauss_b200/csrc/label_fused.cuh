@@ -9,16 +9,20 @@
 // One streamed tile in shared memory serves both products: its channels are
 // the contraction of the first and the columns of the second.
 //
-// Bound by the exponentials of the groups (one per logit: 16 a clock and SM, 512
-// cycles a tile) while there are few channels, by the tensor cores above (a
-// product of 128 x 64 x 16 takes 48 cycles with both operands in shared memory,
-// which is what reading them takes; 32 with one in tensor memory). Measured, in
-// cycles a tile at 18944 x 4096 (rows, classes): bf16 1240 and 1310 (dx, dw) at
-// 16 channels, 1370 and 1630 at 64; fp32 1790 and 1910 at 16, 2840 and 3110 at
-// 64, 6040 and 6650 at 128, where only two streamed tiles fit. The logits are
+// Its floors: one exponential per logit (16 a clock and SM, 512 cycles a tile)
+// while there are few channels, the tensor cores above (a product of 128 x 64 x 16
+// takes 48 cycles with both operands in shared memory, which is what reading them
+// takes; 32 with one in tensor memory). It reaches neither: a group's turn
+// (scores, G, hand-over, next scores) is a chain that is waited for. Measured, in
+// cycles a tile at 18944 x 4096 (rows, classes): bf16 1230 and 1290 (dx, dw) at
+// 16 channels, 1360 and 1630 at 64; fp32 1730 and 1830 at 16 (exponentials 34 and
+// 37 % of their rate, tensor cores 25 and 28 %), 2750 and 3040 at 64, 6000 and 6790
+// at 128 (tensor cores 56 %), where only two streamed tiles fit. The logits are
 // computed twice in all (dx and dw), which costs less than 2 x PARTS bytes a
-// logit of G written and read twice: 640000 x 16 x 256 fp32 takes 158 + 121 us
-// against 405 + 581 + 487 us through scratch.
+// logit of G written and read twice: loss and gradients of 640000 x 16 x 256 fp32
+// take 430 us in all (153 + 117 of them here) against 990 with G through scratch,
+// 100003 x 77 x 4099 2240 against 2900, 640000 x 32 x 128 with its head 645 against
+// 875.
 // acc leaves tensor memory for the registers of eight more warps every
 // `per_segment` tiles: the tensor cores' fp32 additions truncate, and fp32
 // results keep their precision only over short runs of them.

@@ -51,6 +51,8 @@ constexpr float kInf = __builtin_huge_valf();
 constexpr float kNaN = __builtin_nanf("");
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+// Within 2^-22 of the value; below fp32's smallest normal number (2^-126) 0, so
+// smaller entries of a softmax count as none.
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

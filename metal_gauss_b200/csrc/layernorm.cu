@@ -254,7 +254,7 @@ template <typename T>
 struct HeldType<T, true> { using type = int8_t; };
 
 // Threads of the adjoint's block: half as many where a row has one warp, so that
-// blocks of 98 registers a thread (16 channels a lane) leave fewer registers over.
+// blocks of 92 registers a thread (16 channels a lane) leave fewer registers over.
 template <int WARPS>
 constexpr int kBackThreads = WARPS > 1 ? kThreads : 128;
 
@@ -780,11 +780,21 @@ mg_status backward_staged(const Backward& f) {
     return check_launch("layer_norm_backward");
 }
 
-// Where staging wins over single elements by row. Forward: up to 128 channels
-// (500000 x 77 fp32: 93 us against 135, 2000000 x 19: 135 against 324) and above
-// 512, where a team's row fills its registers (100000 x 1001 fp16: 150 us against
-// 356). The adjoint: above 512, where its sums for dw and db do (the same rows:
-// 247 us against 445; but 500000 x 77 fp32: 163 against 150).
+// Staged chunks or single elements by row: us staged/by elements, 2^25 elements
+// in all, fp32 and fp16 ("8": with the 8-bit form):
+//   channels  forward           forward 8          adjoint           adjoint 8
+//   19        117/285  115/305  195/354  197/371
+//   77         84/82    76/156  135/139  127/180
+//   129        98/74    86/131  168/113  156/180
+//   201        78/59    70/115  129/80   125/147
+//   301        74/59    66/127  125/82   113/150   130/108  114/98   170/173  156/163
+//   511        68/49    61/119  111/57   100/133   119/100  106/88   149/139  141/140
+//   601        63/59    55/135  104/78   100/154   129/118   98/119  141/440  137/313
+//   1001       63/49    57/135  115/61    98/147   176/102   96/106  178/322  131/264
+// Forward: staged up to 128 channels and above 512. 16-bit rows would gain from
+// it between those too; fp32 rows above 512 would do without. The adjoint: staged
+// above 512, for the rows held in 8 bits and the 16-bit ones; fp32 rows held in
+// full lose up to 70 us by it.
 template <typename T>
 bool staged(const Forward& f, mg_status* s) {
     if (f.channels > kStageMaxChannels || (f.channels > kBlock8 && f.channels <= 512)) return false;

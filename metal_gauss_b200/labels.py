@@ -93,7 +93,7 @@ def label_loss(features: torch.Tensor, classes: torch.Tensor, labels: torch.Tens
     channels) of the same type (float32, bfloat16 or float16); scale a number
     (a tensor that needs a gradient is refused); labels (...) uint8, int32 or
     int64; bias (n_classes,) float32 or of the features' type, -infinity taking
-    a class out. Pixels labelled ignore_index have loss 0 and
+    a class out (whose embedding is finite all the same). Pixels labelled ignore_index have loss 0 and
     no gradient whatever their features hold, and do not count in a mean. The
     result is float32: one value for reduction "mean" (0 when no pixel takes
     part) or "sum", labels' shape for "none". A row with an infinite logit has
