@@ -74,8 +74,9 @@ def _rows(t: torch.Tensor, what: str) -> tuple[int, int]:
 
 def pack8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """x (..., channels) in 8 bits: codes int8 (..., channels) and scales
-    float32 (..., ceil(channels / 128)), neither differentiable in x. 128 channels with an infinity or a
-    NaN among them read back as NaN; below 1e-30 they read back as 0."""
+    float32 (..., ceil(channels / 128)), neither differentiable in x. 128
+    channels with an infinity or a NaN among them read back as NaN; below 1e-30
+    they read back as 0."""
     code, (n, d) = dtype_code(x, "pack8: x"), _rows(x, "pack8: x")
     check_cuda(x, "pack8: x")
     x = x.detach().contiguous()
@@ -204,10 +205,10 @@ def checkpoint8(fn, x: torch.Tensor, *args) -> torch.Tensor:
     fn again. The result is fn's own; the gradients are those of fn at the x
     that was read back. fn must return one tensor and do the same work both
     times (no random numbers, no running statistics); it runs under the forward
-    pass's autocast state both times. Every other tensor that
-    needs a gradient has to be an argument: one that fn closes over, or that
-    sits in a list among args, makes the backward pass raise. Where no
-    gradient of those inputs is wanted, fn runs by itself and nothing is held."""
+    pass's autocast state both times. Every other tensor that needs a gradient
+    has to be an argument: one that fn closes over, or that sits in a list
+    among args, makes the backward pass raise. Where no gradient of those
+    inputs is wanted, fn runs by itself and nothing is held."""
     dtype_code(x, "checkpoint8: x")
     _rows(x, "checkpoint8: x")
     check_cuda(x, "checkpoint8: x")

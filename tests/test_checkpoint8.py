@@ -52,6 +52,14 @@ def test_a_modules_parameters_get_their_gradients(cuda, form):
     (checkpoint8(fn, x.detach(), *args) * 3).backward()
     assert all(torch.equal(p.grad, q) for p, q in zip(params, want[1:]))
     assert head.frozen.grad is None
+    # asked for the input's gradient alone
+    (gx,) = torch.autograd.grad(checkpoint8(fn, x, *args) * 3, x)
+    assert torch.equal(gx, want[0])
+    # a parameter that trains no more
+    head.weight.requires_grad_(False)
+    gx, gc = torch.autograd.grad(checkpoint8(fn, x, *args) * 3, (x, head.classes))
+    assert torch.equal(gx, want[0]) and torch.equal(gc, want[2])
+    head.weight.requires_grad_(True)
     # a leaf of a module as a plain argument
     w = head.weight
     (got,) = torch.autograd.grad(checkpoint8(lambda t, u: (t * u).sum(), x, w), w)
