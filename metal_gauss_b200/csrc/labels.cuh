@@ -133,6 +133,7 @@ __device__ __forceinline__ uint32_t take_part(float& lo, float& hi) {
 // Parts of the logits' gradient: two also for bf16 features, whose gradients
 // then carry no other rounding than their own (one part alone brings their
 // error from 0.0017 to 0.0028 of the norm).
+// A part below 2^-126 counts as none, so an entry of G under 2^-118 keeps fewer bits.
 template <int PARTS>
 constexpr int kGParts = PARTS == 1 ? 2 : PARTS;
 
